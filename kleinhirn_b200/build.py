@@ -31,7 +31,7 @@ def nvcc() -> str:
 
 
 def _headers_mtime() -> float:
-    hs = list(CSRC.glob("*.h")) + list(CSRC.glob("*.hpp")) + list((ROOT / "include").glob("*.h"))
+    hs = list(CSRC.glob("*.h")) + list(CSRC.glob("*.cuh")) + list(CSRC.glob("*.hpp")) + list((ROOT / "include").glob("*.h"))
     return max((h.stat().st_mtime for h in hs), default=0.0)
 
 
