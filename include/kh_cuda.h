@@ -246,6 +246,122 @@ int kh_attention_f16_noalloc(const void* qkv, const float* mask, void* ctx, cons
  * use ctx. (No counterpart in the reference.) */
 int kh_attention_f16_noalloc_status(void* stream);
 
+/* ---- operators around attention on caller-owned device buffers (no counterpart in the reference) ----
+ * What a layer that reads an encoder's packed states needs beside kh_attention_f16_noalloc: the norm
+ * of every query and key head with the position rotation, attention over states of another length,
+ * and a projection with the low-rank adapters of many requests. Common to the three:
+ * - Every pointer of an argument struct is device memory of the current device (or null where the
+ *   field says so), owned by the caller; strides are in elements. Nothing is allocated. The struct
+ *   itself is host memory and has been read when the call returns.
+ * - The work is queued on `stream` (a cudaStream_t of the current device, NULL for the legacy default
+ *   stream); the call returns once it is queued. Calls may be captured into a CUDA graph; the graph
+ *   then reads the same buffers. The library keeps no state between calls: calls on different streams
+ *   may overlap when they have different outputs and workspaces, and two graphs that may run at the
+ *   same time need a workspace each.
+ * - A workspace needs no initial contents, must be 256-byte aligned and holds nothing afterwards.
+ * - Segment starts ([n + 1] int32, not decreasing) live on the device, so a captured call serves
+ *   other lengths. Starts outside the buffer are cut to its rows. Rows before the first start and
+ *   behind the last are not written.
+ * - Sizes the kernels do not take are KH_ERR_ARG, said before anything is queued. What only the
+ *   device can see (a position outside its table, an adapter id that does not exist, a pipeline wait
+ *   that gave up) is reported by kh_operator_status. */
+
+/* Norm and rotation of the heads of q and k: rows of (q_heads + k_heads) * head_dim values of dtype
+ * (the q heads first, as in a plan's qkv buffer; what follows them in a row is not read). For every
+ * row and head y = x / sqrt(mean(x^2) + eps) * w, then the first rotary_dim values of y are rotated by
+ * the row's position: (a, b) -> (a cos - b sin, b cos + a sin) for the pairs (d, d + rotary_dim / 2),
+ * or (2 d, 2 d + 1) when interleaved, d < rotary_dim / 2. All of it in f32, rounded to dtype once.
+ * cossin: f32 [table_rows][2 * rotary_dim], cos of pair d at column d, sin at rotary_dim + d (the
+ * layout of a plan's cossin buffer). out may be x itself (with the same stride), else they must not
+ * overlap. A position outside [0, table_rows) gives a zero row and a status.
+ * Limits: head_dim even, in [2, 256]; rotary_dim even, in [0, head_dim]; q_heads + k_heads in
+ * [1, 4096]; either count may be 0. Any alignment and stride; 16-byte aligned buffers with strides of
+ * whole 16-byte units are the fast ones. */
+typedef struct kh_qk_norm_rope_args {
+  int32_t dtype;       /* KH_F32 or KH_F16 */
+  int32_t q_heads, k_heads, head_dim;
+  int32_t rotary_dim;  /* 0: no rotation (cossin, positions not read) */
+  int32_t interleaved; /* 0 or 1 */
+  float eps;           /* > 0 */
+  int64_t rows;        /* 0: nothing to do */
+  int64_t x_stride, out_stride; /* >= (q_heads + k_heads) * head_dim */
+  int64_t table_rows;
+  const void* x;
+  void* out;
+  const float* q_weight; /* [head_dim], or null for ones */
+  const float* k_weight; /* [head_dim], or null for ones */
+  const float* cossin;
+  const int32_t* positions; /* [rows] */
+} kh_qk_norm_rope_args;
+int kh_qk_norm_rope(const kh_qk_norm_rope_args* args, void* stream);
+
+/* Attention of packed query rows over the packed states of another length: sequence s has the query
+ * rows [q_starts[s], q_starts[s + 1]) and the state rows [k_starts[s], k_starts[s + 1]); query head h
+ * reads key / value head h / (q_heads / kv_heads); out = softmax(scale q k^T) v over the states whose
+ * key_mask is above 0.5. A row without a kept state is exactly zero, whatever k and v hold there.
+ * f16 operands; scores, sums and the accumulated output in f32, the probabilities rounded to f16 for
+ * the product with v, the output once. max_q and max_k bound the lengths (they size the grid and the
+ * split): of a longer sequence, query rows past max_q are not written and states past max_k not read.
+ * Limits: head_dim 32, 64 or 128; kv_heads divides q_heads (at most 1,024), at most 64 query heads to
+ * one; max_q and max_k at most 2^24; n_seqs at
+ * most 65,535; buffers 16-byte aligned with strides of whole 16-byte units; rows below 2^31. */
+typedef struct kh_cross_attention_args {
+  int32_t n_seqs; /* 0: nothing to do */
+  int32_t q_heads, kv_heads, head_dim;
+  int32_t max_q, max_k; /* >= 0 */
+  float scale;
+  int64_t q_rows, kv_rows; /* rows of the buffers */
+  int64_t q_stride, k_stride, v_stride, out_stride;
+  const void* q; /* f16 [q_rows][q_heads * head_dim] */
+  const void* k; /* f16 [kv_rows][kv_heads * head_dim] */
+  const void* v;
+  void* out;             /* f16 [q_rows][q_heads * head_dim] */
+  const float* key_mask; /* [kv_rows] 1 keep, 0 masked; or null: every state is kept */
+  const int32_t* q_starts; /* [n_seqs + 1] */
+  const int32_t* k_starts; /* [n_seqs + 1] */
+  void* workspace;
+  uint64_t workspace_bytes;
+} kh_cross_attention_args;
+/* Bytes of workspace of such a call (pointers and strides are not read), or -1 and kh_last_error. */
+int64_t kh_cross_attention_f16_workspace(const kh_cross_attention_args* args);
+int kh_cross_attention_f16(const kh_cross_attention_args* args, void* stream);
+
+/* A projection with the low-rank adapters of many requests: rows [seg_starts[i], seg_starts[i + 1])
+ * of x belong to request i, whose adapter is a = seg_adapters[i]:
+ *   out = x w^T + bias + scales[a] (x lora_a[a]^T) lora_b[a]^T
+ * f16 operands, f32 sums, the rank-sized product (with its scale) rounded to f16 once and added to the
+ * same f32 accumulator as the projection; the output is rounded once. A negative id is a request
+ * without an adapter; an id of n_adapters or more counts as none and gives a status.
+ * Limits: k, n and rank multiples of 8, k and n in [8, 65,536], rank in [8, 128] (pad a smaller one
+ * with zeros); n_segs at most 65,535; buffers 16-byte aligned, strides whole 16-byte units; rows
+ * below 2^31 - 256. */
+typedef struct kh_lora_matmul_args {
+  int32_t k, n, rank, n_adapters;
+  int32_t n_segs; /* 0: nothing to do */
+  int64_t rows;   /* rows of the buffers */
+  int64_t x_stride, out_stride;
+  const void* x;      /* f16 [rows][k] */
+  const void* w;      /* f16 [n][k] */
+  const void* bias;   /* f16 [n], or null */
+  const void* lora_a; /* f16 [n_adapters][rank][k] */
+  const void* lora_b; /* f16 [n_adapters][n][rank] */
+  const float* scales; /* [n_adapters], or null for ones */
+  const int32_t* seg_starts;   /* [n_segs + 1] */
+  const int32_t* seg_adapters; /* [n_segs] */
+  void* out; /* f16 [rows][n] */
+  void* workspace;
+  uint64_t workspace_bytes;
+} kh_lora_matmul_args;
+/* Bytes of workspace of such a call (pointers and strides are not read), or -1 and kh_last_error. */
+int64_t kh_lora_matmul_f16_workspace(const kh_lora_matmul_args* args);
+int kh_lora_matmul_f16(const kh_lora_matmul_args* args, void* stream);
+
+/* Waits for `stream` (as cudaStreamSynchronize) and reports what the three operators above met on the
+ * current device since the last report: KH_OK; KH_ERR_ARG for a position outside its table or an
+ * adapter id that does not exist; KH_ERR_CUDA for a pipeline wait that gave up (the output is then
+ * partly written). Reading clears it. Not while a capture is under way. */
+int kh_operator_status(void* stream);
+
 /* ---- failure-path self-tests (no counterpart in the reference) ----
  * They make the failure on purpose, in the forms that leave the GPU usable, so the error
  * handling of a context can be tested on a live device.

@@ -71,6 +71,12 @@ _SIGS = {
     "kh_attention_f16_noalloc": ([_P, _P, _P, _P, ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_float,
                                   ctypes.c_int, _P], ctypes.c_int),
     "kh_attention_f16_noalloc_status": ([_P], ctypes.c_int),
+    "kh_qk_norm_rope": ([_P, _P], ctypes.c_int),
+    "kh_cross_attention_f16_workspace": ([_P], ctypes.c_int64),
+    "kh_cross_attention_f16": ([_P, _P], ctypes.c_int),
+    "kh_lora_matmul_f16_workspace": ([_P], ctypes.c_int64),
+    "kh_lora_matmul_f16": ([_P, _P], ctypes.c_int),
+    "kh_operator_status": ([_P], ctypes.c_int),
     "kh_inject_cuda_error": ([_P, ctypes.c_char_p], ctypes.c_int),
     "kh_selftest_wait_limit": ([_P, ctypes.c_int], ctypes.c_int),
     "kh_selftest_tensor_maps": ([ctypes.c_int, ctypes.c_int], ctypes.c_int64),
@@ -123,6 +129,80 @@ def attention_f16_noalloc_status(stream: int = 0) -> None:
     pipeline wait on the current device gave up since the last report (the report clears it)."""
     lib = load_library()
     _check(lib, lib.kh_attention_f16_noalloc_status(stream or None))
+
+
+class QkNormRopeArgs(ctypes.Structure):
+    """kh_qk_norm_rope_args: fields as in include/kh_cuda.h, pointers as integers (None for null)."""
+    _fields_ = [("dtype", ctypes.c_int32), ("q_heads", ctypes.c_int32), ("k_heads", ctypes.c_int32),
+                ("head_dim", ctypes.c_int32), ("rotary_dim", ctypes.c_int32), ("interleaved", ctypes.c_int32),
+                ("eps", ctypes.c_float), ("rows", ctypes.c_int64), ("x_stride", ctypes.c_int64),
+                ("out_stride", ctypes.c_int64), ("table_rows", ctypes.c_int64), ("x", _P), ("out", _P),
+                ("q_weight", _P), ("k_weight", _P), ("cossin", _P), ("positions", _P)]
+
+
+class CrossAttentionArgs(ctypes.Structure):
+    """kh_cross_attention_args."""
+    _fields_ = [("n_seqs", ctypes.c_int32), ("q_heads", ctypes.c_int32), ("kv_heads", ctypes.c_int32),
+                ("head_dim", ctypes.c_int32), ("max_q", ctypes.c_int32), ("max_k", ctypes.c_int32),
+                ("scale", ctypes.c_float), ("q_rows", ctypes.c_int64), ("kv_rows", ctypes.c_int64),
+                ("q_stride", ctypes.c_int64), ("k_stride", ctypes.c_int64), ("v_stride", ctypes.c_int64),
+                ("out_stride", ctypes.c_int64), ("q", _P), ("k", _P), ("v", _P), ("out", _P), ("key_mask", _P),
+                ("q_starts", _P), ("k_starts", _P), ("workspace", _P), ("workspace_bytes", ctypes.c_uint64)]
+
+
+class LoraMatmulArgs(ctypes.Structure):
+    """kh_lora_matmul_args."""
+    _fields_ = [("k", ctypes.c_int32), ("n", ctypes.c_int32), ("rank", ctypes.c_int32),
+                ("n_adapters", ctypes.c_int32), ("n_segs", ctypes.c_int32), ("rows", ctypes.c_int64),
+                ("x_stride", ctypes.c_int64), ("out_stride", ctypes.c_int64), ("x", _P), ("w", _P), ("bias", _P),
+                ("lora_a", _P), ("lora_b", _P), ("scales", _P), ("seg_starts", _P), ("seg_adapters", _P), ("out", _P),
+                ("workspace", _P), ("workspace_bytes", ctypes.c_uint64)]
+
+
+def _operator(name: str, args, stream: int) -> None:
+    lib = load_library()
+    _check(lib, getattr(lib, name)(ctypes.addressof(args), stream or None))
+
+
+def _workspace_bytes(name: str, args) -> int:
+    lib = load_library()
+    n = int(getattr(lib, name)(ctypes.addressof(args)))
+    if n < 0:
+        raise KhError(1, lib.kh_last_error().decode("utf-8", "replace"))
+    return n
+
+
+def qk_norm_rope(args: QkNormRopeArgs, stream: int = 0) -> None:
+    """kh_qk_norm_rope: per-head norm of q and k rows with the position rotation. Queues the work on
+    `stream`; the caller keeps `args` and its buffers and may call again."""
+    _operator("kh_qk_norm_rope", args, stream)
+
+
+def cross_attention_f16_workspace(args: CrossAttentionArgs) -> int:
+    """Bytes of workspace that cross_attention_f16 needs for these sizes."""
+    return _workspace_bytes("kh_cross_attention_f16_workspace", args)
+
+
+def cross_attention_f16(args: CrossAttentionArgs, stream: int = 0) -> None:
+    """kh_cross_attention_f16: packed query rows over packed states of another length."""
+    _operator("kh_cross_attention_f16", args, stream)
+
+
+def lora_matmul_f16_workspace(args: LoraMatmulArgs) -> int:
+    """Bytes of workspace that lora_matmul_f16 needs for these sizes."""
+    return _workspace_bytes("kh_lora_matmul_f16_workspace", args)
+
+
+def lora_matmul_f16(args: LoraMatmulArgs, stream: int = 0) -> None:
+    """kh_lora_matmul_f16: a projection with the low-rank adapter of each request's rows."""
+    _operator("kh_lora_matmul_f16", args, stream)
+
+
+def operator_status(stream: int = 0) -> None:
+    """kh_operator_status: waits for `stream`; raises KhError if one of the operators above met a
+    position or adapter id outside its table, or gave up a pipeline wait (the report clears it)."""
+    lib = load_library()
+    _check(lib, lib.kh_operator_status(stream or None))
 
 
 def selftest_tensor_maps(threads: int, iters: int) -> int:

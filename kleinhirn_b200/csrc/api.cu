@@ -13,6 +13,7 @@
 
 #include "../../include/kh_cuda.h"
 #include "attn_tc.h"
+#include "device_ops.h"
 #include "gemm_tc.h"
 #include "gemm_tf32.h"
 #include "runtime.h"
@@ -1045,6 +1046,34 @@ int kh_attention_f16_noalloc_status(void* stream) {
     if (code)
       throw kh::CudaError("attention pipeline wait timed out (attention code " + std::to_string(code) + ")");
   });
+}
+
+int kh_qk_norm_rope(const kh_qk_norm_rope_args* args, void* stream) {
+  return guard(nullptr, Latch::No, [&] { kh::qk_norm_rope(args, static_cast<cudaStream_t>(stream)); });
+}
+
+int64_t kh_cross_attention_f16_workspace(const kh_cross_attention_args* args) {
+  int64_t bytes = -1;
+  const int st = guard(nullptr, Latch::No, [&] { bytes = kh::cross_attention_workspace(args); });
+  return st == KH_OK ? bytes : -1;
+}
+
+int kh_cross_attention_f16(const kh_cross_attention_args* args, void* stream) {
+  return guard(nullptr, Latch::No, [&] { kh::cross_attention(args, static_cast<cudaStream_t>(stream)); });
+}
+
+int64_t kh_lora_matmul_f16_workspace(const kh_lora_matmul_args* args) {
+  int64_t bytes = -1;
+  const int st = guard(nullptr, Latch::No, [&] { bytes = kh::lora_matmul_workspace(args); });
+  return st == KH_OK ? bytes : -1;
+}
+
+int kh_lora_matmul_f16(const kh_lora_matmul_args* args, void* stream) {
+  return guard(nullptr, Latch::No, [&] { kh::lora_matmul(args, static_cast<cudaStream_t>(stream)); });
+}
+
+int kh_operator_status(void* stream) {
+  return guard(nullptr, Latch::No, [&] { kh::operator_status(static_cast<cudaStream_t>(stream)); });
 }
 
 int kh_inject_cuda_error(kh_ctx* ctx, const char* what) {

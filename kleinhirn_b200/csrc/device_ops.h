@@ -1,0 +1,37 @@
+// Operators on caller-owned device buffers: the norm and rotation of query and key heads (qk_norm.cu),
+// cross attention to packed states (cross_attn.cu), projections with low-rank adapters (lora.cu).
+#pragma once
+
+#include <cuda_runtime.h>
+
+#include <cstdint>
+
+#include "../../include/kh_cuda.h"
+
+namespace kh {
+
+void qk_norm_rope(const kh_qk_norm_rope_args* a, cudaStream_t st);
+int64_t cross_attention_workspace(const kh_cross_attention_args* a);
+void cross_attention(const kh_cross_attention_args* a, cudaStream_t st);
+int64_t lora_matmul_workspace(const kh_lora_matmul_args* a);
+void lora_matmul(const kh_lora_matmul_args* a, cudaStream_t st);
+
+// Synchronizes `st`; throws what the operators met on the current device since the last report
+// (ArgError: a position or an adapter id outside its table; CudaError: a wait that gave up).
+void operator_status(cudaStream_t st);
+
+// Code each operator's kernels left on the current device (0: none), read and cleared.
+constexpr int OP_BAD_INDEX = 1;  // a position or an adapter id outside its table; others: waits
+int qk_norm_error_code();
+int cross_attention_error_code();
+int lora_error_code();
+
+// Shared argument checks (ArgError with the entry point's name).
+void check_that(bool ok, const char* fn, const char* what);
+// The stream belongs to the current device.
+void check_stream(const char* fn, cudaStream_t st);
+// Memory a kernel on the current device can use: device memory of that device, managed or page-locked
+// host memory. A pointer of another device or of plain host memory would fault in the kernel.
+void check_device_memory(const char* fn, const char* what, const void* p);
+
+}  // namespace kh
