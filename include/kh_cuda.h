@@ -303,13 +303,13 @@ int kh_qk_norm_rope(const kh_qk_norm_rope_args* args, void* stream);
  * the product with v, the output once. max_q and max_k bound the lengths (they size the grid and the
  * split): of a longer sequence, query rows past max_q are not written and states past max_k not read.
  * Limits: head_dim 32, 64 or 128; kv_heads divides q_heads (at most 1,024), at most 64 query heads to
- * one; max_q and max_k at most 2^24; n_seqs at
- * most 65,535; buffers 16-byte aligned with strides of whole 16-byte units; rows below 2^31. */
+ * one; max_q and max_k at most 2^24; n_seqs at most 65,535; buffers 16-byte aligned with strides of
+ * whole 16-byte units; rows below 2^31. */
 typedef struct kh_cross_attention_args {
   int32_t n_seqs; /* 0: nothing to do */
   int32_t q_heads, kv_heads, head_dim;
   int32_t max_q, max_k; /* >= 0 */
-  float scale;
+  float scale; /* > 0, finite */
   int64_t q_rows, kv_rows; /* rows of the buffers */
   int64_t q_stride, k_stride, v_stride, out_stride;
   const void* q; /* f16 [q_rows][q_heads * head_dim] */

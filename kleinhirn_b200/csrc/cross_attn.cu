@@ -1,16 +1,25 @@
 // Cross attention of packed query rows over an encoder's packed states of another length.
 //
-// For query row i of sequence s and query head h, with g = q_heads / kv_heads and the kept states K of
-// s: out = sum_j p_j v_j, p = softmax over j in K of scale q_i,h . k_j,h/g; zero where K is empty.
+// For query row i of sequence s and query head h, with G = q_heads / kv_heads and K the kept states of
+// s: out = sum_j p_j v_j, p the softmax over j in K of scale q_i,h . k_j,h/G; zero where K is empty.
+// Both kernels make one pass over the states with a running reference point m (log2 units) and the sum
+// l of 2^(s - m): m moves only when a score exceeds it by more than 8, so the accumulated output is
+// rescaled seldom and p stays within 2^8, where f16 (the operand of the product with v) rounds it by
+// 2^-11 as anywhere; m, l, scores and the output accumulate in f32.
+// The G query heads of a key head are rows of the same tile (row = query * G + head), so k and v are
+// read once for them.
 //
-// One warp per (query row, head): the warp walks the states with the running maximum m and sum l of
-// the exponentials, its lanes hold D / 32 values of the row each.
+// Which kernel: see takes_rows_kernel. Few rows to a key head (single tokens): bound by reading k and v
+// once, cross_rows_kernel. More: tensor-core products of 128 rows, cross_tile_kernel. Where the rows
+// leave SMs idle, the states of a sequence are split over CTAs, whose partial (m, l, O) the workspace
+// holds and cross_join_kernel adds up in split order.
 
 #include "device_ops.h"
 
 #include <cuda_fp16.h>
 
 #include <algorithm>
+#include <atomic>
 
 #include "runtime.h"
 #include "sm100.cuh"
@@ -30,9 +39,11 @@ struct CrossParams {
   const float* mask;
   const int32_t* q_starts;
   const int32_t* k_starts;
+  float* part_o;   // [nsplit][n_seqs * max_q][q_heads][D]
+  float2* part_ml; // [nsplit][n_seqs * max_q][q_heads]: m, l
   int64_t q_rows, kv_rows, q_stride, k_stride, v_stride, out_stride;
-  int n_seqs, q_heads, kv_heads, max_q, max_k;
-  float scale;
+  int n_seqs, q_heads, kv_heads, G, max_q, max_k, nsplit;
+  float scale_log2;  // scale * log2(e)
 };
 
 // Rows of sequence s in a buffer of `rows`: starts outside it are cut, a longer sequence ends at `most`.
@@ -42,38 +53,651 @@ __device__ __forceinline__ void seq_range(const int32_t* starts, int s, int64_t 
   n = int(min(r1 - r0, int64_t(most)));
 }
 
+// Where the partial result of query i of sequence s, head h, split z lies.
+__device__ __forceinline__ int64_t part_index(const CrossParams& p, int z, int s, int i, int h) {
+  return ((int64_t(z) * p.n_seqs + s) * p.max_q + i) * p.q_heads + h;
+}
+
+// ---- few rows: registers straight from global memory, mma.sync ----
+//
+// One CTA of 4 warps per (split, key head, sequence), rows <= 16 as one m16 block. A warp takes 16
+// states at a time: S = Q K^T in m16n8k16 products, then O += P V with S's accumulator layout as P's
+// operand layout. The sum over the head's values and the order of the states and output columns are
+// free, so every thread loads 16-byte pieces of k and v in the order they lie in memory, with no
+// shared memory and no shuffles: within 32 values of k, the quad lane t holds values 8 t .. 8 t + 7 of
+// q and k alike; of v, it holds the D / 8 values (lane / 4) D / 8 .. of its own four states. Loads
+// run one step ahead. Bound: HBM (2 D 2 bytes per state and key head, each read once).
+
+__device__ __forceinline__ void mma_16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                          uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t pack_half2(float a, float b) {
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+constexpr int RW = 4;      // warps of a CTA
+constexpr int RSTEP = 16;  // states of a warp's step
+
 template <int D>
-__global__ void __launch_bounds__(128) cross_simple_kernel(const CrossParams p) {
-  constexpr int E = D / 32;
-  const int lane = threadIdx.x & 31;
-  const int s = blockIdx.z, h = blockIdx.y;
-  const int i = blockIdx.x * 4 + (threadIdx.x >> 5);
+struct RowsStep {
+  uint4 k[2][D / 32];         // [block of 8 states][32 values]
+  uint32_t v[2][2][D / 16];   // [block][state of the pair][packed values]
+  bool keep[2][2];
+};
+
+template <int D>
+__device__ __forceinline__ void rows_load(RowsStep<D>& r, const CrossParams& p, const __half* kb, const __half* vb,
+                                          const float* mb, int first, int end, int lane) {
+#pragma unroll
+  for (int b = 0; b < 2; ++b) {
+    const int j = first + 8 * b + (lane >> 2);
+#pragma unroll
+    for (int c = 0; c < D / 32; ++c) {
+      r.k[b][c] = make_uint4(0, 0, 0, 0);
+      if (j < end) r.k[b][c] = __ldg(reinterpret_cast<const uint4*>(kb + int64_t(j) * p.k_stride + c * 32 + (lane & 3) * 8));
+    }
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int jv = first + 8 * b + (lane & 3) * 2 + e;
+      const bool keep = jv < end && (!mb || __ldg(mb + jv) > 0.5f);
+      r.keep[b][e] = keep;
+      const __half* row = vb + int64_t(jv) * p.v_stride + (lane >> 2) * (D / 8);
+      // a dropped state's values are never loaded: whatever they hold stays out of the sums
+      if constexpr (D == 32) {
+        uint2 u = make_uint2(0, 0);
+        if (keep) u = __ldg(reinterpret_cast<const uint2*>(row));
+        r.v[b][e][0] = u.x;
+        r.v[b][e][1] = u.y;
+      } else {
+#pragma unroll
+        for (int c = 0; c < D / 64; ++c) {
+          uint4 u = make_uint4(0, 0, 0, 0);
+          if (keep) u = __ldg(reinterpret_cast<const uint4*>(row) + c);
+          r.v[b][e][4 * c] = u.x;
+          r.v[b][e][4 * c + 1] = u.y;
+          r.v[b][e][4 * c + 2] = u.z;
+          r.v[b][e][4 * c + 3] = u.w;
+        }
+      }
+    }
+  }
+}
+
+template <int D>
+__global__ void __launch_bounds__(RW * 32) cross_rows_kernel(const CrossParams p) {
+  constexpr int E = D / 8;  // output columns of 8 at a time
+  __shared__ float so[RW][16][D + 4];
+  __shared__ float sm[RW][16], sl[RW][16];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int split = blockIdx.x, hk = blockIdx.y, s = blockIdx.z;
   int64_t q0, k0;
   int nq, nk;
   seq_range(p.q_starts, s, p.q_rows, p.max_q, q0, nq);
   seq_range(p.k_starts, s, p.kv_rows, p.max_k, k0, nk);
-  if (i >= nq) return;
-  const int hk = h / (p.q_heads / p.kv_heads);
-  float q[E], o[E], m = -INFINITY, l = 0.f;
-  for (int e = 0; e < E; ++e) {
-    q[e] = __half2float(p.q[(q0 + i) * p.q_stride + h * D + e * 32 + lane]) * p.scale;
-    o[e] = 0.f;
+  const int rows = nq * p.G;  // <= 16
+  if (rows == 0) return;
+  // states of this split: whole steps of the CTA's warps
+  const int per = ((nk + p.nsplit - 1) / p.nsplit + RSTEP - 1) / RSTEP * RSTEP;
+  const int begin = min(split * per, nk), end = min(begin + per, nk);
+
+  // A operand: rows lane / 4 and lane / 4 + 8
+  uint32_t qa[D / 32][2][4];
+#pragma unroll
+  for (int c = 0; c < D / 32; ++c)
+#pragma unroll
+    for (int hl = 0; hl < 2; ++hl) {
+      const int r = (lane >> 2) + 8 * hl;
+      uint4 u = make_uint4(0, 0, 0, 0);
+      if (r < rows)
+        u = *reinterpret_cast<const uint4*>(p.q + (q0 + r / p.G) * p.q_stride + (hk * p.G + r % p.G) * D + c * 32 +
+                                            (lane & 3) * 8);
+      qa[c][hl][0] = u.x;
+      qa[c][hl][1] = u.y;
+      qa[c][hl][2] = u.z;
+      qa[c][hl][3] = u.w;
+    }
+
+  const __half* kb = p.k + k0 * p.k_stride + hk * D;
+  const __half* vb = p.v + k0 * p.v_stride + hk * D;
+  const float* mb = p.mask ? p.mask + k0 : nullptr;
+  float o[E][4];
+#pragma unroll
+  for (int e = 0; e < E; ++e) o[e][0] = o[e][1] = o[e][2] = o[e][3] = 0.f;
+  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};  // rows lane / 4 and + 8; l of this thread's states
+
+  RowsStep<D> cur, nxt;
+  int first = begin + warp * RSTEP;
+  if (first < end) rows_load<D>(cur, p, kb, vb, mb, first, end, lane);
+  for (; first < end; first += RW * RSTEP) {
+    if (first + RW * RSTEP < end) rows_load<D>(nxt, p, kb, vb, mb, first + RW * RSTEP, end, lane);
+    float sc[2][4];
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+      sc[b][0] = sc[b][1] = sc[b][2] = sc[b][3] = 0.f;
+#pragma unroll
+      for (int c = 0; c < D / 32; ++c) {
+        const uint4 kk = cur.k[b][c];
+        mma_16816(sc[b], qa[c][0][0], qa[c][1][0], qa[c][0][1], qa[c][1][1], kk.x, kk.y);
+        mma_16816(sc[b], qa[c][0][2], qa[c][1][2], qa[c][0][3], qa[c][1][3], kk.z, kk.w);
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) sc[b][i] = cur.keep[b][i & 1] ? sc[b][i] * p.scale_log2 : -INFINITY;
+    }
+    float top[2];
+#pragma unroll
+    for (int r = 0; r < 2; ++r)
+      top[r] = fmaxf(fmaxf(sc[0][2 * r], sc[0][2 * r + 1]), fmaxf(sc[1][2 * r], sc[1][2 * r + 1]));
+    if (__any_sync(0xffffffffu, top[0] > m[0] + 8.f || top[1] > m[1] + 8.f)) {
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 1));
+        top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 2));
+        const float mn = fmaxf(m[r], top[r]);
+        const float corr = mn > m[r] ? ex2_approx(m[r] - mn) : 1.f;  // (0 from m = -inf)
+        m[r] = mn;
+        l[r] *= corr;
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+          o[e][2 * r] *= corr;
+          o[e][2 * r + 1] *= corr;
+        }
+      }
+    }
+    const float ref[2] = {m[0] == -INFINITY ? 0.f : m[0], m[1] == -INFINITY ? 0.f : m[1]};
+    uint32_t pa[2][2];
+#pragma unroll
+    for (int b = 0; b < 2; ++b)
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        const float x0 = ex2_approx(sc[b][2 * r] - ref[r]), x1 = ex2_approx(sc[b][2 * r + 1] - ref[r]);
+        l[r] += x0 + x1;
+        pa[b][r] = pack_half2(x0, x1);
+      }
+#pragma unroll
+    for (int e2 = 0; e2 < E / 2; ++e2) {
+      // columns 2 e2 and 2 e2 + 1 of the thread's v values: pairs of states side by side
+      const uint32_t u0 = cur.v[0][0][e2], u1 = cur.v[0][1][e2], w0 = cur.v[1][0][e2], w1 = cur.v[1][1][e2];
+      mma_16816(o[2 * e2], pa[0][0], pa[0][1], pa[1][0], pa[1][1], __byte_perm(u0, u1, 0x5410), __byte_perm(w0, w1, 0x5410));
+      mma_16816(o[2 * e2 + 1], pa[0][0], pa[0][1], pa[1][0], pa[1][1], __byte_perm(u0, u1, 0x7632),
+                __byte_perm(w0, w1, 0x7632));
+    }
+    cur = nxt;
   }
-  for (int j = 0; j < nk; ++j) {
-    if (p.mask && !(p.mask[k0 + j] > 0.5f)) continue;
-    float d = 0.f;
-    for (int e = 0; e < E; ++e) d += q[e] * __half2float(p.k[(k0 + j) * p.k_stride + hk * D + e * 32 + lane]);
-    for (int w = 16; w; w >>= 1) d += __shfl_xor_sync(0xffffffffu, d, w);
-    const float mn = fmaxf(m, d);
-    const float c = mn == -INFINITY ? 1.f : expf(m - mn), x = mn == -INFINITY ? 0.f : expf(d - mn);
-    m = mn;
-    l = l * c + x;
-    for (int e = 0; e < E; ++e)
-      o[e] = o[e] * c + x * __half2float(p.v[(k0 + j) * p.v_stride + hk * D + e * 32 + lane]);
+#pragma unroll
+  for (int r = 0; r < 2; ++r) {
+    l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
+    l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
+    const int row = (lane >> 2) + 8 * r;
+    if ((lane & 3) == 0) {
+      sm[warp][row] = m[r];
+      sl[warp][row] = l[r];
+    }
+    // column n = 2 (lane & 3) + i of block e is output value n E + e
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int e = 0; e < E; ++e) so[warp][row][(2 * (lane & 3) + i) * E + e] = o[e][2 * r + i];
   }
-  for (int e = 0; e < E; ++e)
-    p.out[(q0 + i) * p.out_stride + h * D + e * 32 + lane] = __float2half_rn(l > 0.f ? o[e] / l : l);
+  __syncthreads();
+  // the four warps' parts, 8 output values of a row per thread
+  for (int t = threadIdx.x; t < rows * (D / 8); t += RW * 32) {
+    const int row = t / (D / 8), d = t % (D / 8) * 8;
+    float mm = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < RW; ++w) mm = fmaxf(mm, sm[w][row]);
+    float lt = 0.f, acc[8] = {};
+#pragma unroll
+    for (int w = 0; w < RW; ++w) {
+      const float f = sm[w][row] == -INFINITY ? 0.f : ex2_approx(sm[w][row] - mm);
+      lt += f * sl[w][row];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) acc[i] += f * so[w][row][d + i];
+    }
+    const int qi = row / p.G, h = hk * p.G + row % p.G;
+    if (p.nsplit == 1) {
+      const float inv = lt == 0.f ? 0.f : 1.f / lt;
+      uint32_t u[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) u[i] = pack_half2(acc[2 * i] * inv, acc[2 * i + 1] * inv);
+      *reinterpret_cast<uint4*>(p.out + (q0 + qi) * p.out_stride + h * D + d) = make_uint4(u[0], u[1], u[2], u[3]);
+    } else {
+      const int64_t at = part_index(p, split, s, qi, h);
+      float4* dst = reinterpret_cast<float4*>(p.part_o + at * D + d);
+      dst[0] = make_float4(acc[0], acc[1], acc[2], acc[3]);
+      dst[1] = make_float4(acc[4], acc[5], acc[6], acc[7]);
+      if (d == 0) p.part_ml[at] = make_float2(mm, lt);
+    }
+  }
 }
+
+// ---- joining the splits: one warp per (query, head) ----
+
+template <int D>
+__global__ void __launch_bounds__(128) cross_join_kernel(const CrossParams p) {
+  constexpr int V = D / 32;
+  const int lane = threadIdx.x & 31;
+  const int64_t t = int64_t(blockIdx.x) * 4 + (threadIdx.x >> 5);
+  const int64_t per_seq = int64_t(p.max_q) * p.q_heads;
+  const int s = int(t / per_seq);
+  if (s >= p.n_seqs) return;
+  const int i = int((t - s * per_seq) / p.q_heads), h = int(t % p.q_heads);
+  int64_t q0;
+  int nq;
+  seq_range(p.q_starts, s, p.q_rows, p.max_q, q0, nq);
+  if (i >= nq) return;
+  float m = -INFINITY, l = 0.f, o[V] = {};
+  for (int z = 0; z < p.nsplit; ++z) {
+    const int64_t at = part_index(p, z, s, i, h);
+    const float2 ml = p.part_ml[at];
+    if (ml.x == -INFINITY) continue;  // no kept state (its O is not written)
+    const float mn = fmaxf(m, ml.x);
+    const float c = ex2_approx(m - mn), f = ex2_approx(ml.x - mn);
+    m = mn;
+    l = l * c + ml.y * f;
+#pragma unroll
+    for (int e = 0; e < V; ++e) o[e] = o[e] * c + p.part_o[at * D + lane * V + e] * f;
+  }
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  __half* dst = p.out + (q0 + i) * p.out_stride + h * D + lane * V;
+#pragma unroll
+  for (int e = 0; e < V; ++e) dst[e] = __float2half_rn(o[e] * inv);
+}
+
+// ---- tiles of 128 rows on the tensor cores ----
+//
+// One CTA per (block of two row tiles, key head and split, sequence), one CTA per SM, 320 threads:
+//   warp 0     TMA: Q once, tiles of 128 states of K and V into two rings;
+//   warp 1     one thread issues S = Q K^T (M 128, N 128, K = D) into the stream's 128 TMEM columns and
+//              O += P V (A = P from TMEM, V as an MN-major operand) into its O columns;
+//   warps 2-9  softmax, warps 2-5 stream 0 and 6-9 stream 1, one thread per row: 128 scores in
+//              registers, P (f16) written over S in TMEM.
+// The two streams are two row tiles over the same K and V tiles; where the CTA's rows fit one tile,
+// they take its even and odd key tiles instead and add up their (m, l, O) at the end. One stream's
+// softmax runs under the other's products. S of the next tile is issued behind P V of the last one, in
+// order, so P may lie over S, and a full S means that the products before it are done.
+// Key tiles with dropped states (past the end, masked): their scores become -inf and their V rows zero
+// in shared memory, so that nothing they hold reaches a sum.
+
+constexpr int TROWS = 128;
+constexpr int TKEYS = 128;
+constexpr int TTHREADS = 320;
+
+template <int D>
+struct TCfg {
+  static constexpr int PANELS = D == 128 ? 2 : 1;    // columns of a swizzled row: 64 (D 32: 32)
+  static constexpr int PCOLS = D / PANELS;
+  static constexpr int ROWB = PCOLS * 2;             // bytes of a row of a panel: the swizzle width
+  static constexpr int PANEL = 128 * ROWB;
+  static constexpr int TILE = PANELS * PANEL;        // 128 rows of q, k or v
+  static constexpr int KS = D == 128 ? 3 : 4;        // ring stages
+  static constexpr int VS = D == 128 ? 2 : 4;
+  static constexpr int K_OFF = 2 * TILE;             // (Q tiles at 0)
+  static constexpr int V_OFF = K_OFF + KS * TILE;
+  static constexpr int BAR_OFF = V_OFF + VS * TILE;
+  static constexpr int SMEM = (BAR_OFF + 256 + 1024 > 120 * 1024 ? BAR_OFF + 256 + 1024 : 120 * 1024);  // one CTA per SM
+  static constexpr uint64_t LAYOUT = D == 32 ? 4ull : 2ull;  // 64- or 128-byte swizzle
+  static constexpr uint64_t SBO = (8 * ROWB) >> 4;
+  static constexpr uint64_t LBO = PANELS == 2 ? (PANEL >> 4) : 1ull;  // MN-major V: from panel to panel
+  static constexpr uint32_t O_COL = 256;             // TMEM: S of the streams at 0 and 128, then O
+};
+
+template <int D>
+__device__ __forceinline__ uint64_t tile_desc(const void* smem) {
+  using C = TCfg<D>;
+  return ((uint64_t(smem_u32(smem)) >> 4) & 0x3FFFull) | (C::LBO << 16) | (C::SBO << 32) | (1ull << 46) | (C::LAYOUT << 61);
+}
+
+// Values that tcgen05.ld wrote may be used from here on (the compiler keeps uses behind this).
+template <int N>
+__device__ __forceinline__ void settle(uint32_t (&r)[N]) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) asm volatile("" : "+r"(r[i]));
+}
+
+template <int D>
+__global__ void __launch_bounds__(TTHREADS, 1)
+    cross_tile_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant__ CUtensorMap tmk,
+                      const __grid_constant__ CUtensorMap tmv, const CrossParams p) {
+  using C = TCfg<D>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* sQ = smem;
+  uint8_t* sK = smem + C::K_OFF;
+  uint8_t* sV = smem + C::V_OFF;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::BAR_OFF);
+  uint64_t* q_full = bars;
+  uint64_t* s_full = bars + 1;         // [stream]
+  uint64_t* p_full = bars + 3;         // [stream]
+  uint64_t* o_full = bars + 5;         // [stream]
+  uint64_t* drain = bars + 7;
+  uint64_t* k_full = bars + 8;         // [KS]
+  uint64_t* k_empty = k_full + C::KS;
+  uint64_t* v_full = k_empty + C::KS;  // [VS]
+  uint64_t* v_empty = v_full + C::VS;
+  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(v_empty + C::VS);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_holder + 1);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int hk = blockIdx.y % p.kv_heads, split = blockIdx.y / p.kv_heads, s = blockIdx.z;
+  const int G = p.G, qpt = TROWS / G;  // queries of a row tile
+  int64_t q0, k0;
+  int nq, nk;
+  seq_range(p.q_starts, s, p.q_rows, p.max_q, q0, nq);
+  seq_range(p.k_starts, s, p.kv_rows, p.max_k, k0, nk);
+  const int qb = blockIdx.x * 2 * qpt;  // first query of the CTA
+  if (qb >= nq) return;
+  const bool pair = nq - qb > qpt;  // two row tiles (else the streams share one tile's states)
+  // key tiles of this split
+  const int all = (nk + TKEYS - 1) / TKEYS, per = (all + p.nsplit - 1) / p.nsplit;
+  const int t0 = min(split * per, all), nkt = min(t0 + per, all) - t0;
+  const int n_of[2] = {pair ? nkt : (nkt + 1) / 2, pair ? nkt : nkt / 2};
+
+  if (threadIdx.x == 0) {
+    mbar_init(q_full, 1);
+    for (int g = 0; g < 2; ++g) {
+      mbar_init(&s_full[g], 1);
+      mbar_init(&p_full[g], 128);
+      mbar_init(&o_full[g], 1);
+    }
+    mbar_init(drain, 1);
+    for (int i = 0; i < C::KS; ++i) {
+      mbar_init(&k_full[i], 1);
+      mbar_init(&k_empty[i], 1);
+    }
+    for (int i = 0; i < C::VS; ++i) {
+      mbar_init(&v_full[i], 1);
+      mbar_init(&v_empty[i], 1);
+    }
+    *abort_flag = 0;
+    fence_barrier_init();
+    prefetch_tmap(&tmq);
+    prefetch_tmap(&tmk);
+    prefetch_tmap(&tmv);
+  }
+  if (warp == 1) tmem_alloc(tmem_holder, 512);
+  fence_before_sync();
+  __syncthreads();
+  fence_after_sync();
+  const uint32_t tmem = *tmem_holder;
+
+  if (warp == 0) {
+    if (lane == 0 && nkt > 0) {
+      bool ok = true;
+      const int tiles = pair ? 2 : 1;
+      mbar_arrive_expect_tx(q_full, tiles * C::PANELS * qpt * G * C::ROWB);
+      for (int g = 0; g < tiles; ++g)
+        for (int c = 0; c < C::PANELS; ++c)
+          tma_load_3d(sQ + g * C::TILE + c * C::PANEL, &tmq, q_full, c * C::PCOLS, hk * G, int(q0) + qb + g * qpt);
+      uint32_t pend_k = 0, pend_v = 0;  // last issued parity per ring slot (bit 1: issued)
+      auto load = [&](int j, bool is_v) -> bool {
+        const int stages = is_v ? C::VS : C::KS, st = j % stages;
+        const uint32_t u = uint32_t(j / stages) & 1;
+        uint64_t* full = is_v ? &v_full[st] : &k_full[st];
+        if (*abort_flag || !mbar_wait(is_v ? &v_empty[st] : &k_empty[st], u ^ 1, is_v ? 102 : 101)) return false;
+        mbar_arrive_expect_tx(full, C::TILE);
+        uint8_t* dst = (is_v ? sV : sK) + st * C::TILE;
+        for (int c = 0; c < C::PANELS; ++c)
+          tma_load_2d(dst + c * C::PANEL, is_v ? &tmv : &tmk, full, hk * D + c * C::PCOLS, int(k0) + (t0 + j) * TKEYS);
+        uint32_t& pend = is_v ? pend_v : pend_k;
+        pend = (pend & ~(3u << (2 * st))) | ((2u | u) << (2 * st));
+        return true;
+      };
+      ok = load(0, false);
+      for (int j = 0; j < nkt && ok; ++j) {
+        if (j + 1 < nkt) ok = load(j + 1, false);
+        if (ok) ok = load(j, true);
+      }
+      if (!ok) {
+        // every copy this thread issued lands before the CTA ends
+        *abort_flag = 1;
+        mbar_wait(q_full, 0, 103);
+        for (int i = 0; i < C::KS; ++i)
+          if ((pend_k >> (2 * i)) & 2u) mbar_wait(&k_full[i], (pend_k >> (2 * i)) & 1u, 104);
+        for (int i = 0; i < C::VS; ++i)
+          if ((pend_v >> (2 * i)) & 2u) mbar_wait(&v_full[i], (pend_v >> (2 * i)) & 1u, 105);
+      }
+    }
+  } else if (warp == 1) {
+    if (lane == 0 && nkt > 0) {
+      const uint32_t idesc_s = idesc_f16(128, TKEYS);
+      const uint32_t idesc_o = idesc_f16(128, D) | (1u << 16);  // V MN-major
+      auto tile_of = [&](int g, int it) { return pair ? it : 2 * it + g; };
+      auto issue_s = [&](int g, int it) -> bool {
+        const int j = tile_of(g, it), st = j % C::KS;
+        if (*abort_flag || !mbar_wait(&k_full[st], uint32_t(j / C::KS) & 1, 106)) return false;
+        fence_after_sync();
+        const uint64_t dq = tile_desc<D>(sQ + (pair ? g : 0) * C::TILE), dk = tile_desc<D>(sK + st * C::TILE);
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k) {
+          const uint64_t off = uint64_t((k / (C::PCOLS / 16)) * (C::PANEL >> 4) + (k % (C::PCOLS / 16)) * 2);
+          mma_f16(tmem + uint32_t(g * 128), dq + off, dk + off, idesc_s, k ? 1u : 0u);
+        }
+        mma_commit(&s_full[g]);
+        if (!pair || g == 1) mma_commit(&k_empty[st]);
+        return true;
+      };
+      bool ok = mbar_wait(q_full, 0, 107);
+      for (int g = 0; g < 2 && ok; ++g)
+        if (n_of[g] > 0) ok = issue_s(g, 0);
+      for (int it = 0; it < n_of[0] && ok; ++it)
+        for (int g = 0; g < 2 && ok; ++g) {
+          if (it >= n_of[g]) continue;
+          const int j = tile_of(g, it), st = j % C::VS;
+          if (*abort_flag || !mbar_wait(&p_full[g], uint32_t(it) & 1, 108) ||
+              !mbar_wait(&v_full[st], uint32_t(j / C::VS) & 1, 109)) {
+            ok = false;
+            break;
+          }
+          fence_after_sync();
+          const uint64_t dv = tile_desc<D>(sV + st * C::TILE);
+          const uint32_t pa = tmem + uint32_t(g * 128), oa = tmem + C::O_COL + uint32_t(g * D);
+#pragma unroll
+          for (int k = 0; k < TKEYS / 16; ++k)
+            mma_f16_ts(oa, pa + uint32_t(8 * k), dv + uint64_t(k * ((16 * C::ROWB) >> 4)), idesc_o, (it || k) ? 1u : 0u);
+          if (!pair || g == 1) mma_commit(&v_empty[st]);
+          if (it + 1 < n_of[g]) ok = issue_s(g, it + 1);
+          else mma_commit(&o_full[g]);
+        }
+      if (!ok) {
+        *abort_flag = 1;
+        mma_commit(drain);
+        mbar_wait(drain, 0, 110);
+      }
+    }
+  } else {
+    const int g = (warp - 2) >> 2;
+    const int quarter = warp & 3;
+    const int r = quarter * 32 + lane;               // row of the tile = TMEM lane
+    const int key = ((warp - 2) & 3) * 32 + lane;    // 0 .. 127: the V row this thread clears
+    const uint32_t trow = tmem + (uint32_t(quarter * 32) << 16);
+    const uint32_t s_addr = trow + uint32_t(g * 128), o_addr = trow + C::O_COL + uint32_t(g * D);
+    const float* mb = p.mask ? p.mask + k0 : nullptr;
+    bool ok = true;
+    auto wwait = [&](uint64_t* bar, uint32_t parity, int code) -> bool {
+      const bool w = !*abort_flag && mbar_wait(bar, parity, code);
+      return __all_sync(0xffffffffu, w);
+    };
+    float m = -INFINITY, l = 0.f;
+    for (int it = 0; it < n_of[g]; ++it) {
+      const int j = pair ? it : 2 * it + g;
+      const int first = (t0 + j) * TKEYS;  // of the sequence's states
+      // the tile's kept states, as bits (the same for every row)
+      uint32_t km[4];
+      const int left = nk - first;
+      bool whole = left >= TKEYS;
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        const int n = left - 32 * c;
+        km[c] = n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1u;
+      }
+      if (mb) {
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          const int jj = first + 32 * c + lane;
+          km[c] = __ballot_sync(0xffffffffu, jj < nk && __ldg(mb + jj) > 0.5f);
+        }
+        whole = (km[0] & km[1] & km[2] & km[3]) == 0xffffffffu;
+      }
+      if (!wwait(&s_full[g], uint32_t(it) & 1, 111)) { ok = false; break; }
+      fence_after_sync();
+      uint32_t sr[4][32];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) tmem_ld32(s_addr + 32 * c, sr[c]);
+      tmem_ld_wait();
+#pragma unroll
+      for (int c = 0; c < 4; ++c) settle(sr[c]);
+      if (!whole) {
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+#pragma unroll
+          for (int i = 0; i < 32; ++i) sr[c][i] = (km[c] >> i) & 1u ? sr[c][i] : 0xFF800000u;
+      }
+      float mr[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+      for (int c = 0; c < 4; ++c)
+#pragma unroll
+        for (int i = 0; i < 32; i += 2)
+          mr[(i >> 1) & 3] = fmax3(mr[(i >> 1) & 3], __uint_as_float(sr[c][i]), __uint_as_float(sr[c][i + 1]));
+      const float cand = fmaxf(fmaxf(mr[0], mr[1]), fmaxf(mr[2], mr[3])) * p.scale_log2;
+      float corr = 1.f;
+      if (cand > m + 8.f) {  // (also the first kept state: m = -inf)
+        corr = ex2_approx(m - cand);
+        m = cand;
+        l *= corr;
+      }
+      if (it > 0 && __any_sync(0xffffffffu, corr != 1.f)) {
+        // the products before this S are done: O may be rescaled
+#pragma unroll 1
+        for (int c = 0; c < D; c += 32) {
+          uint32_t o[32];
+          tmem_ld32(o_addr + c, o);
+          tmem_ld_wait();
+          settle(o);
+#pragma unroll
+          for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * corr);
+          tmem_st32(o_addr + c, o);
+        }
+        tmem_st_wait();
+      }
+      const float ref = m == -INFINITY ? 0.f : m;
+      float2 ls[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+#pragma unroll
+      for (int c2 = 0; c2 < 2; ++c2) {
+        uint32_t pk[32];
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+          const float2 x = ffma2(make_float2(__uint_as_float(sr[2 * c2 + i / 16][(2 * i) & 31]),
+                                             __uint_as_float(sr[2 * c2 + i / 16][(2 * i + 1) & 31])),
+                                 make_float2(p.scale_log2, p.scale_log2), make_float2(-ref, -ref));
+          const float2 e = make_float2(ex2_approx(x.x), ex2_approx(x.y));
+          ls[i & 1] = fadd2(ls[i & 1], e);
+          const __half2 h = __floats2half2_rn(e.x, e.y);
+          pk[i] = *reinterpret_cast<const uint32_t*>(&h);
+        }
+        tmem_st32(s_addr + 32 * c2, pk);
+      }
+      l += (ls[0].x + ls[0].y) + (ls[1].x + ls[1].y);
+      if (!whole) {
+        const int st = j % C::VS;
+        if (!wwait(&v_full[st], uint32_t(j / C::VS) & 1, 112)) { ok = false; break; }
+        // (in a pair both streams clear the same rows: zeros over zeros)
+        if (!((km[(warp - 2) & 3] >> lane) & 1u)) {
+#pragma unroll
+          for (int c = 0; c < C::PANELS; ++c) {
+            uint4* row = reinterpret_cast<uint4*>(sV + st * C::TILE + c * C::PANEL + key * C::ROWB);
+#pragma unroll
+            for (int e = 0; e < C::ROWB / 16; ++e) row[e] = make_uint4(0, 0, 0, 0);
+          }
+        }
+        fence_proxy_async_smem();
+      }
+      tmem_st_wait();
+      fence_before_sync();
+      mbar_arrive(&p_full[g]);
+    }
+    if (ok && n_of[g] > 0) {
+      ok = wwait(&o_full[g], 0, 113);
+      fence_after_sync();
+    }
+    // this row's share of the output: in a pair the stream's own O; else the two streams' parts, of
+    // which stream g's thread writes the columns [g D / 2, (g + 1) D / 2)
+    const int qi = qb + (pair ? g * qpt : 0) + r / G, h = hk * G + r % G;
+    const bool mine = r < qpt * G && qi < nq;
+    float m_out = m, l_out = l, f0 = 1.f, f1 = 0.f;
+    if (!pair) {
+      float* xm = reinterpret_cast<float*>(sQ + C::TILE);  // the second Q tile is not used
+      float* xl = xm + 256;
+      xm[g * 128 + r] = m;
+      xl[g * 128 + r] = l;
+      fence_before_sync();
+      if (named_bar_any(1 + quarter, 64, !ok)) ok = false;
+      fence_after_sync();
+      const float m0 = xm[r], m1 = xm[128 + r];
+      m_out = fmaxf(m0, m1);
+      f0 = m0 == -INFINITY ? 0.f : ex2_approx(m0 - m_out);
+      f1 = m1 == -INFINITY ? 0.f : ex2_approx(m1 - m_out);
+      l_out = f0 * xl[r] + f1 * xl[128 + r];
+    } else if (m == -INFINITY) {
+      f0 = 0.f;
+    }
+    if (ok) {
+      const bool direct = p.nsplit == 1;
+      const int64_t at = mine && !direct ? part_index(p, split, s, qi, h) : 0;
+      const float inv = direct ? (l_out == 0.f ? 0.f : 1.f / l_out) : 1.f;
+      constexpr int STEP = D / 2 < 32 ? 16 : 32;
+      const int c_begin = pair ? 0 : g * (D / 2), c_end = pair ? D : c_begin + D / 2;
+      const uint32_t o0 = trow + C::O_COL + (pair ? uint32_t(g * D) : 0u);
+#pragma unroll 1
+      for (int c = c_begin; c < c_end; c += STEP) {
+        uint32_t a[STEP], b[STEP];
+        // TMEM of a stream without items was never written: its factor is 0 and it is not read
+        if (n_of[pair ? g : 0] > 0) {
+          if constexpr (STEP == 32) tmem_ld32(o0 + c, a);
+          else tmem_ld16(o0 + c, a);
+        }
+        if (!pair && n_of[1] > 0) {
+          if constexpr (STEP == 32) tmem_ld32(o0 + D + c, b);
+          else tmem_ld16(o0 + D + c, b);
+        }
+        tmem_ld_wait();
+        settle(a);
+        settle(b);
+        float v[STEP];
+#pragma unroll
+        for (int i = 0; i < STEP; ++i)
+          v[i] = ((f0 != 0.f ? __uint_as_float(a[i]) * f0 : 0.f) + (f1 != 0.f ? __uint_as_float(b[i]) * f1 : 0.f)) * inv;
+        if (!mine) continue;
+        if (direct) {
+          uint4* dst = reinterpret_cast<uint4*>(p.out + (q0 + qi) * p.out_stride + h * D + c);
+#pragma unroll
+          for (int i = 0; i < STEP / 8; ++i)
+            dst[i] = make_uint4(pack_half2(v[8 * i], v[8 * i + 1]), pack_half2(v[8 * i + 2], v[8 * i + 3]),
+                                pack_half2(v[8 * i + 4], v[8 * i + 5]), pack_half2(v[8 * i + 6], v[8 * i + 7]));
+        } else {
+          float4* dst = reinterpret_cast<float4*>(p.part_o + at * D + c);
+#pragma unroll
+          for (int i = 0; i < STEP / 4; ++i) dst[i] = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+        }
+      }
+      if (mine && !direct && (pair || g == 0)) p.part_ml[at] = make_float2(m_out, l_out);
+    } else {
+      *abort_flag = 1;
+    }
+  }
+  fence_before_sync();
+  __syncthreads();
+  if (warp == 1) {
+    fence_after_sync();
+    tmem_free(tmem, 512);
+  }
+}
+
+// ---- host side ----
 
 void check_sizes(const char* fn, const kh_cross_attention_args* args) {
   check_that(args != nullptr, fn, "null arguments");
@@ -89,17 +713,73 @@ void check_sizes(const char* fn, const kh_cross_attention_args* args) {
              "q_rows and kv_rows must be in [0, 2^31)");
 }
 
+// One m16 block of rows to a key head: the kernel that streams k and v through registers.
+bool takes_rows_kernel(const kh_cross_attention_args& a) {
+  return int64_t(a.max_q) * (a.q_heads / a.kv_heads) <= 16;
+}
+
+constexpr int SMS = 148;  // of a B200: the split must not depend on the device the size is asked on
+
+// CTAs that a sequence's states are split over: as many as fill the SMs (four CTAs each of the rows
+// kernel, one of the tile kernel), each with enough states to pay for the join.
+int splits(const kh_cross_attention_args& a) {
+  const int64_t G = a.q_heads / a.kv_heads;
+  const bool few = takes_rows_kernel(a);
+  const int64_t blocks = few ? 1 : (int64_t(a.max_q) + 2 * (TROWS / G) - 1) / (2 * (TROWS / G));
+  const int64_t ctas = std::max<int64_t>(1, blocks * a.kv_heads * a.n_seqs);
+  const int64_t want = (few ? 4 * SMS : SMS) / ctas;
+  const int64_t most = few ? a.max_k / (4 * RW * RSTEP) : a.max_k / (4 * TKEYS);
+  return int(std::min<int64_t>(std::max<int64_t>(1, std::min(want, most)), 64));
+}
+
+int64_t round256(int64_t n) { return (n + 255) / 256 * 256; }
+
+template <int D>
+void launch(const CrossParams& p, const kh_cross_attention_args& a, bool states, cudaStream_t st) {
+  if (takes_rows_kernel(a)) {
+    cross_rows_kernel<D><<<dim3(p.nsplit, p.kv_heads, p.n_seqs), RW * 32, 0, st>>>(p);
+  } else {
+    using C = TCfg<D>;
+    static std::atomic<uint64_t> configured{0};
+    once_per_device(configured, [] {
+      KH_CUDA(cudaFuncSetAttribute(cross_tile_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
+    });
+    const int qpt = TROWS / p.G;
+    CUtensorMap tq, tk, tv;
+    encode_tensor_map_f16_3d(&tq, a.q, {uint64_t(D), uint64_t(a.q_heads), uint64_t(a.q_rows)}, D, uint64_t(a.q_stride),
+                             {uint32_t(C::PCOLS), uint32_t(p.G), uint32_t(qpt)}, C::ROWB);
+    tk = tv = tq;  // (without states neither is read)
+    if (states) {
+      const uint64_t cols = uint64_t(a.kv_heads) * D;
+      encode_tensor_map_f16(&tk, a.k, uint64_t(a.kv_rows), cols, uint64_t(a.k_stride), C::PCOLS, TKEYS, C::ROWB);
+      encode_tensor_map_f16(&tv, a.v, uint64_t(a.kv_rows), cols, uint64_t(a.v_stride), C::PCOLS, TKEYS, C::ROWB);
+    }
+    const dim3 grid(unsigned((a.max_q + 2 * qpt - 1) / (2 * qpt)), unsigned(a.kv_heads * p.nsplit), unsigned(a.n_seqs));
+    cross_tile_kernel<D><<<grid, TTHREADS, C::SMEM, st>>>(tq, tk, tv, p);
+  }
+  KH_CUDA(cudaGetLastError());
+  if (p.nsplit > 1) {
+    const int64_t rows = int64_t(p.n_seqs) * p.max_q * p.q_heads;
+    cross_join_kernel<D><<<unsigned((rows + 3) / 4), 128, 0, st>>>(p);
+    KH_CUDA(cudaGetLastError());
+  }
+}
+
 }  // namespace
 
 int64_t cross_attention_workspace(const kh_cross_attention_args* args) {
   check_sizes("kh_cross_attention_f16_workspace", args);
-  return 0;
+  const int n = splits(*args);
+  if (n == 1) return 0;
+  const int64_t parts = int64_t(n) * args->n_seqs * args->max_q * args->q_heads;
+  return round256(parts * args->head_dim * 4) + parts * 8;
 }
 
 void cross_attention(const kh_cross_attention_args* args, cudaStream_t st) {
   const char* fn = "kh_cross_attention_f16";
   check_sizes(fn, args);
   const kh_cross_attention_args& a = *args;
+  check_that(a.scale > 0.f && a.scale <= 1e30f, fn, "scale must be above 0 and finite");
   if (a.n_seqs == 0 || a.max_q == 0 || a.q_rows == 0) return;
   const bool states = a.kv_rows > 0 && a.max_k > 0;
   auto aligned = [](const void* x) { return (reinterpret_cast<uintptr_t>(x) & 15) == 0; };
@@ -144,14 +824,19 @@ void cross_attention(const kh_cross_attention_args* args, cudaStream_t st) {
   p.n_seqs = a.n_seqs;
   p.q_heads = a.q_heads;
   p.kv_heads = a.kv_heads;
+  p.G = a.q_heads / a.kv_heads;
   p.max_q = a.max_q;
   p.max_k = a.max_k;
-  p.scale = a.scale;
-  const dim3 grid((a.max_q + 3) / 4, a.q_heads, a.n_seqs);
-  if (a.head_dim == 32) cross_simple_kernel<32><<<grid, 128, 0, st>>>(p);
-  else if (a.head_dim == 64) cross_simple_kernel<64><<<grid, 128, 0, st>>>(p);
-  else cross_simple_kernel<128><<<grid, 128, 0, st>>>(p);
-  KH_CUDA(cudaGetLastError());
+  p.nsplit = splits(a);
+  p.scale_log2 = a.scale * 1.4426950408889634f;
+  if (p.nsplit > 1) {
+    const int64_t parts = int64_t(p.nsplit) * a.n_seqs * a.max_q * a.q_heads;
+    p.part_o = static_cast<float*>(a.workspace);
+    p.part_ml = reinterpret_cast<float2*>(static_cast<char*>(a.workspace) + round256(parts * a.head_dim * 4));
+  }
+  if (a.head_dim == 32) launch<32>(p, a, states, st);
+  else if (a.head_dim == 64) launch<64>(p, a, states, st);
+  else launch<128>(p, a, states, st);
 }
 
 int cross_attention_error_code() {

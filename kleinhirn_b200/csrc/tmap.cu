@@ -60,6 +60,21 @@ void encode_tensor_map_f16(CUtensorMap* out, const void* ptr, uint64_t rows, uin
   encode_2d(out, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, ptr, rows, cols, row_stride, box_cols, box_rows, swizzle_bytes);
 }
 
+void encode_tensor_map_f16_3d(CUtensorMap* out, const void* ptr, const uint64_t (&dims)[3], uint64_t stride1,
+                              uint64_t stride2, const uint32_t (&box)[3], int swizzle_bytes) {
+  if ((reinterpret_cast<uintptr_t>(ptr) & 15) || stride1 % 8 || stride2 % 8)
+    throw PlanError("tensor map: base or stride not 16-byte aligned");
+  const cuuint64_t d[3] = {dims[0], dims[1], dims[2]};
+  const cuuint64_t strides[2] = {stride1 * 2, stride2 * 2};
+  const cuuint32_t b[3] = {box[0], box[1], box[2]};
+  const cuuint32_t estr[3] = {1, 1, 1};
+  const CUtensorMapSwizzle sw = swizzle_bytes == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B;
+  const CUresult r = encode_fn()(out, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<void*>(ptr), d, strides, b, estr,
+                                 CU_TENSOR_MAP_INTERLEAVE_NONE, sw, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                                 CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) throw CudaError("cuTensorMapEncodeTiled failed: " + std::to_string(int(r)));
+}
+
 CUtensorMap tensor_map_f32(const void* ptr, uint64_t rows, uint64_t cols, uint64_t row_stride, uint32_t box_cols,
                            uint32_t box_rows) {
   // (f32 operands of the 3xTF32 GEMM: 128-byte swizzle; cached and copied out like the f16 maps)

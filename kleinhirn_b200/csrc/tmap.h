@@ -24,6 +24,11 @@ CUtensorMap tensor_map_f32(const void* ptr, uint64_t rows, uint64_t cols, uint64
 void encode_tensor_map_f16(CUtensorMap* out, const void* ptr, uint64_t rows, uint64_t cols, uint64_t row_stride,
                            uint32_t box_cols, uint32_t box_rows, int swizzle_bytes);
 
+// Map of f16 values in three dimensions, the innermost contiguous: dims[i] extents, strides of the
+// outer two in elements, box[i] elements of a tile (dense in shared memory in the same order). Not cached.
+void encode_tensor_map_f16_3d(CUtensorMap* out, const void* ptr, const uint64_t (&dims)[3], uint64_t stride1,
+                              uint64_t stride2, const uint32_t (&box)[3], int swizzle_bytes);
+
 // Self-test of the cache under concurrent use: `threads` host threads fetch `iters` maps each over
 // more keys than the cache keeps; returns how many fetched maps differ from a fresh encoding.
 int64_t selftest_tensor_maps(int threads, int iters);

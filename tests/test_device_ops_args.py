@@ -62,6 +62,8 @@ def test_norm_refusals(kw, text):
     ({"out": None}, "null"), ({"q_starts": None}, "null"), ({"k_starts": None}, "null"), ({"q": P + 8}, "aligned"),
     ({"v": P + 2}, "aligned"), ({"q_stride": 248}, "stride"), ({"k_stride": 120}, "stride"), ({"v_stride": 132}, "stride"),
     ({"out_stride": 252}, "stride"), ({"workspace": P + 64}, "workspace"),
+    ({"scale": 0.0}, "scale"), ({"scale": -0.125}, "scale"), ({"scale": float("inf")}, "scale"),
+    ({"scale": float("nan")}, "scale"), ({"q_heads": 1, "kv_heads": 1, "max_k": 9001, "workspace_bytes": 100}, "workspace"),
 ])
 def test_cross_refusals(kw, text):
     refused(kb.cross_attention_f16, cross(**kw), text)
