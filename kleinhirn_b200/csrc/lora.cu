@@ -1,15 +1,23 @@
 // A projection with the low-rank adapters of many requests.
 //
 // out[t] = x[t] W^T + bias + s_a (x[t] A_a^T) B_a^T, a the adapter of the segment of rows that t lies
-// in. Two steps: h[t] = s_a x[t] A_a^T (rank values a row, rounded to f16: its rounding is 2^-11 of the
-// adapter's own part, as far below the output's as that part is below the projection), then the
-// projection and h B_a^T into the same f32 sum, rounded once.
+// in. Two launches: h[t] = s_a x[t] A_a^T (rank values a row, rounded to f16: 2^-11 of the adapter's
+// own part), then the projection with h B_a^T added to the same f32 accumulators, rounded once. The
+// second launch starts while the first runs (programmatic dependent launch) and waits for it where it
+// needs h, behind the projection's own products.
+//
+// Few rows (takes_rows): bound by reading W, A and B once; lora_shrink_rows_kernel and
+// lora_rows_kernel stream them through registers. Many rows: bound by the tensor cores;
+// lora_shrink_tile_kernel (HBM: reads x once) and lora_pair_kernel. A row tile that holds rows of
+// several adapters takes one more product per adapter, whose output lanes of other rows are switched
+// off in the instruction, so no operand is masked or copied.
 
 #include "device_ops.h"
 
 #include <cuda_fp16.h>
 
 #include <algorithm>
+#include <atomic>
 
 #include "runtime.h"
 #include "sm100.cuh"
@@ -31,17 +39,17 @@ struct LoraParams {
   const int32_t* starts;
   const int32_t* ids;
   __half* out;
-  __half* h;
+  __half* h;  // [rows][rank]
   int64_t rows, x_stride, out_stride;
   int k, n, rank, n_adapters, n_segs;
 };
 
 // Start of segment i, cut to the buffer.
-__device__ __forceinline__ int64_t seg_start(const LoraParams& p, int i) {
-  return min(max(int64_t(p.starts[i]), int64_t(0)), p.rows);
+__device__ __forceinline__ int seg_start(const LoraParams& p, int i) {
+  return int(min(max(int64_t(__ldg(p.starts + i)), int64_t(0)), p.rows));
 }
 // Segment of row t (the last one that starts at or before it), or -1 before the first and behind the last.
-__device__ __forceinline__ int seg_of(const LoraParams& p, int64_t t) {
+__device__ __forceinline__ int seg_of(const LoraParams& p, int t) {
   if (t < seg_start(p, 0) || t >= seg_start(p, p.n_segs)) return -1;
   int lo = 0, hi = p.n_segs - 1;
   while (lo < hi) {
@@ -53,63 +61,747 @@ __device__ __forceinline__ int seg_of(const LoraParams& p, int64_t t) {
 }
 // Adapter of a segment, -1 for none; an id that does not exist counts as none and is reported.
 __device__ __forceinline__ int adapter_of(const LoraParams& p, int seg) {
-  const int a = p.ids[seg];
+  const int a = __ldg(p.ids + seg);
   if (a < p.n_adapters) return a < 0 ? -1 : a;
   atomicCAS(&kh_tc_error, 0, OP_BAD_INDEX);
   return -1;
 }
-
-// One warp per (row, rank index).
-__global__ void __launch_bounds__(256) lora_shrink_simple_kernel(const LoraParams p) {
-  const int64_t t = blockIdx.x;
+// First segment that ends behind row r (n_segs if none), found by a whole warp, 32 probes a round.
+__device__ __forceinline__ int first_seg(const LoraParams& p, int r) {
   const int lane = threadIdx.x & 31;
+  int lo = 0, hi = p.n_segs;
+  while (lo < hi) {
+    const int step = (hi - lo + 31) / 32, i = lo + lane * step;
+    const uint32_t ended = __ballot_sync(0xffffffffu, i < hi && seg_start(p, i + 1) <= r);
+    const int c = ended == 0xffffffffu ? 32 : __ffs(~ended) - 1;  // probes before the first that has not
+    if (c == 0) return lo;
+    hi = min(hi, lo + c * step);
+    lo += (c - 1) * step + 1;
+  }
+  return lo;
+}
+
+__device__ __forceinline__ uint32_t pack_half2(float a, float b) {
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ float dot8(uint4 a, uint4 b, float acc) {
+  const __half2* x = reinterpret_cast<const __half2*>(&a);
+  const __half2* y = reinterpret_cast<const __half2*>(&b);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 u = __half22float2(x[i]), v = __half22float2(y[i]);
+    acc = fmaf(u.x, v.x, fmaf(u.y, v.y, acc));
+  }
+  return acc;
+}
+
+// ---- few rows: h, one CTA of 8 warps per row, a warp two of the rank's dot products at a time ----
+
+__global__ void __launch_bounds__(256) lora_shrink_rows_kernel(const LoraParams p) {
+  launch_dependents();
+  const int t = blockIdx.x, lane = threadIdx.x & 31;
   const int seg = seg_of(p, t);
   if (seg < 0) return;
-  const int a = adapter_of(p, seg);
-  if (a < 0) return;
-  for (int r = threadIdx.x >> 5; r < p.rank; r += 8) {
-    float d = 0.f;
-    for (int i = lane; i < p.k; i += 32)
-      d += __half2float(p.x[t * p.x_stride + i]) * __half2float(p.a[(int64_t(a) * p.rank + r) * p.k + i]);
-    for (int o = 16; o; o >>= 1) d += __shfl_xor_sync(0xffffffffu, d, o);
-    if (lane == 0) p.h[t * p.rank + r] = __float2half_rn(d * (p.scales ? p.scales[a] : 1.f));
+  const int ad = adapter_of(p, seg);
+  if (ad < 0) return;
+  const uint4* x = reinterpret_cast<const uint4*>(p.x + t * p.x_stride);
+  const float s = p.scales ? __ldg(p.scales + ad) : 1.f;
+  const int chunks = p.k / 8;
+  for (int r = (threadIdx.x >> 5) * 2; r < p.rank; r += 16) {  // (the rank is even)
+    const uint4* a0 = reinterpret_cast<const uint4*>(p.a + (int64_t(ad) * p.rank + r) * p.k);
+    const uint4* a1 = a0 + chunks;
+    float d0 = 0.f, d1 = 0.f;
+#pragma unroll 4
+    for (int i = lane; i < chunks; i += 32) {
+      const uint4 v = __ldg(x + i);
+      d0 = dot8(v, __ldg(a0 + i), d0);
+      d1 = dot8(v, __ldg(a1 + i), d1);
+    }
+    for (int o = 16; o; o >>= 1) {
+      d0 += __shfl_xor_sync(0xffffffffu, d0, o);
+      d1 += __shfl_xor_sync(0xffffffffu, d1, o);
+    }
+    if (lane == 0) *reinterpret_cast<uint32_t*>(p.h + int64_t(t) * p.rank + r) = pack_half2(d0 * s, d1 * s);
   }
 }
 
-// 64 x 64 outputs of a CTA, 4 x 4 of a thread.
-__global__ void __launch_bounds__(256) lora_simple_kernel(const LoraParams p) {
-  __shared__ float xs[64][17], ws[64][17];
-  const int64_t t0 = int64_t(blockIdx.x) * 64;
-  const int n0 = blockIdx.y * 64, ty = threadIdx.x / 16, tx = threadIdx.x % 16;
-  float acc[4][4] = {};
-  for (int k0 = 0; k0 < p.k; k0 += 16) {
-    for (int i = threadIdx.x; i < 1024; i += 256) {
-      const int r = i / 16, c = i % 16;
-      xs[r][c] = t0 + r < p.rows && k0 + c < p.k ? __half2float(p.x[(t0 + r) * p.x_stride + k0 + c]) : 0.f;
-      ws[r][c] = n0 + r < p.n && k0 + c < p.k ? __half2float(p.w[int64_t(n0 + r) * p.k + k0 + c]) : 0.f;
+// ---- few rows: the projection ----
+//
+// out^T = W x^T in m16n8k16 products: a CTA owns 128 outputs of NB * 8 rows, 4 warps of 32 outputs by
+// 2 slices of the sum; a cluster of Z CTAs splits the sum further, so that W streams through all SMs,
+// and adds the parts over distributed shared memory in rank order. The order of the values within a
+// sum is free, so a thread loads 16 bytes of W and of x as they lie in memory (quad lane t the values
+// 8 t .. of 32). The adapter's part is a dot product of rank values per output at the end.
+
+constexpr int RN = 128;  // outputs of a CTA
+
+__device__ __forceinline__ void mma_16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                          uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ float ld_cluster_f32(uint32_t addr) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+  return v;
+}
+
+template <int NB>
+struct RowsFrag {
+  uint4 w[2][2];  // [block of 16 outputs][row lane / 4, + 8]
+  uint4 x[NB];
+};
+
+template <int NB>
+__device__ __forceinline__ void rows_load(RowsFrag<NB>& f, const LoraParams& p, int n_first, int t_first, int t_end, int k) {
+  const int lane = threadIdx.x & 31, kk = k + (lane & 3) * 8;
+#pragma unroll
+  for (int mb = 0; mb < 2; ++mb)
+#pragma unroll
+    for (int hl = 0; hl < 2; ++hl) {
+      const int n = n_first + mb * 16 + hl * 8 + (lane >> 2);
+      f.w[mb][hl] = make_uint4(0, 0, 0, 0);
+      if (n < p.n && kk < p.k) f.w[mb][hl] = __ldg(reinterpret_cast<const uint4*>(p.w + int64_t(n) * p.k + kk));
+    }
+#pragma unroll
+  for (int nb = 0; nb < NB; ++nb) {
+    const int t = t_first + nb * 8 + (lane >> 2);
+    f.x[nb] = make_uint4(0, 0, 0, 0);
+    if (t < t_end && kk < p.k) f.x[nb] = __ldg(reinterpret_cast<const uint4*>(p.x + t * p.x_stride + kk));
+  }
+}
+
+template <int NB>
+__global__ void __launch_bounds__(256) lora_rows_kernel(const LoraParams p, int Z) {
+  __shared__ float part[NB * 8][RN + 4];
+  __shared__ int ids[NB * 8];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int nw = warp & 3, kw = warp >> 2;
+  const int z = blockIdx.x % Z, n0 = blockIdx.x / Z * RN;
+  const int begin = seg_start(p, 0), end = seg_start(p, p.n_segs);
+  const int t0 = begin + blockIdx.y * NB * 8;
+  if (t0 >= end) {  // (the whole cluster)
+    wait_primary();
+    return;
+  }
+  const int nt = min(NB * 8, end - t0);
+  if (threadIdx.x < nt) ids[threadIdx.x] = adapter_of(p, seg_of(p, t0 + threadIdx.x));
+
+  float acc[2][NB][4];
+#pragma unroll
+  for (int mb = 0; mb < 2; ++mb)
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) acc[mb][nb][0] = acc[mb][nb][1] = acc[mb][nb][2] = acc[mb][nb][3] = 0.f;
+  const int stride = 2 * Z * 32;
+  RowsFrag<NB> cur, nxt;
+  int k = (z * 2 + kw) * 32;
+  if (k < p.k) rows_load<NB>(cur, p, n0 + nw * 32, t0, end, k);
+  for (; k < p.k; k += stride) {
+    if (k + stride < p.k) rows_load<NB>(nxt, p, n0 + nw * 32, t0, end, k + stride);
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+      for (int mb = 0; mb < 2; ++mb) {
+        const uint4 u = cur.w[mb][0], v = cur.w[mb][1], b = cur.x[nb];
+        mma_16816(acc[mb][nb], u.x, v.x, u.y, v.y, b.x, b.y);
+        mma_16816(acc[mb][nb], u.z, v.z, u.w, v.w, b.z, b.w);
+      }
+    cur = nxt;
+  }
+  // the two slices of this CTA, then the cluster's parts
+  for (int turn = 1; turn >= 0; --turn) {
+    if (kw == turn) {
+#pragma unroll
+      for (int mb = 0; mb < 2; ++mb)
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            float& c = part[nb * 8 + (lane & 3) * 2 + (i & 1)][nw * 32 + mb * 16 + (lane >> 2) + 8 * (i >> 1)];
+            c = turn ? acc[mb][nb][i] : acc[mb][nb][i] + c;
+          }
     }
     __syncthreads();
-    for (int c = 0; c < 16; ++c)
-      for (int i = 0; i < 4; ++i)
-        for (int j = 0; j < 4; ++j) acc[i][j] += xs[ty + 16 * i][c] * ws[tx + 16 * j][c];
-    __syncthreads();
   }
-  for (int i = 0; i < 4; ++i) {
-    const int64_t t = t0 + ty + 16 * i;
+  if (Z > 1) cluster_sync();
+  wait_primary();
+  const int per = RN / Z;
+  for (int e = threadIdx.x; e < nt * per; e += 256) {
+    const int i = e / per, c = z * per + e % per, n = n0 + c, t = t0 + i;
+    if (n >= p.n) continue;
+    float v = 0.f;
+    if (Z == 1) {
+      v = part[i][c];
+    } else {
+      for (int q = 0; q < Z; ++q) v += ld_cluster_f32(cluster_addr(&part[i][c], uint32_t(q)));
+    }
+    if (p.bias) v += __half2float(p.bias[n]);
+    const int ad = ids[i];
+    if (ad >= 0) {
+      const uint4* b = reinterpret_cast<const uint4*>(p.b + (int64_t(ad) * p.n + n) * p.rank);
+      const uint4* h = reinterpret_cast<const uint4*>(p.h + int64_t(t) * p.rank);
+      for (int r = 0; r < p.rank / 8; ++r) v = dot8(h[r], __ldg(b + r), v);
+    }
+    p.out[t * p.out_stride + n] = __float2half_rn(v);
+  }
+  if (Z > 1) cluster_sync();  // no CTA leaves while another reads its part
+}
+
+// ---- many rows: h on the tensor cores ----
+//
+// One cluster of Z CTAs per 128 rows, the CTAs splitting the sum (launches of few tiles). A K block of
+// 64: one tile of x, then for every adapter of the tile's rows its block of A (rank rows) and the
+// products, whose lanes of other rows are off, into one accumulator of 128 x rank. 192 threads:
+// warp 0 TMA, warp 1 MMA, warps 2-5 the scaled f16 rows.
+
+constexpr int SXS = 4;  // x stages
+struct ShrinkPieces {
+  int count;
+  int lo[128], hi[128], id[128];
+};
+
+__device__ __forceinline__ uint32_t lanes_on(int lo, int hi, int word) {
+  const int a = min(max(lo - 32 * word, 0), 32), b = min(max(hi - 32 * word, 0), 32);
+  const uint32_t ub = b >= 32 ? 0xffffffffu : (1u << b) - 1u, ua = a >= 32 ? 0xffffffffu : (1u << a) - 1u;
+  return ub & ~ua;
+}
+
+__global__ void __launch_bounds__(192) lora_shrink_tile_kernel(const __grid_constant__ CUtensorMap tmx,
+                                                               const __grid_constant__ CUtensorMap tma,
+                                                               const LoraParams p, int Z, int astages) {
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ ShrinkPieces pieces;
+  __shared__ uint64_t bars[2 * SXS + 16 + 2];
+  __shared__ uint32_t tmem_holder;
+  __shared__ volatile int abort_flag;
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  const int R16 = (p.rank + 15) / 16 * 16;
+  const int a_bytes = R16 * 128;
+  uint8_t* sX = smem;
+  uint8_t* sA = smem + SXS * 16384;
+  uint64_t *x_full = bars, *x_empty = bars + SXS, *a_full = bars + 2 * SXS, *a_empty = a_full + 8, *done = a_empty + 8,
+           *drain = done + 1;
+  launch_dependents();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int z = blockIdx.x % Z, r0 = int(blockIdx.x / Z) * 128;
+  const uint32_t cols = R16 <= 32 ? 32u : R16 <= 64 ? 64u : 128u;
+  if (warp == 0) {
+    // the adapters of these rows: non-empty runs of rows, in order
+    int n = 0;
+    for (int s = first_seg(p, r0); s < p.n_segs; s += 32) {
+      const int i = s + lane;
+      int lo = 0, hi = 0, id = -1;
+      bool more = i < p.n_segs;
+      if (more) {
+        lo = max(seg_start(p, i), r0) - r0;
+        hi = min(seg_start(p, i + 1), r0 + 128) - r0;
+        more = lo < 128;
+        if (lo < hi) id = adapter_of(p, i);
+      }
+      const uint32_t have = __ballot_sync(0xffffffffu, id >= 0);
+      const int at = n + __popc(have & ((1u << lane) - 1u));
+      if (id >= 0 && at < 128) {
+        pieces.lo[at] = lo;
+        pieces.hi[at] = hi;
+        pieces.id[at] = id;
+      }
+      n += __popc(have);
+      if (!__all_sync(0xffffffffu, more)) break;
+    }
+    if (lane == 0) {
+      pieces.count = min(n, 128);
+      for (int i = 0; i < SXS; ++i) {
+        mbar_init(&x_full[i], 1);
+        mbar_init(&x_empty[i], 1);
+      }
+      for (int i = 0; i < 8; ++i) {
+        mbar_init(&a_full[i], 1);
+        mbar_init(&a_empty[i], 1);
+      }
+      mbar_init(done, 1);
+      mbar_init(drain, 1);
+      abort_flag = 0;
+      fence_barrier_init();
+      prefetch_tmap(&tmx);
+      prefetch_tmap(&tma);
+    }
+  }
+  if (warp == 1) tmem_alloc(&tmem_holder, cols);
+  fence_before_sync();
+  __syncthreads();
+  fence_after_sync();
+  const uint32_t tmem = tmem_holder;
+  const int np = pieces.count;
+  const int nk_all = (p.k + 63) / 64, kps = (nk_all + Z - 1) / Z;
+  const int kb0 = min(z * kps, nk_all), nk = np ? min(kps, nk_all - kb0) : 0;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      bool ok = true;
+      uint32_t pend_x = 0, pend_a = 0;  // two bits a stage: issued, parity
+      int ai = 0;
+      for (int kb = 0; kb < nk && ok; ++kb) {
+        const int xs = kb % SXS;
+        const uint32_t u = uint32_t(kb / SXS) & 1;
+        if (abort_flag || !mbar_wait(&x_empty[xs], u ^ 1, 201)) { ok = false; break; }
+        mbar_arrive_expect_tx(&x_full[xs], 16384);
+        tma_load_2d(sX + xs * 16384, &tmx, &x_full[xs], (kb0 + kb) * 64, r0);
+        pend_x = (pend_x & ~(3u << (2 * xs))) | ((2u | u) << (2 * xs));
+        for (int i = 0; i < np; ++i, ++ai) {
+          const int as = ai % astages;
+          const uint32_t v = uint32_t(ai / astages) & 1;
+          if (abort_flag || !mbar_wait(&a_empty[as], v ^ 1, 202)) { ok = false; break; }
+          mbar_arrive_expect_tx(&a_full[as], a_bytes);
+          tma_load_2d(sA + as * a_bytes, &tma, &a_full[as], (kb0 + kb) * 64, pieces.id[i] * p.rank);
+          pend_a = (pend_a & ~(3u << (2 * as))) | ((2u | v) << (2 * as));
+        }
+      }
+      if (!ok) {
+        abort_flag = 1;
+        for (int i = 0; i < SXS; ++i)
+          if ((pend_x >> (2 * i)) & 2u) mbar_wait(&x_full[i], (pend_x >> (2 * i)) & 1u, 203);
+        for (int i = 0; i < astages; ++i)
+          if ((pend_a >> (2 * i)) & 2u) mbar_wait(&a_full[i], (pend_a >> (2 * i)) & 1u, 204);
+      }
+    }
+  } else if (warp == 1) {
+    if (lane == 0) {
+      const uint32_t idesc = idesc_f16(128, R16);
+      bool ok = true;
+      int ai = 0;
+      for (int kb = 0; kb < nk && ok; ++kb) {
+        const int xs = kb % SXS;
+        if (abort_flag || !mbar_wait(&x_full[xs], uint32_t(kb / SXS) & 1, 205)) { ok = false; break; }
+        const uint64_t dx = desc_sw128(sX + xs * 16384);
+        for (int i = 0; i < np; ++i, ++ai) {
+          const int as = ai % astages;
+          if (abort_flag || !mbar_wait(&a_full[as], uint32_t(ai / astages) & 1, 206)) { ok = false; break; }
+          fence_after_sync();
+          uint32_t off[4];
+#pragma unroll
+          for (int w = 0; w < 4; ++w) off[w] = ~lanes_on(pieces.lo[i], pieces.hi[i], w);
+          const uint64_t da = desc_sw128(sA + as * a_bytes);
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            mma_f16_lanes(tmem, dx + uint64_t(2 * k), da + uint64_t(2 * k), idesc, (kb | k) ? 1u : 0u, off);
+          mma_commit(&a_empty[as]);
+        }
+        if (ok) mma_commit(&x_empty[xs]);
+      }
+      if (!ok) {
+        abort_flag = 1;
+        mma_commit(drain);
+        mbar_wait(drain, 0, 207);
+      }
+      mma_commit(done);  // (after a failure too: nothing is stored then)
+    }
+  } else {
+    const int quarter = warp & 3, r = quarter * 32 + lane, t = r0 + r;
     const int seg = t < p.rows ? seg_of(p, t) : -1;
-    if (seg < 0) continue;
-    const int a = adapter_of(p, seg);
-    for (int j = 0; j < 4; ++j) {
-      const int n = n0 + tx + 16 * j;
-      if (n >= p.n) continue;
-      float v = acc[i][j];
-      if (a >= 0)
-        for (int r = 0; r < p.rank; ++r)
-          v += __half2float(p.h[t * p.rank + r]) * __half2float(p.b[(int64_t(a) * p.n + n) * p.rank + r]);
-      if (p.bias) v += __half2float(p.bias[n]);
-      p.out[t * p.out_stride + n] = __float2half_rn(v);
+    const int ad = seg >= 0 ? adapter_of(p, seg) : -1;
+    const float s = ad >= 0 && p.scales ? __ldg(p.scales + ad) : 1.f;
+    const bool ok = __all_sync(0xffffffffu, mbar_wait(done, 0, 208)) && !abort_flag;
+    fence_after_sync();
+    const uint32_t taddr = tmem + (uint32_t(quarter * 32) << 16);
+    float* part = reinterpret_cast<float*>(smem) + r * (R16 + 1);  // split sums, over the stages (all read)
+#pragma unroll 1
+    for (int c = 0; c < R16; c += 8) {
+      uint32_t v[8];
+      tmem_ld8(taddr + uint32_t(c), v);
+      tmem_ld_wait();
+#pragma unroll
+      for (int i = 0; i < 8; ++i) asm volatile("" : "+r"(v[i]));
+      if (Z > 1) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) part[c + i] = nk > 0 ? __uint_as_float(v[i]) : 0.f;
+      } else if (ok && ad >= 0 && c < p.rank) {
+        *reinterpret_cast<uint4*>(p.h + int64_t(t) * p.rank + c) =
+            make_uint4(pack_half2(__uint_as_float(v[0]) * s, __uint_as_float(v[1]) * s),
+                       pack_half2(__uint_as_float(v[2]) * s, __uint_as_float(v[3]) * s),
+                       pack_half2(__uint_as_float(v[4]) * s, __uint_as_float(v[5]) * s),
+                       pack_half2(__uint_as_float(v[6]) * s, __uint_as_float(v[7]) * s));
+      }
     }
   }
+  fence_before_sync();
+  __syncthreads();
+  if (Z > 1) {
+    cluster_sync();
+    // CTA z adds up rows [z per, (z + 1) per), a thread 8 of a row's values
+    const int per = 128 / Z;
+    const float* base = reinterpret_cast<const float*>(smem);
+    for (int e = threadIdx.x; e < per * (p.rank / 8); e += 192) {
+      const int r = z * per + e / (p.rank / 8), c = e % (p.rank / 8) * 8, t = r0 + r;
+      const int seg = t < p.rows ? seg_of(p, t) : -1;
+      const int ad = seg >= 0 ? adapter_of(p, seg) : -1;
+      if (ad < 0 || abort_flag) continue;
+      const float s = p.scales ? __ldg(p.scales + ad) : 1.f;
+      float v[8] = {};
+      for (int q = 0; q < Z; ++q)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] += ld_cluster_f32(cluster_addr(base + r * (R16 + 1) + c + i, uint32_t(q)));
+      *reinterpret_cast<uint4*>(p.h + int64_t(t) * p.rank + c) =
+          make_uint4(pack_half2(v[0] * s, v[1] * s), pack_half2(v[2] * s, v[3] * s), pack_half2(v[4] * s, v[5] * s),
+                     pack_half2(v[6] * s, v[7] * s));
+    }
+    cluster_sync();
+  }
+  if (warp == 1) {
+    fence_after_sync();
+    tmem_free(tmem, cols);
+  }
+}
+
+// ---- many rows: the projection on CTA pairs ----
+//
+// 256 x BN tiles of a cluster of two CTAs (tcgen05 cta_group::2: each stages its 128 rows of x and
+// BN / 2 rows of W per K block of 64), persistent over the tiles, two accumulators in TMEM so that the
+// epilogue runs under the next tile's products. Behind a tile's K blocks come, in the same ring of
+// stages, the adapters of its rows: the tile's rows of h against the adapter's rows of B, products of
+// ceil(rank / 16) steps whose lanes of other rows are off. The producer warp finds the runs of rows
+// while the K blocks load and hands each one's row range to the MMA thread beside its stage.
+//   warp 0 TMA; warp 1 MMA (first CTA); then a warpgroup per 64 columns: bias, f16, staged and stored by
+//   TMA (tiles with rows that are not to be written: straight from registers).
+
+constexpr int BM = 128;
+constexpr int BK = 64;
+constexpr int A_BYTES = BM * BK * 2;
+constexpr int OUT_BYTES = 128 * 64 * 2;
+
+template <int BN>
+struct PCfg {
+  static constexpr int BH = BN / 2;
+  static constexpr int B_BYTES = BH * BK * 2;
+  static constexpr int STAGE_BYTES = A_BYTES + B_BYTES;
+  static constexpr int NWG = BN / 64;
+  static constexpr int THREADS = 64 + 128 * NWG;
+  static constexpr int STAGES = BN == 256 ? 5 : 6;
+  static constexpr uint32_t TMEM_COLS = 2 * BN;
+  static constexpr int SMEM = STAGES * STAGE_BYTES + NWG * OUT_BYTES + 1024 + 512;
+};
+
+// What a stage holds for the MMA thread: the rows it counts for, its steps of 16, whether the tile ends.
+struct StageNote {
+  int lo, hi, steps, last;
+};
+
+template <int BN>
+__global__ void __launch_bounds__(PCfg<BN>::THREADS, 1)
+    lora_pair_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmW,
+                     const __grid_constant__ CUtensorMap tmH, const __grid_constant__ CUtensorMap tmB,
+                     const __grid_constant__ CUtensorMap tmO, const LoraParams p) {
+  using G = PCfg<BN>;
+  constexpr int STAGES = G::STAGES;
+  constexpr int NWG = G::NWG;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* sA = smem;
+  uint8_t* sB = smem + STAGES * A_BYTES;
+  uint8_t* sOut = sB + STAGES * G::B_BYTES;  // [warpgroup] 16 KB staging tiles
+  uint64_t* full = reinterpret_cast<uint64_t*>(sOut + NWG * OUT_BYTES);
+  uint64_t* empty = full + STAGES;
+  uint64_t* tfull = empty + STAGES;
+  uint64_t* tempty = tfull + 2;
+  uint64_t* drain = tempty + 2;
+  StageNote* notes = reinterpret_cast<StageNote*>(drain + 2);  // [STAGES], 16-byte aligned
+  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(notes + STAGES);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_holder + 1);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_rank();
+  const bool first = rank == 0;
+  const int pair = blockIdx.x >> 1, npairs = gridDim.x >> 1;
+  const int begin = seg_start(p, 0), end = seg_start(p, p.n_segs);  // rows to write
+  const int m_first = begin / (2 * BM), m_tiles = end > begin ? (end + 2 * BM - 1) / (2 * BM) - m_first : 0;
+  const int n_tiles = (p.n + BN - 1) / BN;
+  const int tiles = m_tiles * n_tiles;
+  const int nk = (p.k + BK - 1) / BK;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < STAGES; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(&tfull[b], 1);
+      mbar_init(&tempty[b], 2 * 4 * NWG);  // one arrival per epilogue warp of both CTAs
+    }
+    mbar_init(drain, 1);
+    *abort_flag = 0;
+    fence_barrier_init();
+    prefetch_tmap(&tmX);
+    prefetch_tmap(&tmW);
+    prefetch_tmap(&tmO);
+  }
+  if (warp == 1) tmem_alloc_pair(tmem_holder, G::TMEM_COLS);
+  fence_before_sync();
+  cluster_sync();  // both CTAs' barriers exist before either signals the other
+  fence_after_sync();
+  const uint32_t tmem = *tmem_holder;
+
+  if (warp == 0) {
+    int stage = 0;
+    uint32_t phase = 0;
+    uint32_t issued = 0, last_parity = 0;
+    bool ok = true, waited = false;
+    // one stage: x and W (K block kb, id < 0) or h and B (columns 64 kb of adapter id); by lane 0
+    auto emit = [&](int mb, int nb, int kb, int id, int lo, int hi, int last) -> bool {
+      bool good = true;
+      if (lane == 0) {
+        good = !*abort_flag && mbar_wait(&empty[stage], phase ^ 1, 211);
+        if (good) {
+          if (first) {
+            notes[stage] = {lo, hi, id < 0 ? BK / 16 : (min(p.rank - 64 * kb, 64) + 15) / 16, last};
+            // both CTAs' bytes of the stage complete on the first CTA's barrier
+            mbar_arrive_expect_tx(&full[stage], 2 * G::STAGE_BYTES);
+          }
+          const uint32_t bar = cluster_addr(&full[stage], 0);
+          tma_load_2d_pair(sA + stage * A_BYTES, id < 0 ? &tmX : &tmH, bar, kb * BK, mb * 2 * BM + int(rank) * BM);
+          tma_load_2d_pair(sB + stage * G::B_BYTES, id < 0 ? &tmW : &tmB, bar, kb * BK,
+                           (id < 0 ? 0 : id * p.n) + nb * BN + int(rank) * G::BH);
+          issued |= 1u << stage;
+          last_parity = (last_parity & ~(1u << stage)) | (phase << stage);
+        }
+      }
+      if (++stage == STAGES) {
+        stage = 0;
+        phase ^= 1;
+      }
+      return __shfl_sync(0xffffffffu, good, 0);
+    };
+    const int chunks = (p.rank + 63) / 64;
+    for (int t = pair; t < tiles && ok; t += npairs) {
+      const int mb = m_first + t / n_tiles, nb = t % n_tiles;
+      const int r0 = mb * 2 * BM, r1 = min(r0 + 2 * BM, end);
+      int s = p.n_adapters > 0 ? first_seg(p, r0) : p.n_segs;
+      // the last K block is held back until it is known whether runs follow it
+      for (int kb = 0; kb + 1 < nk && ok; ++kb) ok = emit(mb, nb, kb, -1, 0, 2 * BM, 0);
+      int held_kb = nk - 1, held_id = -1, held_lo = 0, held_hi = 2 * BM;
+      for (bool more = true; more && s < p.n_segs && ok; s += 32) {
+        const int i = s + lane;
+        int lo = 0, hi = 0, id = -1;
+        bool in = i < p.n_segs;
+        if (in) {
+          lo = max(seg_start(p, i), r0) - r0;
+          hi = min(seg_start(p, i + 1), r1) - r0;
+          in = r0 + lo < r1;
+          if (lo < hi) id = adapter_of(p, i);
+        }
+        more = __all_sync(0xffffffffu, in);
+        for (uint32_t have = __ballot_sync(0xffffffffu, id >= 0); have && ok; have &= have - 1) {
+          const int src = __ffs(have) - 1;
+          if (!waited) {
+            wait_primary();  // h is complete
+            waited = true;
+          }
+          const int pid = __shfl_sync(0xffffffffu, id, src);
+          const int plo = __shfl_sync(0xffffffffu, lo, src), phi = __shfl_sync(0xffffffffu, hi, src);
+          for (int c = 0; c < chunks && ok; ++c) {
+            ok = emit(mb, nb, held_kb, held_id, held_lo, held_hi, 0);
+            held_kb = c;
+            held_id = pid;
+            held_lo = plo;
+            held_hi = phi;
+          }
+        }
+      }
+      if (ok) ok = emit(mb, nb, held_kb, held_id, held_lo, held_hi, 1);
+    }
+    if (!ok && lane == 0) {
+      *abort_flag = 1;
+      // the first CTA's barriers count both CTAs' copies: wait for the ones issued
+      if (first)
+        for (int s = 0; s < STAGES; ++s)
+          if (issued & (1u << s)) mbar_wait(&full[s], (last_parity >> s) & 1u, 221);
+    }
+    if (!waited) wait_primary();
+  } else if (warp == 1) {
+    if (lane == 0 && first) {
+      const uint32_t idesc = idesc_f16(2 * BM, BN);
+      int stage = 0;
+      uint32_t phase = 0;
+      int local = 0;
+      bool ok = true;
+      for (int t = pair; t < tiles && ok; t += npairs, ++local) {
+        const int buf = local & 1;
+        const uint32_t tphase = (local >> 1) & 1;
+        if (*abort_flag || !mbar_wait(&tempty[buf], tphase ^ 1, 212)) {
+          ok = false;
+          break;
+        }
+        fence_after_sync();
+        const uint32_t d = tmem + uint32_t(buf * BN);
+        for (int i = 0;; ++i) {
+          if (*abort_flag || !mbar_wait(&full[stage], phase, 213)) {
+            ok = false;
+            break;
+          }
+          fence_after_sync();
+          const uint64_t da = desc_sw128(sA + stage * A_BYTES);
+          const uint64_t db = desc_sw128(sB + stage * G::B_BYTES);
+          const StageNote note = notes[stage];
+          if (i < nk) {
+#pragma unroll
+            for (int k = 0; k < BK / 16; ++k)
+              mma_f16_pair(d, da + uint64_t(k * 2), db + uint64_t(k * 2), idesc, (i | k) != 0 ? 1u : 0u);
+          } else {
+            uint32_t off[8];
+#pragma unroll
+            for (int w = 0; w < 8; ++w) off[w] = ~lanes_on(note.lo, note.hi, w);
+            for (int k = 0; k < note.steps; ++k)
+              mma_f16_pair_lanes(d, da + uint64_t(k * 2), db + uint64_t(k * 2), idesc, 1u, off);
+          }
+          mma_commit_pair_both(&empty[stage]);  // the stage is free again in both CTAs
+          if (++stage == STAGES) {
+            stage = 0;
+            phase ^= 1;
+          }
+          if (note.last) break;
+        }
+        if (!ok) break;
+        mma_commit_pair_both(&tfull[buf]);
+      }
+      if (!ok) {
+        *abort_flag = 1;
+        mma_commit_pair(drain);  // the MMAs in flight finish before the TMEM is freed
+        mbar_wait(drain, 0, 222);
+      }
+    }
+  } else {
+    const int q = warp & 3;
+    const int g = (warp - 2) >> 2;
+    const int r = q * 32 + lane;
+    const bool leader = (warp == 2 + 4 * g) && lane == 0;
+    uint8_t* stile = sOut + g * OUT_BYTES;
+    int local = 0;
+    for (int t = pair; t < tiles; t += npairs, ++local) {
+      const int buf = local & 1;
+      const uint32_t tphase = (local >> 1) & 1;
+      const int mb = m_first + t / n_tiles, nb = t % n_tiles;
+      const int row0 = mb * 2 * BM + int(rank) * BM;  // first row of this CTA's half of the tile
+      const int nc = nb * BN + g * 64;
+      const bool inside = row0 >= begin && row0 + BM <= end;  // every row is to be written
+      if (leader) bulk_wait_read<0>();
+      const bool failed = *abort_flag || !mbar_wait(&tfull[buf], tphase, 214);
+      if (named_bar_any(1 + g, 128, failed)) {  // (and the staging tile is free)
+        *abort_flag = 1;
+        break;
+      }
+      fence_after_sync();
+      const uint32_t taddr = tmem + (uint32_t(q * 32) << 16) + uint32_t(buf * BN + g * 64);
+      const int row = row0 + r;
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        uint32_t a[32];
+        tmem_ld32(taddr + 32 * half, a);
+        tmem_ld_wait();
+#pragma unroll
+        for (int i = 0; i < 32; ++i) asm volatile("" : "+r"(a[i]));
+        if (half == 1) {  // tells the MMA thread that this warp has read its accumulator rows
+          fence_before_sync();
+          __syncwarp();
+          if (lane == 0) mbar_arrive_cluster(cluster_addr(&tempty[buf], 0));
+        }
+#pragma unroll
+        for (int c8 = 0; c8 < 4; ++c8) {
+          const int n = nc + 32 * half + 8 * c8;
+          uint4 bias = make_uint4(0, 0, 0, 0);
+          if (p.bias && n < p.n) bias = __ldg(reinterpret_cast<const uint4*>(p.bias + n));
+          const __half2* bh = reinterpret_cast<const __half2*>(&bias);
+          uint32_t u[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float2 v = fadd2(make_float2(__uint_as_float(a[8 * c8 + 2 * e]), __uint_as_float(a[8 * c8 + 2 * e + 1])),
+                                   __half22float2(bh[e]));
+            u[e] = pack_half2(v.x, v.y);
+          }
+          const uint4 o = make_uint4(u[0], u[1], u[2], u[3]);
+          if (inside) *reinterpret_cast<uint4*>(stile + r * 128 + (((4 * half + c8) ^ (r & 7)) * 16)) = o;
+          else if (row >= begin && row < end && n < p.n)
+            *reinterpret_cast<uint4*>(p.out + row * p.out_stride + n) = o;
+        }
+      }
+      fence_proxy_async_smem();
+      named_bar(1 + g, 128);
+      if (leader && inside) {
+        if (nc < p.n) tma_store_2d(&tmO, stile, nc, row0);
+        bulk_commit();
+      }
+    }
+    if (leader) bulk_wait<0>();
+  }
+  fence_before_sync();
+  cluster_sync();  // neither CTA leaves while the other may still use its shared memory or TMEM
+  if (warp == 1) {
+    fence_after_sync();
+    tmem_free_pair(tmem, G::TMEM_COLS);
+  }
+}
+
+// ---- host side ----
+
+constexpr int SMS = 148;
+
+template <class F, class... A>
+void launch_ex(F* kernel, dim3 grid, int threads, size_t smem, int cluster, bool dependent, cudaStream_t st, A... args) {
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[2];
+  int n = 0;
+  if (cluster > 1) {
+    attr[n].id = cudaLaunchAttributeClusterDimension;
+    attr[n].val.clusterDim.x = unsigned(cluster);
+    attr[n].val.clusterDim.y = 1;
+    attr[n].val.clusterDim.z = 1;
+    ++n;
+  }
+  if (dependent) {
+    attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[n].val.programmaticStreamSerializationAllowed = 1;
+    ++n;
+  }
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(unsigned(threads), 1, 1);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cfg.attrs = attr;
+  cfg.numAttrs = unsigned(n);
+  KH_CUDA(cudaLaunchKernelEx(&cfg, kernel, args...));
+}
+
+// Rows by the register-streaming kernels: W is read once per 64 rows.
+bool takes_rows(const kh_lora_matmul_args& a) { return a.rows <= 64; }
+// h by a CTA per row: few rows, or segments so short that a tile of 128 rows would take a product per
+// row or so.
+bool shrinks_rows(const kh_lora_matmul_args& a) { return a.rows <= 64 || a.rows < 8 * int64_t(a.n_segs); }
+
+template <int NB>
+void launch_rows(const LoraParams& p, int Z, bool dependent, cudaStream_t st) {
+  const dim3 grid(unsigned((p.n + RN - 1) / RN * Z), unsigned((p.rows + NB * 8 - 1) / (NB * 8)));
+  launch_ex(lora_rows_kernel<NB>, grid, 256, 0, Z, dependent, st, p, Z);
+}
+
+template <int BN>
+void launch_pair(const LoraParams& p, const kh_lora_matmul_args& a, bool dependent, cudaStream_t st) {
+  using G = PCfg<BN>;
+  static std::atomic<uint64_t> configured{0};
+  once_per_device(configured, [] {
+    KH_CUDA(cudaFuncSetAttribute(lora_pair_kernel<BN>, cudaFuncAttributeMaxDynamicSharedMemorySize, G::SMEM));
+  });
+  CUtensorMap tx, tw, th, tb, to;
+  encode_tensor_map_f16(&tx, a.x, uint64_t(a.rows), uint64_t(a.k), uint64_t(a.x_stride), BK, BM, 128);
+  encode_tensor_map_f16(&tw, a.w, uint64_t(a.n), uint64_t(a.k), uint64_t(a.k), BK, G::BH, 128);
+  encode_tensor_map_f16(&to, a.out, uint64_t(a.rows), uint64_t(a.n), uint64_t(a.out_stride), 64, BM, 128);
+  th = tb = tw;  // (without adapters neither is read)
+  if (a.n_adapters) {
+    encode_tensor_map_f16(&th, a.workspace, uint64_t(a.rows), uint64_t(a.rank), uint64_t(a.rank), BK, BM, 128);
+    encode_tensor_map_f16(&tb, a.lora_b, uint64_t(a.n_adapters) * a.n, uint64_t(a.rank), uint64_t(a.rank), BK, G::BH, 128);
+  }
+  const int64_t tiles = (a.rows + 2 * BM - 1) / (2 * BM) * ((a.n + BN - 1) / BN);
+  const int pairs = int(std::min<int64_t>(tiles, device_sms() / 2));
+  launch_ex(lora_pair_kernel<BN>, dim3(unsigned(2 * pairs)), G::THREADS, G::SMEM, 2, dependent, st, tx, tw, th, tb, to, p);
 }
 
 void check_sizes(const char* fn, const kh_lora_matmul_args* args) {
@@ -118,7 +810,8 @@ void check_sizes(const char* fn, const kh_lora_matmul_args* args) {
   check_that(a.k >= 8 && a.k <= 65536 && a.k % 8 == 0 && a.n >= 8 && a.n <= 65536 && a.n % 8 == 0, fn,
              "k and n must be multiples of 8, in [8, 65536]");
   check_that(a.rank >= 8 && a.rank <= 128 && a.rank % 8 == 0, fn, "rank must be a multiple of 8, in [8, 128]");
-  check_that(a.n_adapters >= 0 && a.n_adapters <= 65535, fn, "n_adapters must be in [0, 65535]");
+  check_that(a.n_adapters >= 0 && a.n_adapters <= 65535 && int64_t(a.n_adapters) * a.n < (int64_t(1) << 31), fn,
+             "n_adapters must be in [0, 65535], n_adapters * n below 2^31");
   check_that(a.n_segs >= 0 && a.n_segs <= 65535, fn, "n_segs must be in [0, 65535]");
   check_that(a.rows >= 0 && a.rows < (int64_t(1) << 31) - 256, fn, "rows must be in [0, 2^31 - 256)");
 }
@@ -127,7 +820,7 @@ void check_sizes(const char* fn, const kh_lora_matmul_args* args) {
 
 int64_t lora_matmul_workspace(const kh_lora_matmul_args* args) {
   check_sizes("kh_lora_matmul_f16_workspace", args);
-  return args->rows * args->rank * 2;
+  return args->n_adapters ? args->rows * args->rank * 2 : 0;
 }
 
 void lora_matmul(const kh_lora_matmul_args* args, cudaStream_t st) {
@@ -180,10 +873,42 @@ void lora_matmul(const kh_lora_matmul_args* args, cudaStream_t st) {
   p.rank = a.rank;
   p.n_adapters = a.n_adapters;
   p.n_segs = a.n_segs;
-  lora_shrink_simple_kernel<<<unsigned(a.rows), 256, 0, st>>>(p);
-  const dim3 grid(unsigned((a.rows + 63) / 64), unsigned((a.n + 63) / 64));
-  lora_simple_kernel<<<grid, 256, 0, st>>>(p);
-  KH_CUDA(cudaGetLastError());
+  const bool adapters = a.n_adapters > 0;
+  if (adapters) {
+    if (shrinks_rows(a)) {
+      lora_shrink_rows_kernel<<<unsigned(a.rows), 256, 0, st>>>(p);
+      KH_CUDA(cudaGetLastError());
+    } else {
+      const int R16 = (a.rank + 15) / 16 * 16, astages = R16 <= 32 ? 8 : 4;
+      const size_t smem = size_t(SXS) * 16384 + size_t(astages) * R16 * 128 + 1024;
+      static std::atomic<uint64_t> configured{0};
+      once_per_device(configured, [] {
+        KH_CUDA(cudaFuncSetAttribute(lora_shrink_tile_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                     SXS * 16384 + 4 * 128 * 128 + 1024));
+      });
+      CUtensorMap tx, ta;
+      encode_tensor_map_f16(&tx, a.x, uint64_t(a.rows), uint64_t(a.k), uint64_t(a.x_stride), 64, 128, 128);
+      encode_tensor_map_f16(&ta, a.lora_a, uint64_t(a.n_adapters) * a.rank, uint64_t(a.k), uint64_t(a.k), 64, R16, 128);
+      const int64_t tiles = (a.rows + 127) / 128;
+      int Z = 1;  // CTAs that split a tile's sum: while SMs are idle, at least two K blocks each
+      while (Z < 8 && 2 * Z * tiles <= SMS && 4 * Z <= (a.k + 63) / 64) Z *= 2;
+      launch_ex(lora_shrink_tile_kernel, dim3(unsigned(Z * tiles)), 192, smem, Z, false, st, tx, ta, p, Z, astages);
+    }
+  }
+  if (takes_rows(a)) {
+    const int n_tiles = (a.n + RN - 1) / RN;
+    int Z = 1;  // CTAs that split the sum of 128 outputs: while SMs are idle, at least a step a warp
+    while (Z < 8 && 2 * Z * n_tiles <= SMS && 128 * Z <= a.k) Z *= 2;
+    if (a.rows <= 8) launch_rows<1>(p, Z, adapters, st);
+    else if (a.rows <= 16) launch_rows<2>(p, Z, adapters, st);
+    else if (a.rows <= 32) launch_rows<4>(p, Z, adapters, st);
+    else launch_rows<8>(p, Z, adapters, st);
+  } else {
+    // 256 columns a tile where that still gives every pair of SMs one
+    const int64_t wide = (a.rows + 255) / 256 * ((a.n + 255) / 256);
+    if (a.n > 128 && wide >= SMS / 2) launch_pair<256>(p, a, adapters, st);
+    else launch_pair<128>(p, a, adapters, st);
+  }
 }
 
 int lora_error_code() {
