@@ -463,49 +463,60 @@ __global__ void __launch_bounds__(TTHREADS, 1)
       }
     }
   } else if (warp == 1) {
-    if (lane == 0 && nkt > 0) {
+    if (nkt > 0) {  // all lanes in step, one issues
       const uint32_t idesc_s = idesc_f16(128, TKEYS);
       const uint32_t idesc_o = idesc_f16(128, D) | (1u << 16);  // V MN-major
+      const bool lead = elect_one();
+      auto wwait = [&](uint64_t* bar, uint32_t parity, int code) -> bool {
+        return __all_sync(0xffffffffu, !*abort_flag && mbar_wait(bar, parity, code));
+      };
       auto tile_of = [&](int g, int it) { return pair ? it : 2 * it + g; };
       auto issue_s = [&](int g, int it) -> bool {
         const int j = tile_of(g, it), st = j % C::KS;
-        if (*abort_flag || !mbar_wait(&k_full[st], uint32_t(j / C::KS) & 1, 106)) return false;
+        if (!wwait(&k_full[st], uint32_t(j / C::KS) & 1, 106)) return false;
         fence_after_sync();
         const uint64_t dq = tile_desc<D>(sQ + (pair ? g : 0) * C::TILE), dk = tile_desc<D>(sK + st * C::TILE);
+        if (lead) {
 #pragma unroll
-        for (int k = 0; k < D / 16; ++k) {
-          const uint64_t off = uint64_t((k / (C::PCOLS / 16)) * (C::PANEL >> 4) + (k % (C::PCOLS / 16)) * 2);
-          mma_f16(tmem + uint32_t(g * 128), dq + off, dk + off, idesc_s, k ? 1u : 0u);
+          for (int k = 0; k < D / 16; ++k) {
+            const uint64_t off = uint64_t((k / (C::PCOLS / 16)) * (C::PANEL >> 4) + (k % (C::PCOLS / 16)) * 2);
+            mma_f16(tmem + uint32_t(g * 128), dq + off, dk + off, idesc_s, k ? 1u : 0u);
+          }
+          mma_commit(&s_full[g]);
+          if (!pair || g == 1) mma_commit(&k_empty[st]);
         }
-        mma_commit(&s_full[g]);
-        if (!pair || g == 1) mma_commit(&k_empty[st]);
+        __syncwarp();
         return true;
       };
-      bool ok = mbar_wait(q_full, 0, 107);
+      bool ok = wwait(q_full, 0, 107);
       for (int g = 0; g < 2 && ok; ++g)
         if (n_of[g] > 0) ok = issue_s(g, 0);
       for (int it = 0; it < n_of[0] && ok; ++it)
         for (int g = 0; g < 2 && ok; ++g) {
           if (it >= n_of[g]) continue;
           const int j = tile_of(g, it), st = j % C::VS;
-          if (*abort_flag || !mbar_wait(&p_full[g], uint32_t(it) & 1, 108) ||
-              !mbar_wait(&v_full[st], uint32_t(j / C::VS) & 1, 109)) {
+          if (!wwait(&p_full[g], uint32_t(it) & 1, 108) || !wwait(&v_full[st], uint32_t(j / C::VS) & 1, 109)) {
             ok = false;
             break;
           }
           fence_after_sync();
           const uint64_t dv = tile_desc<D>(sV + st * C::TILE);
           const uint32_t pa = tmem + uint32_t(g * 128), oa = tmem + C::O_COL + uint32_t(g * D);
+          const bool last = it + 1 >= n_of[g];
+          if (lead) {
 #pragma unroll
-          for (int k = 0; k < TKEYS / 16; ++k)
-            mma_f16_ts(oa, pa + uint32_t(8 * k), dv + uint64_t(k * ((16 * C::ROWB) >> 4)), idesc_o, (it || k) ? 1u : 0u);
-          if (!pair || g == 1) mma_commit(&v_empty[st]);
-          if (it + 1 < n_of[g]) ok = issue_s(g, it + 1);
-          else mma_commit(&o_full[g]);
+            for (int k = 0; k < TKEYS / 16; ++k)
+              mma_f16_ts(oa, pa + uint32_t(8 * k), dv + uint64_t(k * ((16 * C::ROWB) >> 4)), idesc_o, (it || k) ? 1u : 0u);
+            if (!pair || g == 1) mma_commit(&v_empty[st]);
+            if (last) mma_commit(&o_full[g]);
+          }
+          __syncwarp();
+          if (!last) ok = issue_s(g, it + 1);
         }
       if (!ok) {
         *abort_flag = 1;
-        mma_commit(drain);
+        if (lead) mma_commit(drain);
+        __syncwarp();
         mbar_wait(drain, 0, 110);
       }
     }

@@ -48,17 +48,6 @@ struct LoraParams {
 __device__ __forceinline__ int seg_start(const LoraParams& p, int i) {
   return int(min(max(int64_t(__ldg(p.starts + i)), int64_t(0)), p.rows));
 }
-// Segment of row t (the last one that starts at or before it), or -1 before the first and behind the last.
-__device__ __forceinline__ int seg_of(const LoraParams& p, int t) {
-  if (t < seg_start(p, 0) || t >= seg_start(p, p.n_segs)) return -1;
-  int lo = 0, hi = p.n_segs - 1;
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (seg_start(p, mid) <= t) lo = mid;
-    else hi = mid - 1;
-  }
-  return lo;
-}
 // Adapter of a segment, -1 for none; an id that does not exist counts as none and is reported.
 __device__ __forceinline__ int adapter_of(const LoraParams& p, int seg) {
   const int a = __ldg(p.ids + seg);
@@ -101,8 +90,8 @@ __device__ __forceinline__ float dot8(uint4 a, uint4 b, float acc) {
 __global__ void __launch_bounds__(256) lora_shrink_rows_kernel(const LoraParams p) {
   launch_dependents();
   const int t = blockIdx.x, lane = threadIdx.x & 31;
-  const int seg = seg_of(p, t);
-  if (seg < 0) return;
+  const int seg = first_seg(p, t);
+  if (seg >= p.n_segs || t < seg_start(p, seg) || t >= seg_start(p, p.n_segs)) return;
   const int ad = adapter_of(p, seg);
   if (ad < 0) return;
   const uint4* x = reinterpret_cast<const uint4*>(p.x + t * p.x_stride);
@@ -143,9 +132,12 @@ __device__ __forceinline__ void mma_16816(float (&c)[4], uint32_t a0, uint32_t a
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ float ld_cluster_f32(uint32_t addr) {
-  float v;
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+__device__ __forceinline__ float4 ld_cluster_f32x4(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(addr)
+               : "memory");
   return v;
 }
 
@@ -176,7 +168,7 @@ __device__ __forceinline__ void rows_load(RowsFrag<NB>& f, const LoraParams& p, 
 
 template <int NB>
 __global__ void __launch_bounds__(256) lora_rows_kernel(const LoraParams p, int Z) {
-  __shared__ float part[NB * 8][RN + 4];
+  __shared__ __align__(16) float part[NB * 8][RN + 4];
   __shared__ int ids[NB * 8];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int nw = warp & 3, kw = warp >> 2;
@@ -188,7 +180,6 @@ __global__ void __launch_bounds__(256) lora_rows_kernel(const LoraParams p, int 
     return;
   }
   const int nt = min(NB * 8, end - t0);
-  if (threadIdx.x < nt) ids[threadIdx.x] = adapter_of(p, seg_of(p, t0 + threadIdx.x));
 
   float acc[2][NB][4];
 #pragma unroll
@@ -199,6 +190,24 @@ __global__ void __launch_bounds__(256) lora_rows_kernel(const LoraParams p, int 
   RowsFrag<NB> cur, nxt;
   int k = (z * 2 + kw) * 32;
   if (k < p.k) rows_load<NB>(cur, p, n0 + nw * 32, t0, end, k);
+  // adapters of the CTA's rows, while these loads are under way
+  if (threadIdx.x < NB * 8) ids[threadIdx.x] = -1;
+  __syncthreads();
+  if (p.n_adapters > 0) {
+    for (int s = first_seg(p, t0); s < p.n_segs; s += 256) {
+      const int i = s + threadIdx.x;
+      bool more = i < p.n_segs;
+      if (more) {
+        const int lo = max(seg_start(p, i), t0), hi = min(seg_start(p, i + 1), t0 + nt);
+        more = lo < t0 + nt;
+        if (lo < hi) {
+          const int ad = adapter_of(p, i);
+          for (int t = lo; t < hi; ++t) ids[t - t0] = ad;
+        }
+      }
+      if (!__syncthreads_and(more)) break;
+    }
+  }
   for (; k < p.k; k += stride) {
     if (k + stride < p.k) rows_load<NB>(nxt, p, n0 + nw * 32, t0, end, k + stride);
 #pragma unroll
@@ -228,24 +237,40 @@ __global__ void __launch_bounds__(256) lora_rows_kernel(const LoraParams p, int 
   }
   if (Z > 1) cluster_sync();
   wait_primary();
-  const int per = RN / Z;
+  // four outputs of a row per thread (n is a multiple of 8)
+  const int per = RN / Z / 4;
   for (int e = threadIdx.x; e < nt * per; e += 256) {
-    const int i = e / per, c = z * per + e % per, n = n0 + c, t = t0 + i;
+    const int i = e / per, c = z * (RN / Z) + e % per * 4, n = n0 + c, t = t0 + i;
     if (n >= p.n) continue;
-    float v = 0.f;
+    float v[4] = {};
     if (Z == 1) {
-      v = part[i][c];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[j] = part[i][c + j];
     } else {
-      for (int q = 0; q < Z; ++q) v += ld_cluster_f32(cluster_addr(&part[i][c], uint32_t(q)));
+      float4 u[8];
+#pragma unroll
+      for (int q = 0; q < 8; ++q) u[q] = q < Z ? ld_cluster_f32x4(cluster_addr(&part[i][c], uint32_t(q))) : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int q = 0; q < 8; ++q) v[0] += u[q].x, v[1] += u[q].y, v[2] += u[q].z, v[3] += u[q].w;
     }
-    if (p.bias) v += __half2float(p.bias[n]);
+    if (p.bias) {
+      const uint2 u = __ldg(reinterpret_cast<const uint2*>(p.bias + n));
+      const float2 b0 = __half22float2(*reinterpret_cast<const __half2*>(&u.x)), b1 = __half22float2(*reinterpret_cast<const __half2*>(&u.y));
+      v[0] += b0.x, v[1] += b0.y, v[2] += b1.x, v[3] += b1.y;
+    }
     const int ad = ids[i];
     if (ad >= 0) {
       const uint4* b = reinterpret_cast<const uint4*>(p.b + (int64_t(ad) * p.n + n) * p.rank);
       const uint4* h = reinterpret_cast<const uint4*>(p.h + int64_t(t) * p.rank);
-      for (int r = 0; r < p.rank / 8; ++r) v = dot8(h[r], __ldg(b + r), v);
+      const int chunks = p.rank / 8;
+#pragma unroll 2
+      for (int r = 0; r < chunks; ++r) {
+        const uint4 hv = h[r];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] = dot8(hv, __ldg(b + j * chunks + r), v[j]);
+      }
     }
-    p.out[t * p.out_stride + n] = __float2half_rn(v);
+    *reinterpret_cast<uint2*>(p.out + t * p.out_stride + n) = make_uint2(pack_half2(v[0], v[1]), pack_half2(v[2], v[3]));
   }
   if (Z > 1) cluster_sync();  // no CTA leaves while another reads its part
 }
@@ -260,7 +285,10 @@ __global__ void __launch_bounds__(256) lora_rows_kernel(const LoraParams p, int 
 constexpr int SXS = 4;  // x stages
 struct ShrinkPieces {
   int count;
-  int lo[128], hi[128], id[128];
+  int id[128];
+  uint4 off[128];         // lanes of other rows
+  int row_id[128];        // adapter of each row, -1 for none
+  float row_scale[128];
 };
 
 __device__ __forceinline__ uint32_t lanes_on(int lo, int hi, int word) {
@@ -289,24 +317,31 @@ __global__ void __launch_bounds__(192) lora_shrink_tile_kernel(const __grid_cons
   const int z = blockIdx.x % Z, r0 = int(blockIdx.x / Z) * 128;
   const uint32_t cols = R16 <= 32 ? 32u : R16 <= 64 ? 64u : 128u;
   if (warp == 0) {
+    const int last = seg_start(p, p.n_segs);  // rows from here on are not written
     // the adapters of these rows: non-empty runs of rows, in order
     int n = 0;
+    for (int r = lane; r < 128; r += 32) pieces.row_id[r] = -1;
+    __syncwarp();
     for (int s = first_seg(p, r0); s < p.n_segs; s += 32) {
       const int i = s + lane;
       int lo = 0, hi = 0, id = -1;
       bool more = i < p.n_segs;
       if (more) {
         lo = max(seg_start(p, i), r0) - r0;
-        hi = min(seg_start(p, i + 1), r0 + 128) - r0;
+        hi = min(min(seg_start(p, i + 1), last), r0 + 128) - r0;
         more = lo < 128;
         if (lo < hi) id = adapter_of(p, i);
       }
       const uint32_t have = __ballot_sync(0xffffffffu, id >= 0);
       const int at = n + __popc(have & ((1u << lane) - 1u));
       if (id >= 0 && at < 128) {
-        pieces.lo[at] = lo;
-        pieces.hi[at] = hi;
         pieces.id[at] = id;
+        pieces.off[at] = make_uint4(~lanes_on(lo, hi, 0), ~lanes_on(lo, hi, 1), ~lanes_on(lo, hi, 2), ~lanes_on(lo, hi, 3));
+        const float sc = p.scales ? __ldg(p.scales + id) : 1.f;
+        for (int r = lo; r < hi; ++r) {
+          pieces.row_id[r] = id;
+          pieces.row_scale[r] = sc;
+        }
       }
       n += __popc(have);
       if (!__all_sync(0xffffffffu, more)) break;
@@ -368,45 +403,56 @@ __global__ void __launch_bounds__(192) lora_shrink_tile_kernel(const __grid_cons
       }
     }
   } else if (warp == 1) {
-    if (lane == 0) {
-      const uint32_t idesc = idesc_f16(128, R16);
-      bool ok = true;
-      int ai = 0;
-      for (int kb = 0; kb < nk && ok; ++kb) {
-        const int xs = kb % SXS;
-        if (abort_flag || !mbar_wait(&x_full[xs], uint32_t(kb / SXS) & 1, 205)) { ok = false; break; }
-        const uint64_t dx = desc_sw128(sX + xs * 16384);
-        for (int i = 0; i < np; ++i, ++ai) {
-          const int as = ai % astages;
-          if (abort_flag || !mbar_wait(&a_full[as], uint32_t(ai / astages) & 1, 206)) { ok = false; break; }
-          fence_after_sync();
-          uint32_t off[4];
-#pragma unroll
-          for (int w = 0; w < 4; ++w) off[w] = ~lanes_on(pieces.lo[i], pieces.hi[i], w);
-          const uint64_t da = desc_sw128(sA + as * a_bytes);
+    // all lanes in step, one issues
+    const uint32_t idesc = idesc_f16(128, R16);
+    const bool lead = elect_one();
+    bool ok = true;
+    auto wwait = [&](uint64_t* bar, uint32_t parity, int code) -> bool {
+      return __all_sync(0xffffffffu, !abort_flag && mbar_wait(bar, parity, code));
+    };
+    int as = 0;
+    uint32_t av = 0;
+    for (int kb = 0; kb < nk && ok; ++kb) {
+      const int xs = kb % SXS;
+      if (!wwait(&x_full[xs], uint32_t(kb / SXS) & 1, 205)) { ok = false; break; }
+      const uint64_t dx = desc_sw128(sX + xs * 16384);
+      for (int i = 0; i < np; ++i) {
+        if (!wwait(&a_full[as], av, 206)) { ok = false; break; }
+        fence_after_sync();
+        const uint4 o = pieces.off[i];
+        const uint64_t da = desc_sw128(sA + as * a_bytes);
+        if (lead) {
+          const uint32_t off[4] = {o.x, o.y, o.z, o.w};
 #pragma unroll
           for (int k = 0; k < 4; ++k)
             mma_f16_lanes(tmem, dx + uint64_t(2 * k), da + uint64_t(2 * k), idesc, (kb | k) ? 1u : 0u, off);
           mma_commit(&a_empty[as]);
         }
-        if (ok) mma_commit(&x_empty[xs]);
+        __syncwarp();
+        if (++as == astages) {
+          as = 0;
+          av ^= 1;
+        }
       }
-      if (!ok) {
-        abort_flag = 1;
-        mma_commit(drain);
-        mbar_wait(drain, 0, 207);
-      }
-      mma_commit(done);  // (after a failure too: nothing is stored then)
+      if (ok && lead) mma_commit(&x_empty[xs]);
+      __syncwarp();
     }
+    if (!ok) {
+      abort_flag = 1;
+      if (lead) mma_commit(drain);
+      __syncwarp();
+      mbar_wait(drain, 0, 207);
+    }
+    if (lead) mma_commit(done);  // (after a failure too: nothing is stored then)
+    __syncwarp();
   } else {
     const int quarter = warp & 3, r = quarter * 32 + lane, t = r0 + r;
-    const int seg = t < p.rows ? seg_of(p, t) : -1;
-    const int ad = seg >= 0 ? adapter_of(p, seg) : -1;
-    const float s = ad >= 0 && p.scales ? __ldg(p.scales + ad) : 1.f;
+    const int ad = pieces.row_id[r];
+    const float s = pieces.row_scale[r];  // (read where ad >= 0 only)
     const bool ok = __all_sync(0xffffffffu, mbar_wait(done, 0, 208)) && !abort_flag;
     fence_after_sync();
     const uint32_t taddr = tmem + (uint32_t(quarter * 32) << 16);
-    float* part = reinterpret_cast<float*>(smem) + r * (R16 + 1);  // split sums, over the stages (all read)
+    float* part = reinterpret_cast<float*>(smem) + r * (R16 + 4);  // split sums, over the stages (all read)
 #pragma unroll 1
     for (int c = 0; c < R16; c += 8) {
       uint32_t v[8];
@@ -416,7 +462,10 @@ __global__ void __launch_bounds__(192) lora_shrink_tile_kernel(const __grid_cons
       for (int i = 0; i < 8; ++i) asm volatile("" : "+r"(v[i]));
       if (Z > 1) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) part[c + i] = nk > 0 ? __uint_as_float(v[i]) : 0.f;
+        for (int i = 0; i < 8; i += 4)
+          *reinterpret_cast<float4*>(part + c + i) =
+              nk > 0 ? make_float4(__uint_as_float(v[i]), __uint_as_float(v[i + 1]), __uint_as_float(v[i + 2]), __uint_as_float(v[i + 3]))
+                     : make_float4(0.f, 0.f, 0.f, 0.f);
       } else if (ok && ad >= 0 && c < p.rank) {
         *reinterpret_cast<uint4*>(p.h + int64_t(t) * p.rank + c) =
             make_uint4(pack_half2(__uint_as_float(v[0]) * s, __uint_as_float(v[1]) * s),
@@ -430,22 +479,19 @@ __global__ void __launch_bounds__(192) lora_shrink_tile_kernel(const __grid_cons
   __syncthreads();
   if (Z > 1) {
     cluster_sync();
-    // CTA z adds up rows [z per, (z + 1) per), a thread 8 of a row's values
-    const int per = 128 / Z;
+    // CTA z adds up rows [z per, (z + 1) per), a thread 4 of a row's values
+    const int per = 128 / Z, quads = p.rank / 4;
     const float* base = reinterpret_cast<const float*>(smem);
-    for (int e = threadIdx.x; e < per * (p.rank / 8); e += 192) {
-      const int r = z * per + e / (p.rank / 8), c = e % (p.rank / 8) * 8, t = r0 + r;
-      const int seg = t < p.rows ? seg_of(p, t) : -1;
-      const int ad = seg >= 0 ? adapter_of(p, seg) : -1;
-      if (ad < 0 || abort_flag) continue;
-      const float s = p.scales ? __ldg(p.scales + ad) : 1.f;
-      float v[8] = {};
-      for (int q = 0; q < Z; ++q)
+    for (int e = threadIdx.x; e < per * quads; e += 192) {
+      const int r = z * per + e / quads, c = e % quads * 4;
+      if (pieces.row_id[r] < 0 || abort_flag) continue;
+      const float s = pieces.row_scale[r];
+      float4 u[8], v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] += ld_cluster_f32(cluster_addr(base + r * (R16 + 1) + c + i, uint32_t(q)));
-      *reinterpret_cast<uint4*>(p.h + int64_t(t) * p.rank + c) =
-          make_uint4(pack_half2(v[0] * s, v[1] * s), pack_half2(v[2] * s, v[3] * s), pack_half2(v[4] * s, v[5] * s),
-                     pack_half2(v[6] * s, v[7] * s));
+      for (int q = 0; q < 8; ++q) u[q] = q < Z ? ld_cluster_f32x4(cluster_addr(base + r * (R16 + 4) + c, uint32_t(q))) : v;
+#pragma unroll
+      for (int q = 0; q < 8; ++q) v.x += u[q].x, v.y += u[q].y, v.z += u[q].z, v.w += u[q].w;
+      *reinterpret_cast<uint2*>(p.h + int64_t(r0 + r) * p.rank + c) = make_uint2(pack_half2(v.x * s, v.y * s), pack_half2(v.z * s, v.w * s));
     }
     cluster_sync();
   }
@@ -483,9 +529,11 @@ struct PCfg {
   static constexpr int SMEM = STAGES * STAGE_BYTES + NWG * OUT_BYTES + 1024 + 512;
 };
 
-// What a stage holds for the MMA thread: the rows it counts for, its steps of 16, whether the tile ends.
+// What a stage holds for the MMA warp: the lanes an adapter's product leaves alone, its steps of 16,
+// whether the tile ends.
 struct StageNote {
-  int lo, hi, steps, last;
+  uint4 off[2];
+  int steps, last, pad[2];
 };
 
 template <int BN>
@@ -547,30 +595,31 @@ __global__ void __launch_bounds__(PCfg<BN>::THREADS, 1)
     uint32_t phase = 0;
     uint32_t issued = 0, last_parity = 0;
     bool ok = true, waited = false;
-    // one stage: x and W (K block kb, id < 0) or h and B (columns 64 kb of adapter id); by lane 0
+    // one stage: x and W (K block kb, id < 0) or h and B (columns 64 kb of adapter id for rows [lo, hi))
     auto emit = [&](int mb, int nb, int kb, int id, int lo, int hi, int last) -> bool {
-      bool good = true;
+      if (!__all_sync(0xffffffffu, !*abort_flag && mbar_wait(&empty[stage], phase ^ 1, 211))) return false;
+      if (id >= 0 && lane < 8) reinterpret_cast<uint32_t*>(notes[stage].off)[lane] = ~lanes_on(lo, hi, lane);
+      __syncwarp();
       if (lane == 0) {
-        good = !*abort_flag && mbar_wait(&empty[stage], phase ^ 1, 211);
-        if (good) {
-          if (first) {
-            notes[stage] = {lo, hi, id < 0 ? BK / 16 : (min(p.rank - 64 * kb, 64) + 15) / 16, last};
-            // both CTAs' bytes of the stage complete on the first CTA's barrier
-            mbar_arrive_expect_tx(&full[stage], 2 * G::STAGE_BYTES);
-          }
-          const uint32_t bar = cluster_addr(&full[stage], 0);
-          tma_load_2d_pair(sA + stage * A_BYTES, id < 0 ? &tmX : &tmH, bar, kb * BK, mb * 2 * BM + int(rank) * BM);
-          tma_load_2d_pair(sB + stage * G::B_BYTES, id < 0 ? &tmW : &tmB, bar, kb * BK,
-                           (id < 0 ? 0 : id * p.n) + nb * BN + int(rank) * G::BH);
-          issued |= 1u << stage;
-          last_parity = (last_parity & ~(1u << stage)) | (phase << stage);
+        if (first) {
+          notes[stage].steps = id < 0 ? BK / 16 : (min(p.rank - 64 * kb, 64) + 15) / 16;
+          notes[stage].last = last;
+          // both CTAs' bytes of the stage complete on the first CTA's barrier
+          mbar_arrive_expect_tx(&full[stage], 2 * G::STAGE_BYTES);
         }
+        const uint32_t bar = cluster_addr(&full[stage], 0);
+        tma_load_2d_pair(sA + stage * A_BYTES, id < 0 ? &tmX : &tmH, bar, kb * BK, mb * 2 * BM + int(rank) * BM);
+        tma_load_2d_pair(sB + stage * G::B_BYTES, id < 0 ? &tmW : &tmB, bar, kb * BK,
+                         (id < 0 ? 0 : id * p.n) + nb * BN + int(rank) * G::BH);
       }
+      __syncwarp();
+      issued |= 1u << stage;
+      last_parity = (last_parity & ~(1u << stage)) | (phase << stage);
       if (++stage == STAGES) {
         stage = 0;
         phase ^= 1;
       }
-      return __shfl_sync(0xffffffffu, good, 0);
+      return true;
     };
     const int chunks = (p.rank + 63) / 64;
     for (int t = pair; t < tiles && ok; t += npairs) {
@@ -619,8 +668,12 @@ __global__ void __launch_bounds__(PCfg<BN>::THREADS, 1)
     }
     if (!waited) wait_primary();
   } else if (warp == 1) {
-    if (lane == 0 && first) {
+    if (first) {  // all lanes in step, one issues
       const uint32_t idesc = idesc_f16(2 * BM, BN);
+      const bool lead = elect_one();
+      auto wwait = [&](uint64_t* bar, uint32_t parity, int code) -> bool {
+        return __all_sync(0xffffffffu, !*abort_flag && mbar_wait(bar, parity, code));
+      };
       int stage = 0;
       uint32_t phase = 0;
       int local = 0;
@@ -628,45 +681,54 @@ __global__ void __launch_bounds__(PCfg<BN>::THREADS, 1)
       for (int t = pair; t < tiles && ok; t += npairs, ++local) {
         const int buf = local & 1;
         const uint32_t tphase = (local >> 1) & 1;
-        if (*abort_flag || !mbar_wait(&tempty[buf], tphase ^ 1, 212)) {
+        if (!wwait(&tempty[buf], tphase ^ 1, 212)) {
           ok = false;
           break;
         }
         fence_after_sync();
         const uint32_t d = tmem + uint32_t(buf * BN);
         for (int i = 0;; ++i) {
-          if (*abort_flag || !mbar_wait(&full[stage], phase, 213)) {
+          if (!wwait(&full[stage], phase, 213)) {
             ok = false;
             break;
           }
           fence_after_sync();
           const uint64_t da = desc_sw128(sA + stage * A_BYTES);
           const uint64_t db = desc_sw128(sB + stage * G::B_BYTES);
-          const StageNote note = notes[stage];
+          const int last = notes[stage].last;
           if (i < nk) {
+            if (lead) {
 #pragma unroll
-            for (int k = 0; k < BK / 16; ++k)
-              mma_f16_pair(d, da + uint64_t(k * 2), db + uint64_t(k * 2), idesc, (i | k) != 0 ? 1u : 0u);
+              for (int k = 0; k < BK / 16; ++k)
+                mma_f16_pair(d, da + uint64_t(k * 2), db + uint64_t(k * 2), idesc, (i | k) != 0 ? 1u : 0u);
+              mma_commit_pair_both(&empty[stage]);  // the stage is free again in both CTAs
+            }
           } else {
-            uint32_t off[8];
+            const uint4 o0 = notes[stage].off[0], o1 = notes[stage].off[1];
+            const int steps = notes[stage].steps;
+            if (lead) {
+              const uint32_t off[8] = {o0.x, o0.y, o0.z, o0.w, o1.x, o1.y, o1.z, o1.w};
 #pragma unroll
-            for (int w = 0; w < 8; ++w) off[w] = ~lanes_on(note.lo, note.hi, w);
-            for (int k = 0; k < note.steps; ++k)
-              mma_f16_pair_lanes(d, da + uint64_t(k * 2), db + uint64_t(k * 2), idesc, 1u, off);
+              for (int k = 0; k < BK / 16; ++k)
+                if (k < steps) mma_f16_pair_lanes(d, da + uint64_t(k * 2), db + uint64_t(k * 2), idesc, 1u, off);
+              mma_commit_pair_both(&empty[stage]);
+            }
           }
-          mma_commit_pair_both(&empty[stage]);  // the stage is free again in both CTAs
+          __syncwarp();
           if (++stage == STAGES) {
             stage = 0;
             phase ^= 1;
           }
-          if (note.last) break;
+          if (last) break;
         }
         if (!ok) break;
-        mma_commit_pair_both(&tfull[buf]);
+        if (lead) mma_commit_pair_both(&tfull[buf]);
+        __syncwarp();
       }
       if (!ok) {
         *abort_flag = 1;
-        mma_commit_pair(drain);  // the MMAs in flight finish before the TMEM is freed
+        if (lead) mma_commit_pair(drain);  // the MMAs in flight finish before the TMEM is freed
+        __syncwarp();
         mbar_wait(drain, 0, 222);
       }
     }

@@ -8,8 +8,9 @@
 // Layout: a head is cut into chunks of VEC values (one load each), and a thread owns two chunks of the
 // same head, the pair that the rotation mixes (chunk i and the one R / 2 values on; neighbours when
 // the pairs are neighbours or behind R), so the rotation needs no exchange. LANES threads, a power of
-// two, hold a head and add their squares by shuffles. A thread takes U heads of the same row, so that
-// it loads the angles and weights once, and has 2 U loads in flight.
+// two, hold a head and add their squares by shuffles. A thread takes U heads of the same row: it loads
+// the angles and weights once, folds them into coefficients w cos and w sin (the scale of a head
+// comes last), and has 2 U loads in flight.
 
 #include "device_ops.h"
 
@@ -29,190 +30,230 @@ __device__ int kh_norm_error = 0;
 struct NormParams {
   const void* x;
   void* out;
-  int64_t rows, x_stride, out_stride, table_rows;
+  int64_t x_stride, out_stride, table_rows;
   const float* qw;
   const float* kw;
   const float* cossin;
   const int32_t* positions;
+  uint32_t groups;  // rows * blocks of this launch
   int q_heads, k_heads, D, R;
-  int q_blocks, blocks;  // blocks of U heads of a row: those of q, all
+  uint32_t q_blocks, blocks;  // blocks of U heads of a row: those of q, all
   float eps, inv_d;
   bool interleaved;
 };
 
 template <typename T, int VEC>
-__device__ __forceinline__ void load_chunk(float (&f)[VEC], const T* p) {
-  struct alignas(sizeof(T) * VEC) Raw { T v[VEC]; };
-  const Raw r = *reinterpret_cast<const Raw*>(p);
+struct alignas(sizeof(T) * VEC) Chunk {
+  T v[VEC];
+};
+
+// N consecutive f32 values, in loads as wide as N allows.
+template <int N>
+__device__ __forceinline__ void load_f32(float (&f)[N], const float* p) {
+  const Chunk<float, N> c = *reinterpret_cast<const Chunk<float, N>*>(p);
 #pragma unroll
-  for (int i = 0; i < VEC; ++i) f[i] = float(r.v[i]);
+  for (int i = 0; i < N; ++i) f[i] = c.v[i];
 }
-template <typename T, int VEC>
-__device__ __forceinline__ void store_chunk(T* p, const float (&f)[VEC]) {
-  struct alignas(sizeof(T) * VEC) Raw { T v[VEC]; };
-  Raw r;
+template <>
+__device__ __forceinline__ void load_f32<8>(float (&f)[8], const float* p) {
+  const float4 u = __ldg(reinterpret_cast<const float4*>(p)), v = __ldg(reinterpret_cast<const float4*>(p) + 1);
+  f[0] = u.x, f[1] = u.y, f[2] = u.z, f[3] = u.w, f[4] = v.x, f[5] = v.y, f[6] = v.z, f[7] = v.w;
+}
+
+// Coefficients of one chunk at values [d, d + VEC): its weights times the cosines and sines. `step`:
+// values per angle (1, or 2 when the pairs are neighbours), `angle`: index of the first one.
+template <int VEC, int ANGLES>
+__device__ __forceinline__ void coefficients(float (&wc)[VEC], float (&ws)[VEC], const float* w, const float* cs, int R,
+                                             int d, int angle, bool turned) {
+  if (w) {
+    load_f32<VEC>(wc, w + d);
+  } else {
 #pragma unroll
-  for (int i = 0; i < VEC; ++i) r.v[i] = T(f[i]);
-  *reinterpret_cast<Raw*>(p) = r;
+    for (int e = 0; e < VEC; ++e) wc[e] = 1.f;
+  }
+#pragma unroll
+  for (int e = 0; e < VEC; ++e) ws[e] = 0.f;
+  if (turned) {
+    float c[ANGLES], s[ANGLES];
+    load_f32<ANGLES>(c, cs + angle);
+    load_f32<ANGLES>(s, cs + R + angle);
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+      ws[e] = wc[e] * s[e * ANGLES / VEC];
+      wc[e] *= c[e * ANGLES / VEC];
+    }
+  }
 }
 
 // PAIRS: chunk pairs of a thread (1, or 4 for the one-value chunks of unaligned heads). LANES * PAIRS
 // pairs cover D <= 256.
 template <typename T, int VEC, int PAIRS, int U>
-__global__ void __launch_bounds__(256) qk_norm_rope_kernel(const NormParams p, int lanes) {
-  const int sub = threadIdx.x % lanes;
-  const int64_t group = (int64_t(blockIdx.x) * blockDim.x + threadIdx.x) / lanes;
-  const int64_t row = group / p.blocks;
-  const int block = int(group - row * p.blocks);
-  const bool in = row < p.rows;  // (the threads of a head agree; all stay for the shuffles)
+__global__ void __launch_bounds__(256) qk_norm_rope_kernel(const NormParams p, int lanes_log2) {
+  const uint32_t lanes = 1u << lanes_log2;
+  const uint32_t thread = blockIdx.x * 256u + threadIdx.x;
+  const int sub = int(thread & (lanes - 1));
+  const uint32_t group = thread >> lanes_log2;
+  const uint32_t row = group / p.blocks, block = group - row * p.blocks;
+  const bool in = group < p.groups;  // (the threads of a head agree; all stay for the shuffles)
   const bool is_k = block >= p.q_blocks;
-  const int head0 = (is_k ? block - p.q_blocks : block) * U;
+  const int head0 = int(is_k ? block - p.q_blocks : block) * U;
   const int nheads = in ? min(U, (is_k ? p.k_heads : p.q_heads) - head0) : 0;
   const int first = (is_k ? p.q_heads : 0) + head0;  // among all heads of the row
 
+  int pos = 0;
+  if (in && p.R) pos = p.positions[row];  // (first: the angles depend on it)
+
   const int chunks = p.D / VEC;
-  const int turned = p.interleaved ? 0 : p.R / 2 / VEC;  // pairs whose chunks lie R / 2 apart
+  const int apart = p.interleaved ? 0 : p.R / 2 / VEC;  // pairs whose chunks lie R / 2 values apart
   int c0[PAIRS], c1[PAIRS];
 #pragma unroll
   for (int i = 0; i < PAIRS; ++i) {
-    const int k = sub + i * lanes;
-    c0[i] = k < turned ? k : 2 * k;
-    c1[i] = k < turned ? k + turned : 2 * k + 1;
+    const int k = sub + i * int(lanes);
+    c0[i] = k < apart ? k : 2 * k;
+    c1[i] = k < apart ? k + apart : 2 * k + 1;
     if (c0[i] >= chunks) c0[i] = -1;
     if (c1[i] >= chunks) c1[i] = -1;
   }
 
   const T* xr = static_cast<const T*>(p.x) + row * p.x_stride + int64_t(first) * p.D;
-  float a[U][PAIRS][VEC], b[U][PAIRS][VEC];
+  Chunk<T, VEC> a[U][PAIRS], b[U][PAIRS];
 #pragma unroll
   for (int u = 0; u < U; ++u)
 #pragma unroll
     for (int i = 0; i < PAIRS; ++i) {
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) a[u][i][e] = b[u][i][e] = 0.f;
+      for (int e = 0; e < VEC; ++e) a[u][i].v[e] = b[u][i].v[e] = T(0.f);
       if (u < nheads) {
-        if (c0[i] >= 0) load_chunk<T, VEC>(a[u][i], xr + u * p.D + c0[i] * VEC);
-        if (c1[i] >= 0) load_chunk<T, VEC>(b[u][i], xr + u * p.D + c1[i] * VEC);
+        if (c0[i] >= 0) a[u][i] = *reinterpret_cast<const Chunk<T, VEC>*>(xr + u * p.D + c0[i] * VEC);
+        if (c1[i] >= 0) b[u][i] = *reinterpret_cast<const Chunk<T, VEC>*>(xr + u * p.D + c1[i] * VEC);
       }
     }
 
-  int64_t pos = 0;
-  bool bad = false;
-  if (in && p.R) {
-    pos = p.positions[row];
-    bad = pos < 0 || pos >= p.table_rows;
-    if (bad) {
-      atomicExch(&kh_norm_error, OP_BAD_INDEX);
-      pos = 0;
-    }
+  const bool bad = pos < 0 || (p.R && pos >= p.table_rows);
+  if (bad) {
+    atomicExch(&kh_norm_error, OP_BAD_INDEX);
+    pos = 0;
   }
-  const float* cs = p.cossin + pos * 2 * p.R;
+  const float* cs = p.cossin + int64_t(pos) * 2 * p.R;
   const float* w = is_k ? p.kw : p.qw;
 
   float scale[U];
 #pragma unroll
   for (int u = 0; u < U; ++u) {
-    float ss = 0.f;
+    float s0 = 0.f, s1 = 0.f;
 #pragma unroll
     for (int i = 0; i < PAIRS; ++i)
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) ss += a[u][i][e] * a[u][i][e] + b[u][i][e] * b[u][i][e];
-    for (int o = lanes >> 1; o; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-    scale[u] = rsqrtf(ss * p.inv_d + p.eps);
+      for (int e = 0; e < VEC; ++e) {
+        const float f = float(a[u][i].v[e]), g = float(b[u][i].v[e]);
+        s0 = fmaf(f, f, s0);
+        s1 = fmaf(g, g, s1);
+      }
+    scale[u] = s0 + s1;
   }
+  for (uint32_t o = lanes >> 1; o; o >>= 1)
+#pragma unroll
+    for (int u = 0; u < U; ++u) scale[u] += __shfl_xor_sync(0xffffffffu, scale[u], o);
+#pragma unroll
+  for (int u = 0; u < U; ++u) scale[u] = bad ? 0.f : rsqrtf(fmaf(scale[u], p.inv_d, p.eps));
 
   T* yr = static_cast<T*>(p.out) + row * p.out_stride + int64_t(first) * p.D;
 #pragma unroll
   for (int i = 0; i < PAIRS; ++i) {
-    if (c0[i] < 0) continue;
+    if (c0[i] < 0 || nheads == 0) continue;
     const int d0 = c0[i] * VEC, d1 = c1[i] * VEC;
-    float w0[VEC], w1[VEC], c[VEC], s[VEC], ci[VEC], si[VEC];
-    // angles: pairs apart use (c, s)[e] for (a[e], b[e]); neighbours inside a chunk use (c, s) for the
-    // pairs of a and (ci, si) for those of b
-    const bool apart = sub + i * lanes < turned;
-#pragma unroll
-    for (int e = 0; e < VEC; ++e) {
-      w0[e] = w ? __ldg(w + d0 + e) : 1.f;
-      w1[e] = w && c1[i] >= 0 ? __ldg(w + d1 + e) : 1.f;
-      c[e] = ci[e] = 1.f;
-      s[e] = si[e] = 0.f;
-      if (apart) {
-        c[e] = __ldg(cs + d0 + e);
-        s[e] = __ldg(cs + p.R + d0 + e);
-      } else if (p.interleaved) {
-        if (d0 + e < p.R) {
-          c[e] = __ldg(cs + (d0 + e) / 2);
-          s[e] = __ldg(cs + p.R + (d0 + e) / 2);
-        }
-        if (c1[i] >= 0 && d1 + e < p.R) {
-          ci[e] = __ldg(cs + (d1 + e) / 2);
-          si[e] = __ldg(cs + p.R + (d1 + e) / 2);
-        }
-      }
+    const bool two = c1[i] >= 0, far = sub + i * int(lanes) < apart;
+    const bool near0 = p.interleaved && d0 < p.R, near1 = p.interleaved && two && d1 < p.R;
+    float wc0[VEC], ws0[VEC], wc1[VEC], ws1[VEC];
+    if (p.interleaved) {
+      constexpr int N = VEC == 1 ? 1 : VEC / 2;
+      coefficients<VEC, N>(wc0, ws0, w, cs, p.R, d0, d0 / 2, near0);
+      if (two) coefficients<VEC, N>(wc1, ws1, w, cs, p.R, d1, d1 / 2, near1);
+    } else {
+      coefficients<VEC, VEC>(wc0, ws0, w, cs, p.R, d0, d0, far);
+      if (two) coefficients<VEC, VEC>(wc1, ws1, w, cs, p.R, d1, d0, far);
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       if (u >= nheads) break;
-      float y0[VEC], y1[VEC];
+      float f[VEC], g[VEC], y0[VEC], y1[VEC];
 #pragma unroll
       for (int e = 0; e < VEC; ++e) {
-        y0[e] = a[u][i][e] * scale[u] * w0[e];
-        y1[e] = b[u][i][e] * scale[u] * w1[e];
+        f[e] = float(a[u][i].v[e]);
+        g[e] = float(b[u][i].v[e]);
       }
-      if (apart) {
+      // the partner of a value: in the other chunk, or beside it in its own (VEC 1: the other chunk)
+      if (far || (VEC == 1 && near0)) {
 #pragma unroll
         for (int e = 0; e < VEC; ++e) {
-          const float t = y0[e] * c[e] - y1[e] * s[e];
-          y1[e] = y1[e] * c[e] + y0[e] * s[e];
-          y0[e] = t;
+          y0[e] = fmaf(f[e], wc0[e], -(g[e] * ws1[e]));
+          y1[e] = fmaf(g[e], wc1[e], f[e] * ws0[e]);
         }
-      } else if (p.interleaved) {
-        if constexpr (VEC == 1) {  // the pair is the two one-value chunks
-          const float t = y0[0] * c[0] - y1[0] * s[0];
-          y1[0] = y1[0] * c[0] + y0[0] * s[0];
-          y0[0] = t;
-        } else {
+      } else {
 #pragma unroll
-          for (int e = 0; e < VEC; e += 2) {
-            const float t = y0[e] * c[e] - y0[e + 1] * s[e];
-            y0[e + 1] = y0[e + 1] * c[e] + y0[e] * s[e];
-            y0[e] = t;
-            const float r = y1[e] * ci[e] - y1[e + 1] * si[e];
-            y1[e + 1] = y1[e + 1] * ci[e] + y1[e] * si[e];
-            y1[e] = r;
+        for (int e = 0; e < VEC; ++e) {
+          y0[e] = f[e] * wc0[e];
+          y1[e] = two ? g[e] * wc1[e] : 0.f;
+        }
+        if constexpr (VEC > 1) {
+          if (near0) {
+#pragma unroll
+            for (int e = 0; e < VEC; e += 2) {
+              y0[e] -= f[e + 1] * ws0[e + 1];
+              y0[e + 1] += f[e] * ws0[e];
+            }
+          }
+          if (near1) {
+#pragma unroll
+            for (int e = 0; e < VEC; e += 2) {
+              y1[e] -= g[e + 1] * ws1[e + 1];
+              y1[e + 1] += g[e] * ws1[e];
+            }
           }
         }
       }
-      if (bad) {
+      Chunk<T, VEC> o;
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) y0[e] = y1[e] = 0.f;
+      for (int e = 0; e < VEC; ++e) o.v[e] = T(bad ? 0.f : y0[e] * scale[u]);
+      *reinterpret_cast<Chunk<T, VEC>*>(yr + u * p.D + d0) = o;
+      if (two) {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) o.v[e] = T(bad ? 0.f : y1[e] * scale[u]);
+        *reinterpret_cast<Chunk<T, VEC>*>(yr + u * p.D + d1) = o;
       }
-      store_chunk<T, VEC>(yr + u * p.D + d0, y0);
-      if (c1[i] >= 0) store_chunk<T, VEC>(yr + u * p.D + d1, y1);
     }
   }
 }
 
 template <typename T, int VEC, int PAIRS, int U>
-void launch(NormParams p, cudaStream_t st) {
+void launch(NormParams p, int64_t rows, cudaStream_t st) {
   const int pairs = (p.D / VEC + 1) / 2;
-  int lanes = 1;
-  while (lanes * PAIRS < pairs) lanes *= 2;
-  p.q_blocks = (p.q_heads + U - 1) / U;
-  p.blocks = p.q_blocks + (p.k_heads + U - 1) / U;
-  const int64_t threads = p.rows * p.blocks * lanes;
-  const int64_t grid = (threads + 255) / 256;
-  check_that(grid < (int64_t(1) << 31), "kh_qk_norm_rope", "rows * heads too large");
-  qk_norm_rope_kernel<T, VEC, PAIRS, U><<<unsigned(grid), 256, 0, st>>>(p, lanes);
+  int log2 = 0;
+  while ((PAIRS << log2) < pairs) ++log2;
+  p.q_blocks = uint32_t((p.q_heads + U - 1) / U);
+  p.blocks = p.q_blocks + uint32_t((p.k_heads + U - 1) / U);
+  // 32-bit thread indexes: launches of as many whole rows as stay below 2^31 threads
+  const int64_t most = ((int64_t(1) << 31) - 256) / (int64_t(p.blocks) << log2);
+  for (int64_t r = 0; r < rows; r += most) {
+    const int64_t n = std::min(most, rows - r);
+    NormParams q = p;
+    q.groups = uint32_t(n * p.blocks);
+    q.x = static_cast<const T*>(p.x) + r * p.x_stride;
+    q.out = static_cast<T*>(p.out) + r * p.out_stride;
+    if (p.R) q.positions = p.positions + r;
+    const int64_t threads = (int64_t(q.groups) << log2);
+    qk_norm_rope_kernel<T, VEC, PAIRS, U><<<unsigned((threads + 255) / 256), 256, 0, st>>>(q, log2);
+  }
   KH_CUDA(cudaGetLastError());
 }
 
-// Whether chunks of `vec` values fit the head, its rotation and every row's alignment.
+// Whether chunks of `vec` values fit the head, its rotation and the alignment of rows, angles, weights.
 bool fits(const kh_qk_norm_rope_args& a, int size, int vec) {
   const uintptr_t bytes = uintptr_t(vec) * size;
-  return a.head_dim % vec == 0 && (a.interleaved || (a.rotary_dim / 2) % vec == 0) &&
-         reinterpret_cast<uintptr_t>(a.x) % bytes == 0 && reinterpret_cast<uintptr_t>(a.out) % bytes == 0 &&
-         a.x_stride % vec == 0 && a.out_stride % vec == 0;
+  auto at = [](const void* p, uintptr_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; };
+  return a.head_dim % vec == 0 && (a.interleaved ? a.rotary_dim : a.rotary_dim / 2) % vec == 0 && at(a.x, bytes) &&
+         at(a.out, bytes) && a.x_stride % vec == 0 && a.out_stride % vec == 0 && at(a.q_weight, 16) &&
+         at(a.k_weight, 16) && (a.rotary_dim == 0 || at(a.cossin, 16)) && a.rotary_dim % 4 == 0;
 }
 
 }  // namespace
@@ -268,7 +309,6 @@ void qk_norm_rope(const kh_qk_norm_rope_args* args, cudaStream_t st) {
   NormParams p{};
   p.x = a.x;
   p.out = a.out;
-  p.rows = a.rows;
   p.x_stride = a.x_stride;
   p.out_stride = a.out_stride;
   p.table_rows = a.table_rows;
@@ -284,12 +324,12 @@ void qk_norm_rope(const kh_qk_norm_rope_args* args, cudaStream_t st) {
   p.inv_d = 1.f / float(a.head_dim);
   p.interleaved = a.interleaved != 0;
   if (a.dtype == KH_F16) {
-    if (fits(a, 2, 8)) launch<__half, 8, 1, 2>(p, st);
-    else if (fits(a, 2, 4)) launch<__half, 4, 1, 2>(p, st);
-    else launch<__half, 1, 4, 1>(p, st);
+    if (fits(a, 2, 8)) launch<__half, 8, 1, 4>(p, a.rows, st);
+    else if (fits(a, 2, 4)) launch<__half, 4, 1, 4>(p, a.rows, st);
+    else launch<__half, 1, 4, 1>(p, a.rows, st);
   } else {
-    if (fits(a, 4, 4)) launch<float, 4, 1, 2>(p, st);
-    else launch<float, 1, 4, 1>(p, st);
+    if (fits(a, 4, 4)) launch<float, 4, 1, 4>(p, a.rows, st);
+    else launch<float, 1, 4, 1>(p, a.rows, st);
   }
 }
 

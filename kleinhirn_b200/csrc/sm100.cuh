@@ -195,6 +195,18 @@ __device__ __forceinline__ uint64_t desc_sw128(const void* smem) {
   return ((addr >> 4) & 0x3FFFull) | (1ull << 16) | (64ull << 32) | (1ull << 46) | (2ull << 61);
 }
 
+// True in one lane of a converged warp. An MMA warp runs its loop with all lanes (so that descriptors and
+// addresses stay warp-uniform values) and issues from this one.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(r));
+  return r != 0;
+}
+
 // kind::f16 instruction descriptor: f16 A and B, K-major both, f32 accumulator, M x N.
 __host__ __device__ constexpr uint32_t idesc_f16(int M, int N) {
   return (1u << 4) | (uint32_t(N >> 3) << 17) | (uint32_t(M >> 4) << 24);
