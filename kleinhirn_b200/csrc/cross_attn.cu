@@ -468,7 +468,7 @@ __global__ void __launch_bounds__(TTHREADS, 1)
       const uint32_t idesc_o = idesc_f16(128, D) | (1u << 16);  // V MN-major
       const bool lead = elect_one();
       auto wwait = [&](uint64_t* bar, uint32_t parity, int code) -> bool {
-        return __all_sync(0xffffffffu, !*abort_flag && mbar_wait(bar, parity, code));
+        return __all_sync(0xffffffffu, mbar_wait(bar, parity, code));
       };
       auto tile_of = [&](int g, int it) { return pair ? it : 2 * it + g; };
       auto issue_s = [&](int g, int it) -> bool {

@@ -55,13 +55,16 @@ __device__ __forceinline__ int adapter_of(const LoraParams& p, int seg) {
   atomicCAS(&kh_tc_error, 0, OP_BAD_INDEX);
   return -1;
 }
-// First segment that ends behind row r (n_segs if none), found by a whole warp, 32 probes a round.
+// First segment that ends behind row r (n_segs if none), found by a whole warp, 32 probes a round; with
+// one row to a segment (a step of single tokens) it is segment r, which the first round looks at too.
 __device__ __forceinline__ int first_seg(const LoraParams& p, int r) {
   const int lane = threadIdx.x & 31;
+  const int guess = min(r, p.n_segs - 1), g0 = seg_start(p, guess), g1 = seg_start(p, guess + 1);
   int lo = 0, hi = p.n_segs;
   while (lo < hi) {
     const int step = (hi - lo + 31) / 32, i = lo + lane * step;
     const uint32_t ended = __ballot_sync(0xffffffffu, i < hi && seg_start(p, i + 1) <= r);
+    if (g0 <= r && r < g1) return guess;
     const int c = ended == 0xffffffffu ? 32 : __ffs(~ended) - 1;  // probes before the first that has not
     if (c == 0) return lo;
     hi = min(hi, lo + c * step);
@@ -279,10 +282,13 @@ __global__ void __launch_bounds__(256) lora_rows_kernel(const LoraParams p, int 
 //
 // One cluster of Z CTAs per 128 rows, the CTAs splitting the sum (launches of few tiles). A K block of
 // 64: one tile of x, then for every adapter of the tile's rows its block of A (rank rows) and the
-// products, whose lanes of other rows are off, into one accumulator of 128 x rank. 192 threads:
-// warp 0 TMA, warp 1 MMA, warps 2-5 the scaled f16 rows.
+// products, whose lanes of other rows are off, into one accumulator of 128 x rank. 224 threads:
+// warp 0 loads x (TMA), warp 1 issues the products, warps 2-5 write the scaled f16 rows, warp 6 finds
+// the adapters of the rows, while x loads, and then loads A. (One warp for both loads was the bound: a
+// stage costs its issuing thread some 500 cycles.)
 
 constexpr int SXS = 4;  // x stages
+constexpr int SAS = 8;  // A stages, at most
 struct ShrinkPieces {
   int count;
   int id[128];
@@ -297,12 +303,12 @@ __device__ __forceinline__ uint32_t lanes_on(int lo, int hi, int word) {
   return ub & ~ua;
 }
 
-__global__ void __launch_bounds__(192) lora_shrink_tile_kernel(const __grid_constant__ CUtensorMap tmx,
+__global__ void __launch_bounds__(224) lora_shrink_tile_kernel(const __grid_constant__ CUtensorMap tmx,
                                                                const __grid_constant__ CUtensorMap tma,
                                                                const LoraParams p, int Z, int astages) {
   extern __shared__ uint8_t smem_raw[];
   __shared__ ShrinkPieces pieces;
-  __shared__ uint64_t bars[2 * SXS + 16 + 2];
+  __shared__ uint64_t bars[2 * SXS + 2 * SAS + 3];
   __shared__ uint32_t tmem_holder;
   __shared__ volatile int abort_flag;
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -310,15 +316,63 @@ __global__ void __launch_bounds__(192) lora_shrink_tile_kernel(const __grid_cons
   const int a_bytes = R16 * 128;
   uint8_t* sX = smem;
   uint8_t* sA = smem + SXS * 16384;
-  uint64_t *x_full = bars, *x_empty = bars + SXS, *a_full = bars + 2 * SXS, *a_empty = a_full + 8, *done = a_empty + 8,
-           *drain = done + 1;
+  uint64_t *x_full = bars, *x_empty = x_full + SXS, *a_full = x_empty + SXS, *a_empty = a_full + SAS,
+           *done = a_empty + SAS, *drain = done + 1, *listed = drain + 1;
   launch_dependents();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int z = blockIdx.x % Z, r0 = int(blockIdx.x / Z) * 128;
   const uint32_t cols = R16 <= 32 ? 32u : R16 <= 64 ? 64u : 128u;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < SXS; ++i) {
+      mbar_init(&x_full[i], 1);
+      mbar_init(&x_empty[i], 1);
+    }
+    for (int i = 0; i < SAS; ++i) {
+      mbar_init(&a_full[i], 1);
+      mbar_init(&a_empty[i], 1);
+    }
+    mbar_init(done, 1);
+    mbar_init(drain, 1);
+    mbar_init(listed, 32);
+    abort_flag = 0;
+    fence_barrier_init();
+  }
+  if (warp == 1) tmem_alloc(&tmem_holder, cols);
+  fence_before_sync();
+  __syncthreads();
+  fence_after_sync();
+  const uint32_t tmem = tmem_holder;
+  const int nk_all = (p.k + 63) / 64, kps = (nk_all + Z - 1) / Z;
+  const int kb0 = min(z * kps, nk_all), nk = min(kps, nk_all - kb0);
+  auto wwait = [&](uint64_t* bar, uint32_t parity, int code) -> bool {
+    return __all_sync(0xffffffffu, mbar_wait(bar, parity, code));
+  };
+
   if (warp == 0) {
-    const int last = seg_start(p, p.n_segs);  // rows from here on are not written
+    bool ok = true;
+    int xs = 0, issued = 0;
+    uint32_t u = 0;
+    for (int kb = 0; kb < nk; ++kb) {
+      // past the first round it is known whether any row has an adapter (if none, x was loaded in vain)
+      if (kb == SXS && (!wwait(listed, 0, 200) || pieces.count == 0)) break;
+      if (!wwait(&x_empty[xs], u ^ 1, 201)) { ok = false; break; }
+      if (lane == 0) {
+        mbar_arrive_expect_tx(&x_full[xs], 16384);
+        tma_load_2d(sX + xs * 16384, &tmx, &x_full[xs], (kb0 + kb) * 64, r0);
+      }
+      __syncwarp();
+      ++issued;
+      if (++xs == SXS) {
+        xs = 0;
+        u ^= 1;
+      }
+    }
+    // every copy lands before the CTA ends, also where no product waits for it
+    for (int kb = max(issued - SXS, 0); kb < issued; ++kb) mbar_wait(&x_full[kb % SXS], uint32_t(kb / SXS) & 1, 203);
+    if (!ok) abort_flag = 1;
+  } else if (warp == 6) {
     // the adapters of these rows: non-empty runs of rows, in order
+    const int last = seg_start(p, p.n_segs);  // rows from here on are not written
     int n = 0;
     for (int r = lane; r < 128; r += 32) pieces.row_id[r] = -1;
     __syncwarp();
@@ -346,80 +400,48 @@ __global__ void __launch_bounds__(192) lora_shrink_tile_kernel(const __grid_cons
       n += __popc(have);
       if (!__all_sync(0xffffffffu, more)) break;
     }
-    if (lane == 0) {
-      pieces.count = min(n, 128);
-      for (int i = 0; i < SXS; ++i) {
-        mbar_init(&x_full[i], 1);
-        mbar_init(&x_empty[i], 1);
-      }
-      for (int i = 0; i < 8; ++i) {
-        mbar_init(&a_full[i], 1);
-        mbar_init(&a_empty[i], 1);
-      }
-      mbar_init(done, 1);
-      mbar_init(drain, 1);
-      abort_flag = 0;
-      fence_barrier_init();
-      prefetch_tmap(&tmx);
-      prefetch_tmap(&tma);
-    }
-  }
-  if (warp == 1) tmem_alloc(&tmem_holder, cols);
-  fence_before_sync();
-  __syncthreads();
-  fence_after_sync();
-  const uint32_t tmem = tmem_holder;
-  const int np = pieces.count;
-  const int nk_all = (p.k + 63) / 64, kps = (nk_all + Z - 1) / Z;
-  const int kb0 = min(z * kps, nk_all), nk = np ? min(kps, nk_all - kb0) : 0;
-
-  if (warp == 0) {
-    if (lane == 0) {
-      bool ok = true;
-      uint32_t pend_x = 0, pend_a = 0;  // two bits a stage: issued, parity
-      int ai = 0;
-      for (int kb = 0; kb < nk && ok; ++kb) {
-        const int xs = kb % SXS;
-        const uint32_t u = uint32_t(kb / SXS) & 1;
-        if (abort_flag || !mbar_wait(&x_empty[xs], u ^ 1, 201)) { ok = false; break; }
-        mbar_arrive_expect_tx(&x_full[xs], 16384);
-        tma_load_2d(sX + xs * 16384, &tmx, &x_full[xs], (kb0 + kb) * 64, r0);
-        pend_x = (pend_x & ~(3u << (2 * xs))) | ((2u | u) << (2 * xs));
-        for (int i = 0; i < np; ++i, ++ai) {
-          const int as = ai % astages;
-          const uint32_t v = uint32_t(ai / astages) & 1;
-          if (abort_flag || !mbar_wait(&a_empty[as], v ^ 1, 202)) { ok = false; break; }
+    const int np = min(n, 128);
+    if (lane == 0) pieces.count = np;
+    __syncwarp();
+    mbar_arrive(listed);
+    bool ok = true;
+    int as = 0;
+    uint32_t v = 0, pend = 0;  // pend: two bits a stage: issued, parity
+    for (int kb = 0; kb < nk && ok; ++kb)
+      for (int i = 0; i < np; ++i) {
+        if (!wwait(&a_empty[as], v ^ 1, 202)) { ok = false; break; }
+        if (lane == 0) {
           mbar_arrive_expect_tx(&a_full[as], a_bytes);
           tma_load_2d(sA + as * a_bytes, &tma, &a_full[as], (kb0 + kb) * 64, pieces.id[i] * p.rank);
-          pend_a = (pend_a & ~(3u << (2 * as))) | ((2u | v) << (2 * as));
+        }
+        __syncwarp();
+        pend = (pend & ~(3u << (2 * as))) | ((2u | v) << (2 * as));
+        if (++as == astages) {
+          as = 0;
+          v ^= 1;
         }
       }
-      if (!ok) {
-        abort_flag = 1;
-        for (int i = 0; i < SXS; ++i)
-          if ((pend_x >> (2 * i)) & 2u) mbar_wait(&x_full[i], (pend_x >> (2 * i)) & 1u, 203);
-        for (int i = 0; i < astages; ++i)
-          if ((pend_a >> (2 * i)) & 2u) mbar_wait(&a_full[i], (pend_a >> (2 * i)) & 1u, 204);
-      }
+    if (!ok) {
+      abort_flag = 1;
+      for (int i = 0; i < astages; ++i)
+        if ((pend >> (2 * i)) & 2u) mbar_wait(&a_full[i], (pend >> (2 * i)) & 1u, 204);
     }
   } else if (warp == 1) {
     // all lanes in step, one issues
     const uint32_t idesc = idesc_f16(128, R16);
     const bool lead = elect_one();
-    bool ok = true;
-    auto wwait = [&](uint64_t* bar, uint32_t parity, int code) -> bool {
-      return __all_sync(0xffffffffu, !abort_flag && mbar_wait(bar, parity, code));
-    };
+    bool ok = wwait(listed, 0, 209);
+    const int np = ok ? pieces.count : 0;
     int as = 0;
     uint32_t av = 0;
-    for (int kb = 0; kb < nk && ok; ++kb) {
+    for (int kb = 0; kb < nk && np && ok; ++kb) {
       const int xs = kb % SXS;
       if (!wwait(&x_full[xs], uint32_t(kb / SXS) & 1, 205)) { ok = false; break; }
       const uint64_t dx = desc_sw128(sX + xs * 16384);
       for (int i = 0; i < np; ++i) {
+        const uint4 o = pieces.off[i];
         if (!wwait(&a_full[as], av, 206)) { ok = false; break; }
         fence_after_sync();
-        const uint4 o = pieces.off[i];
         const uint64_t da = desc_sw128(sA + as * a_bytes);
         if (lead) {
           const uint32_t off[4] = {o.x, o.y, o.z, o.w};
@@ -447,10 +469,11 @@ __global__ void __launch_bounds__(192) lora_shrink_tile_kernel(const __grid_cons
     __syncwarp();
   } else {
     const int quarter = warp & 3, r = quarter * 32 + lane, t = r0 + r;
-    const int ad = pieces.row_id[r];
-    const float s = pieces.row_scale[r];  // (read where ad >= 0 only)
-    const bool ok = __all_sync(0xffffffffu, mbar_wait(done, 0, 208)) && !abort_flag;
+    const bool ok = wwait(listed, 0, 210) && wwait(done, 0, 208) && !abort_flag;
     fence_after_sync();
+    const int ad = ok ? pieces.row_id[r] : -1;
+    const float s = pieces.row_scale[r];  // (used where ad >= 0)
+    const bool any = nk > 0 && pieces.count > 0;  // else the accumulator was never written
     const uint32_t taddr = tmem + (uint32_t(quarter * 32) << 16);
     float* part = reinterpret_cast<float*>(smem) + r * (R16 + 4);  // split sums, over the stages (all read)
 #pragma unroll 1
@@ -464,9 +487,9 @@ __global__ void __launch_bounds__(192) lora_shrink_tile_kernel(const __grid_cons
 #pragma unroll
         for (int i = 0; i < 8; i += 4)
           *reinterpret_cast<float4*>(part + c + i) =
-              nk > 0 ? make_float4(__uint_as_float(v[i]), __uint_as_float(v[i + 1]), __uint_as_float(v[i + 2]), __uint_as_float(v[i + 3]))
-                     : make_float4(0.f, 0.f, 0.f, 0.f);
-      } else if (ok && ad >= 0 && c < p.rank) {
+              any ? make_float4(__uint_as_float(v[i]), __uint_as_float(v[i + 1]), __uint_as_float(v[i + 2]), __uint_as_float(v[i + 3]))
+                  : make_float4(0.f, 0.f, 0.f, 0.f);
+      } else if (ad >= 0 && c < p.rank) {
         *reinterpret_cast<uint4*>(p.h + int64_t(t) * p.rank + c) =
             make_uint4(pack_half2(__uint_as_float(v[0]) * s, __uint_as_float(v[1]) * s),
                        pack_half2(__uint_as_float(v[2]) * s, __uint_as_float(v[3]) * s),
@@ -482,7 +505,7 @@ __global__ void __launch_bounds__(192) lora_shrink_tile_kernel(const __grid_cons
     // CTA z adds up rows [z per, (z + 1) per), a thread 4 of a row's values
     const int per = 128 / Z, quads = p.rank / 4;
     const float* base = reinterpret_cast<const float*>(smem);
-    for (int e = threadIdx.x; e < per * quads; e += 192) {
+    for (int e = threadIdx.x; e < per * quads; e += 224) {
       const int r = z * per + e / quads, c = e % quads * 4;
       if (pieces.row_id[r] < 0 || abort_flag) continue;
       const float s = pieces.row_scale[r];
@@ -507,10 +530,11 @@ __global__ void __launch_bounds__(192) lora_shrink_tile_kernel(const __grid_cons
 // BN / 2 rows of W per K block of 64), persistent over the tiles, two accumulators in TMEM so that the
 // epilogue runs under the next tile's products. Behind a tile's K blocks come, in the same ring of
 // stages, the adapters of its rows: the tile's rows of h against the adapter's rows of B, products of
-// ceil(rank / 16) steps whose lanes of other rows are off. The producer warp finds the runs of rows
-// while the K blocks load and hands each one's row range to the MMA thread beside its stage.
+// ceil(rank / 16) steps whose lanes of other rows are off.
 //   warp 0 TMA; warp 1 MMA (first CTA); then a warpgroup per 64 columns: bias, f16, staged and stored by
-//   TMA (tiles with rows that are not to be written: straight from registers).
+//   TMA (tiles with rows that are not to be written: straight from registers); the last warp finds the
+//   adapters of the tiles ahead, in lists of up to 16 runs of rows (found by the TMA warp itself, the
+//   dependent loads of the search held up the K blocks: 7 % on 65,536 rows of 768 -> 2,304).
 
 constexpr int BM = 128;
 constexpr int BK = 64;
@@ -523,10 +547,10 @@ struct PCfg {
   static constexpr int B_BYTES = BH * BK * 2;
   static constexpr int STAGE_BYTES = A_BYTES + B_BYTES;
   static constexpr int NWG = BN / 64;
-  static constexpr int THREADS = 64 + 128 * NWG;
+  static constexpr int THREADS = 64 + 128 * NWG + 32;
   static constexpr int STAGES = BN == 256 ? 5 : 6;
   static constexpr uint32_t TMEM_COLS = 2 * BN;
-  static constexpr int SMEM = STAGES * STAGE_BYTES + NWG * OUT_BYTES + 1024 + 512;
+  static constexpr int SMEM = STAGES * STAGE_BYTES + NWG * OUT_BYTES + 1024 + 512 + 1280;
 };
 
 // What a stage holds for the MMA warp: the lanes an adapter's product leaves alone, its steps of 16,
@@ -534,6 +558,13 @@ struct PCfg {
 struct StageNote {
   uint4 off[2];
   int steps, last, pad[2];
+};
+
+// Runs of rows of a tile: the adapter and the lanes of other rows; more: the tile has another list.
+struct RunList {
+  int count, more, pad[2];
+  int id[16];
+  uint32_t off[16][8];
 };
 
 template <int BN>
@@ -554,8 +585,11 @@ __global__ void __launch_bounds__(PCfg<BN>::THREADS, 1)
   uint64_t* tfull = empty + STAGES;
   uint64_t* tempty = tfull + 2;
   uint64_t* drain = tempty + 2;
-  StageNote* notes = reinterpret_cast<StageNote*>(drain + 2);  // [STAGES], 16-byte aligned
-  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(notes + STAGES);
+  uint64_t* list_full = drain + 2;  // [2]
+  uint64_t* list_empty = list_full + 2;
+  StageNote* notes = reinterpret_cast<StageNote*>(list_empty + 2);  // [STAGES], 16-byte aligned
+  RunList* lists = reinterpret_cast<RunList*>(notes + STAGES);      // [2]
+  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(lists + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_holder + 1);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -578,6 +612,10 @@ __global__ void __launch_bounds__(PCfg<BN>::THREADS, 1)
       mbar_init(&tempty[b], 2 * 4 * NWG);  // one arrival per epilogue warp of both CTAs
     }
     mbar_init(drain, 1);
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(&list_full[b], 1);
+      mbar_init(&list_empty[b], 1);
+    }
     *abort_flag = 0;
     fence_barrier_init();
     prefetch_tmap(&tmX);
@@ -595,10 +633,11 @@ __global__ void __launch_bounds__(PCfg<BN>::THREADS, 1)
     uint32_t phase = 0;
     uint32_t issued = 0, last_parity = 0;
     bool ok = true, waited = false;
-    // one stage: x and W (K block kb, id < 0) or h and B (columns 64 kb of adapter id for rows [lo, hi))
-    auto emit = [&](int mb, int nb, int kb, int id, int lo, int hi, int last) -> bool {
-      if (!__all_sync(0xffffffffu, !*abort_flag && mbar_wait(&empty[stage], phase ^ 1, 211))) return false;
-      if (id >= 0 && lane < 8) reinterpret_cast<uint32_t*>(notes[stage].off)[lane] = ~lanes_on(lo, hi, lane);
+    // one stage: x and W (K block kb, id < 0) or h and B (columns 64 kb of adapter id); lane w < 8 has
+    // word w of the lanes that are off
+    auto emit = [&](int mb, int nb, int kb, int id, uint32_t off, int last) -> bool {
+      if (!__all_sync(0xffffffffu, mbar_wait(&empty[stage], phase ^ 1, 211))) return false;
+      if (id >= 0 && lane < 8) reinterpret_cast<uint32_t*>(notes[stage].off)[lane] = off;
       __syncwarp();
       if (lane == 0) {
         if (first) {
@@ -622,42 +661,43 @@ __global__ void __launch_bounds__(PCfg<BN>::THREADS, 1)
       return true;
     };
     const int chunks = (p.rank + 63) / 64;
+    int list = 0;
+    uint32_t lphase = 0;
     for (int t = pair; t < tiles && ok; t += npairs) {
       const int mb = m_first + t / n_tiles, nb = t % n_tiles;
-      const int r0 = mb * 2 * BM, r1 = min(r0 + 2 * BM, end);
-      int s = p.n_adapters > 0 ? first_seg(p, r0) : p.n_segs;
-      // the last K block is held back until it is known whether runs follow it
-      for (int kb = 0; kb + 1 < nk && ok; ++kb) ok = emit(mb, nb, kb, -1, 0, 2 * BM, 0);
-      int held_kb = nk - 1, held_id = -1, held_lo = 0, held_hi = 2 * BM;
-      for (bool more = true; more && s < p.n_segs && ok; s += 32) {
-        const int i = s + lane;
-        int lo = 0, hi = 0, id = -1;
-        bool in = i < p.n_segs;
-        if (in) {
-          lo = max(seg_start(p, i), r0) - r0;
-          hi = min(seg_start(p, i + 1), r1) - r0;
-          in = r0 + lo < r1;
-          if (lo < hi) id = adapter_of(p, i);
+      for (int kb = 0; kb + 1 < nk && ok; ++kb) ok = emit(mb, nb, kb, -1, 0u, 0);
+      // a stage is held back until it is known whether another follows it
+      int held_kb = nk - 1, held_id = -1;
+      uint32_t held_off = 0;
+      for (bool more = p.n_adapters > 0; more && ok;) {
+        if (!__all_sync(0xffffffffu, mbar_wait(&list_full[list], lphase, 216))) {
+          ok = false;
+          break;
         }
-        more = __all_sync(0xffffffffu, in);
-        for (uint32_t have = __ballot_sync(0xffffffffu, id >= 0); have && ok; have &= have - 1) {
-          const int src = __ffs(have) - 1;
-          if (!waited) {
-            wait_primary();  // h is complete
-            waited = true;
-          }
-          const int pid = __shfl_sync(0xffffffffu, id, src);
-          const int plo = __shfl_sync(0xffffffffu, lo, src), phi = __shfl_sync(0xffffffffu, hi, src);
+        const int count = lists[list].count;
+        more = lists[list].more != 0;
+        if (count > 0 && !waited) {
+          wait_primary();  // h is complete
+          waited = true;
+        }
+        for (int i = 0; i < count && ok; ++i) {
+          const int id = lists[list].id[i];
+          const uint32_t off = lists[list].off[i][lane & 7];
           for (int c = 0; c < chunks && ok; ++c) {
-            ok = emit(mb, nb, held_kb, held_id, held_lo, held_hi, 0);
+            ok = emit(mb, nb, held_kb, held_id, held_off, 0);
             held_kb = c;
-            held_id = pid;
-            held_lo = plo;
-            held_hi = phi;
+            held_id = id;
+            held_off = off;
           }
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&list_empty[list]);
+        if (++list == 2) {
+          list = 0;
+          lphase ^= 1;
         }
       }
-      if (ok) ok = emit(mb, nb, held_kb, held_id, held_lo, held_hi, 1);
+      if (ok) ok = emit(mb, nb, held_kb, held_id, held_off, 1);
     }
     if (!ok && lane == 0) {
       *abort_flag = 1;
@@ -672,7 +712,7 @@ __global__ void __launch_bounds__(PCfg<BN>::THREADS, 1)
       const uint32_t idesc = idesc_f16(2 * BM, BN);
       const bool lead = elect_one();
       auto wwait = [&](uint64_t* bar, uint32_t parity, int code) -> bool {
-        return __all_sync(0xffffffffu, !*abort_flag && mbar_wait(bar, parity, code));
+        return __all_sync(0xffffffffu, mbar_wait(bar, parity, code));
       };
       int stage = 0;
       uint32_t phase = 0;
@@ -731,6 +771,49 @@ __global__ void __launch_bounds__(PCfg<BN>::THREADS, 1)
         __syncwarp();
         mbar_wait(drain, 0, 222);
       }
+    }
+  } else if (warp == 2 + 4 * NWG) {
+    if (p.n_adapters > 0) {
+      int list = 0;
+      uint32_t lphase = 0;
+      bool ok = true;
+      for (int t = pair; t < tiles && ok; t += npairs) {
+        const int r0 = (m_first + t / n_tiles) * 2 * BM, r1 = min(r0 + 2 * BM, end);
+        int s = first_seg(p, r0);
+        for (bool more = true; more && ok; s += 16) {
+          const int i = s + lane;  // lanes 0-15 take a segment each
+          int lo = 0, hi = 0, id = -1;
+          bool in = lane < 16 && i < p.n_segs;
+          if (in) {
+            lo = max(seg_start(p, i), r0) - r0;
+            hi = min(seg_start(p, i + 1), r1) - r0;
+            in = r0 + lo < r1;
+            if (lo < hi) id = adapter_of(p, i);
+          }
+          more = (__ballot_sync(0xffffffffu, in) & 0xffffu) == 0xffffu;
+          const uint32_t have = __ballot_sync(0xffffffffu, id >= 0);
+          if (have == 0 && more) continue;  // (empty segments)
+          ok = __all_sync(0xffffffffu, mbar_wait(&list_empty[list], lphase ^ 1, 215));
+          if (!ok) break;
+          if (id >= 0) {
+            const int at = __popc(have & ((1u << lane) - 1u));
+            lists[list].id[at] = id;
+#pragma unroll
+            for (int w = 0; w < 8; ++w) lists[list].off[at][w] = ~lanes_on(lo, hi, w);
+          }
+          if (lane == 0) {
+            lists[list].count = __popc(have);
+            lists[list].more = more;
+          }
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&list_full[list]);
+          if (++list == 2) {
+            list = 0;
+            lphase ^= 1;
+          }
+        }
+      }
+      if (!ok) *abort_flag = 1;
     }
   } else {
     const int q = warp & 3;
@@ -941,7 +1024,7 @@ void lora_matmul(const kh_lora_matmul_args* args, cudaStream_t st) {
       lora_shrink_rows_kernel<<<unsigned(a.rows), 256, 0, st>>>(p);
       KH_CUDA(cudaGetLastError());
     } else {
-      const int R16 = (a.rank + 15) / 16 * 16, astages = R16 <= 32 ? 8 : 4;
+      const int R16 = (a.rank + 15) / 16 * 16, astages = R16 <= 32 ? SAS : 4;
       const size_t smem = size_t(SXS) * 16384 + size_t(astages) * R16 * 128 + 1024;
       static std::atomic<uint64_t> configured{0};
       once_per_device(configured, [] {
@@ -954,7 +1037,7 @@ void lora_matmul(const kh_lora_matmul_args* args, cudaStream_t st) {
       const int64_t tiles = (a.rows + 127) / 128;
       int Z = 1;  // CTAs that split a tile's sum: while SMs are idle, at least two K blocks each
       while (Z < 8 && 2 * Z * tiles <= SMS && 4 * Z <= (a.k + 63) / 64) Z *= 2;
-      launch_ex(lora_shrink_tile_kernel, dim3(unsigned(Z * tiles)), 192, smem, Z, false, st, tx, ta, p, Z, astages);
+      launch_ex(lora_shrink_tile_kernel, dim3(unsigned(Z * tiles)), 224, smem, Z, false, st, tx, ta, p, Z, astages);
     }
   }
   if (takes_rows(a)) {
