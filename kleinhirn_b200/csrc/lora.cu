@@ -6,8 +6,8 @@
 // second launch starts while the first runs (programmatic dependent launch) and waits for it where it
 // needs h, behind the projection's own products.
 //
-// Few rows (takes_rows): bound by reading W, A and B once; lora_shrink_rows_kernel and
-// lora_rows_kernel stream them through registers. Many rows: bound by the tensor cores;
+// Few rows (takes_few): bound by reading W, A and B once; lora_shrink_rows_kernel and
+// lora_few_kernel. Many rows: bound by the tensor cores;
 // lora_shrink_tile_kernel (HBM: reads x once) and lora_pair_kernel. A row tile that holds rows of
 // several adapters takes one more product per adapter, whose output lanes of other rows are switched
 // off in the instruction, so no operand is masked or copied.
@@ -88,9 +88,9 @@ __device__ __forceinline__ float dot8(uint4 a, uint4 b, float acc) {
   return acc;
 }
 
-// ---- few rows: h, one CTA of 8 warps per row, a warp two of the rank's dot products at a time ----
+// ---- few rows: h, one CTA of 16 warps per row, a warp one of the rank's dot products at a time ----
 
-__global__ void __launch_bounds__(256) lora_shrink_rows_kernel(const LoraParams p) {
+__global__ void __launch_bounds__(512) lora_shrink_rows_kernel(const LoraParams p) {
   launch_dependents();
   const int t = blockIdx.x, lane = threadIdx.x & 31;
   const int seg = first_seg(p, t);
@@ -100,41 +100,42 @@ __global__ void __launch_bounds__(256) lora_shrink_rows_kernel(const LoraParams 
   const uint4* x = reinterpret_cast<const uint4*>(p.x + t * p.x_stride);
   const float s = p.scales ? __ldg(p.scales + ad) : 1.f;
   const int chunks = p.k / 8;
-  for (int r = (threadIdx.x >> 5) * 2; r < p.rank; r += 16) {  // (the rank is even)
-    const uint4* a0 = reinterpret_cast<const uint4*>(p.a + (int64_t(ad) * p.rank + r) * p.k);
-    const uint4* a1 = a0 + chunks;
-    float d0 = 0.f, d1 = 0.f;
+  for (int r = threadIdx.x >> 5; r < p.rank; r += 16) {
+    const uint4* a = reinterpret_cast<const uint4*>(p.a + (int64_t(ad) * p.rank + r) * p.k);
+    float d = 0.f;
+    int i = lane;
+    for (; i + 7 * 32 < chunks; i += 8 * 32) {  // eight loads of each in flight
+      uint4 u[8], v[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        u[j] = __ldg(a + i + 32 * j);
+        v[j] = __ldg(x + i + 32 * j);
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) d = dot8(u[j], v[j], d);
+    }
 #pragma unroll 4
-    for (int i = lane; i < chunks; i += 32) {
-      const uint4 v = __ldg(x + i);
-      d0 = dot8(v, __ldg(a0 + i), d0);
-      d1 = dot8(v, __ldg(a1 + i), d1);
-    }
-    for (int o = 16; o; o >>= 1) {
-      d0 += __shfl_xor_sync(0xffffffffu, d0, o);
-      d1 += __shfl_xor_sync(0xffffffffu, d1, o);
-    }
-    if (lane == 0) *reinterpret_cast<uint32_t*>(p.h + int64_t(t) * p.rank + r) = pack_half2(d0 * s, d1 * s);
+    for (; i < chunks; i += 32) d = dot8(__ldg(a + i), __ldg(x + i), d);
+    for (int o = 16; o; o >>= 1) d += __shfl_xor_sync(0xffffffffu, d, o);
+    if (lane == 0) p.h[int64_t(t) * p.rank + r] = __float2half_rn(d * s);
   }
 }
 
 // ---- few rows: the projection ----
 //
-// out^T = W x^T in m16n8k16 products: a CTA owns 128 outputs of NB * 8 rows, 4 warps of 32 outputs by
-// 2 slices of the sum; a cluster of Z CTAs splits the sum further, so that W streams through all SMs,
-// and adds the parts over distributed shared memory in rank order. The order of the values within a
-// sum is free, so a thread loads 16 bytes of W and of x as they lie in memory (quad lane t the values
-// 8 t .. of 32). The adapter's part is a dot product of rank values per output at the end.
+// out^T = W x^T: the 128 rows of the MMA are outputs and its columns the (up to 128) rows of x, so that
+// few rows waste no tensor work and W streams once through a deep ring. A cluster of Z CTAs splits the
+// sum of 128 outputs, until about every SM takes part in reading W, and adds the parts over distributed
+// shared memory in rank order, each CTA for its share of the rows. The adapter's part is a dot product
+// of rank values per output there. Warp 0 TMA, warp 1 MMA, warps 2-9 the outputs (lane = output, two
+// warps to 32 of them), warp 10 finds the rows' adapters meanwhile.
+// FUSED: where all adapters' A together have at most 128 rows, they are a second operand tile of every
+// stage, h comes out of the same pass over x, and there is no launch before this one.
 
-constexpr int RN = 128;  // outputs of a CTA
+constexpr int FT = 128;      // rows of x, at most
+constexpr int FTHREADS = 352;
+constexpr int FSMEM = 200 * 1024;
 
-__device__ __forceinline__ void mma_16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
-                                          uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
 __device__ __forceinline__ float4 ld_cluster_f32x4(uint32_t addr) {
   float4 v;
   asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
@@ -143,139 +144,259 @@ __device__ __forceinline__ float4 ld_cluster_f32x4(uint32_t addr) {
                : "memory");
   return v;
 }
-
-template <int NB>
-struct RowsFrag {
-  uint4 w[2][2];  // [block of 16 outputs][row lane / 4, + 8]
-  uint4 x[NB];
-};
-
-template <int NB>
-__device__ __forceinline__ void rows_load(RowsFrag<NB>& f, const LoraParams& p, int n_first, int t_first, int t_end, int k) {
-  const int lane = threadIdx.x & 31, kk = k + (lane & 3) * 8;
-#pragma unroll
-  for (int mb = 0; mb < 2; ++mb)
-#pragma unroll
-    for (int hl = 0; hl < 2; ++hl) {
-      const int n = n_first + mb * 16 + hl * 8 + (lane >> 2);
-      f.w[mb][hl] = make_uint4(0, 0, 0, 0);
-      if (n < p.n && kk < p.k) f.w[mb][hl] = __ldg(reinterpret_cast<const uint4*>(p.w + int64_t(n) * p.k + kk));
-    }
-#pragma unroll
-  for (int nb = 0; nb < NB; ++nb) {
-    const int t = t_first + nb * 8 + (lane >> 2);
-    f.x[nb] = make_uint4(0, 0, 0, 0);
-    if (t < t_end && kk < p.k) f.x[nb] = __ldg(reinterpret_cast<const uint4*>(p.x + t * p.x_stride + kk));
-  }
+__device__ __forceinline__ float ld_cluster_f32(uint32_t addr) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+  return v;
 }
 
-template <int NB>
-__global__ void __launch_bounds__(256) lora_rows_kernel(const LoraParams p, int Z) {
-  __shared__ __align__(16) float part[NB * 8][RN + 4];
-  __shared__ int ids[NB * 8];
+// cols: rows of x rounded up to the MMA's steps of 16; a stage: 16 KB of W, FUSED 16 KB of A (of them
+// a_bytes loaded), cols * 128 bytes of x.
+template <bool FUSED>
+__global__ void __launch_bounds__(FTHREADS, 1)
+    lora_few_kernel(const __grid_constant__ CUtensorMap tmx, const __grid_constant__ CUtensorMap tmw,
+                    const __grid_constant__ CUtensorMap tma, const LoraParams p, int Z, int cols, int stages, int a_bytes) {
+  constexpr int X_OFF = FUSED ? 32768 : 16384;
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ uint64_t bars[2 * 12 + 2];
+  __shared__ uint32_t tmem_holder;
+  __shared__ volatile int abort_flag;
+  __shared__ int ids[FT];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int nw = warp & 3, kw = warp >> 2;
-  const int z = blockIdx.x % Z, n0 = blockIdx.x / Z * RN;
+  const int z = blockIdx.x % Z, n0 = int(blockIdx.x / Z) * 128;
   const int begin = seg_start(p, 0), end = seg_start(p, p.n_segs);
-  const int t0 = begin + blockIdx.y * NB * 8;
+  const int t0 = begin + int(blockIdx.y) * FT;
   if (t0 >= end) {  // (the whole cluster)
     wait_primary();
     return;
   }
-  const int nt = min(NB * 8, end - t0);
-
-  float acc[2][NB][4];
-#pragma unroll
-  for (int mb = 0; mb < 2; ++mb)
-#pragma unroll
-    for (int nb = 0; nb < NB; ++nb) acc[mb][nb][0] = acc[mb][nb][1] = acc[mb][nb][2] = acc[mb][nb][3] = 0.f;
-  const int stride = 2 * Z * 32;
-  RowsFrag<NB> cur, nxt;
-  int k = (z * 2 + kw) * 32;
-  if (k < p.k) rows_load<NB>(cur, p, n0 + nw * 32, t0, end, k);
-  // adapters of the CTA's rows, while these loads are under way
-  if (threadIdx.x < NB * 8) ids[threadIdx.x] = -1;
+  const int nt = min(FT, end - t0);
+  const int x_bytes = cols * 128, stage_bytes = X_OFF + x_bytes;
+  uint64_t *full = bars, *empty = bars + stages, *done = bars + 24, *drain = bars + 25;
+  const uint32_t tcols = (cols <= 32 ? 32u : cols <= 64 ? 64u : 128u) * (FUSED ? 2 : 1);
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < stages; ++i) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], 1);
+    }
+    mbar_init(done, 1);
+    mbar_init(drain, 1);
+    abort_flag = 0;
+    fence_barrier_init();
+  }
+  if (warp == 1) tmem_alloc(&tmem_holder, tcols);
+  fence_before_sync();
   __syncthreads();
-  if (p.n_adapters > 0) {
-    for (int s = first_seg(p, t0); s < p.n_segs; s += 256) {
-      const int i = s + threadIdx.x;
-      bool more = i < p.n_segs;
-      if (more) {
-        const int lo = max(seg_start(p, i), t0), hi = min(seg_start(p, i + 1), t0 + nt);
-        more = lo < t0 + nt;
-        if (lo < hi) {
-          const int ad = adapter_of(p, i);
-          for (int t = lo; t < hi; ++t) ids[t - t0] = ad;
+  fence_after_sync();
+  const uint32_t tmem = tmem_holder;
+  const int nk_all = (p.k + 63) / 64, kps = (nk_all + Z - 1) / Z;
+  const int kb0 = min(z * kps, nk_all), nk = min(kps, nk_all - kb0);
+  auto wwait = [&](uint64_t* bar, uint32_t parity, int code) -> bool {
+    return __all_sync(0xffffffffu, mbar_wait(bar, parity, code));
+  };
+
+  if (warp == 0) {
+    bool ok = true;
+    int st = 0;
+    uint32_t ph = 0, pend = 0;
+    for (int kb = 0; kb < nk; ++kb) {
+      if (!wwait(&empty[st], ph ^ 1, 231)) { ok = false; break; }
+      if (lane == 0) {
+        mbar_arrive_expect_tx(&full[st], uint32_t(16384 + x_bytes + (FUSED ? a_bytes : 0)));
+        tma_load_2d(smem + st * stage_bytes, &tmw, &full[st], (kb0 + kb) * 64, n0);
+        if (FUSED) tma_load_2d(smem + st * stage_bytes + 16384, &tma, &full[st], (kb0 + kb) * 64, 0);
+        tma_load_2d(smem + st * stage_bytes + X_OFF, &tmx, &full[st], (kb0 + kb) * 64, t0);
+      }
+      __syncwarp();
+      pend = (pend & ~(3u << (2 * st))) | ((2u | ph) << (2 * st));
+      if (++st == stages) {
+        st = 0;
+        ph ^= 1;
+      }
+    }
+    if (!ok) {
+      abort_flag = 1;
+      for (int i = 0; i < stages; ++i)
+        if ((pend >> (2 * i)) & 2u) mbar_wait(&full[i], (pend >> (2 * i)) & 1u, 232);
+    }
+  } else if (warp == 1) {
+    // all lanes in step, one issues
+    const uint32_t idesc = idesc_f16(128, cols);
+    const bool lead = elect_one();
+    bool ok = true;
+    int st = 0;
+    uint32_t ph = 0;
+    for (int kb = 0; kb < nk; ++kb) {
+      if (!wwait(&full[st], ph, 233)) { ok = false; break; }
+      fence_after_sync();
+      const uint64_t dw = desc_sw128(smem + st * stage_bytes), dx = desc_sw128(smem + st * stage_bytes + X_OFF);
+      if (lead) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) mma_f16(tmem, dw + uint64_t(2 * k), dx + uint64_t(2 * k), idesc, (kb | k) ? 1u : 0u);
+        if (FUSED) {  // (rows of the A tile past the adapters hold anything; so do their lanes)
+          const uint64_t da = desc_sw128(smem + st * stage_bytes + 16384);
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            mma_f16(tmem + tcols / 2, da + uint64_t(2 * k), dx + uint64_t(2 * k), idesc, (kb | k) ? 1u : 0u);
+        }
+        mma_commit(&empty[st]);
+      }
+      __syncwarp();
+      if (++st == stages) {
+        st = 0;
+        ph ^= 1;
+      }
+    }
+    if (!ok) {
+      abort_flag = 1;
+      if (lead) mma_commit(drain);
+      __syncwarp();
+      mbar_wait(drain, 0, 234);
+    }
+    if (lead) mma_commit(done);  // (after a failure too: nothing is stored then)
+    __syncwarp();
+  } else if (warp == 10) {
+    for (int t = lane; t < FT; t += 32) ids[t] = -1;
+    __syncwarp();
+    if (p.n_adapters > 0) {
+      for (int s = first_seg(p, t0); s < p.n_segs; s += 32) {
+        const int i = s + lane;
+        bool more = i < p.n_segs;
+        if (more) {
+          const int lo = max(seg_start(p, i), t0), hi = min(seg_start(p, i + 1), t0 + nt);
+          more = lo < t0 + nt;
+          if (lo < hi) {
+            const int ad = adapter_of(p, i);
+            for (int t = lo; t < hi; ++t) ids[t - t0] = ad;
+          }
+        }
+        if (!__all_sync(0xffffffffu, more)) break;
+      }
+    }
+    __syncwarp();
+    named_bar(1, 32 * 9);
+  } else {
+    // rows of B that this thread will need, towards L2 while W streams
+    named_bar(1, 32 * 9);
+    const int n = n0 + (warp & 3) * 32 + lane;
+    if (n < p.n)
+      for (int g = z * 2 + ((warp - 2) >> 2); g * 4 < nt; g += 2 * Z)
+        for (int j = 0; j < 4; ++j)
+          if (ids[g * 4 + j] >= 0 && (j == 0 || ids[g * 4 + j] != ids[g * 4 + j - 1]))
+            for (int r = 0; r < p.rank; r += 64) prefetch_l2(p.b + (int64_t(ids[g * 4 + j]) * p.n + n) * p.rank + r);
+    // the accumulator (lane = output, column = row of x) as part[row of x][output], over the stages,
+    // which all have been read
+    const int quarter = warp & 3, half = (warp - 2) >> 2;
+    const bool ok = wwait(done, 0, 235);
+    fence_after_sync();
+    float* part = reinterpret_cast<float*>(smem) + quarter * 32 + lane;
+    const uint32_t taddr = tmem + (uint32_t(quarter * 32) << 16);
+    if (!ok) abort_flag = 1;
+#pragma unroll 1
+    for (int c = 16 * half; c < cols; c += 32) {
+      uint32_t v[16];
+      tmem_ld16(taddr + uint32_t(c), v);
+      tmem_ld_wait();
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        asm volatile("" : "+r"(v[i]));
+        part[(c + i) * 128] = nk > 0 ? __uint_as_float(v[i]) : 0.f;
+      }
+      if (FUSED) {  // the adapters' lanes behind it
+        tmem_ld16(taddr + tcols / 2 + uint32_t(c), v);
+        tmem_ld_wait();
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          asm volatile("" : "+r"(v[i]));
+          part[(cols + c + i) * 128] = nk > 0 ? __uint_as_float(v[i]) : 0.f;
         }
       }
-      if (!__syncthreads_and(more)) break;
     }
   }
-  for (; k < p.k; k += stride) {
-    if (k + stride < p.k) rows_load<NB>(nxt, p, n0 + nw * 32, t0, end, k + stride);
+  fence_before_sync();
+  __syncthreads();
+  if (Z > 1) cluster_sync();
+  const float* part = reinterpret_cast<const float*>(smem);
+  const int chunks = p.rank / 8;
+  __half* hs = reinterpret_cast<__half*>(smem + size_t(FUSED ? 2 : 1) * cols * 512);  // FUSED: h, [row of x][rank]
+  if (FUSED) {
+    // h of this CTA's rows of x: the parts of the row's own adapter, scaled
+    for (int e = threadIdx.x; e < nt * p.rank; e += FTHREADS) {
+      const int i = e / p.rank, r = e - i * p.rank, ad = ids[i];
+      if (ad < 0 || (i / 8) % Z != z) continue;  // (groups z * 2 and z * 2 + 1 of four rows, and on by 2 Z)
+      const float* src = part + (cols + i) * 128 + ad * p.rank + r;
+      float d = 0.f;
+      if (Z == 1) {
+        d = *src;
+      } else {
+        float u[8];
 #pragma unroll
-    for (int nb = 0; nb < NB; ++nb)
+        for (int q = 0; q < 8; ++q) u[q] = q < Z ? ld_cluster_f32(cluster_addr(src, uint32_t(q))) : 0.f;
 #pragma unroll
-      for (int mb = 0; mb < 2; ++mb) {
-        const uint4 u = cur.w[mb][0], v = cur.w[mb][1], b = cur.x[nb];
-        mma_16816(acc[mb][nb], u.x, v.x, u.y, v.y, b.x, b.y);
-        mma_16816(acc[mb][nb], u.z, v.z, u.w, v.w, b.z, b.w);
+        for (int q = 0; q < 8; ++q) d += u[q];
       }
-    cur = nxt;
-  }
-  // the two slices of this CTA, then the cluster's parts
-  for (int turn = 1; turn >= 0; --turn) {
-    if (kw == turn) {
-#pragma unroll
-      for (int mb = 0; mb < 2; ++mb)
-#pragma unroll
-        for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            float& c = part[nb * 8 + (lane & 3) * 2 + (i & 1)][nw * 32 + mb * 16 + (lane >> 2) + 8 * (i >> 1)];
-            c = turn ? acc[mb][nb][i] : acc[mb][nb][i] + c;
-          }
+      hs[e] = __float2half_rn(d * (p.scales ? __ldg(p.scales + ad) : 1.f));
     }
     __syncthreads();
+  } else {
+    wait_primary();
   }
-  if (Z > 1) cluster_sync();
-  wait_primary();
-  // four outputs of a row per thread (n is a multiple of 8)
-  const int per = RN / Z / 4;
-  for (int e = threadIdx.x; e < nt * per; e += 256) {
-    const int i = e / per, c = z * (RN / Z) + e % per * 4, n = n0 + c, t = t0 + i;
-    if (n >= p.n) continue;
-    float v[4] = {};
-    if (Z == 1) {
+  if (warp >= 2 && warp < 10 && !abort_flag) {
+    const int c = (warp & 3) * 32 + lane, n = n0 + c, half = (warp - 2) >> 2;
+    const float bias = p.bias && n < p.n ? __half2float(p.bias[n]) : 0.f;
+    // groups of four rows of x, dealt to the cluster's CTAs and the two warps of these outputs
+    for (int g = z * 2 + half; g * 4 < nt; g += 2 * Z) {
+      float v[4];
+      int ad[4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) v[j] = part[i][c + j];
-    } else {
-      float4 u[8];
-#pragma unroll
-      for (int q = 0; q < 8; ++q) u[q] = q < Z ? ld_cluster_f32x4(cluster_addr(&part[i][c], uint32_t(q))) : make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-      for (int q = 0; q < 8; ++q) v[0] += u[q].x, v[1] += u[q].y, v[2] += u[q].z, v[3] += u[q].w;
-    }
-    if (p.bias) {
-      const uint2 u = __ldg(reinterpret_cast<const uint2*>(p.bias + n));
-      const float2 b0 = __half22float2(*reinterpret_cast<const __half2*>(&u.x)), b1 = __half22float2(*reinterpret_cast<const __half2*>(&u.y));
-      v[0] += b0.x, v[1] += b0.y, v[2] += b1.x, v[3] += b1.y;
-    }
-    const int ad = ids[i];
-    if (ad >= 0) {
-      const uint4* b = reinterpret_cast<const uint4*>(p.b + (int64_t(ad) * p.n + n) * p.rank);
-      const uint4* h = reinterpret_cast<const uint4*>(p.h + int64_t(t) * p.rank);
-      const int chunks = p.rank / 8;
-#pragma unroll 2
-      for (int r = 0; r < chunks; ++r) {
-        const uint4 hv = h[r];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) v[j] = dot8(hv, __ldg(b + j * chunks + r), v[j]);
+      for (int j = 0; j < 4; ++j) {
+        const int i = g * 4 + j;
+        v[j] = bias;
+        ad[j] = i < nt && n < p.n ? ids[i] : -1;
       }
+      if (Z == 1) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] += part[(g * 4 + j) * 128 + c];
+      } else {
+        float u[4][8];
+#pragma unroll
+        for (int q = 0; q < 8; ++q)
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            u[j][q] = q < Z ? ld_cluster_f32(cluster_addr(part + (g * 4 + j) * 128 + c, uint32_t(q))) : 0.f;
+#pragma unroll
+        for (int q = 0; q < 8; ++q)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) v[j] += u[j][q];
+      }
+      if (ad[0] >= 0 || ad[1] >= 0 || ad[2] >= 0 || ad[3] >= 0) {
+        const uint4* h = FUSED ? reinterpret_cast<const uint4*>(hs + g * 4 * p.rank)
+                               : reinterpret_cast<const uint4*>(p.h + int64_t(t0 + g * 4) * p.rank);
+        const bool same = ad[0] == ad[1] && ad[1] == ad[2] && ad[2] == ad[3];
+#pragma unroll 4
+        for (int r = 0; r < chunks; ++r) {
+          uint4 b[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            b[j] = j ? b[0] : make_uint4(0, 0, 0, 0);
+            if (ad[j] >= 0 && !(j && same)) b[j] = __ldg(reinterpret_cast<const uint4*>(p.b + (int64_t(ad[j]) * p.n + n) * p.rank) + r);
+          }
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if (ad[j] >= 0) v[j] = dot8(h[j * chunks + r], b[j], v[j]);
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (g * 4 + j < nt && n < p.n) p.out[(t0 + g * 4 + j) * p.out_stride + n] = __float2half_rn(v[j]);
     }
-    *reinterpret_cast<uint2*>(p.out + t * p.out_stride + n) = make_uint2(pack_half2(v[0], v[1]), pack_half2(v[2], v[3]));
   }
   if (Z > 1) cluster_sync();  // no CTA leaves while another reads its part
+  if (warp == 1) {
+    fence_after_sync();
+    tmem_free(tmem, tcols);
+  }
 }
 
 // ---- many rows: h on the tensor cores ----
@@ -305,7 +426,7 @@ __device__ __forceinline__ uint32_t lanes_on(int lo, int hi, int word) {
 
 __global__ void __launch_bounds__(224) lora_shrink_tile_kernel(const __grid_constant__ CUtensorMap tmx,
                                                                const __grid_constant__ CUtensorMap tma,
-                                                               const LoraParams p, int Z, int astages) {
+                                                               const LoraParams p, int Z, int xstages, int astages) {
   extern __shared__ uint8_t smem_raw[];
   __shared__ ShrinkPieces pieces;
   __shared__ uint64_t bars[2 * SXS + 2 * SAS + 3];
@@ -315,7 +436,7 @@ __global__ void __launch_bounds__(224) lora_shrink_tile_kernel(const __grid_cons
   const int R16 = (p.rank + 15) / 16 * 16;
   const int a_bytes = R16 * 128;
   uint8_t* sX = smem;
-  uint8_t* sA = smem + SXS * 16384;
+  uint8_t* sA = smem + xstages * 16384;
   uint64_t *x_full = bars, *x_empty = x_full + SXS, *a_full = x_empty + SXS, *a_empty = a_full + SAS,
            *done = a_empty + SAS, *drain = done + 1, *listed = drain + 1;
   launch_dependents();
@@ -354,7 +475,7 @@ __global__ void __launch_bounds__(224) lora_shrink_tile_kernel(const __grid_cons
     uint32_t u = 0;
     for (int kb = 0; kb < nk; ++kb) {
       // past the first round it is known whether any row has an adapter (if none, x was loaded in vain)
-      if (kb == SXS && (!wwait(listed, 0, 200) || pieces.count == 0)) break;
+      if (kb == xstages && (!wwait(listed, 0, 200) || pieces.count == 0)) break;
       if (!wwait(&x_empty[xs], u ^ 1, 201)) { ok = false; break; }
       if (lane == 0) {
         mbar_arrive_expect_tx(&x_full[xs], 16384);
@@ -362,13 +483,14 @@ __global__ void __launch_bounds__(224) lora_shrink_tile_kernel(const __grid_cons
       }
       __syncwarp();
       ++issued;
-      if (++xs == SXS) {
+      if (++xs == xstages) {
         xs = 0;
         u ^= 1;
       }
     }
     // every copy lands before the CTA ends, also where no product waits for it
-    for (int kb = max(issued - SXS, 0); kb < issued; ++kb) mbar_wait(&x_full[kb % SXS], uint32_t(kb / SXS) & 1, 203);
+    for (int kb = max(issued - xstages, 0); kb < issued; ++kb)
+      mbar_wait(&x_full[kb % xstages], uint32_t(kb / xstages) & 1, 203);
     if (!ok) abort_flag = 1;
   } else if (warp == 6) {
     // the adapters of these rows: non-empty runs of rows, in order
@@ -432,11 +554,10 @@ __global__ void __launch_bounds__(224) lora_shrink_tile_kernel(const __grid_cons
     const bool lead = elect_one();
     bool ok = wwait(listed, 0, 209);
     const int np = ok ? pieces.count : 0;
-    int as = 0;
-    uint32_t av = 0;
+    int as = 0, xs = 0;
+    uint32_t av = 0, xv = 0;
     for (int kb = 0; kb < nk && np && ok; ++kb) {
-      const int xs = kb % SXS;
-      if (!wwait(&x_full[xs], uint32_t(kb / SXS) & 1, 205)) { ok = false; break; }
+      if (!wwait(&x_full[xs], xv, 205)) { ok = false; break; }
       const uint64_t dx = desc_sw128(sX + xs * 16384);
       for (int i = 0; i < np; ++i) {
         const uint4 o = pieces.off[i];
@@ -458,6 +579,10 @@ __global__ void __launch_bounds__(224) lora_shrink_tile_kernel(const __grid_cons
       }
       if (ok && lead) mma_commit(&x_empty[xs]);
       __syncwarp();
+      if (++xs == xstages) {
+        xs = 0;
+        xv ^= 1;
+      }
     }
     if (!ok) {
       abort_flag = 1;
@@ -916,16 +1041,36 @@ void launch_ex(F* kernel, dim3 grid, int threads, size_t smem, int cluster, bool
   KH_CUDA(cudaLaunchKernelEx(&cfg, kernel, args...));
 }
 
-// Rows by the register-streaming kernels: W is read once per 64 rows.
-bool takes_rows(const kh_lora_matmul_args& a) { return a.rows <= 64; }
-// h by a CTA per row: few rows, or segments so short that a tile of 128 rows would take a product per
-// row or so.
-bool shrinks_rows(const kh_lora_matmul_args& a) { return a.rows <= 64 || a.rows < 8 * int64_t(a.n_segs); }
+// h by a CTA per row: few rows (each reads its adapter's A through L2), or segments so short that a tile
+// of 128 rows would take a product per row or so.
+bool shrinks_rows(const kh_lora_matmul_args& a) {
+  return a.rows < 8 * int64_t(a.n_segs) || (a.rows <= FT && a.rows * a.rank * int64_t(a.k) <= (int64_t(1) << 24));
+}
+// Rows of x as the columns of the product: W is read once per 128 rows.
+bool takes_few(const kh_lora_matmul_args& a) { return a.rows <= FT || (a.rows <= 4 * FT && a.rows < 8 * int64_t(a.n_segs)); }
+// h from the same launch: every cluster makes it for itself, so A is read once per 128 outputs.
+bool fuses(const kh_lora_matmul_args& a) { return takes_few(a) && a.n_adapters > 0 && a.n_adapters * a.rank <= 128; }
 
-template <int NB>
-void launch_rows(const LoraParams& p, int Z, bool dependent, cudaStream_t st) {
-  const dim3 grid(unsigned((p.n + RN - 1) / RN * Z), unsigned((p.rows + NB * 8 - 1) / (NB * 8)));
-  launch_ex(lora_rows_kernel<NB>, grid, 256, 0, Z, dependent, st, p, Z);
+template <bool FUSED>
+void launch_few(const LoraParams& p, const kh_lora_matmul_args& a, cudaStream_t st) {
+  static std::atomic<uint64_t> configured{0};
+  once_per_device(configured, [] {
+    KH_CUDA(cudaFuncSetAttribute(lora_few_kernel<FUSED>, cudaFuncAttributeMaxDynamicSharedMemorySize, FSMEM + 1024));
+  });
+  const int cols = int(std::min<int64_t>(FT, (a.rows + 15) / 16 * 16));
+  const int stages = std::min(12, FSMEM / ((FUSED ? 32768 : 16384) + cols * 128));
+  const int n_tiles = (a.n + 127) / 128, nk = (a.k + 63) / 64;
+  int Z = 1;  // CTAs that split the sum of 128 outputs: while SMs are idle, at least a K block each
+  while (Z < 8 && 2 * Z * n_tiles <= SMS && 2 * Z <= nk) Z *= 2;
+  CUtensorMap tx, tw, ta;
+  encode_tensor_map_f16(&tx, a.x, uint64_t(a.rows), uint64_t(a.k), uint64_t(a.x_stride), 64, uint32_t(cols), 128);
+  encode_tensor_map_f16(&tw, a.w, uint64_t(a.n), uint64_t(a.k), uint64_t(a.k), 64, 128, 128);
+  ta = tw;
+  const int a_rows = a.n_adapters * a.rank;
+  if (FUSED) encode_tensor_map_f16(&ta, a.lora_a, uint64_t(a_rows), uint64_t(a.k), uint64_t(a.k), 64, uint32_t(a_rows), 128);
+  const dim3 grid(unsigned(n_tiles * Z), unsigned((a.rows + FT - 1) / FT));
+  launch_ex(lora_few_kernel<FUSED>, grid, FTHREADS, FSMEM + 1024, Z, !FUSED && a.n_adapters > 0, st, tx, tw, ta, p, Z, cols,
+            stages, a_rows * 128);
 }
 
 template <int BN>
@@ -965,7 +1110,7 @@ void check_sizes(const char* fn, const kh_lora_matmul_args* args) {
 
 int64_t lora_matmul_workspace(const kh_lora_matmul_args* args) {
   check_sizes("kh_lora_matmul_f16_workspace", args);
-  return args->n_adapters ? args->rows * args->rank * 2 : 0;
+  return args->n_adapters && !fuses(*args) ? args->rows * args->rank * 2 : 0;
 }
 
 void lora_matmul(const kh_lora_matmul_args* args, cudaStream_t st) {
@@ -1019,13 +1164,12 @@ void lora_matmul(const kh_lora_matmul_args* args, cudaStream_t st) {
   p.n_adapters = a.n_adapters;
   p.n_segs = a.n_segs;
   const bool adapters = a.n_adapters > 0;
-  if (adapters) {
+  if (adapters && !fuses(a)) {
     if (shrinks_rows(a)) {
-      lora_shrink_rows_kernel<<<unsigned(a.rows), 256, 0, st>>>(p);
+      lora_shrink_rows_kernel<<<unsigned(a.rows), 512, 0, st>>>(p);
       KH_CUDA(cudaGetLastError());
     } else {
-      const int R16 = (a.rank + 15) / 16 * 16, astages = R16 <= 32 ? SAS : 4;
-      const size_t smem = size_t(SXS) * 16384 + size_t(astages) * R16 * 128 + 1024;
+      const int R16 = (a.rank + 15) / 16 * 16;
       static std::atomic<uint64_t> configured{0};
       once_per_device(configured, [] {
         KH_CUDA(cudaFuncSetAttribute(lora_shrink_tile_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
@@ -1037,17 +1181,15 @@ void lora_matmul(const kh_lora_matmul_args* args, cudaStream_t st) {
       const int64_t tiles = (a.rows + 127) / 128;
       int Z = 1;  // CTAs that split a tile's sum: while SMs are idle, at least two K blocks each
       while (Z < 8 && 2 * Z * tiles <= SMS && 4 * Z <= (a.k + 63) / 64) Z *= 2;
-      launch_ex(lora_shrink_tile_kernel, dim3(unsigned(Z * tiles)), 224, smem, Z, false, st, tx, ta, p, Z, astages);
+      // many tiles: rings so short that four CTAs share an SM (up to rank 32) and cover each other's waits
+      const int xstages = tiles > 2 * SMS ? 2 : SXS, astages = R16 > 32 || tiles > 2 * SMS ? 4 : SAS;
+      const size_t smem = size_t(xstages) * 16384 + size_t(astages) * R16 * 128 + 1024;
+      launch_ex(lora_shrink_tile_kernel, dim3(unsigned(Z * tiles)), 224, smem, Z, false, st, tx, ta, p, Z, xstages, astages);
     }
   }
-  if (takes_rows(a)) {
-    const int n_tiles = (a.n + RN - 1) / RN;
-    int Z = 1;  // CTAs that split the sum of 128 outputs: while SMs are idle, at least a step a warp
-    while (Z < 8 && 2 * Z * n_tiles <= SMS && 128 * Z <= a.k) Z *= 2;
-    if (a.rows <= 8) launch_rows<1>(p, Z, adapters, st);
-    else if (a.rows <= 16) launch_rows<2>(p, Z, adapters, st);
-    else if (a.rows <= 32) launch_rows<4>(p, Z, adapters, st);
-    else launch_rows<8>(p, Z, adapters, st);
+  if (takes_few(a)) {
+    if (fuses(a)) launch_few<true>(p, a, st);
+    else launch_few<false>(p, a, st);
   } else {
     // 256 columns a tile where that still gives every pair of SMs one
     const int64_t wide = (a.rows + 255) / 256 * ((a.n + 255) / 256);
