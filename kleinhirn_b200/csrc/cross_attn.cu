@@ -310,12 +310,13 @@ __global__ void __launch_bounds__(128) cross_join_kernel(const CrossParams p) {
 
 // ---- tiles of 128 rows on the tensor cores ----
 //
-// One CTA per (block of two row tiles, key head and split, sequence), one CTA per SM, 320 threads:
+// One CTA per (block of two row tiles, key head and split, sequence), one CTA per SM, 384 threads:
 //   warp 0     TMA: Q once, tiles of 128 states of K and V into two rings;
 //   warp 1     one thread issues S = Q K^T (M 128, N 128, K = D) into the stream's 128 TMEM columns and
 //              O += P V (A = P from TMEM, V as an MN-major operand) into its O columns;
-//   warps 2-9  softmax, warps 2-5 stream 0 and 6-9 stream 1, one thread per row: 128 scores in
-//              registers, P (f16) written over S in TMEM.
+//   warps 4-11 softmax, warps 4-7 stream 0 and 8-11 stream 1, one thread per row: 128 scores in
+//              registers, P (f16) written over S in TMEM, in two halves, the first of which goes into
+//              its products while the second is computed.
 // The two streams are two row tiles over the same K and V tiles; where the CTA's rows fit one tile,
 // they take its even and odd key tiles instead and add up their (m, l, O) at the end. One stream's
 // softmax runs under the other's products. S of the next tile is issued behind P V of the last one, in
@@ -323,9 +324,15 @@ __global__ void __launch_bounds__(128) cross_join_kernel(const CrossParams p) {
 // Key tiles with dropped states (past the end, masked): their scores become -inf and their V rows zero
 // in shared memory, so that nothing they hold reaches a sum.
 
+// Pairs of eight whose exponentials go to the FMA pipe.
+constexpr int EXP_FMA = 2;
+
 constexpr int TROWS = 128;
 constexpr int TKEYS = 128;
-constexpr int TTHREADS = 320;
+constexpr int TTHREADS = 384;
+// Registers a thread: the launch's 168 x 384 are dealt again, as the softmax warps hold a row of 128 scores
+// (56 x 128 + 224 x 256 = 168 x 384).
+constexpr int REGS_ISSUE = 56, REGS_SOFTMAX = 224;
 
 template <int D>
 struct TCfg {
@@ -352,6 +359,28 @@ __device__ __forceinline__ uint64_t tile_desc(const void* smem) {
   return ((uint64_t(smem_u32(smem)) >> 4) & 0x3FFFull) | (C::LBO << 16) | (C::SBO << 32) | (1ull << 46) | (C::LAYOUT << 61);
 }
 
+// 2^x of two values on the FMA pipe (the special-function unit gives 4 results a clock and SM quarter, which
+// would bound the softmax): x = n + f with n the nearest whole number (Cody and Waite's reduction, by
+// adding and taking off 1.5 2^23, whose low bits are then n; 127 more make them the exponent field) and 2^f
+// by the polynomial of degree 4 of least relative error on [-1/2, 1/2] (Remez exchange): 2.6e-6, 2^-18.5,
+// against the 2^-11 of the f16 that p becomes. x below -126 (a dropped score is -inf) gives 2^-126, whose
+// f16 is 0; NaN stays NaN.
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float2 exp2_fma(float2 x) {
+  x = make_float2(max_nan(x.x, -126.f), max_nan(x.y, -126.f));
+  const float2 t = fadd2(x, make_float2(12582912.f + 127.f, 12582912.f + 127.f));
+  const float2 f = fadd2(x, fsub2(make_float2(12582912.f + 127.f, 12582912.f + 127.f), t));
+  float2 q = ffma2(make_float2(0.009570102207362652f, 0.009570102207362652f), f, make_float2(0.05591785907745361f, 0.05591785907745361f));
+  q = ffma2(q, f, make_float2(0.240247443318367f, 0.240247443318367f));
+  q = ffma2(q, f, make_float2(0.6931217908859253f, 0.6931217908859253f));
+  q = ffma2(q, f, make_float2(0.9999992847442627f, 0.9999992847442627f));
+  return fmul2(q, make_float2(__uint_as_float(__float_as_uint(t.x) << 23), __uint_as_float(__float_as_uint(t.y) << 23)));
+}
+
 // Values that tcgen05.ld wrote may be used from here on (the compiler keeps uses behind this).
 template <int N>
 __device__ __forceinline__ void settle(uint32_t (&r)[N]) {
@@ -372,10 +401,10 @@ __global__ void __launch_bounds__(TTHREADS, 1)
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::BAR_OFF);
   uint64_t* q_full = bars;
   uint64_t* s_full = bars + 1;         // [stream]
-  uint64_t* p_full = bars + 3;         // [stream]
-  uint64_t* o_full = bars + 5;         // [stream]
-  uint64_t* drain = bars + 7;
-  uint64_t* k_full = bars + 8;         // [KS]
+  uint64_t* p_full = bars + 3;         // [stream][half]
+  uint64_t* o_full = bars + 7;         // [stream]
+  uint64_t* drain = bars + 9;
+  uint64_t* k_full = bars + 10;        // [KS]
   uint64_t* k_empty = k_full + C::KS;
   uint64_t* v_full = k_empty + C::KS;  // [VS]
   uint64_t* v_empty = v_full + C::VS;
@@ -401,7 +430,8 @@ __global__ void __launch_bounds__(TTHREADS, 1)
     mbar_init(q_full, 1);
     for (int g = 0; g < 2; ++g) {
       mbar_init(&s_full[g], 1);
-      mbar_init(&p_full[g], 128);
+      mbar_init(&p_full[2 * g], 128);
+      mbar_init(&p_full[2 * g + 1], 128);
       mbar_init(&o_full[g], 1);
     }
     mbar_init(drain, 1);
@@ -425,8 +455,9 @@ __global__ void __launch_bounds__(TTHREADS, 1)
   fence_after_sync();
   const uint32_t tmem = *tmem_holder;
 
-  if (warp == 0) {
-    if (lane == 0 && nkt > 0) {
+  if (warp < 4) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGS_ISSUE));
+    if (warp == 0 && lane == 0 && nkt > 0) {
       bool ok = true;
       const int tiles = pair ? 2 : 1;
       mbar_arrive_expect_tx(q_full, tiles * C::PANELS * qpt * G * C::ROWB);
@@ -462,8 +493,7 @@ __global__ void __launch_bounds__(TTHREADS, 1)
           if ((pend_v >> (2 * i)) & 2u) mbar_wait(&v_full[i], (pend_v >> (2 * i)) & 1u, 105);
       }
     }
-  } else if (warp == 1) {
-    if (nkt > 0) {  // all lanes in step, one issues
+    if (warp == 1 && nkt > 0) {  // all lanes in step, one issues
       const uint32_t idesc_s = idesc_f16(128, TKEYS);
       const uint32_t idesc_o = idesc_f16(128, D) | (1u << 16);  // V MN-major
       const bool lead = elect_one();
@@ -495,7 +525,7 @@ __global__ void __launch_bounds__(TTHREADS, 1)
         for (int g = 0; g < 2 && ok; ++g) {
           if (it >= n_of[g]) continue;
           const int j = tile_of(g, it), st = j % C::VS;
-          if (!wwait(&p_full[g], uint32_t(it) & 1, 108) || !wwait(&v_full[st], uint32_t(j / C::VS) & 1, 109)) {
+          if (!wwait(&v_full[st], uint32_t(j / C::VS) & 1, 109) || !wwait(&p_full[2 * g], uint32_t(it) & 1, 108)) {
             ok = false;
             break;
           }
@@ -505,8 +535,18 @@ __global__ void __launch_bounds__(TTHREADS, 1)
           const bool last = it + 1 >= n_of[g];
           if (lead) {
 #pragma unroll
-            for (int k = 0; k < TKEYS / 16; ++k)
+            for (int k = 0; k < TKEYS / 32; ++k)
               mma_f16_ts(oa, pa + uint32_t(8 * k), dv + uint64_t(k * ((16 * C::ROWB) >> 4)), idesc_o, (it || k) ? 1u : 0u);
+          }
+          if (!wwait(&p_full[2 * g + 1], uint32_t(it) & 1, 114)) {
+            ok = false;
+            break;
+          }
+          fence_after_sync();
+          if (lead) {
+#pragma unroll
+            for (int k = TKEYS / 32; k < TKEYS / 16; ++k)
+              mma_f16_ts(oa, pa + uint32_t(8 * k), dv + uint64_t(k * ((16 * C::ROWB) >> 4)), idesc_o, 1u);
             if (!pair || g == 1) mma_commit(&v_empty[st]);
             if (last) mma_commit(&o_full[g]);
           }
@@ -521,38 +561,46 @@ __global__ void __launch_bounds__(TTHREADS, 1)
       }
     }
   } else {
-    const int g = (warp - 2) >> 2;
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(REGS_SOFTMAX));
+    const int g = (warp - 4) >> 2;
     const int quarter = warp & 3;
-    const int r = quarter * 32 + lane;               // row of the tile = TMEM lane
-    const int key = ((warp - 2) & 3) * 32 + lane;    // 0 .. 127: the V row this thread clears
+    const int r = quarter * 32 + lane;  // row of the tile = TMEM lane; also the V row this thread clears
     const uint32_t trow = tmem + (uint32_t(quarter * 32) << 16);
     const uint32_t s_addr = trow + uint32_t(g * 128), o_addr = trow + C::O_COL + uint32_t(g * D);
     const float* mb = p.mask ? p.mask + k0 : nullptr;
     bool ok = true;
     auto wwait = [&](uint64_t* bar, uint32_t parity, int code) -> bool {
-      const bool w = !*abort_flag && mbar_wait(bar, parity, code);
-      return __all_sync(0xffffffffu, w);
+      return __all_sync(0xffffffffu, mbar_wait(bar, parity, code));
     };
+    // mask values of a tile's states, lane by lane (0 past the end), loaded a tile ahead
+    float mk[4];
+    auto load_mask = [&](int it) {
+      const int first = (t0 + (pair ? it : 2 * it + g)) * TKEYS;
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        const int jj = first + 32 * c + lane;
+        mk[c] = it < n_of[g] && jj < nk ? __ldg(mb + jj) : 0.f;
+      }
+    };
+    if (mb) load_mask(0);
     float m = -INFINITY, l = 0.f;
     for (int it = 0; it < n_of[g]; ++it) {
       const int j = pair ? it : 2 * it + g;
-      const int first = (t0 + j) * TKEYS;  // of the sequence's states
-      // the tile's kept states, as bits (the same for every row)
+      const int left = nk - (t0 + j) * TKEYS;
+      // a tile with states to drop: which are kept, as bits (the same for every row)
       uint32_t km[4];
-      const int left = nk - first;
       bool whole = left >= TKEYS;
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        const int n = left - 32 * c;
-        km[c] = n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1u;
-      }
       if (mb) {
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          const int jj = first + 32 * c + lane;
-          km[c] = __ballot_sync(0xffffffffu, jj < nk && __ldg(mb + jj) > 0.5f);
-        }
+        for (int c = 0; c < 4; ++c) km[c] = __ballot_sync(0xffffffffu, mk[c] > 0.5f);
         whole = (km[0] & km[1] & km[2] & km[3]) == 0xffffffffu;
+        load_mask(it + 1);
+      } else if (!whole) {
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          const int n = left - 32 * c;
+          km[c] = n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1u;
+        }
       }
       if (!wwait(&s_full[g], uint32_t(it) & 1, 111)) { ok = false; break; }
       fence_after_sync();
@@ -567,6 +615,18 @@ __global__ void __launch_bounds__(TTHREADS, 1)
         for (int c = 0; c < 4; ++c)
 #pragma unroll
           for (int i = 0; i < 32; ++i) sr[c][i] = (km[c] >> i) & 1u ? sr[c][i] : 0xFF800000u;
+        // (in a pair both streams clear the same V rows: zeros over zeros)
+        const int st = j % C::VS;
+        if (!wwait(&v_full[st], uint32_t(j / C::VS) & 1, 112)) { ok = false; break; }
+        if (!((km[quarter] >> lane) & 1u)) {
+#pragma unroll
+          for (int c = 0; c < C::PANELS; ++c) {
+            uint4* row = reinterpret_cast<uint4*>(sV + st * C::TILE + c * C::PANEL + r * C::ROWB);
+#pragma unroll
+            for (int e = 0; e < C::ROWB / 16; ++e) row[e] = make_uint4(0, 0, 0, 0);
+          }
+        }
+        fence_proxy_async_smem();
       }
       float mr[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
@@ -575,25 +635,25 @@ __global__ void __launch_bounds__(TTHREADS, 1)
         for (int i = 0; i < 32; i += 2)
           mr[(i >> 1) & 3] = fmax3(mr[(i >> 1) & 3], __uint_as_float(sr[c][i]), __uint_as_float(sr[c][i + 1]));
       const float cand = fmaxf(fmaxf(mr[0], mr[1]), fmaxf(mr[2], mr[3])) * p.scale_log2;
-      float corr = 1.f;
-      if (cand > m + 8.f) {  // (also the first kept state: m = -inf)
-        corr = ex2_approx(m - cand);
-        m = cand;
+      const bool moves = cand > m + 8.f;  // (also the first kept state: m = -inf)
+      if (__any_sync(0xffffffffu, moves)) {
+        const float corr = moves ? ex2_approx(m - cand) : 1.f;
+        if (moves) m = cand;
         l *= corr;
-      }
-      if (it > 0 && __any_sync(0xffffffffu, corr != 1.f)) {
-        // the products before this S are done: O may be rescaled
+        if (it > 0) {
+          // the products before this S are done: O may be rescaled
 #pragma unroll 1
-        for (int c = 0; c < D; c += 32) {
-          uint32_t o[32];
-          tmem_ld32(o_addr + c, o);
-          tmem_ld_wait();
-          settle(o);
+          for (int c = 0; c < D; c += 32) {
+            uint32_t o[32];
+            tmem_ld32(o_addr + c, o);
+            tmem_ld_wait();
+            settle(o);
 #pragma unroll
-          for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * corr);
-          tmem_st32(o_addr + c, o);
+            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * corr);
+            tmem_st32(o_addr + c, o);
+          }
+          tmem_st_wait();
         }
-        tmem_st_wait();
       }
       const float ref = m == -INFINITY ? 0.f : m;
       float2 ls[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
@@ -605,31 +665,17 @@ __global__ void __launch_bounds__(TTHREADS, 1)
           const float2 x = ffma2(make_float2(__uint_as_float(sr[2 * c2 + i / 16][(2 * i) & 31]),
                                              __uint_as_float(sr[2 * c2 + i / 16][(2 * i + 1) & 31])),
                                  make_float2(p.scale_log2, p.scale_log2), make_float2(-ref, -ref));
-          const float2 e = make_float2(ex2_approx(x.x), ex2_approx(x.y));
+          const float2 e = (i & 7) < EXP_FMA ? exp2_fma(x) : make_float2(ex2_approx(x.x), ex2_approx(x.y));
           ls[i & 1] = fadd2(ls[i & 1], e);
           const __half2 h = __floats2half2_rn(e.x, e.y);
           pk[i] = *reinterpret_cast<const uint32_t*>(&h);
         }
         tmem_st32(s_addr + 32 * c2, pk);
+        tmem_st_wait();
+        fence_before_sync();
+        mbar_arrive(&p_full[2 * g + c2]);
       }
       l += (ls[0].x + ls[0].y) + (ls[1].x + ls[1].y);
-      if (!whole) {
-        const int st = j % C::VS;
-        if (!wwait(&v_full[st], uint32_t(j / C::VS) & 1, 112)) { ok = false; break; }
-        // (in a pair both streams clear the same rows: zeros over zeros)
-        if (!((km[(warp - 2) & 3] >> lane) & 1u)) {
-#pragma unroll
-          for (int c = 0; c < C::PANELS; ++c) {
-            uint4* row = reinterpret_cast<uint4*>(sV + st * C::TILE + c * C::PANEL + key * C::ROWB);
-#pragma unroll
-            for (int e = 0; e < C::ROWB / 16; ++e) row[e] = make_uint4(0, 0, 0, 0);
-          }
-        }
-        fence_proxy_async_smem();
-      }
-      tmem_st_wait();
-      fence_before_sync();
-      mbar_arrive(&p_full[g]);
     }
     if (ok && n_of[g] > 0) {
       ok = wwait(&o_full[g], 0, 113);

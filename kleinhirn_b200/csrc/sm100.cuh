@@ -181,6 +181,8 @@ __device__ __forceinline__ float2 fadd2(float2 a, float2 b) {
   return bits_f2(r);
 }
 
+__device__ __forceinline__ float2 fsub2(float2 a, float2 b) { return fadd2(a, make_float2(-b.x, -b.y)); }
+
 // Three-input maximum (one instruction on sm_100).
 __device__ __forceinline__ float fmax3(float a, float b, float c) {
   float r;
