@@ -310,47 +310,55 @@ __global__ void __launch_bounds__(128) cross_join_kernel(const CrossParams p) {
 
 // ---- tiles of 128 rows on the tensor cores ----
 //
-// One CTA per (block of two row tiles, key head and split, sequence), one CTA per SM, 384 threads:
-//   warp 0     TMA: Q once, tiles of 128 states of K and V into two rings;
-//   warp 1     one thread issues S = Q K^T (M 128, N 128, K = D) into the stream's 128 TMEM columns and
-//              O += P V (A = P from TMEM, V as an MN-major operand) into its O columns;
-//   warps 4-11 softmax, warps 4-7 stream 0 and 8-11 stream 1, one thread per row: 128 scores in
-//              registers, P (f16) written over S in TMEM, in two halves, the first of which goes into
-//              its products while the second is computed.
+// One CTA per (block of two row tiles, key head and split, sequence):
+//   warp 0     TMA: Q once, tiles of KEYS states of K and V into two rings;
+//   warp 1     issues S = Q K^T (M 128, N KEYS, K = D) into the stream's TMEM columns and O += P V (A = P
+//              from TMEM, V as an MN-major operand) into its O columns;
+//   8 warps    softmax, four to a stream, one thread per row: its KEYS scores in registers, P (f16)
+//              written over S in TMEM.
 // The two streams are two row tiles over the same K and V tiles; where the CTA's rows fit one tile,
-// they take its even and odd key tiles instead and add up their (m, l, O) at the end. One stream's
-// softmax runs under the other's products. S of the next tile is issued behind P V of the last one, in
-// order, so P may lie over S, and a full S means that the products before it are done.
+// they take its even and odd key tiles instead and add up their (m, l, O) at the end. S of the next
+// tile is issued behind P V of the last one, in order, so P may lie over S, and a full S means that the
+// products before it are done; one stream's softmax runs under the other's products.
 // Key tiles with dropped states (past the end, masked): their scores become -inf and their V rows zero
 // in shared memory, so that nothing they hold reaches a sum.
-
-// Pairs of eight whose exponentials go to the FMA pipe.
-constexpr int EXP_FMA = 2;
+//
+// Bound: the softmax threads. A row tile of 128 x 128 scores takes the special-function unit 1,024
+// cycles (4 lanes a clock on each quarter of the SM), its products 512 (D 64) or 1,024 (D 128). Heads of
+// 128 fill TMEM with one CTA per SM (KEYS 128; 168 registers a thread are dealt again, so that a softmax
+// thread holds its row); smaller heads run two CTAs per SM (KEYS 64), whose four softmax warps on each
+// quarter cover one another's waits, and one CTA's ends the other's beginning.
 
 constexpr int TROWS = 128;
-constexpr int TKEYS = 128;
-constexpr int TTHREADS = 384;
-// Registers a thread: the launch's 168 x 384 are dealt again, as the softmax warps hold a row of 128 scores
-// (56 x 128 + 224 x 256 = 168 x 384).
-constexpr int REGS_ISSUE = 56, REGS_SOFTMAX = 224;
 
 template <int D>
 struct TCfg {
-  static constexpr int PANELS = D == 128 ? 2 : 1;    // columns of a swizzled row: 64 (D 32: 32)
+  static constexpr bool ONE = D == 128;              // one CTA per SM
+  static constexpr int KEYS = ONE ? 128 : 64;
+  static constexpr int EXP_FMA = ONE ? 2 : 0;        // pairs of eight whose exponentials go to the FMA pipe
+  static constexpr int HALVES = ONE ? 2 : 1;         // parts in which P goes into its products
+  static constexpr int FIRST = ONE ? 4 : 2;          // first softmax warp (setmaxnreg acts on whole warpgroups)
+  static constexpr int THREADS = 32 * (FIRST + 8);
+  // 56 x 128 + 224 x 256 = 168 x 384, the registers of the launch
+  static constexpr int REGS_ISSUE = 56, REGS_SOFTMAX = 224;
+  static constexpr int PANELS = ONE ? 2 : 1;         // columns of a swizzled row: 64 (D 32: 32)
   static constexpr int PCOLS = D / PANELS;
   static constexpr int ROWB = PCOLS * 2;             // bytes of a row of a panel: the swizzle width
-  static constexpr int PANEL = 128 * ROWB;
-  static constexpr int TILE = PANELS * PANEL;        // 128 rows of q, k or v
-  static constexpr int KS = D == 128 ? 3 : 4;        // ring stages
-  static constexpr int VS = D == 128 ? 2 : 4;
-  static constexpr int K_OFF = 2 * TILE;             // (Q tiles at 0)
-  static constexpr int V_OFF = K_OFF + KS * TILE;
-  static constexpr int BAR_OFF = V_OFF + VS * TILE;
-  static constexpr int SMEM = (BAR_OFF + 256 + 1024 > 120 * 1024 ? BAR_OFF + 256 + 1024 : 120 * 1024);  // one CTA per SM
+  static constexpr int QPANEL = TROWS * ROWB, QTILE = PANELS * QPANEL;
+  static constexpr int KPANEL = KEYS * ROWB, KTILE = PANELS * KPANEL;
+  static constexpr int KS = ONE ? 3 : 4, VS = ONE ? 2 : 4;  // ring stages
+  static constexpr int K_OFF = 2 * QTILE;
+  static constexpr int V_OFF = K_OFF + KS * KTILE;
+  static constexpr int BAR_OFF = V_OFF + VS * KTILE;
+  static constexpr int LUT_OFF = BAR_OFF + 256;             // 4 bits as 4 words, [16]
+  static constexpr int USED = LUT_OFF + 256 + 1024;
+  // as much as keeps a third CTA (its TMEM) off the SM
+  static constexpr int SMEM = ONE || USED > 100 * 1024 ? USED : 100 * 1024;
+  static constexpr uint32_t S_STRIDE = ONE ? 128 : 64;      // TMEM: S of the streams, then O
+  static constexpr uint32_t O_COL = 2 * S_STRIDE, COLS = ONE ? 512 : 256;
   static constexpr uint64_t LAYOUT = D == 32 ? 4ull : 2ull;  // 64- or 128-byte swizzle
   static constexpr uint64_t SBO = (8 * ROWB) >> 4;
-  static constexpr uint64_t LBO = PANELS == 2 ? (PANEL >> 4) : 1ull;  // MN-major V: from panel to panel
-  static constexpr uint32_t O_COL = 256;             // TMEM: S of the streams at 0 and 128, then O
+  static constexpr uint64_t LBO = PANELS == 2 ? (KPANEL >> 4) : 1ull;  // MN-major V: from panel to panel
 };
 
 template <int D>
@@ -359,25 +367,25 @@ __device__ __forceinline__ uint64_t tile_desc(const void* smem) {
   return ((uint64_t(smem_u32(smem)) >> 4) & 0x3FFFull) | (C::LBO << 16) | (C::SBO << 32) | (1ull << 46) | (C::LAYOUT << 61);
 }
 
-// 2^x of two values on the FMA pipe (the special-function unit gives 4 results a clock and SM quarter, which
-// would bound the softmax): x = n + f with n the nearest whole number (Cody and Waite's reduction, by
-// adding and taking off 1.5 2^23, whose low bits are then n; 127 more make them the exponent field) and 2^f
-// by the polynomial of degree 4 of least relative error on [-1/2, 1/2] (Remez exchange): 2.6e-6, 2^-18.5,
-// against the 2^-11 of the f16 that p becomes. x below -126 (a dropped score is -inf) gives 2^-126, whose
-// f16 is 0; NaN stays NaN.
+// 2^x of two values on the FMA pipe: x = n + f with n the nearest whole number (Cody and Waite's reduction,
+// by adding and taking off 1.5 2^23, whose low bits are then n; 127 more make them the exponent field) and
+// 2^f by the polynomial of degree 4 of least relative error on [-1/2, 1/2] (Remez exchange): 2.6e-6,
+// 2^-18.5, against the 2^-11 of the f16 that p becomes. x below -126 (a dropped score is -inf) gives
+// 2^-126, whose f16 is 0; NaN stays NaN.
 __device__ __forceinline__ float max_nan(float a, float b) {
   float r;
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
   return r;
 }
+__device__ __forceinline__ float2 twice(float a) { return make_float2(a, a); }
 __device__ __forceinline__ float2 exp2_fma(float2 x) {
   x = make_float2(max_nan(x.x, -126.f), max_nan(x.y, -126.f));
-  const float2 t = fadd2(x, make_float2(12582912.f + 127.f, 12582912.f + 127.f));
-  const float2 f = fadd2(x, fsub2(make_float2(12582912.f + 127.f, 12582912.f + 127.f), t));
-  float2 q = ffma2(make_float2(0.009570102207362652f, 0.009570102207362652f), f, make_float2(0.05591785907745361f, 0.05591785907745361f));
-  q = ffma2(q, f, make_float2(0.240247443318367f, 0.240247443318367f));
-  q = ffma2(q, f, make_float2(0.6931217908859253f, 0.6931217908859253f));
-  q = ffma2(q, f, make_float2(0.9999992847442627f, 0.9999992847442627f));
+  const float2 t = fadd2(x, twice(12582912.f + 127.f));
+  const float2 f = fadd2(x, ffma2(t, twice(-1.f), twice(12582912.f + 127.f)));
+  float2 q = ffma2(twice(0.009570102207362652f), f, twice(0.05591785907745361f));
+  q = ffma2(q, f, twice(0.240247443318367f));
+  q = ffma2(q, f, twice(0.6931217908859253f));
+  q = ffma2(q, f, twice(0.9999992847442627f));
   return fmul2(q, make_float2(__uint_as_float(__float_as_uint(t.x) << 23), __uint_as_float(__float_as_uint(t.y) << 23)));
 }
 
@@ -388,11 +396,23 @@ __device__ __forceinline__ void settle(uint32_t (&r)[N]) {
   for (int i = 0; i < N; ++i) asm volatile("" : "+r"(r[i]));
 }
 
+// Barrier of the two warps of a quarter. The ids are constants: with an id in a register a CTA counts as
+// using all 16 barriers, and a second one does not fit the SM.
+__device__ __forceinline__ bool quarter_any(int quarter, bool pred) {
+  switch (quarter) {
+    case 0: return named_bar_any<1>(64, pred);
+    case 1: return named_bar_any<2>(64, pred);
+    case 2: return named_bar_any<3>(64, pred);
+    default: return named_bar_any<4>(64, pred);
+  }
+}
+
 template <int D>
-__global__ void __launch_bounds__(TTHREADS, 1)
+__global__ void __launch_bounds__(TCfg<D>::THREADS, TCfg<D>::ONE ? 1 : 2)
     cross_tile_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant__ CUtensorMap tmk,
                       const __grid_constant__ CUtensorMap tmv, const CrossParams p) {
   using C = TCfg<D>;
+  constexpr int KEYS = C::KEYS;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* sQ = smem;
@@ -422,9 +442,9 @@ __global__ void __launch_bounds__(TTHREADS, 1)
   if (qb >= nq) return;
   const bool pair = nq - qb > qpt;  // two row tiles (else the streams share one tile's states)
   // key tiles of this split
-  const int all = (nk + TKEYS - 1) / TKEYS, per = (all + p.nsplit - 1) / p.nsplit;
+  const int all = (nk + KEYS - 1) / KEYS, per = (all + p.nsplit - 1) / p.nsplit;
   const int t0 = min(split * per, all), nkt = min(t0 + per, all) - t0;
-  const int n_of[2] = {pair ? nkt : (nkt + 1) / 2, pair ? nkt : nkt / 2};
+  const int n0_of = pair ? nkt : (nkt + 1) / 2, n1_of = pair ? nkt : nkt / 2;  // tiles of the streams
 
   if (threadIdx.x == 0) {
     mbar_init(q_full, 1);
@@ -449,31 +469,36 @@ __global__ void __launch_bounds__(TTHREADS, 1)
     prefetch_tmap(&tmk);
     prefetch_tmap(&tmv);
   }
-  if (warp == 1) tmem_alloc(tmem_holder, 512);
+  const uint4* lut4 = reinterpret_cast<const uint4*>(smem + C::LUT_OFF);
+  if (threadIdx.x < 64) reinterpret_cast<uint32_t*>(smem + C::LUT_OFF)[threadIdx.x] = (threadIdx.x >> 2 >> (threadIdx.x & 3)) & 1u ? ~0u : 0u;
+  if (warp == 1) tmem_alloc(tmem_holder, C::COLS);
   fence_before_sync();
   __syncthreads();
   fence_after_sync();
   const uint32_t tmem = *tmem_holder;
+  auto wwait = [&](uint64_t* bar, uint32_t parity, int code) -> bool {
+    return __all_sync(0xffffffffu, mbar_wait(bar, parity, code));
+  };
 
-  if (warp < 4) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGS_ISSUE));
+  if (warp < C::FIRST) {
+    if constexpr (C::ONE) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::REGS_ISSUE));
     if (warp == 0 && lane == 0 && nkt > 0) {
       bool ok = true;
       const int tiles = pair ? 2 : 1;
       mbar_arrive_expect_tx(q_full, tiles * C::PANELS * qpt * G * C::ROWB);
       for (int g = 0; g < tiles; ++g)
         for (int c = 0; c < C::PANELS; ++c)
-          tma_load_3d(sQ + g * C::TILE + c * C::PANEL, &tmq, q_full, c * C::PCOLS, hk * G, int(q0) + qb + g * qpt);
+          tma_load_3d(sQ + g * C::QTILE + c * C::QPANEL, &tmq, q_full, c * C::PCOLS, hk * G, int(q0) + qb + g * qpt);
       uint32_t pend_k = 0, pend_v = 0;  // last issued parity per ring slot (bit 1: issued)
       auto load = [&](int j, bool is_v) -> bool {
         const int stages = is_v ? C::VS : C::KS, st = j % stages;
         const uint32_t u = uint32_t(j / stages) & 1;
         uint64_t* full = is_v ? &v_full[st] : &k_full[st];
-        if (*abort_flag || !mbar_wait(is_v ? &v_empty[st] : &k_empty[st], u ^ 1, is_v ? 102 : 101)) return false;
-        mbar_arrive_expect_tx(full, C::TILE);
-        uint8_t* dst = (is_v ? sV : sK) + st * C::TILE;
+        if (!mbar_wait(is_v ? &v_empty[st] : &k_empty[st], u ^ 1, is_v ? 102 : 101)) return false;
+        mbar_arrive_expect_tx(full, C::KTILE);
+        uint8_t* dst = (is_v ? sV : sK) + st * C::KTILE;
         for (int c = 0; c < C::PANELS; ++c)
-          tma_load_2d(dst + c * C::PANEL, is_v ? &tmv : &tmk, full, hk * D + c * C::PCOLS, int(k0) + (t0 + j) * TKEYS);
+          tma_load_2d(dst + c * C::KPANEL, is_v ? &tmv : &tmk, full, hk * D + c * C::PCOLS, int(k0) + (t0 + j) * KEYS);
         uint32_t& pend = is_v ? pend_v : pend_k;
         pend = (pend & ~(3u << (2 * st))) | ((2u | u) << (2 * st));
         return true;
@@ -494,65 +519,67 @@ __global__ void __launch_bounds__(TTHREADS, 1)
       }
     }
     if (warp == 1 && nkt > 0) {  // all lanes in step, one issues
-      const uint32_t idesc_s = idesc_f16(128, TKEYS);
+      const uint32_t idesc_s = idesc_f16(128, KEYS);
       const uint32_t idesc_o = idesc_f16(128, D) | (1u << 16);  // V MN-major
       const bool lead = elect_one();
-      auto wwait = [&](uint64_t* bar, uint32_t parity, int code) -> bool {
-        return __all_sync(0xffffffffu, mbar_wait(bar, parity, code));
-      };
-      auto tile_of = [&](int g, int it) { return pair ? it : 2 * it + g; };
-      auto issue_s = [&](int g, int it) -> bool {
-        const int j = tile_of(g, it), st = j % C::KS;
-        if (!wwait(&k_full[st], uint32_t(j / C::KS) & 1, 106)) return false;
-        fence_after_sync();
-        const uint64_t dq = tile_desc<D>(sQ + (pair ? g : 0) * C::TILE), dk = tile_desc<D>(sK + st * C::TILE);
-        if (lead) {
-#pragma unroll
-          for (int k = 0; k < D / 16; ++k) {
-            const uint64_t off = uint64_t((k / (C::PCOLS / 16)) * (C::PANEL >> 4) + (k % (C::PCOLS / 16)) * 2);
-            mma_f16(tmem + uint32_t(g * 128), dq + off, dk + off, idesc_s, k ? 1u : 0u);
-          }
-          mma_commit(&s_full[g]);
-          if (!pair || g == 1) mma_commit(&k_empty[st]);
+      // Tile `it` of stream g: tile `it` of the split in a pair, else 2 it + g. A ring stage is waited for by
+      // its first product and freed behind its last (stream 1's in a pair).
+      const uint64_t dq0 = tile_desc<D>(sQ), dk0 = tile_desc<D>(sK), dv0 = tile_desc<D>(sV);
+      constexpr uint64_t Q16 = uint64_t(C::QTILE >> 4), K16 = uint64_t(C::KTILE >> 4);
+      int ks = 0, vs = 0;       // ring stages of the next K and V tile
+      uint32_t kp = 0, vp = 0;  // and their parities
+      auto issue_s = [&](int g) -> bool {
+        if (!pair || g == 0) {
+          if (!wwait(&k_full[ks], kp, 106)) return false;
+          fence_after_sync();
         }
-        __syncwarp();
+        const uint64_t dq = dq0 + (pair && g ? Q16 : 0ull), dk = dk0 + ks * K16;
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k) {
+          const int panel = k / (C::PCOLS / 16), step = k % (C::PCOLS / 16);
+          mma_f16_if(lead, tmem + uint32_t(g) * C::S_STRIDE, dq + uint64_t(panel * (C::QPANEL >> 4) + step * 2),
+                     dk + uint64_t(panel * (C::KPANEL >> 4) + step * 2), idesc_s, k ? 1u : 0u);
+        }
+        mma_commit_if(lead, &s_full[g]);
+        if (!pair || g == 1) {
+          mma_commit_if(lead, &k_empty[ks]);
+          if (++ks == C::KS) {
+            ks = 0;
+            kp ^= 1;
+          }
+        }
         return true;
       };
-      bool ok = wwait(q_full, 0, 107);
-      for (int g = 0; g < 2 && ok; ++g)
-        if (n_of[g] > 0) ok = issue_s(g, 0);
-      for (int it = 0; it < n_of[0] && ok; ++it)
-        for (int g = 0; g < 2 && ok; ++g) {
-          if (it >= n_of[g]) continue;
-          const int j = tile_of(g, it), st = j % C::VS;
-          if (!wwait(&v_full[st], uint32_t(j / C::VS) & 1, 109) || !wwait(&p_full[2 * g], uint32_t(it) & 1, 108)) {
-            ok = false;
-            break;
-          }
-          fence_after_sync();
-          const uint64_t dv = tile_desc<D>(sV + st * C::TILE);
-          const uint32_t pa = tmem + uint32_t(g * 128), oa = tmem + C::O_COL + uint32_t(g * D);
-          const bool last = it + 1 >= n_of[g];
-          if (lead) {
+      auto issue_o = [&](int g, int it, bool last) -> bool {
+        if ((!pair || g == 0) && !wwait(&v_full[vs], vp, 109)) return false;
+        const uint64_t dv = dv0 + vs * K16;
+        const uint32_t pa = tmem + uint32_t(g) * C::S_STRIDE, oa = tmem + C::O_COL + uint32_t(g * D);
 #pragma unroll
-            for (int k = 0; k < TKEYS / 32; ++k)
-              mma_f16_ts(oa, pa + uint32_t(8 * k), dv + uint64_t(k * ((16 * C::ROWB) >> 4)), idesc_o, (it || k) ? 1u : 0u);
+        for (int k = 0; k < KEYS / 16; ++k) {
+          if (k % (KEYS / 16 / C::HALVES) == 0) {
+            if (!wwait(&p_full[2 * g + (k ? 1 : 0)], uint32_t(it) & 1, 108)) return false;
+            fence_after_sync();
           }
-          if (!wwait(&p_full[2 * g + 1], uint32_t(it) & 1, 114)) {
-            ok = false;
-            break;
-          }
-          fence_after_sync();
-          if (lead) {
-#pragma unroll
-            for (int k = TKEYS / 32; k < TKEYS / 16; ++k)
-              mma_f16_ts(oa, pa + uint32_t(8 * k), dv + uint64_t(k * ((16 * C::ROWB) >> 4)), idesc_o, 1u);
-            if (!pair || g == 1) mma_commit(&v_empty[st]);
-            if (last) mma_commit(&o_full[g]);
-          }
-          __syncwarp();
-          if (!last) ok = issue_s(g, it + 1);
+          mma_f16_ts_if(lead, oa, pa + uint32_t(8 * k), dv + uint64_t(k * ((16 * C::ROWB) >> 4)), idesc_o, (it || k) ? 1u : 0u);
         }
+        if (last) mma_commit_if(lead, &o_full[g]);
+        if (!pair || g == 1) {
+          mma_commit_if(lead, &v_empty[vs]);
+          if (++vs == C::VS) {
+            vs = 0;
+            vp ^= 1;
+          }
+        }
+        return true;
+      };
+      bool ok = wwait(q_full, 0, 107) && issue_s(0) && (n1_of == 0 || issue_s(1));
+      for (int it = 0; it < n0_of && ok; ++it) {
+        const bool two = it < n1_of, next0 = it + 1 < n0_of, next1 = it + 1 < n1_of;
+        ok = issue_o(0, it, !next0);
+        if (next0) ok = ok && issue_s(0);
+        if (two) ok = ok && issue_o(1, it, !next1);
+        if (next1) ok = ok && issue_s(1);
+      }
       if (!ok) {
         *abort_flag = 1;
         if (lead) mma_commit(drain);
@@ -561,76 +588,90 @@ __global__ void __launch_bounds__(TTHREADS, 1)
       }
     }
   } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(REGS_SOFTMAX));
-    const int g = (warp - 4) >> 2;
+    if constexpr (C::ONE) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::REGS_SOFTMAX));
+    const int g = (warp - C::FIRST) >> 2;
     const int quarter = warp & 3;
-    const int r = quarter * 32 + lane;  // row of the tile = TMEM lane; also the V row this thread clears
+    const int r = quarter * 32 + lane;  // row of the tile = TMEM lane
     const uint32_t trow = tmem + (uint32_t(quarter * 32) << 16);
-    const uint32_t s_addr = trow + uint32_t(g * 128), o_addr = trow + C::O_COL + uint32_t(g * D);
+    const uint32_t s_addr = trow + uint32_t(g) * C::S_STRIDE, o_addr = trow + C::O_COL + uint32_t(g * D);
+    const int n_mine = g ? n1_of : n0_of;
     const float* mb = p.mask ? p.mask + k0 : nullptr;
     bool ok = true;
-    auto wwait = [&](uint64_t* bar, uint32_t parity, int code) -> bool {
-      return __all_sync(0xffffffffu, mbar_wait(bar, parity, code));
-    };
+    constexpr int W = KEYS / 32;  // words of a tile's states
     // mask values of a tile's states, lane by lane (0 past the end), loaded a tile ahead
-    float mk[4];
+    float mk[W];
     auto load_mask = [&](int it) {
-      const int first = (t0 + (pair ? it : 2 * it + g)) * TKEYS;
+      const int first = (t0 + (pair ? it : 2 * it + g)) * KEYS;
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
+      for (int c = 0; c < W; ++c) {
         const int jj = first + 32 * c + lane;
-        mk[c] = it < n_of[g] && jj < nk ? __ldg(mb + jj) : 0.f;
+        mk[c] = it < n_mine && jj < nk ? __ldg(mb + jj) : 0.f;
       }
     };
     if (mb) load_mask(0);
     float m = -INFINITY, l = 0.f;
-    for (int it = 0; it < n_of[g]; ++it) {
+    for (int it = 0; it < n_mine; ++it) {
       const int j = pair ? it : 2 * it + g;
-      const int left = nk - (t0 + j) * TKEYS;
+      const int left = nk - (t0 + j) * KEYS;
       // a tile with states to drop: which are kept, as bits (the same for every row)
-      uint32_t km[4];
-      bool whole = left >= TKEYS;
+      uint32_t km[W];
+      bool whole = left >= KEYS;
       if (mb) {
+        uint32_t every = 0xffffffffu;
 #pragma unroll
-        for (int c = 0; c < 4; ++c) km[c] = __ballot_sync(0xffffffffu, mk[c] > 0.5f);
-        whole = (km[0] & km[1] & km[2] & km[3]) == 0xffffffffu;
+        for (int c = 0; c < W; ++c) {
+          km[c] = __ballot_sync(0xffffffffu, mk[c] > 0.5f);
+          every &= km[c];
+        }
+        whole = every == 0xffffffffu;
         load_mask(it + 1);
       } else if (!whole) {
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
+        for (int c = 0; c < W; ++c) {
           const int n = left - 32 * c;
           km[c] = n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1u;
         }
       }
       if (!wwait(&s_full[g], uint32_t(it) & 1, 111)) { ok = false; break; }
       fence_after_sync();
-      uint32_t sr[4][32];
+      uint32_t sr[W][32];
 #pragma unroll
-      for (int c = 0; c < 4; ++c) tmem_ld32(s_addr + 32 * c, sr[c]);
+      for (int c = 0; c < W; ++c) tmem_ld32(s_addr + 32 * c, sr[c]);
       tmem_ld_wait();
 #pragma unroll
-      for (int c = 0; c < 4; ++c) settle(sr[c]);
+      for (int c = 0; c < W; ++c) settle(sr[c]);
       if (!whole) {
 #pragma unroll
-        for (int c = 0; c < 4; ++c)
+        for (int c = 0; c < W; ++c)
 #pragma unroll
-          for (int i = 0; i < 32; ++i) sr[c][i] = (km[c] >> i) & 1u ? sr[c][i] : 0xFF800000u;
-        // (in a pair both streams clear the same V rows: zeros over zeros)
-        const int st = j % C::VS;
+          for (int i = 0; i < 32; i += 4) {
+            const uint4 keep = lut4[(km[c] >> i) & 15u];
+            sr[c][i] = (sr[c][i] & keep.x) | (~keep.x & 0xFF800000u);
+            sr[c][i + 1] = (sr[c][i + 1] & keep.y) | (~keep.y & 0xFF800000u);
+            sr[c][i + 2] = (sr[c][i + 2] & keep.z) | (~keep.z & 0xFF800000u);
+            sr[c][i + 3] = (sr[c][i + 3] & keep.w) | (~keep.w & 0xFF800000u);
+          }
+        // a thread clears its share of the dropped V rows (in a pair both streams clear the same ones: zeros
+        // over zeros): a row of KEYS 128, half a row of KEYS 64
+        const int st = j % C::VS, vr = r % KEYS;
         if (!wwait(&v_full[st], uint32_t(j / C::VS) & 1, 112)) { ok = false; break; }
-        if (!((km[quarter] >> lane) & 1u)) {
+        uint32_t word = km[0];
+#pragma unroll
+        for (int c = 1; c < W; ++c) word = vr / 32 == c ? km[c] : word;
+        if (!((word >> lane) & 1u)) {
+          constexpr int BYTES = C::ROWB * KEYS / 128;
 #pragma unroll
           for (int c = 0; c < C::PANELS; ++c) {
-            uint4* row = reinterpret_cast<uint4*>(sV + st * C::TILE + c * C::PANEL + r * C::ROWB);
+            uint4* row = reinterpret_cast<uint4*>(sV + st * C::KTILE + c * C::KPANEL + vr * C::ROWB + r / KEYS * BYTES);
 #pragma unroll
-            for (int e = 0; e < C::ROWB / 16; ++e) row[e] = make_uint4(0, 0, 0, 0);
+            for (int e = 0; e < BYTES / 16; ++e) row[e] = make_uint4(0, 0, 0, 0);
           }
         }
         fence_proxy_async_smem();
       }
       float mr[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-      for (int c = 0; c < 4; ++c)
+      for (int c = 0; c < W; ++c)
 #pragma unroll
         for (int i = 0; i < 32; i += 2)
           mr[(i >> 1) & 3] = fmax3(mr[(i >> 1) & 3], __uint_as_float(sr[c][i]), __uint_as_float(sr[c][i + 1]));
@@ -643,41 +684,44 @@ __global__ void __launch_bounds__(TTHREADS, 1)
         if (it > 0) {
           // the products before this S are done: O may be rescaled
 #pragma unroll 1
-          for (int c = 0; c < D; c += 32) {
-            uint32_t o[32];
-            tmem_ld32(o_addr + c, o);
+          for (int c = 0; c < D; c += 16) {
+            uint32_t o[16];
+            tmem_ld16(o_addr + c, o);
             tmem_ld_wait();
             settle(o);
 #pragma unroll
-            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * corr);
-            tmem_st32(o_addr + c, o);
+            for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * corr);
+            tmem_st16(o_addr + c, o);
           }
           tmem_st_wait();
         }
       }
       const float ref = m == -INFINITY ? 0.f : m;
       float2 ls[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+      constexpr int CHUNK = C::ONE ? 32 : 8;  // packed pairs stored at a time, as the registers allow
 #pragma unroll
-      for (int c2 = 0; c2 < 2; ++c2) {
-        uint32_t pk[32];
+      for (int c = 0; c < KEYS / 2; c += CHUNK) {
+        uint32_t pk[CHUNK];
 #pragma unroll
-        for (int i = 0; i < 32; ++i) {
-          const float2 x = ffma2(make_float2(__uint_as_float(sr[2 * c2 + i / 16][(2 * i) & 31]),
-                                             __uint_as_float(sr[2 * c2 + i / 16][(2 * i + 1) & 31])),
-                                 make_float2(p.scale_log2, p.scale_log2), make_float2(-ref, -ref));
-          const float2 e = (i & 7) < EXP_FMA ? exp2_fma(x) : make_float2(ex2_approx(x.x), ex2_approx(x.y));
+        for (int i = 0; i < CHUNK; ++i) {
+          const int k = 2 * (c + i);
+          const float2 x = ffma2(make_float2(__uint_as_float(sr[k / 32][k & 31]), __uint_as_float(sr[k / 32][(k + 1) & 31])),
+                                 twice(p.scale_log2), twice(-ref));
+          const float2 e = (i & 7) < C::EXP_FMA ? exp2_fma(x) : make_float2(ex2_approx(x.x), ex2_approx(x.y));
           ls[i & 1] = fadd2(ls[i & 1], e);
-          const __half2 h = __floats2half2_rn(e.x, e.y);
-          pk[i] = *reinterpret_cast<const uint32_t*>(&h);
+          pk[i] = pack_half2(e.x, e.y);
         }
-        tmem_st32(s_addr + 32 * c2, pk);
-        tmem_st_wait();
-        fence_before_sync();
-        mbar_arrive(&p_full[2 * g + c2]);
+        if constexpr (C::ONE) tmem_st32(s_addr + c, pk);
+        else tmem_st8(s_addr + c, pk);
+        if ((c + CHUNK) % (KEYS / 2 / C::HALVES) == 0) {
+          tmem_st_wait();
+          fence_before_sync();
+          mbar_arrive(&p_full[2 * g + (c + CHUNK == KEYS / 2 ? C::HALVES - 1 : 0)]);
+        }
       }
       l += (ls[0].x + ls[0].y) + (ls[1].x + ls[1].y);
     }
-    if (ok && n_of[g] > 0) {
+    if (ok && n_mine > 0) {
       ok = wwait(&o_full[g], 0, 113);
       fence_after_sync();
     }
@@ -687,12 +731,12 @@ __global__ void __launch_bounds__(TTHREADS, 1)
     const bool mine = r < qpt * G && qi < nq;
     float m_out = m, l_out = l, f0 = 1.f, f1 = 0.f;
     if (!pair) {
-      float* xm = reinterpret_cast<float*>(sQ + C::TILE);  // the second Q tile is not used
+      float* xm = reinterpret_cast<float*>(sQ + C::QTILE);  // the second Q tile is not used
       float* xl = xm + 256;
       xm[g * 128 + r] = m;
       xl[g * 128 + r] = l;
       fence_before_sync();
-      if (named_bar_any(1 + quarter, 64, !ok)) ok = false;
+      if (quarter_any(quarter, !ok)) ok = false;
       fence_after_sync();
       const float m0 = xm[r], m1 = xm[128 + r];
       m_out = fmaxf(m0, m1);
@@ -706,39 +750,32 @@ __global__ void __launch_bounds__(TTHREADS, 1)
       const bool direct = p.nsplit == 1;
       const int64_t at = mine && !direct ? part_index(p, split, s, qi, h) : 0;
       const float inv = direct ? (l_out == 0.f ? 0.f : 1.f / l_out) : 1.f;
-      constexpr int STEP = D / 2 < 32 ? 16 : 32;
       const int c_begin = pair ? 0 : g * (D / 2), c_end = pair ? D : c_begin + D / 2;
       const uint32_t o0 = trow + C::O_COL + (pair ? uint32_t(g * D) : 0u);
 #pragma unroll 1
-      for (int c = c_begin; c < c_end; c += STEP) {
-        uint32_t a[STEP], b[STEP];
+      for (int c = c_begin; c < c_end; c += 16) {
+        uint32_t a[16], b[16];
         // TMEM of a stream without items was never written: its factor is 0 and it is not read
-        if (n_of[pair ? g : 0] > 0) {
-          if constexpr (STEP == 32) tmem_ld32(o0 + c, a);
-          else tmem_ld16(o0 + c, a);
-        }
-        if (!pair && n_of[1] > 0) {
-          if constexpr (STEP == 32) tmem_ld32(o0 + D + c, b);
-          else tmem_ld16(o0 + D + c, b);
-        }
+        if ((pair ? n_mine : n0_of) > 0) tmem_ld16(o0 + c, a);
+        if (!pair && n1_of > 0) tmem_ld16(o0 + D + c, b);
         tmem_ld_wait();
         settle(a);
         settle(b);
-        float v[STEP];
+        float v[16];
 #pragma unroll
-        for (int i = 0; i < STEP; ++i)
+        for (int i = 0; i < 16; ++i)
           v[i] = ((f0 != 0.f ? __uint_as_float(a[i]) * f0 : 0.f) + (f1 != 0.f ? __uint_as_float(b[i]) * f1 : 0.f)) * inv;
         if (!mine) continue;
         if (direct) {
           uint4* dst = reinterpret_cast<uint4*>(p.out + (q0 + qi) * p.out_stride + h * D + c);
 #pragma unroll
-          for (int i = 0; i < STEP / 8; ++i)
+          for (int i = 0; i < 2; ++i)
             dst[i] = make_uint4(pack_half2(v[8 * i], v[8 * i + 1]), pack_half2(v[8 * i + 2], v[8 * i + 3]),
                                 pack_half2(v[8 * i + 4], v[8 * i + 5]), pack_half2(v[8 * i + 6], v[8 * i + 7]));
         } else {
           float4* dst = reinterpret_cast<float4*>(p.part_o + at * D + c);
 #pragma unroll
-          for (int i = 0; i < STEP / 4; ++i) dst[i] = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+          for (int i = 0; i < 4; ++i) dst[i] = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
         }
       }
       if (mine && !direct && (pair || g == 0)) p.part_ml[at] = make_float2(m_out, l_out);
@@ -750,7 +787,7 @@ __global__ void __launch_bounds__(TTHREADS, 1)
   __syncthreads();
   if (warp == 1) {
     fence_after_sync();
-    tmem_free(tmem, 512);
+    tmem_free(tmem, C::COLS);
   }
 }
 
@@ -778,14 +815,14 @@ bool takes_rows_kernel(const kh_cross_attention_args& a) {
 constexpr int SMS = 148;  // of a B200: the split must not depend on the device the size is asked on
 
 // CTAs that a sequence's states are split over: as many as fill the SMs (four CTAs each of the rows
-// kernel, one of the tile kernel), each with enough states to pay for the join.
+// kernel, one or two of the tile kernel), each with enough states to pay for the join.
 int splits(const kh_cross_attention_args& a) {
   const int64_t G = a.q_heads / a.kv_heads;
   const bool few = takes_rows_kernel(a);
   const int64_t blocks = few ? 1 : (int64_t(a.max_q) + 2 * (TROWS / G) - 1) / (2 * (TROWS / G));
   const int64_t ctas = std::max<int64_t>(1, blocks * a.kv_heads * a.n_seqs);
-  const int64_t want = (few ? 4 * SMS : SMS) / ctas;
-  const int64_t most = few ? a.max_k / (4 * RW * RSTEP) : a.max_k / (4 * TKEYS);
+  const int64_t want = (few ? 4 * SMS : a.head_dim == 128 ? SMS : 2 * SMS) / ctas;
+  const int64_t most = few ? a.max_k / (4 * RW * RSTEP) : a.max_k / 512;
   return int(std::min<int64_t>(std::max<int64_t>(1, std::min(want, most)), 64));
 }
 
@@ -808,11 +845,11 @@ void launch(const CrossParams& p, const kh_cross_attention_args& a, bool states,
     tk = tv = tq;  // (without states neither is read)
     if (states) {
       const uint64_t cols = uint64_t(a.kv_heads) * D;
-      encode_tensor_map_f16(&tk, a.k, uint64_t(a.kv_rows), cols, uint64_t(a.k_stride), C::PCOLS, TKEYS, C::ROWB);
-      encode_tensor_map_f16(&tv, a.v, uint64_t(a.kv_rows), cols, uint64_t(a.v_stride), C::PCOLS, TKEYS, C::ROWB);
+      encode_tensor_map_f16(&tk, a.k, uint64_t(a.kv_rows), cols, uint64_t(a.k_stride), C::PCOLS, C::KEYS, C::ROWB);
+      encode_tensor_map_f16(&tv, a.v, uint64_t(a.kv_rows), cols, uint64_t(a.v_stride), C::PCOLS, C::KEYS, C::ROWB);
     }
     const dim3 grid(unsigned((a.max_q + 2 * qpt - 1) / (2 * qpt)), unsigned(a.kv_heads * p.nsplit), unsigned(a.n_seqs));
-    cross_tile_kernel<D><<<grid, TTHREADS, C::SMEM, st>>>(tq, tk, tv, p);
+    cross_tile_kernel<D><<<grid, C::THREADS, C::SMEM, st>>>(tq, tk, tv, p);
   }
   KH_CUDA(cudaGetLastError());
   if (p.nsplit > 1) {
