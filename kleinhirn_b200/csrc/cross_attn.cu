@@ -311,7 +311,8 @@ __global__ void __launch_bounds__(128) cross_join_kernel(const CrossParams p) {
 // ---- tiles of 128 rows on the tensor cores ----
 //
 // One CTA per (block of two row tiles, key head and split, sequence):
-//   warp 0     TMA: Q once, tiles of KEYS states of K and V into two rings;
+//   warp 0     TMA: Q once, tiles of KEYS states of K and V into two rings; it also clears the dropped
+//              states' rows of V tiles (past the end, masked) before they are used;
 //   warp 1     issues S = Q K^T (M 128, N KEYS, K = D) into the stream's TMEM columns and O += P V (A = P
 //              from TMEM, V as an MN-major operand) into its O columns;
 //   8 warps    softmax, four to a stream, one thread per row: its KEYS scores in registers, P (f16)
@@ -320,8 +321,9 @@ __global__ void __launch_bounds__(128) cross_join_kernel(const CrossParams p) {
 // they take its even and odd key tiles instead and add up their (m, l, O) at the end. S of the next
 // tile is issued behind P V of the last one, in order, so P may lie over S, and a full S means that the
 // products before it are done; one stream's softmax runs under the other's products.
-// Key tiles with dropped states (past the end, masked): their scores become -inf and their V rows zero
-// in shared memory, so that nothing they hold reaches a sum.
+// Key tiles with dropped states: their scores become -inf and their V rows zero in shared memory, so
+// that nothing they hold reaches a sum. (The rows cleared by the softmax warps, which then wait for V and
+// fence: 59 against XX us a CTA's loop, 301-499 queries on 700-1,500 states with one in seven masked.)
 //
 // Bound: the softmax threads. A row tile of 128 x 128 scores takes the special-function unit 1,024
 // cycles (4 lanes a clock on each quarter of the SM), its products 512 (D 64) or 1,024 (D 128). Heads of
@@ -350,8 +352,7 @@ struct TCfg {
   static constexpr int K_OFF = 2 * QTILE;
   static constexpr int V_OFF = K_OFF + KS * KTILE;
   static constexpr int BAR_OFF = V_OFF + VS * KTILE;
-  static constexpr int LUT_OFF = BAR_OFF + 256;             // 4 bits as 4 words, [16]
-  static constexpr int USED = LUT_OFF + 256 + 1024;
+  static constexpr int USED = BAR_OFF + 320 + 1024;
   // as much as keeps a third CTA (its TMEM) off the SM
   static constexpr int SMEM = ONE || USED > 100 * 1024 ? USED : 100 * 1024;
   static constexpr uint32_t S_STRIDE = ONE ? 128 : 64;      // TMEM: S of the streams, then O
@@ -424,11 +425,13 @@ __global__ void __launch_bounds__(TCfg<D>::THREADS, TCfg<D>::ONE ? 1 : 2)
   uint64_t* p_full = bars + 3;         // [stream][half]
   uint64_t* o_full = bars + 7;         // [stream]
   uint64_t* drain = bars + 9;
-  uint64_t* k_full = bars + 10;        // [KS]
+  uint64_t* v_tail = bars + 10;        // without a mask: the last tile's rows are cleared
+  uint64_t* k_full = bars + 11;        // [KS]
   uint64_t* k_empty = k_full + C::KS;
   uint64_t* v_full = k_empty + C::KS;  // [VS]
   uint64_t* v_empty = v_full + C::VS;
-  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(v_empty + C::VS);
+  uint64_t* v_clear = v_empty + C::VS;  // [VS] with a mask: the stage's dropped rows are cleared
+  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(v_clear + C::VS);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_holder + 1);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -462,15 +465,15 @@ __global__ void __launch_bounds__(TCfg<D>::THREADS, TCfg<D>::ONE ? 1 : 2)
     for (int i = 0; i < C::VS; ++i) {
       mbar_init(&v_full[i], 1);
       mbar_init(&v_empty[i], 1);
+      mbar_init(&v_clear[i], 1);
     }
+    mbar_init(v_tail, 1);
     *abort_flag = 0;
     fence_barrier_init();
     prefetch_tmap(&tmq);
     prefetch_tmap(&tmk);
     prefetch_tmap(&tmv);
   }
-  const uint4* lut4 = reinterpret_cast<const uint4*>(smem + C::LUT_OFF);
-  if (threadIdx.x < 64) reinterpret_cast<uint32_t*>(smem + C::LUT_OFF)[threadIdx.x] = (threadIdx.x >> 2 >> (threadIdx.x & 3)) & 1u ? ~0u : 0u;
   if (warp == 1) tmem_alloc(tmem_holder, C::COLS);
   fence_before_sync();
   __syncthreads();
@@ -482,34 +485,75 @@ __global__ void __launch_bounds__(TCfg<D>::THREADS, TCfg<D>::ONE ? 1 : 2)
 
   if (warp < C::FIRST) {
     if constexpr (C::ONE) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::REGS_ISSUE));
-    if (warp == 0 && lane == 0 && nkt > 0) {
-      bool ok = true;
+    if (warp == 0 && nkt > 0) {
       const int tiles = pair ? 2 : 1;
-      mbar_arrive_expect_tx(q_full, tiles * C::PANELS * qpt * G * C::ROWB);
-      for (int g = 0; g < tiles; ++g)
-        for (int c = 0; c < C::PANELS; ++c)
-          tma_load_3d(sQ + g * C::QTILE + c * C::QPANEL, &tmq, q_full, c * C::PCOLS, hk * G, int(q0) + qb + g * qpt);
+      if (lane == 0) {
+        mbar_arrive_expect_tx(q_full, tiles * C::PANELS * qpt * G * C::ROWB);
+        for (int g = 0; g < tiles; ++g)
+          for (int c = 0; c < C::PANELS; ++c)
+            tma_load_3d(sQ + g * C::QTILE + c * C::QPANEL, &tmq, q_full, c * C::PCOLS, hk * G, int(q0) + qb + g * qpt);
+      }
       uint32_t pend_k = 0, pend_v = 0;  // last issued parity per ring slot (bit 1: issued)
       auto load = [&](int j, bool is_v) -> bool {
-        const int stages = is_v ? C::VS : C::KS, st = j % stages;
-        const uint32_t u = uint32_t(j / stages) & 1;
+        if (j >= nkt) return true;
+        const int st = is_v ? j % C::VS : j % C::KS;
+        const uint32_t u = uint32_t(is_v ? j / C::VS : j / C::KS) & 1;
         uint64_t* full = is_v ? &v_full[st] : &k_full[st];
-        if (!mbar_wait(is_v ? &v_empty[st] : &k_empty[st], u ^ 1, is_v ? 102 : 101)) return false;
-        mbar_arrive_expect_tx(full, C::KTILE);
-        uint8_t* dst = (is_v ? sV : sK) + st * C::KTILE;
-        for (int c = 0; c < C::PANELS; ++c)
-          tma_load_2d(dst + c * C::KPANEL, is_v ? &tmv : &tmk, full, hk * D + c * C::PCOLS, int(k0) + (t0 + j) * KEYS);
+        if (!wwait(is_v ? &v_empty[st] : &k_empty[st], u ^ 1, is_v ? 102 : 101)) return false;
+        if (lane == 0) {
+          mbar_arrive_expect_tx(full, C::KTILE);
+          uint8_t* dst = (is_v ? sV : sK) + st * C::KTILE;
+          for (int c = 0; c < C::PANELS; ++c)
+            tma_load_2d(dst + c * C::KPANEL, is_v ? &tmv : &tmk, full, hk * D + c * C::PCOLS, int(k0) + (t0 + j) * KEYS);
+        }
+        __syncwarp();
         uint32_t& pend = is_v ? pend_v : pend_k;
         pend = (pend & ~(3u << (2 * st))) | ((2u | u) << (2 * st));
         return true;
       };
-      ok = load(0, false);
-      for (int j = 0; j < nkt && ok; ++j) {
-        if (j + 1 < nkt) ok = load(j + 1, false);
-        if (ok) ok = load(j, true);
+      // mask values of a tile's states, lane by lane (0 past the end), loaded a tile ahead
+      float mk[KEYS / 32];
+      auto load_mask = [&](int j) {
+#pragma unroll
+        for (int i = 0; i < KEYS / 32; ++i) {
+          const int jj = (t0 + j) * KEYS + 32 * i + lane;
+          mk[i] = jj < nk ? (p.mask ? __ldg(p.mask + k0 + jj) : 1.f) : 0.f;
+        }
+      };
+      // Tile j's rows are looked at before V of tile j + AHEAD is loaded, whose slot is free once the product
+      // of tile j - AHEAD is done: the clearing runs ahead of the products.
+      constexpr int AHEAD = C::VS / 2;
+      bool ok = load(0, false);
+      for (int j = 0; j < AHEAD && ok; ++j) ok = load(j + 1, false) && load(j, true);
+      if (p.mask) load_mask(0);
+      for (int j = 0; j < nkt && ok; ok = ok && load(j + AHEAD + 1, false) && load(j + AHEAD, true), ++j) {
+        if (!p.mask && (t0 + j + 1) * KEYS <= nk) continue;
+        if (!p.mask) load_mask(j);
+        const int st = j % C::VS;
+        uint32_t dropped = 0;  // bit i: state 32 i + lane of the tile
+#pragma unroll
+        for (int i = 0; i < KEYS / 32; ++i) dropped |= mk[i] > 0.5f ? 0u : 1u << i;
+        if (p.mask) load_mask(j + 1);
+        if (__any_sync(0xffffffffu, dropped != 0)) {
+          ok = wwait(&v_full[st], uint32_t(j / C::VS) & 1, 112);
+          if (!ok) break;
+          // a lane clears its own rows, starting at a piece of its own so that the lanes spread over the banks
+          constexpr int PIECES = C::ROWB / 16;
+#pragma unroll
+          for (int i = 0; i < KEYS / 32; ++i)
+            if ((dropped >> i) & 1u) {
+              uint8_t* row = sV + st * C::KTILE + (32 * i + lane) * C::ROWB;
+#pragma unroll
+              for (int e = 0; e < PIECES * C::PANELS; ++e)
+                *reinterpret_cast<uint4*>(row + e / PIECES * C::KPANEL + ((e + lane) % PIECES) * 16) = make_uint4(0, 0, 0, 0);
+            }
+          fence_proxy_async_smem();
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(p.mask ? &v_clear[st] : v_tail);
       }
       if (!ok) {
-        // every copy this thread issued lands before the CTA ends
+        // every copy this warp issued lands before the CTA ends
         *abort_flag = 1;
         mbar_wait(q_full, 0, 103);
         for (int i = 0; i < C::KS; ++i)
@@ -526,6 +570,7 @@ __global__ void __launch_bounds__(TCfg<D>::THREADS, TCfg<D>::ONE ? 1 : 2)
       // its first product and freed behind its last (stream 1's in a pair).
       const uint64_t dq0 = tile_desc<D>(sQ), dk0 = tile_desc<D>(sK), dv0 = tile_desc<D>(sV);
       constexpr uint64_t Q16 = uint64_t(C::QTILE >> 4), K16 = uint64_t(C::KTILE >> 4);
+      const bool ragged = (t0 + nkt) * KEYS > nk;  // the last tile has states past the end
       int ks = 0, vs = 0;       // ring stages of the next K and V tile
       uint32_t kp = 0, vp = 0;  // and their parities
       auto issue_s = [&](int g) -> bool {
@@ -551,7 +596,11 @@ __global__ void __launch_bounds__(TCfg<D>::THREADS, TCfg<D>::ONE ? 1 : 2)
         return true;
       };
       auto issue_o = [&](int g, int it, bool last) -> bool {
-        if ((!pair || g == 0) && !wwait(&v_full[vs], vp, 109)) return false;
+        if (!pair || g == 0) {
+          if (!wwait(&v_full[vs], vp, 109)) return false;
+          if (p.mask ? !wwait(&v_clear[vs], vp, 114) : (ragged && (pair ? it : 2 * it + g) == nkt - 1 && !wwait(v_tail, 0, 115)))
+            return false;
+        }
         const uint64_t dv = dv0 + vs * K16;
         const uint32_t pa = tmem + uint32_t(g) * C::S_STRIDE, oa = tmem + C::O_COL + uint32_t(g * D);
 #pragma unroll
@@ -644,30 +693,7 @@ __global__ void __launch_bounds__(TCfg<D>::THREADS, TCfg<D>::ONE ? 1 : 2)
 #pragma unroll
         for (int c = 0; c < W; ++c)
 #pragma unroll
-          for (int i = 0; i < 32; i += 4) {
-            const uint4 keep = lut4[(km[c] >> i) & 15u];
-            sr[c][i] = (sr[c][i] & keep.x) | (~keep.x & 0xFF800000u);
-            sr[c][i + 1] = (sr[c][i + 1] & keep.y) | (~keep.y & 0xFF800000u);
-            sr[c][i + 2] = (sr[c][i + 2] & keep.z) | (~keep.z & 0xFF800000u);
-            sr[c][i + 3] = (sr[c][i + 3] & keep.w) | (~keep.w & 0xFF800000u);
-          }
-        // a thread clears its share of the dropped V rows (in a pair both streams clear the same ones: zeros
-        // over zeros): a row of KEYS 128, half a row of KEYS 64
-        const int st = j % C::VS, vr = r % KEYS;
-        if (!wwait(&v_full[st], uint32_t(j / C::VS) & 1, 112)) { ok = false; break; }
-        uint32_t word = km[0];
-#pragma unroll
-        for (int c = 1; c < W; ++c) word = vr / 32 == c ? km[c] : word;
-        if (!((word >> lane) & 1u)) {
-          constexpr int BYTES = C::ROWB * KEYS / 128;
-#pragma unroll
-          for (int c = 0; c < C::PANELS; ++c) {
-            uint4* row = reinterpret_cast<uint4*>(sV + st * C::KTILE + c * C::KPANEL + vr * C::ROWB + r / KEYS * BYTES);
-#pragma unroll
-            for (int e = 0; e < BYTES / 16; ++e) row[e] = make_uint4(0, 0, 0, 0);
-          }
-        }
-        fence_proxy_async_smem();
+          for (int i = 0; i < 32; ++i) sr[c][i] = (km[c] >> i) & 1u ? sr[c][i] : 0xFF800000u;
       }
       float mr[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
