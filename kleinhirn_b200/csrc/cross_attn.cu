@@ -12,7 +12,7 @@
 // Which kernel: see takes_rows_kernel. Few rows to a key head (single tokens): bound by reading k and v
 // once, cross_rows_kernel. More: tensor-core products of 128 rows, cross_tile_kernel. Where the rows
 // leave SMs idle, the states of a sequence are split over CTAs, whose partial (m, l, O) the workspace
-// holds and cross_join_kernel adds up in split order.
+// holds and cross_join_kernel adds up in a fixed order.
 
 #include "device_ops.h"
 
@@ -58,15 +58,16 @@ __device__ __forceinline__ int64_t part_index(const CrossParams& p, int z, int s
   return ((int64_t(z) * p.n_seqs + s) * p.max_q + i) * p.q_heads + h;
 }
 
-// ---- few rows: registers straight from global memory, mma.sync ----
+// ---- few rows: one m16 block on mma.sync ----
 //
-// One CTA of 4 warps per (split, key head, sequence), rows <= 16 as one m16 block. A warp takes 16
-// states at a time: S = Q K^T in m16n8k16 products, then O += P V with S's accumulator layout as P's
-// operand layout. The sum over the head's values and the order of the states and output columns are
-// free, so every thread loads 16-byte pieces of k and v in the order they lie in memory, with no
-// shared memory and no shuffles: within 32 values of k, the quad lane t holds values 8 t .. 8 t + 7 of
-// q and k alike; of v, it holds the D / 8 values (lane / 4) D / 8 .. of its own four states. Loads
-// run one step ahead. Bound: HBM (2 D 2 bytes per state and key head, each read once).
+// One CTA of 4 warps per (split, key head, sequence), rows <= 16 as one m16 block. Each warp has a ring
+// of its own, filled by TMA with boxes of 16 states of K and V, and no other warp to wait for until the
+// end. A step of 16 states: S = Q K^T in m16n8k16 products, then O += P V with S's accumulator layout as
+// P's operand layout. The sum over the head's values and the order of the output columns are free, so a
+// thread takes 16-byte pieces of k and v as they lie: within 32 values of k, the quad lane t holds values
+// 8 t .. 8 t + 7 of q and k alike; of v, it holds the D / 8 values (lane / 4) D / 8 .. of its four states.
+// Bound: HBM (2 D 2 bytes per state and key head, each read once), by the bytes in flight: 64 requests of
+// one query on 200-512 states, 12 heads of 64, took 25 us with loads one step ahead in registers.
 
 __device__ __forceinline__ void mma_16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                           uint32_t b1) {
@@ -81,69 +82,67 @@ __device__ __forceinline__ uint32_t pack_half2(float a, float b) {
 }
 
 constexpr int RW = 4;      // warps of a CTA
-constexpr int RSTEP = 16;  // states of a warp's step
+constexpr int RSTEP = 16;  // states of a step
 
 template <int D>
-struct RowsStep {
-  uint4 k[2][D / 32];         // [block of 8 states][32 values]
-  uint32_t v[2][2][D / 16];   // [block][state of the pair][packed values]
-  bool keep[2][2];
+struct RCfg {
+  static constexpr int STAGES = D == 128 ? 3 : 4;
+  static constexpr int PANELS = D == 128 ? 2 : 1, PCOLS = D / PANELS, ROWB = PCOLS * 2;
+  static constexpr int PANEL = RSTEP * ROWB, TILE = PANELS * PANEL;  // 16 rows of k or v
+  static constexpr int RING = STAGES * 2 * TILE;                     // of a warp
+  static constexpr int PART = RW * 16 * (D + 4) * 4;                 // the warps' O at the end, over the rings
+  static constexpr int SMEM = (RW * RING > PART ? RW * RING : PART) + 1024;
+  // byte offset of 16-byte piece c of row r in a swizzled tile
+  static __device__ __forceinline__ int at(int r, int c) {
+    if (D == 32) return r * 64 + ((c ^ ((r >> 1) & 3)) * 16);
+    return (c >> 3) * PANEL + r * 128 + (((c & 7) ^ (r & 7)) * 16);
+  }
 };
 
 template <int D>
-__device__ __forceinline__ void rows_load(RowsStep<D>& r, const CrossParams& p, const __half* kb, const __half* vb,
-                                          const float* mb, int first, int end, int lane) {
-#pragma unroll
-  for (int b = 0; b < 2; ++b) {
-    const int j = first + 8 * b + (lane >> 2);
-#pragma unroll
-    for (int c = 0; c < D / 32; ++c) {
-      r.k[b][c] = make_uint4(0, 0, 0, 0);
-      if (j < end) r.k[b][c] = __ldg(reinterpret_cast<const uint4*>(kb + int64_t(j) * p.k_stride + c * 32 + (lane & 3) * 8));
-    }
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      const int jv = first + 8 * b + (lane & 3) * 2 + e;
-      const bool keep = jv < end && (!mb || __ldg(mb + jv) > 0.5f);
-      r.keep[b][e] = keep;
-      const __half* row = vb + int64_t(jv) * p.v_stride + (lane >> 2) * (D / 8);
-      // a dropped state's values are never loaded: whatever they hold stays out of the sums
-      if constexpr (D == 32) {
-        uint2 u = make_uint2(0, 0);
-        if (keep) u = __ldg(reinterpret_cast<const uint2*>(row));
-        r.v[b][e][0] = u.x;
-        r.v[b][e][1] = u.y;
-      } else {
-#pragma unroll
-        for (int c = 0; c < D / 64; ++c) {
-          uint4 u = make_uint4(0, 0, 0, 0);
-          if (keep) u = __ldg(reinterpret_cast<const uint4*>(row) + c);
-          r.v[b][e][4 * c] = u.x;
-          r.v[b][e][4 * c + 1] = u.y;
-          r.v[b][e][4 * c + 2] = u.z;
-          r.v[b][e][4 * c + 3] = u.w;
-        }
-      }
-    }
-  }
-}
-
-template <int D>
-__global__ void __launch_bounds__(RW * 32) cross_rows_kernel(const CrossParams p) {
+__global__ void __launch_bounds__(RW * 32)
+    cross_rows_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant__ CUtensorMap tmv, const CrossParams p) {
+  using C = RCfg<D>;
   constexpr int E = D / 8;  // output columns of 8 at a time
-  __shared__ float so[RW][16][D + 4];
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ uint64_t bars[RW][C::STAGES];
   __shared__ float sm[RW][16], sl[RW][16];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int split = blockIdx.x, hk = blockIdx.y, s = blockIdx.z;
+  if (lane == 0) {
+    for (int i = 0; i < C::STAGES; ++i) mbar_init(&bars[warp][i], 1);
+    fence_barrier_init();
+    if (warp == 0) {
+      prefetch_tmap(&tmk);
+      prefetch_tmap(&tmv);
+    }
+  }
+  __syncwarp();
   int64_t q0, k0;
   int nq, nk;
   seq_range(p.q_starts, s, p.q_rows, p.max_q, q0, nq);
   seq_range(p.k_starts, s, p.kv_rows, p.max_k, k0, nk);
   const int rows = nq * p.G;  // <= 16
   if (rows == 0) return;
-  // states of this split: whole steps of the CTA's warps
+  // states of this split, in whole steps
   const int per = ((nk + p.nsplit - 1) / p.nsplit + RSTEP - 1) / RSTEP * RSTEP;
   const int begin = min(split * per, nk), end = min(begin + per, nk);
+  const int steps = ((end - begin + RSTEP - 1) / RSTEP - warp + RW - 1) / RW;  // of this warp: warp, warp + 4, ..
+
+  uint8_t* ring = smem + warp * C::RING;
+  auto load = [&](int i) {  // step i of this warp into its stage
+    if (lane == 0) {
+      const int st = i % C::STAGES, y = int(k0) + begin + (i * RW + warp) * RSTEP;
+      uint64_t* bar = &bars[warp][st];
+      mbar_arrive_expect_tx(bar, 2 * C::TILE);
+      for (int c = 0; c < C::PANELS; ++c) {
+        tma_load_2d(ring + st * 2 * C::TILE + c * C::PANEL, &tmk, bar, hk * D + c * C::PCOLS, y);
+        tma_load_2d(ring + st * 2 * C::TILE + C::TILE + c * C::PANEL, &tmv, bar, hk * D + c * C::PCOLS, y);
+      }
+    }
+  };
+  for (int i = 0; i < min(steps, C::STAGES); ++i) load(i);
 
   // A operand: rows lane / 4 and lane / 4 + 8
   uint32_t qa[D / 32][2][4];
@@ -162,32 +161,67 @@ __global__ void __launch_bounds__(RW * 32) cross_rows_kernel(const CrossParams p
       qa[c][hl][3] = u.w;
     }
 
-  const __half* kb = p.k + k0 * p.k_stride + hk * D;
-  const __half* vb = p.v + k0 * p.v_stride + hk * D;
   const float* mb = p.mask ? p.mask + k0 : nullptr;
   float o[E][4];
 #pragma unroll
   for (int e = 0; e < E; ++e) o[e][0] = o[e][1] = o[e][2] = o[e][3] = 0.f;
   float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};  // rows lane / 4 and + 8; l of this thread's states
-
-  RowsStep<D> cur, nxt;
-  int first = begin + warp * RSTEP;
-  if (first < end) rows_load<D>(cur, p, kb, vb, mb, first, end, lane);
-  for (; first < end; first += RW * RSTEP) {
-    if (first + RW * RSTEP < end) rows_load<D>(nxt, p, kb, vb, mb, first + RW * RSTEP, end, lane);
+  bool ok = true;
+  int used = 0;  // steps whose loads have been waited for
+  for (int i = 0; i < steps; ++i) {
+    const int st = i % C::STAGES, first = begin + (i * RW + warp) * RSTEP;
+    bool keep[2][2];
+#pragma unroll
+    for (int b = 0; b < 2; ++b)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int j = first + 8 * b + (lane & 3) * 2 + e;
+        keep[b][e] = j < end && (!mb || __ldg(mb + j) > 0.5f);
+      }
+    if (!__all_sync(0xffffffffu, mbar_wait(&bars[warp][st], uint32_t(i / C::STAGES) & 1, 120))) {
+      ok = false;
+      break;
+    }
+    ++used;
+    const uint8_t* tk = ring + st * 2 * C::TILE;
+    const uint8_t* tv = tk + C::TILE;
     float sc[2][4];
 #pragma unroll
     for (int b = 0; b < 2; ++b) {
       sc[b][0] = sc[b][1] = sc[b][2] = sc[b][3] = 0.f;
 #pragma unroll
       for (int c = 0; c < D / 32; ++c) {
-        const uint4 kk = cur.k[b][c];
+        const uint4 kk = *reinterpret_cast<const uint4*>(tk + C::at(8 * b + (lane >> 2), 4 * c + (lane & 3)));
         mma_16816(sc[b], qa[c][0][0], qa[c][1][0], qa[c][0][1], qa[c][1][1], kk.x, kk.y);
         mma_16816(sc[b], qa[c][0][2], qa[c][1][2], qa[c][0][3], qa[c][1][3], kk.z, kk.w);
       }
 #pragma unroll
-      for (int i = 0; i < 4; ++i) sc[b][i] = cur.keep[b][i & 1] ? sc[b][i] * p.scale_log2 : -INFINITY;
+      for (int e = 0; e < 4; ++e) sc[b][e] = keep[b][e & 1] ? sc[b][e] * p.scale_log2 : -INFINITY;
     }
+    // v of this thread's states; a dropped one's values stay out of the sums whatever they hold
+    uint32_t v[2][2][D / 16];
+#pragma unroll
+    for (int b = 0; b < 2; ++b)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int r = 8 * b + (lane & 3) * 2 + e;
+        if constexpr (D == 32) {
+          const uint2 u = *reinterpret_cast<const uint2*>(tv + C::at(r, lane >> 3) + ((lane >> 2) & 1) * 8);
+          v[b][e][0] = keep[b][e] ? u.x : 0u;
+          v[b][e][1] = keep[b][e] ? u.y : 0u;
+        } else {
+#pragma unroll
+          for (int c = 0; c < D / 64; ++c) {
+            const uint4 u = *reinterpret_cast<const uint4*>(tv + C::at(r, (lane >> 2) * (D / 64) + c));
+            v[b][e][4 * c] = keep[b][e] ? u.x : 0u;
+            v[b][e][4 * c + 1] = keep[b][e] ? u.y : 0u;
+            v[b][e][4 * c + 2] = keep[b][e] ? u.z : 0u;
+            v[b][e][4 * c + 3] = keep[b][e] ? u.w : 0u;
+          }
+        }
+      }
+    __syncwarp();  // the stage has been read
+    if (i + C::STAGES < steps) load(i + C::STAGES);
     float top[2];
 #pragma unroll
     for (int r = 0; r < 2; ++r)
@@ -221,13 +255,16 @@ __global__ void __launch_bounds__(RW * 32) cross_rows_kernel(const CrossParams p
 #pragma unroll
     for (int e2 = 0; e2 < E / 2; ++e2) {
       // columns 2 e2 and 2 e2 + 1 of the thread's v values: pairs of states side by side
-      const uint32_t u0 = cur.v[0][0][e2], u1 = cur.v[0][1][e2], w0 = cur.v[1][0][e2], w1 = cur.v[1][1][e2];
+      const uint32_t u0 = v[0][0][e2], u1 = v[0][1][e2], w0 = v[1][0][e2], w1 = v[1][1][e2];
       mma_16816(o[2 * e2], pa[0][0], pa[0][1], pa[1][0], pa[1][1], __byte_perm(u0, u1, 0x5410), __byte_perm(w0, w1, 0x5410));
       mma_16816(o[2 * e2 + 1], pa[0][0], pa[0][1], pa[1][0], pa[1][1], __byte_perm(u0, u1, 0x7632),
                 __byte_perm(w0, w1, 0x7632));
     }
-    cur = nxt;
   }
+  if (!ok)  // every copy this warp issued lands before the rings are used again
+    for (int i = used; i < min(steps, used + C::STAGES); ++i) mbar_wait(&bars[warp][i % C::STAGES], uint32_t(i / C::STAGES) & 1, 121);
+  __syncthreads();
+  float* so = reinterpret_cast<float*>(smem);  // [warp][16][D + 4]
 #pragma unroll
   for (int r = 0; r < 2; ++r) {
     l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
@@ -237,11 +274,15 @@ __global__ void __launch_bounds__(RW * 32) cross_rows_kernel(const CrossParams p
       sm[warp][row] = m[r];
       sl[warp][row] = l[r];
     }
-    // column n = 2 (lane & 3) + i of block e is output value n E + e
+    if (row < rows) {
+      // column n = 2 (lane & 3) + i of block e is output value n E + e
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
+      for (int i = 0; i < 2; ++i)
 #pragma unroll
-      for (int e = 0; e < E; ++e) so[warp][row][(2 * (lane & 3) + i) * E + e] = o[e][2 * r + i];
+        for (int e = 0; e < E; e += 4)
+          *reinterpret_cast<float4*>(so + (warp * 16 + row) * (D + 4) + (2 * (lane & 3) + i) * E + e) =
+              make_float4(o[e][2 * r + i], o[e + 1][2 * r + i], o[e + 2][2 * r + i], o[e + 3][2 * r + i]);
+    }
   }
   __syncthreads();
   // the four warps' parts, 8 output values of a row per thread
@@ -256,7 +297,7 @@ __global__ void __launch_bounds__(RW * 32) cross_rows_kernel(const CrossParams p
       const float f = sm[w][row] == -INFINITY ? 0.f : ex2_approx(sm[w][row] - mm);
       lt += f * sl[w][row];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) acc[i] += f * so[w][row][d + i];
+      for (int i = 0; i < 8; ++i) acc[i] += f * so[(w * 16 + row) * (D + 4) + d + i];
     }
     const int qi = row / p.G, h = hk * p.G + row % p.G;
     if (p.nsplit == 1) {
@@ -275,37 +316,47 @@ __global__ void __launch_bounds__(RW * 32) cross_rows_kernel(const CrossParams p
   }
 }
 
-// ---- joining the splits: one warp per (query, head) ----
+// ---- joining the splits: one CTA of 4 warps per (query, head), a warp every fourth split ----
 
 template <int D>
 __global__ void __launch_bounds__(128) cross_join_kernel(const CrossParams p) {
   constexpr int V = D / 32;
-  const int lane = threadIdx.x & 31;
-  const int64_t t = int64_t(blockIdx.x) * 4 + (threadIdx.x >> 5);
+  __shared__ float so[4][D], sl[4];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t t = blockIdx.x;
   const int64_t per_seq = int64_t(p.max_q) * p.q_heads;
   const int s = int(t / per_seq);
-  if (s >= p.n_seqs) return;
   const int i = int((t - s * per_seq) / p.q_heads), h = int(t % p.q_heads);
   int64_t q0;
   int nq;
   seq_range(p.q_starts, s, p.q_rows, p.max_q, q0, nq);
   if (i >= nq) return;
-  float m = -INFINITY, l = 0.f, o[V] = {};
-  for (int z = 0; z < p.nsplit; ++z) {
+  // the largest reference point first (a lane per split), then the sums, with independent loads
+  float m = -INFINITY;
+  for (int z = lane; z < p.nsplit; z += 32) m = fmaxf(m, p.part_ml[part_index(p, z, s, i, h)].x);
+  for (int w = 16; w; w >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, w));
+  float l = 0.f, o[V] = {};
+#pragma unroll 4
+  for (int z = warp; z < p.nsplit; z += 4) {
     const int64_t at = part_index(p, z, s, i, h);
     const float2 ml = p.part_ml[at];
-    if (ml.x == -INFINITY) continue;  // no kept state (its O is not written)
-    const float mn = fmaxf(m, ml.x);
-    const float c = ex2_approx(m - mn), f = ex2_approx(ml.x - mn);
-    m = mn;
-    l = l * c + ml.y * f;
+    float v[V];
 #pragma unroll
-    for (int e = 0; e < V; ++e) o[e] = o[e] * c + p.part_o[at * D + lane * V + e] * f;
+    for (int e = 0; e < V; ++e) v[e] = p.part_o[at * D + lane * V + e];
+    const float f = ml.x == -INFINITY ? 0.f : ex2_approx(ml.x - m);
+    l += f * ml.y;
+#pragma unroll
+    for (int e = 0; e < V; ++e) o[e] += f == 0.f ? 0.f : f * v[e];  // (without a kept state O holds anything)
   }
-  const float inv = l == 0.f ? 0.f : 1.f / l;
-  __half* dst = p.out + (q0 + i) * p.out_stride + h * D + lane * V;
 #pragma unroll
-  for (int e = 0; e < V; ++e) dst[e] = __float2half_rn(o[e] * inv);
+  for (int e = 0; e < V; ++e) so[warp][lane * V + e] = o[e];
+  if (lane == 0) sl[warp] = l;
+  __syncthreads();
+  l = (sl[0] + sl[1]) + (sl[2] + sl[3]);
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  if (threadIdx.x < D)
+    p.out[(q0 + i) * p.out_stride + h * D + threadIdx.x] =
+        __float2half_rn(((so[0][threadIdx.x] + so[1][threadIdx.x]) + (so[2][threadIdx.x] + so[3][threadIdx.x])) * inv);
 }
 
 // ---- tiles of 128 rows on the tensor cores ----
@@ -322,8 +373,8 @@ __global__ void __launch_bounds__(128) cross_join_kernel(const CrossParams p) {
 // tile is issued behind P V of the last one, in order, so P may lie over S, and a full S means that the
 // products before it are done; one stream's softmax runs under the other's products.
 // Key tiles with dropped states: their scores become -inf and their V rows zero in shared memory, so
-// that nothing they hold reaches a sum. (The rows cleared by the softmax warps, which then wait for V and
-// fence: 59 against XX us a CTA's loop, 301-499 queries on 700-1,500 states with one in seven masked.)
+// that nothing they hold reaches a sum. (Cleared by the softmax warps, which then wait for V and fence:
+// 74 us against 62, 301-499 queries on 700-1,500 states with one in seven masked, 16 sequences.)
 //
 // Bound: the softmax threads. A row tile of 128 x 128 scores takes the special-function unit 1,024
 // cycles (4 lanes a clock on each quarter of the SM), its products 512 (D 64) or 1,024 (D 128). Heads of
@@ -856,8 +907,25 @@ int64_t round256(int64_t n) { return (n + 255) / 256 * 256; }
 
 template <int D>
 void launch(const CrossParams& p, const kh_cross_attention_args& a, bool states, cudaStream_t st) {
+  CUtensorMap tk, tv;
+  auto state_maps = [&](int box_cols, int box_rows, int row_bytes) {
+    const uint64_t cols = uint64_t(a.kv_heads) * D;
+    encode_tensor_map_f16(&tk, a.k, uint64_t(a.kv_rows), cols, uint64_t(a.k_stride), uint32_t(box_cols), uint32_t(box_rows), row_bytes);
+    encode_tensor_map_f16(&tv, a.v, uint64_t(a.kv_rows), cols, uint64_t(a.v_stride), uint32_t(box_cols), uint32_t(box_rows), row_bytes);
+  };
   if (takes_rows_kernel(a)) {
-    cross_rows_kernel<D><<<dim3(p.nsplit, p.kv_heads, p.n_seqs), RW * 32, 0, st>>>(p);
+    using C = RCfg<D>;
+    static std::atomic<uint64_t> configured{0};
+    once_per_device(configured, [] {
+      KH_CUDA(cudaFuncSetAttribute(cross_rows_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
+    });
+    // (without states no map is read; any valid one will do)
+    if (states) state_maps(C::PCOLS, RSTEP, C::ROWB);
+    else {
+      encode_tensor_map_f16(&tk, a.q, uint64_t(a.q_rows), uint64_t(a.q_heads) * D, uint64_t(a.q_stride), C::PCOLS, RSTEP, C::ROWB);
+      tv = tk;
+    }
+    cross_rows_kernel<D><<<dim3(p.nsplit, p.kv_heads, p.n_seqs), RW * 32, C::SMEM, st>>>(tk, tv, p);
   } else {
     using C = TCfg<D>;
     static std::atomic<uint64_t> configured{0};
@@ -865,22 +933,18 @@ void launch(const CrossParams& p, const kh_cross_attention_args& a, bool states,
       KH_CUDA(cudaFuncSetAttribute(cross_tile_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
     });
     const int qpt = TROWS / p.G;
-    CUtensorMap tq, tk, tv;
+    CUtensorMap tq;
     encode_tensor_map_f16_3d(&tq, a.q, {uint64_t(D), uint64_t(a.q_heads), uint64_t(a.q_rows)}, D, uint64_t(a.q_stride),
                              {uint32_t(C::PCOLS), uint32_t(p.G), uint32_t(qpt)}, C::ROWB);
-    tk = tv = tq;  // (without states neither is read)
-    if (states) {
-      const uint64_t cols = uint64_t(a.kv_heads) * D;
-      encode_tensor_map_f16(&tk, a.k, uint64_t(a.kv_rows), cols, uint64_t(a.k_stride), C::PCOLS, C::KEYS, C::ROWB);
-      encode_tensor_map_f16(&tv, a.v, uint64_t(a.kv_rows), cols, uint64_t(a.v_stride), C::PCOLS, C::KEYS, C::ROWB);
-    }
+    if (states) state_maps(C::PCOLS, C::KEYS, C::ROWB);
+    else tk = tv = tq;
     const dim3 grid(unsigned((a.max_q + 2 * qpt - 1) / (2 * qpt)), unsigned(a.kv_heads * p.nsplit), unsigned(a.n_seqs));
     cross_tile_kernel<D><<<grid, C::THREADS, C::SMEM, st>>>(tq, tk, tv, p);
   }
   KH_CUDA(cudaGetLastError());
   if (p.nsplit > 1) {
     const int64_t rows = int64_t(p.n_seqs) * p.max_q * p.q_heads;
-    cross_join_kernel<D><<<unsigned((rows + 3) / 4), 128, 0, st>>>(p);
+    cross_join_kernel<D><<<unsigned(rows), 128, 0, st>>>(p);
     KH_CUDA(cudaGetLastError());
   }
 }
