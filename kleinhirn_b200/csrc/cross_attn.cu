@@ -60,7 +60,7 @@ __device__ __forceinline__ int64_t part_index(const CrossParams& p, int z, int s
 
 // ---- few rows: one m16 block on mma.sync ----
 //
-// One CTA of 4 warps per (split, key head, sequence), rows <= 16 as one m16 block. Each warp has a ring
+// One CTA of RW warps per (split, key head, sequence), rows <= 16 as one m16 block. Each warp has a ring
 // of its own, filled by TMA with boxes of 16 states of K and V, and no other warp to wait for until the
 // end. A step of 16 states: S = Q K^T in m16n8k16 products, then O += P V with S's accumulator layout as
 // P's operand layout. The sum over the head's values and the order of the output columns are free, so a
@@ -81,10 +81,9 @@ __device__ __forceinline__ uint32_t pack_half2(float a, float b) {
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-constexpr int RW = 4;      // warps of a CTA
 constexpr int RSTEP = 16;  // states of a step
 
-template <int D>
+template <int D, int RW>
 struct RCfg {
   static constexpr int STAGES = D == 128 ? 3 : 4;
   static constexpr int PANELS = D == 128 ? 2 : 1, PCOLS = D / PANELS, ROWB = PCOLS * 2;
@@ -99,10 +98,10 @@ struct RCfg {
   }
 };
 
-template <int D>
+template <int D, int RW>
 __global__ void __launch_bounds__(RW * 32)
     cross_rows_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant__ CUtensorMap tmv, const CrossParams p) {
-  using C = RCfg<D>;
+  using C = RCfg<D, RW>;
   constexpr int E = D / 8;  // output columns of 8 at a time
   extern __shared__ uint8_t smem_raw[];
   __shared__ uint64_t bars[RW][C::STAGES];
@@ -128,7 +127,7 @@ __global__ void __launch_bounds__(RW * 32)
   // states of this split, in whole steps
   const int per = ((nk + p.nsplit - 1) / p.nsplit + RSTEP - 1) / RSTEP * RSTEP;
   const int begin = min(split * per, nk), end = min(begin + per, nk);
-  const int steps = ((end - begin + RSTEP - 1) / RSTEP - warp + RW - 1) / RW;  // of this warp: warp, warp + 4, ..
+  const int steps = ((end - begin + RSTEP - 1) / RSTEP - warp + RW - 1) / RW;  // of this warp: warp, warp + RW, ..
 
   uint8_t* ring = smem + warp * C::RING;
   auto load = [&](int i) {  // step i of this warp into its stage
@@ -285,7 +284,7 @@ __global__ void __launch_bounds__(RW * 32)
     }
   }
   __syncthreads();
-  // the four warps' parts, 8 output values of a row per thread
+  // the warps' parts, 8 output values of a row per thread
   for (int t = threadIdx.x; t < rows * (D / 8); t += RW * 32) {
     const int row = t / (D / 8), d = t % (D / 8) * 8;
     float mm = -INFINITY;
@@ -393,7 +392,7 @@ struct TCfg {
   static constexpr int FIRST = ONE ? 4 : 2;          // first softmax warp (setmaxnreg acts on whole warpgroups)
   static constexpr int THREADS = 32 * (FIRST + 8);
   // 56 x 128 + 224 x 256 = 168 x 384, the registers of the launch
-  static constexpr int REGS_ISSUE = 56, REGS_SOFTMAX = 224;
+  static constexpr int REGS_ISSUE = 56, REGS_SOFTMAX = 224;  // (ONE)
   static constexpr int PANELS = ONE ? 2 : 1;         // columns of a swizzled row: 64 (D 32: 32)
   static constexpr int PCOLS = D / PANELS;
   static constexpr int ROWB = PCOLS * 2;             // bytes of a row of a panel: the swizzle width
@@ -535,7 +534,7 @@ __global__ void __launch_bounds__(TCfg<D>::THREADS, TCfg<D>::ONE ? 1 : 2)
   };
 
   if (warp < C::FIRST) {
-    if constexpr (C::ONE) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::REGS_ISSUE));
+    if (C::ONE) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::REGS_ISSUE));
     if (warp == 0 && nkt > 0) {
       const int tiles = pair ? 2 : 1;
       if (lane == 0) {
@@ -688,7 +687,7 @@ __global__ void __launch_bounds__(TCfg<D>::THREADS, TCfg<D>::ONE ? 1 : 2)
       }
     }
   } else {
-    if constexpr (C::ONE) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::REGS_SOFTMAX));
+    if (C::ONE) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::REGS_SOFTMAX));
     const int g = (warp - C::FIRST) >> 2;
     const int quarter = warp & 3;
     const int r = quarter * 32 + lane;  // row of the tile = TMEM lane
@@ -899,11 +898,20 @@ int splits(const kh_cross_attention_args& a) {
   const int64_t blocks = few ? 1 : (int64_t(a.max_q) + 2 * (TROWS / G) - 1) / (2 * (TROWS / G));
   const int64_t ctas = std::max<int64_t>(1, blocks * a.kv_heads * a.n_seqs);
   const int64_t want = (few ? 4 * SMS : a.head_dim == 128 ? SMS : 2 * SMS) / ctas;
-  const int64_t most = few ? a.max_k / (4 * RW * RSTEP) : a.max_k / 512;
+  const int64_t most = few ? a.max_k / 256 : a.max_k / 512;
   return int(std::min<int64_t>(std::max<int64_t>(1, std::min(want, most)), 64));
 }
 
 int64_t round256(int64_t n) { return (n + 255) / 256 * 256; }
+
+template <int D, int RW>
+void launch_rows(const CUtensorMap& tk, const CUtensorMap& tv, const CrossParams& p, cudaStream_t st) {
+  static std::atomic<uint64_t> configured{0};
+  once_per_device(configured, [] {
+    KH_CUDA(cudaFuncSetAttribute(cross_rows_kernel<D, RW>, cudaFuncAttributeMaxDynamicSharedMemorySize, RCfg<D, RW>::SMEM));
+  });
+  cross_rows_kernel<D, RW><<<dim3(p.nsplit, p.kv_heads, p.n_seqs), RW * 32, RCfg<D, RW>::SMEM, st>>>(tk, tv, p);
+}
 
 template <int D>
 void launch(const CrossParams& p, const kh_cross_attention_args& a, bool states, cudaStream_t st) {
@@ -914,18 +922,19 @@ void launch(const CrossParams& p, const kh_cross_attention_args& a, bool states,
     encode_tensor_map_f16(&tv, a.v, uint64_t(a.kv_rows), cols, uint64_t(a.v_stride), uint32_t(box_cols), uint32_t(box_rows), row_bytes);
   };
   if (takes_rows_kernel(a)) {
-    using C = RCfg<D>;
-    static std::atomic<uint64_t> configured{0};
-    once_per_device(configured, [] {
-      KH_CUDA(cudaFuncSetAttribute(cross_rows_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
-    });
     // (without states no map is read; any valid one will do)
+    using C = RCfg<D, 4>;
     if (states) state_maps(C::PCOLS, RSTEP, C::ROWB);
     else {
       encode_tensor_map_f16(&tk, a.q, uint64_t(a.q_rows), uint64_t(a.q_heads) * D, uint64_t(a.q_stride), C::PCOLS, RSTEP, C::ROWB);
       tv = tk;
     }
-    cross_rows_kernel<D><<<dim3(p.nsplit, p.kv_heads, p.n_seqs), RW * 32, C::SMEM, st>>>(tk, tv, p);
+    // Few CTAs are over soonest with four warps each (one request, 12 heads, 128 states: 3.6 us against
+    // 4.5 with two); many, that run one after another on an SM, with two (64 requests, 12 heads, 200-512
+    // states: 17.5 us against 20.6).
+    const bool many = int64_t(p.n_seqs) * p.kv_heads * p.nsplit >= 2 * SMS;
+    if (many) launch_rows<D, 2>(tk, tv, p, st);
+    else launch_rows<D, 4>(tk, tv, p, st);
   } else {
     using C = TCfg<D>;
     static std::atomic<uint64_t> configured{0};
