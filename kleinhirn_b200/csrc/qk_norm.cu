@@ -42,17 +42,36 @@ struct NormParams {
   bool interleaved;
 };
 
+// A chunk of VEC values, moved as one word of its size (a copy of an array of halves is VEC loads).
+template <int BYTES> struct Word;
+template <> struct Word<16> { typedef uint4 type; };
+template <> struct Word<8> { typedef uint2 type; };
+template <> struct Word<4> { typedef uint32_t type; };
+template <> struct Word<2> { typedef uint16_t type; };
 template <typename T, int VEC>
-struct alignas(sizeof(T) * VEC) Chunk {
-  T v[VEC];
+struct Chunk {
+  typedef typename Word<sizeof(T) * VEC>::type W;
+  W w;
+  __device__ __forceinline__ float get(int i) const { return float(reinterpret_cast<const T*>(&w)[i]); }
+  __device__ __forceinline__ void set(int i, float f) { reinterpret_cast<T*>(&w)[i] = T(f); }
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int i = 0; i < int(sizeof(W) / (sizeof(W) >= 4 ? 4 : 2)); ++i) {
+      if (sizeof(W) >= 4) reinterpret_cast<uint32_t*>(&w)[i] = 0u;
+      else reinterpret_cast<uint16_t*>(&w)[i] = 0;
+    }
+  }
+  __device__ __forceinline__ void load(const T* p) { w = *reinterpret_cast<const W*>(p); }
+  __device__ __forceinline__ void store(T* p) const { *reinterpret_cast<W*>(p) = w; }
 };
 
 // N consecutive f32 values, in loads as wide as N allows.
 template <int N>
 __device__ __forceinline__ void load_f32(float (&f)[N], const float* p) {
-  const Chunk<float, N> c = *reinterpret_cast<const Chunk<float, N>*>(p);
+  Chunk<float, N> c;
+  c.load(p);
 #pragma unroll
-  for (int i = 0; i < N; ++i) f[i] = c.v[i];
+  for (int i = 0; i < N; ++i) f[i] = c.get(i);
 }
 template <>
 __device__ __forceinline__ void load_f32<8>(float (&f)[8], const float* p) {
@@ -121,11 +140,11 @@ __global__ void __launch_bounds__(256) qk_norm_rope_kernel(const NormParams p, i
   for (int u = 0; u < U; ++u)
 #pragma unroll
     for (int i = 0; i < PAIRS; ++i) {
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) a[u][i].v[e] = b[u][i].v[e] = T(0.f);
+      a[u][i].clear();
+      b[u][i].clear();
       if (u < nheads) {
-        if (c0[i] >= 0) a[u][i] = *reinterpret_cast<const Chunk<T, VEC>*>(xr + u * p.D + c0[i] * VEC);
-        if (c1[i] >= 0) b[u][i] = *reinterpret_cast<const Chunk<T, VEC>*>(xr + u * p.D + c1[i] * VEC);
+        if (c0[i] >= 0) a[u][i].load(xr + u * p.D + c0[i] * VEC);
+        if (c1[i] >= 0) b[u][i].load(xr + u * p.D + c1[i] * VEC);
       }
     }
 
@@ -145,7 +164,7 @@ __global__ void __launch_bounds__(256) qk_norm_rope_kernel(const NormParams p, i
     for (int i = 0; i < PAIRS; ++i)
 #pragma unroll
       for (int e = 0; e < VEC; ++e) {
-        const float f = float(a[u][i].v[e]), g = float(b[u][i].v[e]);
+        const float f = a[u][i].get(e), g = b[u][i].get(e);
         s0 = fmaf(f, f, s0);
         s1 = fmaf(g, g, s1);
       }
@@ -179,8 +198,8 @@ __global__ void __launch_bounds__(256) qk_norm_rope_kernel(const NormParams p, i
       float f[VEC], g[VEC], y0[VEC], y1[VEC];
 #pragma unroll
       for (int e = 0; e < VEC; ++e) {
-        f[e] = float(a[u][i].v[e]);
-        g[e] = float(b[u][i].v[e]);
+        f[e] = a[u][i].get(e);
+        g[e] = b[u][i].get(e);
       }
       // the partner of a value: in the other chunk, or beside it in its own (VEC 1: the other chunk)
       if (far || (VEC == 1 && near0)) {
@@ -214,12 +233,12 @@ __global__ void __launch_bounds__(256) qk_norm_rope_kernel(const NormParams p, i
       }
       Chunk<T, VEC> o;
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) o.v[e] = T(bad ? 0.f : y0[e] * scale[u]);
-      *reinterpret_cast<Chunk<T, VEC>*>(yr + u * p.D + d0) = o;
+      for (int e = 0; e < VEC; ++e) o.set(e, bad ? 0.f : y0[e] * scale[u]);
+      o.store(yr + u * p.D + d0);
       if (two) {
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) o.v[e] = T(bad ? 0.f : y1[e] * scale[u]);
-        *reinterpret_cast<Chunk<T, VEC>*>(yr + u * p.D + d1) = o;
+        for (int e = 0; e < VEC; ++e) o.set(e, bad ? 0.f : y1[e] * scale[u]);
+        o.store(yr + u * p.D + d1);
       }
     }
   }
