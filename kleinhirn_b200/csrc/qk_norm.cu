@@ -19,6 +19,7 @@
 #include <algorithm>
 
 #include "runtime.h"
+#include "sm100.cuh"
 #include "tmap.h"
 
 namespace kh {
@@ -60,6 +61,19 @@ struct Chunk {
       if (sizeof(W) >= 4) reinterpret_cast<uint32_t*>(&w)[i] = 0u;
       else reinterpret_cast<uint16_t*>(&w)[i] = 0;
     }
+  }
+  __device__ __forceinline__ float2 pair(int i) const {
+    if constexpr (sizeof(T) == 2) return __half22float2(reinterpret_cast<const __half2*>(&w)[i / 2]);
+    else return reinterpret_cast<const float2*>(&w)[i / 2];
+  }
+  __device__ __forceinline__ void set_pair(int i, float2 f) {
+    if constexpr (sizeof(T) == 2) reinterpret_cast<__half2*>(&w)[i / 2] = __float22half2_rn(f);
+    else reinterpret_cast<float2*>(&w)[i / 2] = f;
+  }
+  __device__ __forceinline__ void shuffle(int src) {
+#pragma unroll
+    for (int i = 0; i < int(sizeof(W) / 4); ++i)
+      reinterpret_cast<uint32_t*>(&w)[i] = __shfl_sync(0xffffffffu, reinterpret_cast<uint32_t*>(&w)[i], src);
   }
   __device__ __forceinline__ void load(const T* p) { w = *reinterpret_cast<const W*>(p); }
   __device__ __forceinline__ void store(T* p) const { *reinterpret_cast<W*>(p) = w; }
@@ -104,7 +118,118 @@ __device__ __forceinline__ void coefficients(float (&wc)[VEC], float (&ws)[VEC],
   }
 }
 
-// PAIRS: chunk pairs of a thread (1, or 4 for the one-value chunks of unaligned heads). LANES * PAIRS
+// The usual heads (up to 32 chunks): a thread owns one chunk of U heads of a row, so a warp's loads and
+// stores are whole heads side by side; the chunk that the rotation mixes with comes from its lane. MODE:
+// 0 no rotation, 1 pairs R / 2 apart, 2 neighbouring pairs. Next to the loads it is the instructions that
+// count (packed f32x2 arithmetic, one mode to a kernel): 65,536 rows of 24 heads of 64 take 77 us (5.3 TB/s;
+// 91 us with every mode in one kernel, 160 instructions to a chunk, and 83 us with the kernel below).
+template <typename T, int VEC, int U, int MODE>
+__global__ void __launch_bounds__(256) qk_norm_rope_lanes_kernel(const NormParams p, int lanes_log2) {
+  const uint32_t lanes = 1u << lanes_log2;
+  const uint32_t thread = blockIdx.x * 256u + threadIdx.x;
+  const int c = int(thread & (lanes - 1));  // chunk
+  const uint32_t group = thread >> lanes_log2;
+  const uint32_t row = group / p.blocks, block = group - row * p.blocks;
+  const bool in = group < p.groups && c < p.D / VEC;  // (all stay for the shuffles)
+  const bool is_k = block >= p.q_blocks;
+  const int head0 = int(is_k ? block - p.q_blocks : block) * U;
+  const int nheads = in ? min(U, (is_k ? p.k_heads : p.q_heads) - head0) : 0;
+  const int d = c * VEC;
+
+  int pos = 0;
+  if (MODE && in) pos = __ldg(p.positions + row);  // (first: the angles depend on it)
+  const int64_t col = int64_t((is_k ? p.q_heads : 0) + head0) * p.D + d;
+  const T* xr = static_cast<const T*>(p.x) + row * p.x_stride + col;
+  Chunk<T, VEC> a[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    a[u].clear();
+    if (u < nheads) a[u].load(xr + u * p.D);
+  }
+  // y = (x wc + partner's x ws) * scale: ws is the partner's weight times the sine, with its sign
+  const float* w = is_k ? p.kw : p.qw;
+  float wc[VEC], ws[VEC];
+#pragma unroll
+  for (int e = 0; e < VEC; ++e) wc[e] = 1.f, ws[e] = 0.f;
+  if (in && w) load_f32<VEC>(wc, w + d);
+  const int half = p.R / 2 / VEC;  // chunks of half the rotated part
+  const bool turned = MODE && in && d < p.R;
+  int other = c;
+  if constexpr (MODE != 0) {
+    if (pos < 0 || pos >= p.table_rows) {  // the row comes out zero
+      atomicExch(&kh_norm_error, OP_BAD_INDEX);
+      pos = 0;
+#pragma unroll
+      for (int u = 0; u < U; ++u) a[u].clear();
+    }
+    const float* cs = p.cossin + int64_t(pos) * 2 * p.R;
+    if (MODE == 1 && turned) {
+      other = c < half ? c + half : c - half;
+      float co[VEC], si[VEC], wo[VEC];
+      const int angle = (c < half ? c : other) * VEC;
+      load_f32<VEC>(co, cs + angle);
+      load_f32<VEC>(si, cs + p.R + angle);
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) wo[e] = 1.f;
+      if (w) load_f32<VEC>(wo, w + other * VEC);
+      const float sign = c < half ? -1.f : 1.f;
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        ws[e] = sign * wo[e] * si[e];
+        wc[e] *= co[e];
+      }
+    } else if (MODE == 2 && turned) {
+      float co[VEC / 2], si[VEC / 2];
+      load_f32<VEC / 2>(co, cs + d / 2);
+      load_f32<VEC / 2>(si, cs + p.R + d / 2);
+#pragma unroll
+      for (int e = 0; e < VEC; e += 2) {
+        ws[e] = -wc[e + 1] * si[e / 2];
+        ws[e + 1] = wc[e] * si[e / 2];
+        wc[e] *= co[e / 2];
+        wc[e + 1] *= co[e / 2];
+      }
+    }
+  }
+
+  float scale[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    float2 ss = make_float2(0.f, 0.f);
+#pragma unroll
+    for (int e = 0; e < VEC; e += 2) ss = sm100::ffma2(a[u].pair(e), a[u].pair(e), ss);
+    scale[u] = ss.x + ss.y;
+  }
+  for (uint32_t o = lanes >> 1; o; o >>= 1)
+#pragma unroll
+    for (int u = 0; u < U; ++u) scale[u] += __shfl_xor_sync(0xffffffffu, scale[u], o);
+
+  const int src = (threadIdx.x & 31) - c + other;
+  T* yr = static_cast<T*>(p.out) + row * p.out_stride + col;
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const float sc = rsqrtf(fmaf(scale[u], p.inv_d, p.eps));
+    Chunk<T, VEC> b = a[u];
+    if (MODE == 1) b.shuffle(src);
+    // (an unturned value has no partner: 0 times an infinity next to it must not reach it)
+    if (MODE && !turned) b.clear();
+    if (u >= nheads) continue;
+    Chunk<T, VEC> o;
+#pragma unroll
+    for (int e = 0; e < VEC; e += 2) {
+      float2 y = sm100::fmul2(a[u].pair(e), make_float2(wc[e], wc[e + 1]));
+      if (MODE) {
+        float2 g = b.pair(e);
+        if (MODE == 2) g = make_float2(g.y, g.x);
+        y = sm100::ffma2(g, make_float2(ws[e], ws[e + 1]), y);
+      }
+      o.set_pair(e, sm100::fmul2(y, make_float2(sc, sc)));
+    }
+    o.store(yr + u * p.D);
+  }
+}
+
+// Heads of more chunks, and unaligned ones. PAIRS: chunk pairs of a thread (1, or 4 for the one-value chunks of unaligned heads). LANES * PAIRS
 // pairs cover D <= 256.
 template <typename T, int VEC, int PAIRS, int U>
 __global__ void __launch_bounds__(256) qk_norm_rope_kernel(const NormParams p, int lanes_log2) {
@@ -244,11 +369,12 @@ __global__ void __launch_bounds__(256) qk_norm_rope_kernel(const NormParams p, i
   }
 }
 
+// PAIRS 0: the kernel with one chunk to a thread.
 template <typename T, int VEC, int PAIRS, int U>
 void launch(NormParams p, int64_t rows, cudaStream_t st) {
-  const int pairs = (p.D / VEC + 1) / 2;
+  const int units = PAIRS ? (p.D / VEC + 1) / 2 : p.D / VEC;
   int log2 = 0;
-  while ((PAIRS << log2) < pairs) ++log2;
+  while ((std::max(PAIRS, 1) << log2) < units) ++log2;
   p.q_blocks = uint32_t((p.q_heads + U - 1) / U);
   p.blocks = p.q_blocks + uint32_t((p.k_heads + U - 1) / U);
   // 32-bit thread indexes: launches of as many whole rows as stay below 2^31 threads
@@ -261,7 +387,14 @@ void launch(NormParams p, int64_t rows, cudaStream_t st) {
     q.out = static_cast<T*>(p.out) + r * p.out_stride;
     if (p.R) q.positions = p.positions + r;
     const int64_t threads = (int64_t(q.groups) << log2);
-    qk_norm_rope_kernel<T, VEC, PAIRS, U><<<unsigned((threads + 255) / 256), 256, 0, st>>>(q, log2);
+    const unsigned grid = unsigned((threads + 255) / 256);
+    if constexpr (PAIRS == 0) {
+      if (!p.R) qk_norm_rope_lanes_kernel<T, VEC, U, 0><<<grid, 256, 0, st>>>(q, log2);
+      else if (!p.interleaved) qk_norm_rope_lanes_kernel<T, VEC, U, 1><<<grid, 256, 0, st>>>(q, log2);
+      else qk_norm_rope_lanes_kernel<T, VEC, U, 2><<<grid, 256, 0, st>>>(q, log2);
+    } else {
+      qk_norm_rope_kernel<T, VEC, PAIRS, U><<<grid, 256, 0, st>>>(q, log2);
+    }
   }
   KH_CUDA(cudaGetLastError());
 }
@@ -343,11 +476,12 @@ void qk_norm_rope(const kh_qk_norm_rope_args* args, cudaStream_t st) {
   p.inv_d = 1.f / float(a.head_dim);
   p.interleaved = a.interleaved != 0;
   if (a.dtype == KH_F16) {
-    if (fits(a, 2, 8)) launch<__half, 8, 1, 4>(p, a.rows, st);
-    else if (fits(a, 2, 4)) launch<__half, 4, 1, 4>(p, a.rows, st);
+    if (fits(a, 2, 8)) launch<__half, 8, 0, 4>(p, a.rows, st);
+    else if (fits(a, 2, 4) && a.head_dim <= 128) launch<__half, 4, 0, 4>(p, a.rows, st);
     else launch<__half, 1, 4, 1>(p, a.rows, st);
   } else {
-    if (fits(a, 4, 4)) launch<float, 4, 1, 4>(p, a.rows, st);
+    if (fits(a, 4, 4) && a.head_dim <= 128) launch<float, 4, 0, 4>(p, a.rows, st);
+    else if (fits(a, 4, 4)) launch<float, 4, 1, 2>(p, a.rows, st);
     else launch<float, 1, 4, 1>(p, a.rows, st);
   }
 }
