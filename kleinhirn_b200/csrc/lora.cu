@@ -150,6 +150,70 @@ __device__ __forceinline__ float ld_cluster_f32(uint32_t addr) {
   return v;
 }
 
+// The outputs n0 + c of groups of RG rows of x, dealt to the cluster's CTAs and the two warps of these
+// outputs: the parts of the sum, the bias and the dot product with h, rounded once.
+template <int RG>
+__device__ __forceinline__ void few_outputs(const LoraParams& p, const float* part, const int* ids, const __half* h, int n0,
+                                            int t0, int nt, int z, int Z, int c, int half) {
+  const int n = n0 + c;
+  if (n >= p.n) return;
+  const float bias = p.bias ? __half2float(p.bias[n]) : 0.f;
+  const int chunks = p.rank / 8;
+  for (int g = z * 2 + half; g * RG < nt; g += 2 * Z) {
+    float v[RG];
+    int ad[RG];
+    bool any = false, same = true;
+#pragma unroll
+    for (int j = 0; j < RG; ++j) {
+      const int i = g * RG + j;
+      v[j] = bias;
+      ad[j] = i < nt ? ids[i] : -1;
+      any |= ad[j] >= 0;
+      same &= ad[j] == ad[0];
+    }
+    if (Z == 1) {
+#pragma unroll
+      for (int j = 0; j < RG; ++j) v[j] += part[(g * RG + j) * 128 + c];
+    } else {
+      float u[RG][8];
+#pragma unroll
+      for (int q = 0; q < 8; ++q)
+#pragma unroll
+        for (int j = 0; j < RG; ++j)
+          u[j][q] = q < Z ? ld_cluster_f32(cluster_addr(part + (g * RG + j) * 128 + c, uint32_t(q))) : 0.f;
+#pragma unroll
+      for (int q = 0; q < 8; ++q)
+#pragma unroll
+        for (int j = 0; j < RG; ++j) v[j] += u[j][q];
+    }
+    if (any && same) {  // the rows of one adapter: its row of B once
+      const uint4* b = reinterpret_cast<const uint4*>(p.b + (int64_t(ad[0]) * p.n + n) * p.rank);
+#pragma unroll 8
+      for (int r = 0; r < chunks; ++r) {
+        const uint4 br = __ldg(b + r);
+#pragma unroll
+        for (int j = 0; j < RG; ++j) v[j] = dot8(*reinterpret_cast<const uint4*>(h + (g * RG + j) * p.rank + 8 * r), br, v[j]);
+      }
+    } else if (any) {
+#pragma unroll 2
+      for (int r = 0; r < chunks; ++r) {
+        uint4 b[RG];
+#pragma unroll
+        for (int j = 0; j < RG; ++j) {
+          b[j] = make_uint4(0, 0, 0, 0);
+          if (ad[j] >= 0) b[j] = __ldg(reinterpret_cast<const uint4*>(p.b + (int64_t(ad[j]) * p.n + n) * p.rank) + r);
+        }
+#pragma unroll
+        for (int j = 0; j < RG; ++j)
+          if (ad[j] >= 0) v[j] = dot8(*reinterpret_cast<const uint4*>(h + (g * RG + j) * p.rank + 8 * r), b[j], v[j]);
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < RG; ++j)
+      if (g * RG + j < nt) p.out[(t0 + g * RG + j) * p.out_stride + n] = __float2half_rn(v[j]);
+  }
+}
+
 // cols: rows of x rounded up to the MMA's steps of 16; a stage: 16 KB of W, FUSED 16 KB of A (of them
 // a_bytes loaded), cols * 128 bytes of x.
 template <bool FUSED>
@@ -281,10 +345,10 @@ __global__ void __launch_bounds__(FTHREADS, 1)
     named_bar(1, 32 * 9);
     const int n = n0 + (warp & 3) * 32 + lane;
     if (n < p.n)
-      for (int g = z * 2 + ((warp - 2) >> 2); g * 4 < nt; g += 2 * Z)
-        for (int j = 0; j < 4; ++j)
-          if (ids[g * 4 + j] >= 0 && (j == 0 || ids[g * 4 + j] != ids[g * 4 + j - 1]))
-            for (int r = 0; r < p.rank; r += 64) prefetch_l2(p.b + (int64_t(ids[g * 4 + j]) * p.n + n) * p.rank + r);
+      for (int g = z * 2 + ((warp - 2) >> 2), rg = nt > 8 * Z ? 8 : 4; g * rg < nt; g += 2 * Z)
+        for (int j = g * rg; j < min(g * rg + rg, nt); ++j)
+          if (ids[j] >= 0 && (j == g * rg || ids[j] != ids[j - 1]))
+            for (int r = 0; r < p.rank; r += 64) prefetch_l2(p.b + (int64_t(ids[j]) * p.n + n) * p.rank + r);
     // the accumulator (lane = output, column = row of x) as part[row of x][output], over the stages,
     // which all have been read
     const int quarter = warp & 3, half = (warp - 2) >> 2;
@@ -318,79 +382,43 @@ __global__ void __launch_bounds__(FTHREADS, 1)
   __syncthreads();
   if (Z > 1) cluster_sync();
   const float* part = reinterpret_cast<const float*>(smem);
-  const int chunks = p.rank / 8;
-  __half* hs = reinterpret_cast<__half*>(smem + size_t(FUSED ? 2 : 1) * cols * 512);  // FUSED: h, [row of x][rank]
+  const bool wide = nt > 8 * Z;  // rows enough for groups of eight
+  const int group = wide ? 8 : 4;
+  const __half* h;
   if (FUSED) {
-    // h of this CTA's rows of x: the parts of the row's own adapter, scaled
-    for (int e = threadIdx.x; e < nt * p.rank; e += FTHREADS) {
-      const int i = e / p.rank, r = e - i * p.rank, ad = ids[i];
-      if (ad < 0 || (i / 8) % Z != z) continue;  // (groups z * 2 and z * 2 + 1 of four rows, and on by 2 Z)
-      const float* src = part + (cols + i) * 128 + ad * p.rank + r;
-      float d = 0.f;
-      if (Z == 1) {
-        d = *src;
-      } else {
-        float u[8];
+    // h of this CTA's rows of x: the parts of the row's own adapter, scaled; a warp per row
+    __half* hs = reinterpret_cast<__half*>(smem + size_t(2) * cols * 512);  // [row of x][rank]
+    for (int k = warp; k < FT; k += FTHREADS / 32) {
+      const int i = (k / (2 * group) * Z + z) * 2 * group + k % (2 * group);  // k-th row of this CTA's groups
+      if (i >= nt) break;
+      const int ad = ids[i];
+      if (ad < 0) continue;
+      const float sc = p.scales ? __ldg(p.scales + ad) : 1.f;
+      for (int r = lane; r < p.rank; r += 32) {
+        const float* src = part + (cols + i) * 128 + ad * p.rank + r;
+        float d = 0.f;
+        if (Z == 1) {
+          d = *src;
+        } else {
+          float u[8];
 #pragma unroll
-        for (int q = 0; q < 8; ++q) u[q] = q < Z ? ld_cluster_f32(cluster_addr(src, uint32_t(q))) : 0.f;
+          for (int q = 0; q < 8; ++q) u[q] = q < Z ? ld_cluster_f32(cluster_addr(src, uint32_t(q))) : 0.f;
 #pragma unroll
-        for (int q = 0; q < 8; ++q) d += u[q];
+          for (int q = 0; q < 8; ++q) d += u[q];
+        }
+        hs[i * p.rank + r] = __float2half_rn(d * sc);
       }
-      hs[e] = __float2half_rn(d * (p.scales ? __ldg(p.scales + ad) : 1.f));
     }
     __syncthreads();
+    h = hs;
   } else {
     wait_primary();
+    h = p.h + int64_t(t0) * p.rank;
   }
   if (warp >= 2 && warp < 10 && !abort_flag) {
-    const int c = (warp & 3) * 32 + lane, n = n0 + c, half = (warp - 2) >> 2;
-    const float bias = p.bias && n < p.n ? __half2float(p.bias[n]) : 0.f;
-    // groups of four rows of x, dealt to the cluster's CTAs and the two warps of these outputs
-    for (int g = z * 2 + half; g * 4 < nt; g += 2 * Z) {
-      float v[4];
-      int ad[4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int i = g * 4 + j;
-        v[j] = bias;
-        ad[j] = i < nt && n < p.n ? ids[i] : -1;
-      }
-      if (Z == 1) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) v[j] += part[(g * 4 + j) * 128 + c];
-      } else {
-        float u[4][8];
-#pragma unroll
-        for (int q = 0; q < 8; ++q)
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-            u[j][q] = q < Z ? ld_cluster_f32(cluster_addr(part + (g * 4 + j) * 128 + c, uint32_t(q))) : 0.f;
-#pragma unroll
-        for (int q = 0; q < 8; ++q)
-#pragma unroll
-          for (int j = 0; j < 4; ++j) v[j] += u[j][q];
-      }
-      if (ad[0] >= 0 || ad[1] >= 0 || ad[2] >= 0 || ad[3] >= 0) {
-        const uint4* h = FUSED ? reinterpret_cast<const uint4*>(hs + g * 4 * p.rank)
-                               : reinterpret_cast<const uint4*>(p.h + int64_t(t0 + g * 4) * p.rank);
-        const bool same = ad[0] == ad[1] && ad[1] == ad[2] && ad[2] == ad[3];
-#pragma unroll 4
-        for (int r = 0; r < chunks; ++r) {
-          uint4 b[4];
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            b[j] = j ? b[0] : make_uint4(0, 0, 0, 0);
-            if (ad[j] >= 0 && !(j && same)) b[j] = __ldg(reinterpret_cast<const uint4*>(p.b + (int64_t(ad[j]) * p.n + n) * p.rank) + r);
-          }
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-            if (ad[j] >= 0) v[j] = dot8(h[j * chunks + r], b[j], v[j]);
-        }
-      }
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (g * 4 + j < nt && n < p.n) p.out[(t0 + g * 4 + j) * p.out_stride + n] = __float2half_rn(v[j]);
-    }
+    const int c = (warp & 3) * 32 + lane, half = (warp - 2) >> 2;
+    if (wide) few_outputs<8>(p, part, ids, h, n0, t0, nt, z, Z, c, half);
+    else few_outputs<4>(p, part, ids, h, n0, t0, nt, z, Z, c, half);
   }
   if (Z > 1) cluster_sync();  // no CTA leaves while another reads its part
   if (warp == 1) {
@@ -674,7 +702,7 @@ struct PCfg {
   static constexpr int NWG = BN / 64;
   static constexpr int THREADS = 64 + 128 * NWG + 32;
   static constexpr int STAGES = BN == 256 ? 5 : 6;
-  static constexpr uint32_t TMEM_COLS = 2 * BN;
+  static constexpr uint32_t TMEM_COLS = BN == 128 ? 256 : 512;
   static constexpr int SMEM = STAGES * STAGE_BYTES + NWG * OUT_BYTES + 1024 + 512 + 1280;
 };
 
@@ -758,42 +786,54 @@ __global__ void __launch_bounds__(PCfg<BN>::THREADS, 1)
     uint32_t phase = 0;
     uint32_t issued = 0, last_parity = 0;
     bool ok = true, waited = false;
-    // one stage: x and W (K block kb, id < 0) or h and B (columns 64 kb of adapter id); lane w < 8 has
-    // word w of the lanes that are off
-    auto emit = [&](int mb, int nb, int kb, int id, uint32_t off, int last) -> bool {
-      if (!__all_sync(0xffffffffu, mbar_wait(&empty[stage], phase ^ 1, 211))) return false;
-      if (id >= 0 && lane < 8) reinterpret_cast<uint32_t*>(notes[stage].off)[lane] = off;
-      __syncwarp();
-      if (lane == 0) {
-        if (first) {
-          notes[stage].steps = id < 0 ? BK / 16 : (min(p.rank - 64 * kb, 64) + 15) / 16;
-          notes[stage].last = last;
-          // both CTAs' bytes of the stage complete on the first CTA's barrier
-          mbar_arrive_expect_tx(&full[stage], 2 * G::STAGE_BYTES);
-        }
-        const uint32_t bar = cluster_addr(&full[stage], 0);
-        tma_load_2d_pair(sA + stage * A_BYTES, id < 0 ? &tmX : &tmH, bar, kb * BK, mb * 2 * BM + int(rank) * BM);
-        tma_load_2d_pair(sB + stage * G::B_BYTES, id < 0 ? &tmW : &tmB, bar, kb * BK,
-                         (id < 0 ? 0 : id * p.n) + nb * BN + int(rank) * G::BH);
-      }
-      __syncwarp();
+    const bool lead = elect_one();
+    const uint32_t full0 = cluster_addr(&full[0], 0);  // both CTAs' bytes complete on the first CTA's barriers
+    // One stage, all lanes in step: columns [64 kb, 64 kb + 64) of x and W, or of h and an adapter's
+    // rows of B.
+    auto emit = [&](const CUtensorMap* ma, const CUtensorMap* mbm, int kb, int row_a, int row_b) {
+      mbar_arrive_expect_tx_if(lead && first, &full[stage], 2 * G::STAGE_BYTES);
+      const uint32_t bar = full0 + uint32_t(stage) * 8u;
+      tma_load_2d_pair_if(lead, sA + stage * A_BYTES, ma, bar, kb * BK, row_a);
+      tma_load_2d_pair_if(lead, sB + stage * G::B_BYTES, mbm, bar, kb * BK, row_b);
       issued |= 1u << stage;
       last_parity = (last_parity & ~(1u << stage)) | (phase << stage);
       if (++stage == STAGES) {
         stage = 0;
         phase ^= 1;
       }
-      return true;
     };
+    auto room = [&]() -> bool { return __all_sync(0xffffffffu, mbar_wait(&empty[stage], phase ^ 1, 211)); };
     const int chunks = (p.rank + 63) / 64;
     int list = 0;
     uint32_t lphase = 0;
     for (int t = pair; t < tiles && ok; t += npairs) {
       const int mb = m_first + t / n_tiles, nb = t % n_tiles;
-      for (int kb = 0; kb + 1 < nk && ok; ++kb) ok = emit(mb, nb, kb, -1, 0u, 0);
-      // a stage is held back until it is known whether another follows it
+      const int row_a = mb * 2 * BM + int(rank) * BM, row_b = nb * BN + int(rank) * G::BH;
+      for (int kb = 0; kb + 1 < nk; ++kb) {
+        if (!room()) {
+          ok = false;
+          break;
+        }
+        emit(&tmX, &tmW, kb, row_a, row_b);
+      }
+      // A stage is held back until it is known whether another follows it: the MMA warp is told with the
+      // last K block and with every run of rows whether the tile ends there.
       int held_kb = nk - 1, held_id = -1;
-      uint32_t held_off = 0;
+      uint32_t held_off = 0;  // lane w < 8: word w of the lanes that are off
+      auto flush = [&](bool last) {
+        if (!ok || !room()) {
+          ok = false;
+          return;
+        }
+        if (first) {
+          if (held_id >= 0 && lane < 8) reinterpret_cast<uint32_t*>(notes[stage].off)[lane] = held_off;
+          if (lane == 8) notes[stage].steps = (min(p.rank - 64 * held_kb, 64) + 15) / 16;
+          if (lane == 9) notes[stage].last = last;
+          __syncwarp();  // before the arrival that the MMA warp waits for
+        }
+        if (held_id < 0) emit(&tmX, &tmW, held_kb, row_a, row_b);
+        else emit(&tmH, &tmB, held_kb, row_a, held_id * p.n + row_b);
+      };
       for (bool more = p.n_adapters > 0; more && ok;) {
         if (!__all_sync(0xffffffffu, mbar_wait(&list_full[list], lphase, 216))) {
           ok = false;
@@ -809,7 +849,7 @@ __global__ void __launch_bounds__(PCfg<BN>::THREADS, 1)
           const int id = lists[list].id[i];
           const uint32_t off = lists[list].off[i][lane & 7];
           for (int c = 0; c < chunks && ok; ++c) {
-            ok = emit(mb, nb, held_kb, held_id, held_off, 0);
+            flush(false);
             held_kb = c;
             held_id = id;
             held_off = off;
@@ -822,7 +862,7 @@ __global__ void __launch_bounds__(PCfg<BN>::THREADS, 1)
           lphase ^= 1;
         }
       }
-      if (ok) ok = emit(mb, nb, held_kb, held_id, held_off, 1);
+      flush(true);
     }
     if (!ok && lane == 0) {
       *abort_flag = 1;
@@ -839,6 +879,7 @@ __global__ void __launch_bounds__(PCfg<BN>::THREADS, 1)
       auto wwait = [&](uint64_t* bar, uint32_t parity, int code) -> bool {
         return __all_sync(0xffffffffu, mbar_wait(bar, parity, code));
       };
+      const uint64_t da0 = desc_sw128(sA), db0 = desc_sw128(sB);
       int stage = 0;
       uint32_t phase = 0;
       int local = 0;
@@ -858,16 +899,13 @@ __global__ void __launch_bounds__(PCfg<BN>::THREADS, 1)
             break;
           }
           fence_after_sync();
-          const uint64_t da = desc_sw128(sA + stage * A_BYTES);
-          const uint64_t db = desc_sw128(sB + stage * G::B_BYTES);
-          const int last = notes[stage].last;
+          const uint64_t da = da0 + uint64_t(stage * (A_BYTES >> 4)), db = db0 + uint64_t(stage * (G::B_BYTES >> 4));
+          const bool last = i + 1 >= nk && notes[stage].last;
           if (i < nk) {
-            if (lead) {
 #pragma unroll
-              for (int k = 0; k < BK / 16; ++k)
-                mma_f16_pair(d, da + uint64_t(k * 2), db + uint64_t(k * 2), idesc, (i | k) != 0 ? 1u : 0u);
-              mma_commit_pair_both(&empty[stage]);  // the stage is free again in both CTAs
-            }
+            for (int k = 0; k < BK / 16; ++k)
+              mma_f16_pair_if(lead, d, da + uint64_t(k * 2), db + uint64_t(k * 2), idesc, (i | k) != 0 ? 1u : 0u);
+            mma_commit_pair_both_if(lead, &empty[stage]);  // the stage is free again in both CTAs
           } else {
             const uint4 o0 = notes[stage].off[0], o1 = notes[stage].off[1];
             const int steps = notes[stage].steps;
@@ -1191,9 +1229,12 @@ void lora_matmul(const kh_lora_matmul_args* args, cudaStream_t st) {
     if (fuses(a)) launch_few<true>(p, a, st);
     else launch_few<false>(p, a, st);
   } else {
-    // 256 columns a tile where that still gives every pair of SMs one
-    const int64_t wide = (a.rows + 255) / 256 * ((a.n + 255) / 256);
-    if (a.n > 128 && wide >= SMS / 2) launch_pair<256>(p, a, adapters, st);
+    // The tile width whose rounds over the SM pairs are over soonest; a narrower tile costs a little more
+    // than its share (the same x for fewer columns).
+    const int64_t m_tiles = (a.rows + 255) / 256, pairs = device_sms() / 2;
+    auto cost = [&](int bn) { return double((m_tiles * ((a.n + bn - 1) / bn) + pairs - 1) / pairs) * (bn + 24); };
+    if (cost(256) <= cost(192) && cost(256) <= cost(128)) launch_pair<256>(p, a, adapters, st);
+    else if (cost(192) <= cost(128)) launch_pair<192>(p, a, adapters, st);
     else launch_pair<128>(p, a, adapters, st);
   }
 }

@@ -406,6 +406,43 @@ __device__ __forceinline__ void tma_load_2d_pair(void* dst, const CUtensorMap* m
       "l"(map), "r"(bar), "r"(x), "r"(y)
       : "memory");
 }
+// The same, and the arrival that announces its bytes, under a predicate (see mma_f16_if).
+__device__ __forceinline__ void tma_load_2d_pair_if(bool lead, void* dst, const CUtensorMap* map, uint32_t bar, int x, int y) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\t"
+      "setp.ne.b32 q, %5, 0;\n\t"
+      "@q cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], "
+      "[%2];\n\t}" ::"r"(smem_u32(dst)),
+      "l"(map), "r"(bar), "r"(x), "r"(y), "r"(uint32_t(lead))
+      : "memory");
+}
+__device__ __forceinline__ void mbar_arrive_expect_tx_if(bool lead, uint64_t* bar, uint32_t bytes) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\t"
+      "setp.ne.b32 q, %2, 0;\n\t"
+      "@q mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n\t}" ::"r"(smem_u32(bar)),
+      "r"(bytes), "r"(uint32_t(lead))
+      : "memory");
+}
+__device__ __forceinline__ void mma_f16_pair_if(bool lead, uint32_t tmem_d, uint64_t da, uint64_t db, uint32_t idesc,
+                                                uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "setp.ne.b32 q, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem_d),
+      "l"(da), "l"(db), "r"(idesc), "r"(acc), "r"(uint32_t(lead))
+      : "memory");
+}
+__device__ __forceinline__ void mma_commit_pair_both_if(bool lead, const uint64_t* bar) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\t"
+      "setp.ne.b32 q, %2, 0;\n\t"
+      "@q tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;\n\t}" ::"r"(
+          smem_u32(bar)),
+      "h"(uint16_t(3)), "r"(uint32_t(lead))
+      : "memory");
+}
 // MMA of a CTA pair, issued by one thread of the first CTA: A rows [0, 128) and B rows
 // [0, N/2) from this CTA's shared memory, A rows [128, 256) and B rows [N/2, N) from the same
 // offsets in the peer's; each CTA's TMEM holds its 128 rows of D.
