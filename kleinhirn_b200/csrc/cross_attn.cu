@@ -360,15 +360,15 @@ __global__ void __launch_bounds__(128) cross_join_kernel(const CrossParams p) {
 
 // ---- tiles of 128 rows on the tensor cores ----
 //
-// One CTA per (block of two row tiles, key head and split, sequence):
+// One CTA per (block of row tiles, key head and split, sequence):
 //   warp 0     TMA: Q once, tiles of KEYS states of K and V into two rings; it also clears the dropped
 //              states' rows of V tiles (past the end, masked) before they are used;
 //   warp 1     issues S = Q K^T (M 128, N KEYS, K = D) into the stream's TMEM columns and O += P V (A = P
 //              from TMEM, V as an MN-major operand) into its O columns;
 //   8 warps    softmax, four to a stream, one thread per row: its KEYS scores in registers, P (f16)
 //              written over S in TMEM.
-// The two streams are two row tiles over the same K and V tiles; where the CTA's rows fit one tile,
-// they take its even and odd key tiles instead and add up their (m, l, O) at the end. S of the next
+// The two streams are two row tiles over the same K and V tiles (heads of 128); where the CTA's rows fit
+// one tile, they take its even and odd key tiles instead and add up their (m, l, O) at the end. S of the next
 // tile is issued behind P V of the last one, in order, so P may lie over S, and a full S means that the
 // products before it are done; one stream's softmax runs under the other's products.
 // Key tiles with dropped states: their scores become -inf and their V rows zero in shared memory, so
@@ -378,16 +378,18 @@ __global__ void __launch_bounds__(128) cross_join_kernel(const CrossParams p) {
 // Bound: the softmax threads. A row tile of 128 x 128 scores takes the special-function unit 1,024
 // cycles (4 lanes a clock on each quarter of the SM), its products 512 (D 64) or 1,024 (D 128). Heads of
 // 128 fill TMEM with one CTA per SM (KEYS 128; 168 registers a thread are dealt again, so that a softmax
-// thread holds its row); smaller heads run two CTAs per SM (KEYS 64), whose four softmax warps on each
-// quarter cover one another's waits, and one CTA's ends the other's beginning.
+// thread holds its row); smaller heads run two CTAs per SM (KEYS 64, one row tile each: 16 heads of 64,
+// 2,048 queries on 4,096 states, 186 us against 202 with two), whose four softmax warps on each quarter
+// cover one another's waits, and one CTA's end the other's beginning. (Some of the exponentials by a
+// polynomial on the FMA pipe instead: no faster, as the clock falls with the power they take.)
 
 constexpr int TROWS = 128;
 
 template <int D>
 struct TCfg {
   static constexpr bool ONE = D == 128;              // one CTA per SM
+  static constexpr int ROW_TILES = ONE ? 2 : 1;      // of a CTA, at most
   static constexpr int KEYS = ONE ? 128 : 64;
-  static constexpr int EXP_FMA = ONE ? 2 : 0;        // pairs of eight whose exponentials go to the FMA pipe
   static constexpr int HALVES = ONE ? 2 : 1;         // parts in which P goes into its products
   static constexpr int FIRST = ONE ? 4 : 2;          // first softmax warp (setmaxnreg acts on whole warpgroups)
   static constexpr int THREADS = 32 * (FIRST + 8);
@@ -399,7 +401,8 @@ struct TCfg {
   static constexpr int QPANEL = TROWS * ROWB, QTILE = PANELS * QPANEL;
   static constexpr int KPANEL = KEYS * ROWB, KTILE = PANELS * KPANEL;
   static constexpr int KS = ONE ? 3 : 4, VS = ONE ? 2 : 4;  // ring stages
-  static constexpr int K_OFF = 2 * QTILE;
+  // (with one row tile, 2 KB beside it to exchange the streams' m and l; with two, the unused second tile)
+  static constexpr int K_OFF = ROW_TILES == 2 ? 2 * QTILE : QTILE + 2048;
   static constexpr int V_OFF = K_OFF + KS * KTILE;
   static constexpr int BAR_OFF = V_OFF + VS * KTILE;
   static constexpr int USED = BAR_OFF + 320 + 1024;
@@ -418,27 +421,7 @@ __device__ __forceinline__ uint64_t tile_desc(const void* smem) {
   return ((uint64_t(smem_u32(smem)) >> 4) & 0x3FFFull) | (C::LBO << 16) | (C::SBO << 32) | (1ull << 46) | (C::LAYOUT << 61);
 }
 
-// 2^x of two values on the FMA pipe: x = n + f with n the nearest whole number (Cody and Waite's reduction,
-// by adding and taking off 1.5 2^23, whose low bits are then n; 127 more make them the exponent field) and
-// 2^f by the polynomial of degree 4 of least relative error on [-1/2, 1/2] (Remez exchange): 2.6e-6,
-// 2^-18.5, against the 2^-11 of the f16 that p becomes. x below -126 (a dropped score is -inf) gives
-// 2^-126, whose f16 is 0; NaN stays NaN.
-__device__ __forceinline__ float max_nan(float a, float b) {
-  float r;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
-  return r;
-}
 __device__ __forceinline__ float2 twice(float a) { return make_float2(a, a); }
-__device__ __forceinline__ float2 exp2_fma(float2 x) {
-  x = make_float2(max_nan(x.x, -126.f), max_nan(x.y, -126.f));
-  const float2 t = fadd2(x, twice(12582912.f + 127.f));
-  const float2 f = fadd2(x, ffma2(t, twice(-1.f), twice(12582912.f + 127.f)));
-  float2 q = ffma2(twice(0.009570102207362652f), f, twice(0.05591785907745361f));
-  q = ffma2(q, f, twice(0.240247443318367f));
-  q = ffma2(q, f, twice(0.6931217908859253f));
-  q = ffma2(q, f, twice(0.9999992847442627f));
-  return fmul2(q, make_float2(__uint_as_float(__float_as_uint(t.x) << 23), __uint_as_float(__float_as_uint(t.y) << 23)));
-}
 
 // Values that tcgen05.ld wrote may be used from here on (the compiler keeps uses behind this).
 template <int N>
@@ -491,9 +474,9 @@ __global__ void __launch_bounds__(TCfg<D>::THREADS, TCfg<D>::ONE ? 1 : 2)
   int nq, nk;
   seq_range(p.q_starts, s, p.q_rows, p.max_q, q0, nq);
   seq_range(p.k_starts, s, p.kv_rows, p.max_k, k0, nk);
-  const int qb = blockIdx.x * 2 * qpt;  // first query of the CTA
+  const int qb = blockIdx.x * C::ROW_TILES * qpt;  // first query of the CTA
   if (qb >= nq) return;
-  const bool pair = nq - qb > qpt;  // two row tiles (else the streams share one tile's states)
+  const bool pair = C::ROW_TILES == 2 && nq - qb > qpt;  // two row tiles (else the streams share one tile's states)
   // key tiles of this split
   const int all = (nk + KEYS - 1) / KEYS, per = (all + p.nsplit - 1) / p.nsplit;
   const int t0 = min(split * per, all), nkt = min(t0 + per, all) - t0;
@@ -783,7 +766,7 @@ __global__ void __launch_bounds__(TCfg<D>::THREADS, TCfg<D>::ONE ? 1 : 2)
           const int k = 2 * (c + i);
           const float2 x = ffma2(make_float2(__uint_as_float(sr[k / 32][k & 31]), __uint_as_float(sr[k / 32][(k + 1) & 31])),
                                  twice(p.scale_log2), twice(-ref));
-          const float2 e = (i & 7) < C::EXP_FMA ? exp2_fma(x) : make_float2(ex2_approx(x.x), ex2_approx(x.y));
+          const float2 e = make_float2(ex2_approx(x.x), ex2_approx(x.y));
           ls[i & 1] = fadd2(ls[i & 1], e);
           pk[i] = pack_half2(e.x, e.y);
         }
@@ -807,7 +790,7 @@ __global__ void __launch_bounds__(TCfg<D>::THREADS, TCfg<D>::ONE ? 1 : 2)
     const bool mine = r < qpt * G && qi < nq;
     float m_out = m, l_out = l, f0 = 1.f, f1 = 0.f;
     if (!pair) {
-      float* xm = reinterpret_cast<float*>(sQ + C::QTILE);  // the second Q tile is not used
+      float* xm = reinterpret_cast<float*>(sQ + C::QTILE);
       float* xl = xm + 256;
       xm[g * 128 + r] = m;
       xl[g * 128 + r] = l;
@@ -895,7 +878,8 @@ constexpr int SMS = 148;  // of a B200: the split must not depend on the device 
 int splits(const kh_cross_attention_args& a) {
   const int64_t G = a.q_heads / a.kv_heads;
   const bool few = takes_rows_kernel(a);
-  const int64_t blocks = few ? 1 : (int64_t(a.max_q) + 2 * (TROWS / G) - 1) / (2 * (TROWS / G));
+  const int64_t cta_rows = (a.head_dim == 128 ? 2 : 1) * (TROWS / G);
+  const int64_t blocks = few ? 1 : (a.max_q + cta_rows - 1) / cta_rows;
   const int64_t ctas = std::max<int64_t>(1, blocks * a.kv_heads * a.n_seqs);
   const int64_t want = (few ? 4 * SMS : a.head_dim == 128 ? SMS : 2 * SMS) / ctas;
   const int64_t most = few ? a.max_k / 256 : a.max_k / 512;
@@ -947,7 +931,8 @@ void launch(const CrossParams& p, const kh_cross_attention_args& a, bool states,
                              {uint32_t(C::PCOLS), uint32_t(p.G), uint32_t(qpt)}, C::ROWB);
     if (states) state_maps(C::PCOLS, C::KEYS, C::ROWB);
     else tk = tv = tq;
-    const dim3 grid(unsigned((a.max_q + 2 * qpt - 1) / (2 * qpt)), unsigned(a.kv_heads * p.nsplit), unsigned(a.n_seqs));
+    const int rows = C::ROW_TILES * qpt;
+    const dim3 grid(unsigned((a.max_q + rows - 1) / rows), unsigned(a.kv_heads * p.nsplit), unsigned(a.n_seqs));
     cross_tile_kernel<D><<<grid, C::THREADS, C::SMEM, st>>>(tq, tk, tv, p);
   }
   KH_CUDA(cudaGetLastError());
