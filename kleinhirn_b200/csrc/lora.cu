@@ -48,13 +48,13 @@ struct LoraParams {
 __device__ __forceinline__ int seg_start(const LoraParams& p, int i) {
   return int(min(max(int64_t(__ldg(p.starts + i)), int64_t(0)), p.rows));
 }
-// Adapter of a segment, -1 for none; an id that does not exist counts as none and is reported.
-__device__ __forceinline__ int adapter_of(const LoraParams& p, int seg) {
-  const int a = __ldg(p.ids + seg);
-  if (a < p.n_adapters) return a < 0 ? -1 : a;
+// An id as an adapter, -1 for none; one that does not exist counts as none and is reported.
+__device__ __forceinline__ int known_adapter(const LoraParams& p, int id) {
+  if (id < p.n_adapters) return id < 0 ? -1 : id;
   atomicCAS(&kh_tc_error, 0, OP_BAD_INDEX);
   return -1;
 }
+__device__ __forceinline__ int adapter_of(const LoraParams& p, int seg) { return known_adapter(p, __ldg(p.ids + seg)); }
 // First segment that ends behind row r (n_segs if none), found by a whole warp, 32 probes a round; with
 // one row to a segment (a step of single tokens) it is segment r, which the first round looks at too.
 __device__ __forceinline__ int first_seg(const LoraParams& p, int r) {
@@ -324,18 +324,27 @@ __global__ void __launch_bounds__(FTHREADS, 1)
     for (int t = lane; t < FT; t += 32) ids[t] = -1;
     __syncwarp();
     if (p.n_adapters > 0) {
-      for (int s = first_seg(p, t0); s < p.n_segs; s += 32) {
-        const int i = s + lane;
-        bool more = i < p.n_segs;
-        if (more) {
-          const int lo = max(seg_start(p, i), t0), hi = min(seg_start(p, i + 1), t0 + nt);
-          more = lo < t0 + nt;
-          if (lo < hi) {
-            const int ad = adapter_of(p, i);
-            for (int t = lo; t < hi; ++t) ids[t - t0] = ad;
+      for (int s = first_seg(p, t0), more = 1; more && s < p.n_segs; s += 128) {
+        // four segments a lane, their loads together
+        int lo[4], hi[4], id[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int i = s + 32 * j + lane;
+          lo[j] = hi[j] = t0 + nt;
+          id[j] = -1;
+          if (i < p.n_segs) {
+            lo[j] = max(seg_start(p, i), t0);
+            hi[j] = min(seg_start(p, i + 1), t0 + nt);
+            id[j] = __ldg(p.ids + i);
           }
         }
-        if (!__all_sync(0xffffffffu, more)) break;
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (lo[j] < hi[j]) {
+            const int ad = known_adapter(p, id[j]);
+            for (int t = lo[j]; t < hi[j]; ++t) ids[t - t0] = ad;
+          }
+        more = __all_sync(0xffffffffu, lo[3] < t0 + nt);
       }
     }
     __syncwarp();
@@ -384,41 +393,41 @@ __global__ void __launch_bounds__(FTHREADS, 1)
   const float* part = reinterpret_cast<const float*>(smem);
   const bool wide = nt > 8 * Z;  // rows enough for groups of eight
   const int group = wide ? 8 : 4;
-  const __half* h;
-  if (FUSED) {
-    // h of this CTA's rows of x: the parts of the row's own adapter, scaled; a warp per row
-    __half* hs = reinterpret_cast<__half*>(smem + size_t(2) * cols * 512);  // [row of x][rank]
+  // h of this CTA's rows of x, in shared memory, a warp per row
+  __half* hs = reinterpret_cast<__half*>(smem + size_t(FUSED ? 2 : 1) * cols * 512);  // [row of x][rank]
+  if (!FUSED) wait_primary();
+  if (p.n_adapters > 0) {
     for (int k = warp; k < FT; k += FTHREADS / 32) {
       const int i = (k / (2 * group) * Z + z) * 2 * group + k % (2 * group);  // k-th row of this CTA's groups
       if (i >= nt) break;
       const int ad = ids[i];
       if (ad < 0) continue;
-      const float sc = p.scales ? __ldg(p.scales + ad) : 1.f;
-      for (int r = lane; r < p.rank; r += 32) {
-        const float* src = part + (cols + i) * 128 + ad * p.rank + r;
-        float d = 0.f;
-        if (Z == 1) {
-          d = *src;
-        } else {
-          float u[8];
+      if (FUSED) {  // the parts of the row's own adapter, scaled
+        const float sc = p.scales ? __ldg(p.scales + ad) : 1.f;
+        for (int r = lane; r < p.rank; r += 32) {
+          const float* src = part + (cols + i) * 128 + ad * p.rank + r;
+          float d = 0.f;
+          if (Z == 1) {
+            d = *src;
+          } else {
+            float u[8];
 #pragma unroll
-          for (int q = 0; q < 8; ++q) u[q] = q < Z ? ld_cluster_f32(cluster_addr(src, uint32_t(q))) : 0.f;
+            for (int q = 0; q < 8; ++q) u[q] = q < Z ? ld_cluster_f32(cluster_addr(src, uint32_t(q))) : 0.f;
 #pragma unroll
-          for (int q = 0; q < 8; ++q) d += u[q];
+            for (int q = 0; q < 8; ++q) d += u[q];
+          }
+          hs[i * p.rank + r] = __float2half_rn(d * sc);
         }
-        hs[i * p.rank + r] = __float2half_rn(d * sc);
+      } else if (lane < p.rank / 8) {
+        reinterpret_cast<uint4*>(hs + i * p.rank)[lane] = reinterpret_cast<const uint4*>(p.h + int64_t(t0 + i) * p.rank)[lane];
       }
     }
     __syncthreads();
-    h = hs;
-  } else {
-    wait_primary();
-    h = p.h + int64_t(t0) * p.rank;
   }
   if (warp >= 2 && warp < 10 && !abort_flag) {
     const int c = (warp & 3) * 32 + lane, half = (warp - 2) >> 2;
-    if (wide) few_outputs<8>(p, part, ids, h, n0, t0, nt, z, Z, c, half);
-    else few_outputs<4>(p, part, ids, h, n0, t0, nt, z, Z, c, half);
+    if (wide) few_outputs<8>(p, part, ids, hs, n0, t0, nt, z, Z, c, half);
+    else few_outputs<4>(p, part, ids, hs, n0, t0, nt, z, Z, c, half);
   }
   if (Z > 1) cluster_sync();  // no CTA leaves while another reads its part
   if (warp == 1) {
@@ -526,29 +535,38 @@ __global__ void __launch_bounds__(224) lora_shrink_tile_kernel(const __grid_cons
     int n = 0;
     for (int r = lane; r < 128; r += 32) pieces.row_id[r] = -1;
     __syncwarp();
-    for (int s = first_seg(p, r0); s < p.n_segs; s += 32) {
-      const int i = s + lane;
-      int lo = 0, hi = 0, id = -1;
-      bool more = i < p.n_segs;
-      if (more) {
-        lo = max(seg_start(p, i), r0) - r0;
-        hi = min(min(seg_start(p, i + 1), last), r0 + 128) - r0;
-        more = lo < 128;
-        if (lo < hi) id = adapter_of(p, i);
-      }
-      const uint32_t have = __ballot_sync(0xffffffffu, id >= 0);
-      const int at = n + __popc(have & ((1u << lane) - 1u));
-      if (id >= 0 && at < 128) {
-        pieces.id[at] = id;
-        pieces.off[at] = make_uint4(~lanes_on(lo, hi, 0), ~lanes_on(lo, hi, 1), ~lanes_on(lo, hi, 2), ~lanes_on(lo, hi, 3));
-        const float sc = p.scales ? __ldg(p.scales + id) : 1.f;
-        for (int r = lo; r < hi; ++r) {
-          pieces.row_id[r] = id;
-          pieces.row_scale[r] = sc;
+    for (int s = first_seg(p, r0), more = 1; more && s < p.n_segs; s += 128) {
+      // four segments a lane, their loads together
+      int lo[4], hi[4], id[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int i = s + 32 * j + lane;
+        lo[j] = hi[j] = 128;
+        id[j] = -1;
+        if (i < p.n_segs) {
+          lo[j] = max(seg_start(p, i), r0) - r0;
+          hi[j] = min(min(seg_start(p, i + 1), last), r0 + 128) - r0;
+          id[j] = __ldg(p.ids + i);
         }
       }
-      n += __popc(have);
-      if (!__all_sync(0xffffffffu, more)) break;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int ad = lo[j] < hi[j] ? known_adapter(p, id[j]) : -1;
+        const uint32_t have = __ballot_sync(0xffffffffu, ad >= 0);
+        const int at = n + __popc(have & ((1u << lane) - 1u));
+        if (ad >= 0 && at < 128) {
+          pieces.id[at] = ad;
+          pieces.off[at] = make_uint4(~lanes_on(lo[j], hi[j], 0), ~lanes_on(lo[j], hi[j], 1), ~lanes_on(lo[j], hi[j], 2),
+                                      ~lanes_on(lo[j], hi[j], 3));
+          const float sc = p.scales ? __ldg(p.scales + ad) : 1.f;
+          for (int r = lo[j]; r < hi[j]; ++r) {
+            pieces.row_id[r] = ad;
+            pieces.row_scale[r] = sc;
+          }
+        }
+        n += __popc(have);
+      }
+      more = __all_sync(0xffffffffu, lo[3] < 128);
     }
     const int np = min(n, 128);
     if (lane == 0) pieces.count = np;
@@ -1051,6 +1069,10 @@ __global__ void __launch_bounds__(PCfg<BN>::THREADS, 1)
 
 // ---- host side ----
 
+// CTAs in clusters, one an SM, that surely run at once: the SMs come in groups of 16 to 18, of which a
+// cluster of 8 leaves up to two idle (18 clusters of 8 took two rounds: 11 us against 5.8 for 18 of 4, 32
+// rows 512 -> 2,304).
+constexpr int CLUSTER_CTAS = 128;
 constexpr int SMS = 148;
 
 template <class F, class... A>
@@ -1099,7 +1121,7 @@ void launch_few(const LoraParams& p, const kh_lora_matmul_args& a, cudaStream_t 
   const int stages = std::min(12, FSMEM / ((FUSED ? 32768 : 16384) + cols * 128));
   const int n_tiles = (a.n + 127) / 128, nk = (a.k + 63) / 64;
   int Z = 1;  // CTAs that split the sum of 128 outputs: while SMs are idle, at least a K block each
-  while (Z < 8 && 2 * Z * n_tiles <= SMS && 2 * Z <= nk) Z *= 2;
+  while (Z < 8 && 2 * Z * n_tiles <= CLUSTER_CTAS && 2 * Z <= nk) Z *= 2;
   CUtensorMap tx, tw, ta;
   encode_tensor_map_f16(&tx, a.x, uint64_t(a.rows), uint64_t(a.k), uint64_t(a.x_stride), 64, uint32_t(cols), 128);
   encode_tensor_map_f16(&tw, a.w, uint64_t(a.n), uint64_t(a.k), uint64_t(a.k), 64, 128, 128);
@@ -1218,7 +1240,7 @@ void lora_matmul(const kh_lora_matmul_args* args, cudaStream_t st) {
       encode_tensor_map_f16(&ta, a.lora_a, uint64_t(a.n_adapters) * a.rank, uint64_t(a.k), uint64_t(a.k), 64, R16, 128);
       const int64_t tiles = (a.rows + 127) / 128;
       int Z = 1;  // CTAs that split a tile's sum: while SMs are idle, at least two K blocks each
-      while (Z < 8 && 2 * Z * tiles <= SMS && 4 * Z <= (a.k + 63) / 64) Z *= 2;
+      while (Z < 8 && 2 * Z * tiles <= CLUSTER_CTAS && 4 * Z <= (a.k + 63) / 64) Z *= 2;
       // many tiles: rings so short that four CTAs share an SM (up to rank 32) and cover each other's waits
       const int xstages = tiles > 2 * SMS ? 2 : SXS, astages = R16 > 32 || tiles > 2 * SMS ? 4 : SAS;
       const size_t smem = size_t(xstages) * 16384 + size_t(astages) * R16 * 128 + 1024;
