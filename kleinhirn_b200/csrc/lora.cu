@@ -10,7 +10,7 @@
 // lora_few_kernel. Many rows: bound by the tensor cores;
 // lora_shrink_tile_kernel (HBM: reads x once) and lora_pair_kernel. A row tile that holds rows of
 // several adapters takes one more product per adapter, whose output lanes of other rows are switched
-// off in the instruction, so no operand is masked or copied.
+// off in the instruction, so no operand is masked or copied, and rows of one adapter need not be neighbours.
 
 #include "device_ops.h"
 
@@ -447,7 +447,7 @@ __global__ void __launch_bounds__(FTHREADS, 1)
 
 constexpr int SXS = 4;  // x stages
 constexpr int SAS = 8;  // A stages, at most
-struct ShrinkPieces {
+struct ShrinkPieces {  // the adapters of a tile
   int count;
   int id[128];
   uint4 off[128];         // lanes of other rows
@@ -530,7 +530,7 @@ __global__ void __launch_bounds__(224) lora_shrink_tile_kernel(const __grid_cons
       mbar_wait(&x_full[kb % xstages], uint32_t(kb / xstages) & 1, 203);
     if (!ok) abort_flag = 1;
   } else if (warp == 6) {
-    // the adapters of these rows: non-empty runs of rows, in order
+    // the adapters of these rows, each with all its rows
     const int last = seg_start(p, p.n_segs);  // rows from here on are not written
     int n = 0;
     for (int r = lane; r < 128; r += 32) pieces.row_id[r] = -1;
@@ -552,23 +552,34 @@ __global__ void __launch_bounds__(224) lora_shrink_tile_kernel(const __grid_cons
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const int ad = lo[j] < hi[j] ? known_adapter(p, id[j]) : -1;
-        const uint32_t have = __ballot_sync(0xffffffffu, ad >= 0);
-        const int at = n + __popc(have & ((1u << lane) - 1u));
-        if (ad >= 0 && at < 128) {
+        // an adapter that is in the list already takes these rows too; a new one's first lane adds it
+        int at = -1;
+        for (int k = 0; k < n; ++k) at = pieces.id[k] == ad ? k : at;
+        const uint32_t peers = __match_any_sync(0xffffffffu, ad);
+        const bool adds = ad >= 0 && at < 0 && lane == __ffs(peers) - 1;
+        const uint32_t added = __ballot_sync(0xffffffffu, adds);
+        if (ad >= 0 && at < 0) at = n + __popc(added & ((1u << (__ffs(peers) - 1)) - 1u));
+        if (adds) {
           pieces.id[at] = ad;
-          pieces.off[at] = make_uint4(~lanes_on(lo[j], hi[j], 0), ~lanes_on(lo[j], hi[j], 1), ~lanes_on(lo[j], hi[j], 2),
-                                      ~lanes_on(lo[j], hi[j], 3));
+          pieces.off[at] = make_uint4(~0u, ~0u, ~0u, ~0u);
+        }
+        __syncwarp();
+        if (ad >= 0) {
+          uint32_t* off = reinterpret_cast<uint32_t*>(&pieces.off[at]);
+#pragma unroll
+          for (int w = 0; w < 4; ++w) atomicAnd(off + w, ~lanes_on(lo[j], hi[j], w));
           const float sc = p.scales ? __ldg(p.scales + ad) : 1.f;
           for (int r = lo[j]; r < hi[j]; ++r) {
             pieces.row_id[r] = ad;
             pieces.row_scale[r] = sc;
           }
         }
-        n += __popc(have);
+        n += __popc(added);  // (at most 128: every one has a row of its own)
+        __syncwarp();
       }
       more = __all_sync(0xffffffffu, lo[3] < 128);
     }
-    const int np = min(n, 128);
+    const int np = n;
     if (lane == 0) pieces.count = np;
     __syncwarp();
     mbar_arrive(listed);
@@ -704,7 +715,7 @@ __global__ void __launch_bounds__(224) lora_shrink_tile_kernel(const __grid_cons
 // ceil(rank / 16) steps whose lanes of other rows are off.
 //   warp 0 TMA; warp 1 MMA (first CTA); then a warpgroup per 64 columns: bias, f16, staged and stored by
 //   TMA (tiles with rows that are not to be written: straight from registers); the last warp finds the
-//   adapters of the tiles ahead, in lists of up to 16 runs of rows (found by the TMA warp itself, the
+//   adapters of the tiles ahead, in lists of up to 16 from 32 segments (found by the TMA warp itself, the
 //   dependent loads of the search held up the K blocks: 7 % on 65,536 rows of 768 -> 2,304).
 
 constexpr int BM = 128;
@@ -731,7 +742,7 @@ struct StageNote {
   int steps, last, pad[2];
 };
 
-// Runs of rows of a tile: the adapter and the lanes of other rows; more: the tile has another list.
+// Adapters of a tile and the lanes of other rows; more: the tile has another list.
 struct RunList {
   int count, more, pad[2];
   int id[16];
@@ -961,36 +972,42 @@ __global__ void __launch_bounds__(PCfg<BN>::THREADS, 1)
       for (int t = pair; t < tiles && ok; t += npairs) {
         const int r0 = (m_first + t / n_tiles) * 2 * BM, r1 = min(r0 + 2 * BM, end);
         int s = first_seg(p, r0);
-        for (bool more = true; more && ok; s += 16) {
-          const int i = s + lane;  // lanes 0-15 take a segment each
+        for (bool more = true; more && ok; s += 32) {
+          const int i = s + lane;
           int lo = 0, hi = 0, id = -1;
-          bool in = lane < 16 && i < p.n_segs;
+          bool in = i < p.n_segs;
           if (in) {
             lo = max(seg_start(p, i), r0) - r0;
             hi = min(seg_start(p, i + 1), r1) - r0;
             in = r0 + lo < r1;
             if (lo < hi) id = adapter_of(p, i);
           }
-          more = (__ballot_sync(0xffffffffu, in) & 0xffffu) == 0xffffu;
-          const uint32_t have = __ballot_sync(0xffffffffu, id >= 0);
-          if (have == 0 && more) continue;  // (empty segments)
-          ok = __all_sync(0xffffffffu, mbar_wait(&list_empty[list], lphase ^ 1, 215));
-          if (!ok) break;
-          if (id >= 0) {
-            const int at = __popc(have & ((1u << lane) - 1u));
-            lists[list].id[at] = id;
+          more = __all_sync(0xffffffffu, in);
+          // the adapters of these segments, each with all its rows, numbered by their first lanes
+          const uint32_t peers = __match_any_sync(0xffffffffu, id);
+          const uint32_t firsts = __ballot_sync(0xffffffffu, id >= 0 && lane == __ffs(peers) - 1);
+          const int at = __popc(firsts & ((1u << (__ffs(peers) - 1)) - 1u)), count = __popc(firsts);
+          if (count == 0 && more) continue;
+          for (int base = 0; ok && (base == 0 || base < count); base += 16) {
+            ok = __all_sync(0xffffffffu, mbar_wait(&list_empty[list], lphase ^ 1, 215));
+            if (!ok) break;
+            for (int w = lane; w < 128; w += 32) (&lists[list].off[0][0])[w] = ~0u;
+            __syncwarp();
+            if (id >= 0 && at >= base && at < base + 16) {
+              lists[list].id[at - base] = id;  // (the same from all its lanes)
 #pragma unroll
-            for (int w = 0; w < 8; ++w) lists[list].off[at][w] = ~lanes_on(lo, hi, w);
-          }
-          if (lane == 0) {
-            lists[list].count = __popc(have);
-            lists[list].more = more;
-          }
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&list_full[list]);
-          if (++list == 2) {
-            list = 0;
-            lphase ^= 1;
+              for (int w = 0; w < 8; ++w) atomicAnd(&lists[list].off[at - base][w], ~lanes_on(lo, hi, w));
+            }
+            if (lane == 0) {
+              lists[list].count = min(count - base, 16);
+              lists[list].more = more || base + 16 < count;
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&list_full[list]);
+            if (++list == 2) {
+              list = 0;
+              lphase ^= 1;
+            }
           }
         }
       }
@@ -1101,13 +1118,17 @@ void launch_ex(F* kernel, dim3 grid, int threads, size_t smem, int cluster, bool
   KH_CUDA(cudaLaunchKernelEx(&cfg, kernel, args...));
 }
 
-// h by a CTA per row: few rows (each reads its adapter's A through L2), or segments so short that a tile
-// of 128 rows would take a product per row or so.
+// Whether a tile of 128 rows holds so many adapters (no more than it has segments) that a product for
+// each costs more than the tile is worth.
+bool scattered(const kh_lora_matmul_args& a) { return a.rows < 8 * int64_t(a.n_segs) && a.n_adapters > 16; }
+// h by a CTA per row: few rows (each reads its adapter's A through L2), or scattered ones (400 rows of 40
+// adapters, 1,024 -> 4,096: the whole call 63 us, with h by tiles 80; 1,000 rows of 100: 38 against 47).
 bool shrinks_rows(const kh_lora_matmul_args& a) {
-  return a.rows < 8 * int64_t(a.n_segs) || (a.rows <= FT && a.rows * a.rank * int64_t(a.k) <= (int64_t(1) << 24));
+  return scattered(a) || (a.rows <= FT && a.rows * a.rank * int64_t(a.k) <= (int64_t(1) << 24));
 }
-// Rows of x as the columns of the product: W is read once per 128 rows.
-bool takes_few(const kh_lora_matmul_args& a) { return a.rows <= FT || (a.rows <= 4 * FT && a.rows < 8 * int64_t(a.n_segs)); }
+// Rows of x as the columns of the product: W is read once per 128 rows. Scattered rows take it up to four
+// times (250 rows of 100 adapters, 768 -> 2,304: 36 us against 94; 400 of 40, 1,024 -> 4,096: 63 against 179).
+bool takes_few(const kh_lora_matmul_args& a) { return a.rows <= FT || (a.rows <= 4 * FT && scattered(a)); }
 // h from the same launch: every cluster makes it for itself, so A is read once per 128 outputs.
 bool fuses(const kh_lora_matmul_args& a) { return takes_few(a) && a.n_adapters > 0 && a.n_adapters * a.rank <= 128; }
 

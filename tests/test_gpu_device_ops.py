@@ -632,3 +632,11 @@ def test_captured_lengths_change():
         want, tol = cross_ref(q, k, v, nq, nk, H, KV, D, scale)
         close(out[nq[0]:nq[-1]], want[nq[0]:nq[-1]], tol[nq[0]:nq[-1]])
         assert (out[:nq[0]] == 7).all() and (out[nq[-1]:] == 7).all()
+
+
+def test_lora_adapters_scattered_over_short_segments():
+    """Few adapters over many short segments: the rows of one adapter of a tile are no neighbours."""
+    lens = [1 + (i * 7) % 9 for i in range(200)]
+    for na in (2, 5, 40):
+        x, w, bias, a, b, scales, st = lora_case(60 + na, lens, 256, 328, 24, na)
+        lora_check(x, w, bias, a, b, scales, st, [(i * 5) % (na + 1) - 1 for i in range(200)])
