@@ -275,8 +275,8 @@ int kh_attention_f16_noalloc_status(void* stream);
  * layout of a plan's cossin buffer). out may be x itself (with the same stride), else they must not
  * overlap. A position outside [0, table_rows) gives a zero row and a status.
  * Limits: head_dim even, in [2, 256]; rotary_dim even, in [0, head_dim]; q_heads + k_heads in
- * [1, 4096]; either count may be 0. Any alignment and stride; 16-byte aligned buffers with strides of
- * whole 16-byte units are the fast ones. */
+ * [1, 4096]; either count may be 0; rows and strides below 2^31. Any alignment and stride; 16-byte
+ * aligned buffers with strides of whole 16-byte units are the fast ones. */
 typedef struct kh_qk_norm_rope_args {
   int32_t dtype;       /* KH_F32 or KH_F16 */
   int32_t q_heads, k_heads, head_dim;
@@ -302,9 +302,10 @@ int kh_qk_norm_rope(const kh_qk_norm_rope_args* args, void* stream);
  * f16 operands; scores, sums and the accumulated output in f32, the probabilities rounded to f16 for
  * the product with v, the output once. max_q and max_k bound the lengths (they size the grid and the
  * split): of a longer sequence, query rows past max_q are not written and states past max_k not read.
+ * out may be q itself (with the same stride); else it shares no value with what the call reads.
  * Limits: head_dim 32, 64 or 128; kv_heads divides q_heads (at most 1,024), at most 64 query heads to
  * one; max_q and max_k at most 2^24; n_seqs at most 65,535; buffers 16-byte aligned with strides of
- * whole 16-byte units; rows below 2^31. */
+ * whole 16-byte units; rows and strides below 2^31. */
 typedef struct kh_cross_attention_args {
   int32_t n_seqs; /* 0: nothing to do */
   int32_t q_heads, kv_heads, head_dim;
@@ -322,7 +323,8 @@ typedef struct kh_cross_attention_args {
   void* workspace;
   uint64_t workspace_bytes;
 } kh_cross_attention_args;
-/* Bytes of workspace of such a call (pointers and strides are not read), or -1 and kh_last_error. */
+/* Bytes of workspace of such a call (pointers and strides are not read), or -1 and kh_last_error. They
+ * depend on the head counts, n_seqs, max_q and max_k, and need not grow with each of them. */
 int64_t kh_cross_attention_f16_workspace(const kh_cross_attention_args* args);
 int kh_cross_attention_f16(const kh_cross_attention_args* args, void* stream);
 
@@ -331,10 +333,11 @@ int kh_cross_attention_f16(const kh_cross_attention_args* args, void* stream);
  *   out = x w^T + bias + scales[a] (x lora_a[a]^T) lora_b[a]^T
  * f16 operands, f32 sums, the rank-sized product (with its scale) rounded to f16 once and added to the
  * same f32 accumulator as the projection; the output is rounded once. A negative id is a request
- * without an adapter; an id of n_adapters or more counts as none and gives a status.
+ * without an adapter; an id of n_adapters or more counts as none and gives a status. out shares no
+ * value with what the call reads (not in place).
  * Limits: k, n and rank multiples of 8, k and n in [8, 65,536], rank in [8, 128] (pad a smaller one
- * with zeros); n_segs at most 65,535; buffers 16-byte aligned, strides whole 16-byte units; rows
- * below 2^31 - 256. */
+ * with zeros); n_adapters and n_segs at most 65,535, n_adapters * n below 2^31 - 512; buffers 16-byte
+ * aligned, strides whole 16-byte units below 2^31; rows below 2^31 - 256. */
 typedef struct kh_lora_matmul_args {
   int32_t k, n, rank, n_adapters;
   int32_t n_segs; /* 0: nothing to do */
@@ -352,7 +355,8 @@ typedef struct kh_lora_matmul_args {
   void* workspace;
   uint64_t workspace_bytes;
 } kh_lora_matmul_args;
-/* Bytes of workspace of such a call (pointers and strides are not read), or -1 and kh_last_error. */
+/* Bytes of workspace of such a call (pointers and strides are not read), or -1 and kh_last_error:
+ * 2 * rows * rank, 0 without adapters. */
 int64_t kh_lora_matmul_f16_workspace(const kh_lora_matmul_args* args);
 int kh_lora_matmul_f16(const kh_lora_matmul_args* args, void* stream);
 

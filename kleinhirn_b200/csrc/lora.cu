@@ -1181,8 +1181,8 @@ void check_sizes(const char* fn, const kh_lora_matmul_args* args) {
   check_that(a.k >= 8 && a.k <= 65536 && a.k % 8 == 0 && a.n >= 8 && a.n <= 65536 && a.n % 8 == 0, fn,
              "k and n must be multiples of 8, in [8, 65536]");
   check_that(a.rank >= 8 && a.rank <= 128 && a.rank % 8 == 0, fn, "rank must be a multiple of 8, in [8, 128]");
-  check_that(a.n_adapters >= 0 && a.n_adapters <= 65535 && int64_t(a.n_adapters) * a.n < (int64_t(1) << 31), fn,
-             "n_adapters must be in [0, 65535], n_adapters * n below 2^31");
+  check_that(a.n_adapters >= 0 && a.n_adapters <= 65535 && int64_t(a.n_adapters) * a.n < (int64_t(1) << 31) - 512, fn,
+             "n_adapters must be in [0, 65535], n_adapters * n below 2^31 - 512");
   check_that(a.n_segs >= 0 && a.n_segs <= 65535, fn, "n_segs must be in [0, 65535]");
   check_that(a.rows >= 0 && a.rows < (int64_t(1) << 31) - 256, fn, "rows must be in [0, 2^31 - 256)");
 }
@@ -1191,7 +1191,8 @@ void check_sizes(const char* fn, const kh_lora_matmul_args* args) {
 
 int64_t lora_matmul_workspace(const kh_lora_matmul_args* args) {
   check_sizes("kh_lora_matmul_f16_workspace", args);
-  return args->n_adapters && !fuses(*args) ? args->rows * args->rank * 2 : 0;
+  // (the same whichever kernels take the call, so that a workspace for the most rows serves fewer)
+  return args->n_adapters ? args->rows * args->rank * 2 : 0;
 }
 
 void lora_matmul(const kh_lora_matmul_args* args, cudaStream_t st) {
@@ -1209,6 +1210,7 @@ void lora_matmul(const kh_lora_matmul_args* args, cudaStream_t st) {
   check_that(a.x_stride >= a.k && a.out_stride >= a.n && a.x_stride < lim && a.out_stride < lim &&
                  a.x_stride % 8 == 0 && a.out_stride % 8 == 0,
              fn, "strides must be multiples of 8, at least k and n, below 2^31");
+  check_that(a.x != a.out, fn, "out may not be x: every row of x is read for all outputs");
   const int64_t need = lora_matmul_workspace(args);
   check_that(need == 0 || (a.workspace && int64_t(a.workspace_bytes) >= need), fn, "workspace too small");
   check_that((reinterpret_cast<uintptr_t>(a.workspace) & 255) == 0, fn, "workspace must be 256-byte aligned");

@@ -229,8 +229,8 @@ __global__ void __launch_bounds__(256) qk_norm_rope_lanes_kernel(const NormParam
   }
 }
 
-// Heads of more chunks, and unaligned ones. PAIRS: chunk pairs of a thread (1, or 4 for the one-value chunks of unaligned heads). LANES * PAIRS
-// pairs cover D <= 256.
+// Heads of more chunks, and unaligned ones. PAIRS: chunk pairs of a thread (1, or 4 for the one-value
+// chunks of unaligned heads). LANES * PAIRS pairs cover D <= 256.
 template <typename T, int VEC, int PAIRS, int U>
 __global__ void __launch_bounds__(256) qk_norm_rope_kernel(const NormParams p, int lanes_log2) {
   const uint32_t lanes = 1u << lanes_log2;
@@ -423,11 +423,12 @@ void qk_norm_rope(const kh_qk_norm_rope_args* args, cudaStream_t st) {
              fn, "q_heads + k_heads must be in [1, 4096]");
   check_that(a.interleaved == 0 || a.interleaved == 1, fn, "interleaved must be 0 or 1");
   check_that(a.eps > 0.f, fn, "eps must be above 0");
-  check_that(a.rows >= 0 && a.rows < (int64_t(1) << 40), fn, "rows must be in [0, 2^40)");
+  check_that(a.rows >= 0 && a.rows < (int64_t(1) << 31), fn, "rows must be in [0, 2^31)");
   const int64_t width = int64_t(a.q_heads + a.k_heads) * a.head_dim;
   check_that(a.x_stride >= width && a.out_stride >= width && a.x_stride < (int64_t(1) << 31) &&
                  a.out_stride < (int64_t(1) << 31),
              fn, "strides must be at least (q_heads + k_heads) * head_dim and below 2^31");
+  check_that(a.rows * std::max(a.x_stride, a.out_stride) < (int64_t(1) << 48), fn, "rows * stride must be below 2^48");
   if (a.rows == 0) return;
   const int size = a.dtype == KH_F16 ? 2 : 4;
   check_that(a.x && a.out, fn, "null x or out");

@@ -81,6 +81,28 @@ def test_lora_refusals(kw, text):
     refused(kb.lora_matmul_f16, lora(**kw), text)
 
 
+@pytest.mark.parametrize("call,args,text", [
+    (kb.qk_norm_rope, norm(rows=1 << 31), "rows"),
+    (kb.qk_norm_rope, norm(rows=(1 << 31) - 1, x_stride=(1 << 31) - 1), "stride"),
+    (kb.qk_norm_rope, norm(x_stride=1 << 31), "stride"),
+    (kb.lora_matmul_f16, lora(n=65528, n_adapters=32773), "n_adapters"),
+    (kb.lora_matmul_f16, lora(n_adapters=65536), "n_adapters"),
+    (kb.lora_matmul_f16, lora(rows=(1 << 31) - 256), "rows"),
+    (kb.lora_matmul_f16, lora(x_stride=1 << 31), "stride"),
+    (kb.lora_matmul_f16, lora(out=P), "out may not be x"),
+    (kb.cross_attention_f16, cross(v_stride=1 << 31), "stride"),
+])
+def test_limits_and_aliases_are_refused(call, args, text):
+    refused(call, args, text)
+
+
+def test_lora_workspace_grows_with_the_rows_alone():
+    for rows in (0, 1, 128, 129, 70000):
+        for na, segs in ((1, 1), (40, 60000)):
+            assert kb.lora_matmul_f16_workspace(lora(rows=rows, rank=16, n_adapters=na, n_segs=segs)) == rows * 32
+    assert kb.lora_matmul_f16_workspace(lora(n_adapters=0)) == 0
+
+
 def test_null_arguments_are_refused():
     lib = kb.load_library()
     for name in ("kh_qk_norm_rope", "kh_cross_attention_f16", "kh_lora_matmul_f16"):

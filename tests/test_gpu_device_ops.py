@@ -640,3 +640,91 @@ def test_lora_adapters_scattered_over_short_segments():
     for na in (2, 5, 40):
         x, w, bias, a, b, scales, st = lora_case(60 + na, lens, 256, 328, 24, na)
         lora_check(x, w, bias, a, b, scales, st, [(i * 5) % (na + 1) - 1 for i in range(200)])
+
+
+@pytest.mark.parametrize("K,N,R", [(256, 512, 72), (72, 136, 128), (1536, 264, 8)])
+def test_lora_scattered_rows_of_many_adapters(K, N, R):
+    """Few rows a segment and many adapters, over several blocks of 128 rows that do not start at 0."""
+    lens = [(i * 5) % 4 for i in range(200)]
+    x, w, bias, a, b, scales, st = lora_case(K, lens, K, N, R, 90, pad=8, first=7)
+    lora_check(x, w, bias, a, b, scales, st, [(i * 11) % 91 - 1 for i in range(200)])
+
+
+@pytest.mark.parametrize("ql,kl", [([1, 3], [900, 40]), ([150, 300], [260, 90]), ([20], [4000])])
+def test_cross_in_place(ql, kl):
+    """out may be q, whichever kernel takes the call, with split states too."""
+    H, KV, D = 4, 2, 64
+    q, k, v, qs, ks, scale = cross_case(51, ql, kl, H, KV, D)
+    want, tol = cross_ref(q, k, v, qs, ks, H, KV, D, scale)
+    behind = q[qs[-1]:].clone()
+    a = cross_args(q, k, v, q, i32(qs), i32(ks), H, KV, D, scale, max(ql), max(kl))
+    kb().cross_attention_f16(a, stream())
+    kb().operator_status(stream())
+    close(q[:qs[-1]], want[:qs[-1]], tol[:qs[-1]])
+    assert torch_().equal(q[qs[-1]:], behind)
+
+
+def test_offsets_past_32_bits():
+    """Rows whose value offsets, and byte offsets, pass 2^31: the last rows of wide strided buffers."""
+    torch = torch_()
+    rows, width = 17000, 140000  # 2.4e9 values
+    buf = torch.empty(rows, width, dtype=torch.float16, device="cuda")
+    g = gen(52)
+    tail = 300
+    buf[-tail:, :768] = randn(g, tail, 768)
+    first, qs, ks, mq, mk = rows - tail, [rows - tail, rows - 190, rows - 180], [rows - tail, rows - 90, rows], 110, 210
+    H, KV, D = 4, 2, 64
+    q, k, v = buf[:, :256], buf[:, 256:384], buf[:, 384:512]
+    cut = [s - first for s in qs], [s - first for s in ks]
+    small = [t[-tail:].clone() for t in (q, k, v)]
+    want, tol = cross_ref(*small, cut[0], cut[1], H, KV, D, 0.125)
+    for max_q in (mq, 4):
+        out = buf[:, 512:768]
+        out[-tail:] = 7
+        a = cross_args(q, k, v, out, i32(qs), i32(ks), H, KV, D, 0.125, max_q, mk)
+        kb().cross_attention_f16(a, stream())
+        kb().operator_status(stream())
+        for s in range(2):
+            n = min(max_q, qs[s + 1] - qs[s])
+            r = slice(cut[0][s], cut[0][s] + n)
+            close(out[-tail:][r], want[r], tol[r])
+            assert (out[-tail:][cut[0][s] + n:cut[0][s + 1]] == 7).all()
+    w, a_, b_ = randn(g, 256, 256, scale=1 / 16), randn(g, 2, 8, 256, scale=1 / 16), randn(g, 2, 256, 8)
+    for lens in ([200, 100], [2, 3]):
+        st = [rows - tail, rows - tail + lens[0], rows - tail + sum(lens)]
+        out = buf[:, 512:768]
+        kb().lora_matmul_f16(lora_args(q, w, None, a_, b_, None, i32(st), i32([1, 0]), out), stream())
+        kb().operator_status(stream())
+        want, tol = lora_ref(small[0], w, None, a_, b_, None, [s - first for s in st], [1, 0])
+        n = sum(lens)
+        close(out[-tail:][:n], want[:n], tol[:n])
+    table, pos = angle_table(rows, 64), torch.arange(rows, device="cuda").int()
+    kb().qk_norm_rope(norm_args(q, q, 2, 2, 64, 64, False, table, pos, None, None), stream())
+    kb().operator_status(stream())
+    want, top = norm_ref(small[0], 2, 2, 64, 64, False, table, pos[-tail:], None, None)
+    close(q[-tail:], want, norm_tol(small[0], want, top))
+
+
+def test_two_captured_layers_replayed_at_once():
+    """Two graphs with workspaces of their own, replayed on two streams at the same time."""
+    torch = torch_()
+    ts = [layer(gen(71 + i), [1] * 20, [300 + i] * 20) for i in range(2)] + [layer(gen(73), [60, 200], [590, 90])]
+    graphs, want = [], []
+    for t in ts:
+        t["call"](stream())
+        torch.cuda.synchronize()
+        want.append(t["y"].clone())
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            t["call"](torch.cuda.current_stream().cuda_stream)
+        t["y"].zero_()
+    streams = [torch.cuda.Stream() for _ in ts]
+    torch.cuda.synchronize()
+    for _ in range(10):
+        for g, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                g.replay()
+    torch.cuda.synchronize()
+    kb().operator_status(stream())
+    for t, w in zip(ts, want):
+        assert torch.equal(t["y"], w)
