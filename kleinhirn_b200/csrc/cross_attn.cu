@@ -44,6 +44,7 @@ struct CrossParams {
   int64_t q_rows, kv_rows, q_stride, k_stride, v_stride, out_stride;
   int n_seqs, q_heads, kv_heads, G, max_q, max_k, nsplit;
   float scale_log2;  // scale * log2(e)
+  bool wide;         // 16 columns of out are aligned to their 32 bytes
 };
 
 // Rows of sequence s in a buffer of `rows`: starts outside it are cut, a longer sequence ends at `most`.
@@ -419,6 +420,13 @@ template <int D>
 __device__ __forceinline__ uint64_t tile_desc(const void* smem) {
   using C = TCfg<D>;
   return ((uint64_t(smem_u32(smem)) >> 4) & 0x3FFFull) | (C::LBO << 16) | (C::SBO << 32) | (1ull << 46) | (C::LAYOUT << 61);
+}
+
+// 32 aligned bytes, a whole sector, in one store.
+__device__ __forceinline__ void store_32(void* dst, const uint32_t (&u)[8]) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(dst), "r"(u[0]), "r"(u[1]), "r"(u[2]), "r"(u[3]),
+               "r"(u[4]), "r"(u[5]), "r"(u[6]), "r"(u[7])
+               : "memory");
 }
 
 __device__ __forceinline__ float2 twice(float a) { return make_float2(a, a); }
@@ -826,15 +834,22 @@ __global__ void __launch_bounds__(TCfg<D>::THREADS, TCfg<D>::ONE ? 1 : 2)
           v[i] = ((f0 != 0.f ? __uint_as_float(a[i]) * f0 : 0.f) + (f1 != 0.f ? __uint_as_float(b[i]) * f1 : 0.f)) * inv;
         if (!mine) continue;
         if (direct) {
-          uint4* dst = reinterpret_cast<uint4*>(p.out + (q0 + qi) * p.out_stride + h * D + c);
+          __half* dst = p.out + (q0 + qi) * p.out_stride + h * D + c;
+          uint32_t u[8];
 #pragma unroll
-          for (int i = 0; i < 2; ++i)
-            dst[i] = make_uint4(pack_half2(v[8 * i], v[8 * i + 1]), pack_half2(v[8 * i + 2], v[8 * i + 3]),
-                                pack_half2(v[8 * i + 4], v[8 * i + 5]), pack_half2(v[8 * i + 6], v[8 * i + 7]));
+          for (int i = 0; i < 8; ++i) u[i] = pack_half2(v[2 * i], v[2 * i + 1]);
+          if (p.wide) {
+            store_32(dst, u);
+          } else {
+            reinterpret_cast<uint4*>(dst)[0] = make_uint4(u[0], u[1], u[2], u[3]);
+            reinterpret_cast<uint4*>(dst)[1] = make_uint4(u[4], u[5], u[6], u[7]);
+          }
         } else {
-          float4* dst = reinterpret_cast<float4*>(p.part_o + at * D + c);
+          uint32_t u[2][8];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) dst[i] = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+          for (int i = 0; i < 16; ++i) u[i / 8][i % 8] = __float_as_uint(v[i]);
+          store_32(p.part_o + at * D + c, u[0]);
+          store_32(p.part_o + at * D + c + 8, u[1]);
         }
       }
       if (mine && !direct && (pair || g == 0)) p.part_ml[at] = make_float2(m_out, l_out);
@@ -1007,6 +1022,7 @@ void cross_attention(const kh_cross_attention_args* args, cudaStream_t st) {
   p.max_k = a.max_k;
   p.nsplit = splits(a);
   p.scale_log2 = a.scale * 1.4426950408889634f;
+  p.wide = reinterpret_cast<uintptr_t>(a.out) % 32 == 0 && a.out_stride % 16 == 0;
   if (p.nsplit > 1) {
     const int64_t parts = int64_t(p.nsplit) * a.n_seqs * a.max_q * a.q_heads;
     p.part_o = static_cast<float*>(a.workspace);
