@@ -126,9 +126,11 @@ __global__ void __launch_bounds__(512) lora_shrink_rows_kernel(const LoraParams 
 // out^T = W x^T: the 128 rows of the MMA are outputs and its columns the (up to 128) rows of x, so that
 // few rows waste no tensor work and W streams once through a deep ring. A cluster of Z CTAs splits the
 // sum of 128 outputs, until about every SM takes part in reading W, and adds the parts over distributed
-// shared memory in rank order, each CTA for its share of the rows. The adapter's part is a dot product
-// of rank values per output there. Warp 0 TMA, warp 1 MMA, warps 2-9 the outputs (lane = output, two
-// warps to 32 of them), warp 10 finds the rows' adapters meanwhile.
+// shared memory in rank order, each CTA for its share of the rows, in groups of eight. The adapters' part
+// of a group is m16n8k16 products of B's rows as they lie in memory with the group's h, one adapter's rows
+// of it at a time (as dot products, a thread to an output, 120 rows of 4 adapters of rank 64, 4,096 ->
+// 4,096, took 49 us; so, 36). Warp 0 TMA, warp 1 MMA, warps 2-9 16 outputs each, warp 10 finds the rows'
+// adapters meanwhile.
 // FUSED: where all adapters' A together have at most 128 rows, they are a second operand tile of every
 // stage, h comes out of the same pass over x, and there is no launch before this one.
 
@@ -149,75 +151,94 @@ __device__ __forceinline__ float ld_cluster_f32(uint32_t addr) {
   asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
   return v;
 }
+__device__ __forceinline__ void mma_16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                          uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
 
-// The outputs n0 + c of groups of RG rows of x, dealt to the cluster's CTAs and the two warps of these
-// outputs: the parts of the sum, the bias and the dot product with h, rounded once.
-template <int RG>
-__device__ __forceinline__ void few_outputs(const LoraParams& p, const float* part, const int* ids, const __half* h, int n0,
-                                            int t0, int nt, int z, int Z, int c, int half) {
-  const int n = n0 + c;
-  if (n >= p.n) return;
-  const float bias = p.bias ? __half2float(p.bias[n]) : 0.f;
-  const int chunks = p.rank / 8;
-  for (int g = z * 2 + half; g * RG < nt; g += 2 * Z) {
-    float v[RG];
-    int ad[RG];
-    bool any = false, same = true;
-#pragma unroll
-    for (int j = 0; j < RG; ++j) {
-      const int i = g * RG + j;
-      v[j] = bias;
-      ad[j] = i < nt ? ids[i] : -1;
-      any |= ad[j] >= 0;
-      same &= ad[j] == ad[0];
+constexpr int PS = 132;  // row stride of the parts of the sum: [row of x][output], f32
+
+// The adapters' part: products of B's rows, 16 outputs to a warp, with the h of eight rows of x, one
+// adapter's rows of them at a time (zeros for the others). A CTA's products go through its groups of rows,
+// a group's adapters and the rank's sixteens, eight of one group to a batch, whose loads of B are in flight
+// together: those of the first from before the sum is done, the others' under the products before them.
+// The order of the rank's values is free: the quad lane q takes the values 4 q .. 4 q + 3 of 16, of B and h.
+struct Products {
+  int g;             // group
+  int mine;          // adapter of the row of x that this lane holds h of
+  uint32_t leaders;  // a lane for each adapter that is left
+  int k;             // first of the adapter's rank values that are left
+  // the next group with an adapter, from g on
+  __device__ __forceinline__ void find(const int* ids, int nt, int step) {
+    const int lane = threadIdx.x & 31;
+    for (; g * 8 < nt; g += step) {
+      mine = ids[g * 8 + (lane >> 2)];
+      const uint32_t same = __match_any_sync(0xffffffffu, mine);
+      leaders = __ballot_sync(0xffffffffu, mine >= 0 && lane == __ffs(same) - 1);
+      if (leaders) return;
     }
-    if (Z == 1) {
-#pragma unroll
-      for (int j = 0; j < RG; ++j) v[j] += part[(g * RG + j) * 128 + c];
-    } else {
-      float u[RG][8];
-#pragma unroll
-      for (int q = 0; q < 8; ++q)
-#pragma unroll
-        for (int j = 0; j < RG; ++j)
-          u[j][q] = q < Z ? ld_cluster_f32(cluster_addr(part + (g * RG + j) * 128 + c, uint32_t(q))) : 0.f;
-#pragma unroll
-      for (int q = 0; q < 8; ++q)
-#pragma unroll
-        for (int j = 0; j < RG; ++j) v[j] += u[j][q];
-    }
-    if (any && same) {  // the rows of one adapter: its row of B once
-      const uint4* b = reinterpret_cast<const uint4*>(p.b + (int64_t(ad[0]) * p.n + n) * p.rank);
-#pragma unroll 8
-      for (int r = 0; r < chunks; ++r) {
-        const uint4 br = __ldg(b + r);
-#pragma unroll
-        for (int j = 0; j < RG; ++j) v[j] = dot8(*reinterpret_cast<const uint4*>(h + (g * RG + j) * p.rank + 8 * r), br, v[j]);
-      }
-    } else if (any) {
-#pragma unroll 2
-      for (int r = 0; r < chunks; ++r) {
-        uint4 b[RG];
-#pragma unroll
-        for (int j = 0; j < RG; ++j) {
-          b[j] = make_uint4(0, 0, 0, 0);
-          if (ad[j] >= 0) b[j] = __ldg(reinterpret_cast<const uint4*>(p.b + (int64_t(ad[j]) * p.n + n) * p.rank) + r);
-        }
-#pragma unroll
-        for (int j = 0; j < RG; ++j)
-          if (ad[j] >= 0) v[j] = dot8(*reinterpret_cast<const uint4*>(h + (g * RG + j) * p.rank + 8 * r), b[j], v[j]);
-      }
-    }
-#pragma unroll
-    for (int j = 0; j < RG; ++j)
-      if (g * RG + j < nt) p.out[(t0 + g * RG + j) * p.out_stride + n] = __float2half_rn(v[j]);
   }
+  __device__ __forceinline__ int adapter() const { return __shfl_sync(0xffffffffu, mine, __ffs(leaders) - 1); }
+  __device__ __forceinline__ void next(int rank) {
+    k += 16;
+    if (k >= rank) {
+      k = 0;
+      leaders &= leaders - 1;
+    }
+  }
+};
+// b: B at this lane's output and rank values, of adapter 0; low, high: its outputs lane / 4 and + 8 exist
+__device__ __forceinline__ void load_batch(const LoraParams& p, Products& s, const int* ids, int nt, int step, const __half* b,
+                                           bool low, bool high, uint2 (&lo)[8], uint2 (&hi)[8]) {
+  const int q4 = (threadIdx.x & 3) * 4;
+  const bool some = s.g * 8 < nt;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    lo[i] = hi[i] = make_uint2(0, 0);
+    if (some && s.leaders) {
+      const __half* src = b + s.adapter() * (int64_t(p.n) * p.rank) + s.k;
+      if (s.k + q4 < p.rank) {
+        if (low) lo[i] = __ldg(reinterpret_cast<const uint2*>(src));
+        if (high) hi[i] = __ldg(reinterpret_cast<const uint2*>(src + 8 * p.rank));
+      }
+      s.next(p.rank);
+    }
+  }
+  if (some && !s.leaders) {
+    s.g += step;
+    s.find(ids, nt, step);
+  }
+}
+// part: the sum at row 0 of x and this lane's output; hs: h [row of x][rank + 8]
+__device__ __forceinline__ void use_batch(const LoraParams& p, Products s, const __half* hs, float* part, const uint2 (&lo)[8],
+                                          const uint2 (&hi)[8]) {
+  const int lane = threadIdx.x & 31, q4 = (lane & 3) * 4;
+  float* dst = part + (s.g * 8 + 2 * (lane & 3)) * PS;
+  float acc[4] = {dst[0], dst[PS], dst[8], dst[PS + 8]};
+  const __half* h = hs + (s.g * 8 + (lane >> 2)) * (p.rank + 8) + q4;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    uint2 v = make_uint2(0, 0);
+    if (s.leaders) {
+      if (s.adapter() == s.mine && s.k + q4 < p.rank) v = *reinterpret_cast<const uint2*>(h + s.k);
+      s.next(p.rank);
+    }
+    mma_16816(acc, lo[i].x, hi[i].x, lo[i].y, hi[i].y, v.x, v.y);
+  }
+  dst[0] = acc[0];
+  dst[PS] = acc[1];
+  dst[8] = acc[2];
+  dst[PS + 8] = acc[3];
 }
 
 // cols: rows of x rounded up to the MMA's steps of 16; a stage: 16 KB of W, FUSED 16 KB of A (of them
 // a_bytes loaded), cols * 128 bytes of x.
+// (registers: what leaves an SM room for a CTA of lora_shrink_rows_kernel)
 template <bool FUSED>
-__global__ void __launch_bounds__(FTHREADS, 1)
+__global__ void __maxnreg__(FUSED ? 168 : 112)
     lora_few_kernel(const __grid_constant__ CUtensorMap tmx, const __grid_constant__ CUtensorMap tmw,
                     const __grid_constant__ CUtensorMap tma, const LoraParams p, int Z, int cols, int stages, int a_bytes) {
   constexpr int X_OFF = FUSED ? 32768 : 16384;
@@ -259,6 +280,12 @@ __global__ void __launch_bounds__(FTHREADS, 1)
   auto wwait = [&](uint64_t* bar, uint32_t parity, int code) -> bool {
     return __all_sync(0xffffffffu, mbar_wait(bar, parity, code));
   };
+  // (warps 2-9)
+  Products loaded, used;
+  uint2 b_lo[8], b_hi[8];
+  const int m = n0 + 16 * (warp - 2) + (lane >> 2);  // output of this lane's rows of B
+  const bool low = m < p.n, high = m + 8 < p.n;
+  const __half* b_at = p.b + int64_t(m) * p.rank + (lane & 3) * 4;
 
   if (warp == 0) {
     bool ok = true;
@@ -350,14 +377,12 @@ __global__ void __launch_bounds__(FTHREADS, 1)
     __syncwarp();
     named_bar(1, 32 * 9);
   } else {
-    // rows of B that this thread will need, towards L2 while W streams
     named_bar(1, 32 * 9);
-    const int n = n0 + (warp & 3) * 32 + lane;
-    if (n < p.n)
-      for (int g = z * 2 + ((warp - 2) >> 2), rg = nt > 8 * Z ? 8 : 4; g * rg < nt; g += 2 * Z)
-        for (int j = g * rg; j < min(g * rg + rg, nt); ++j)
-          if (ids[j] >= 0 && (j == g * rg || ids[j] != ids[j - 1]))
-            for (int r = 0; r < p.rank; r += 64) prefetch_l2(p.b + (int64_t(ids[j]) * p.n + n) * p.rank + r);
+    loaded.g = z;
+    loaded.k = 0;
+    loaded.find(ids, nt, Z);
+    used = loaded;
+    load_batch(p, loaded, ids, nt, Z, b_at, low, high, b_lo, b_hi);
     // the accumulator (lane = output, column = row of x) as part[row of x][output], over the stages,
     // which all have been read
     const int quarter = warp & 3, half = (warp - 2) >> 2;
@@ -374,7 +399,7 @@ __global__ void __launch_bounds__(FTHREADS, 1)
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
         asm volatile("" : "+r"(v[i]));
-        part[(c + i) * 128] = nk > 0 ? __uint_as_float(v[i]) : 0.f;
+        part[(c + i) * PS] = nk > 0 ? __uint_as_float(v[i]) : 0.f;
       }
       if (FUSED) {  // the adapters' lanes behind it
         tmem_ld16(taddr + tcols / 2 + uint32_t(c), v);
@@ -382,7 +407,7 @@ __global__ void __launch_bounds__(FTHREADS, 1)
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
           asm volatile("" : "+r"(v[i]));
-          part[(cols + c + i) * 128] = nk > 0 ? __uint_as_float(v[i]) : 0.f;
+          part[(cols + c + i) * PS] = nk > 0 ? __uint_as_float(v[i]) : 0.f;
         }
       }
     }
@@ -390,22 +415,20 @@ __global__ void __launch_bounds__(FTHREADS, 1)
   fence_before_sync();
   __syncthreads();
   if (Z > 1) cluster_sync();
-  const float* part = reinterpret_cast<const float*>(smem);
-  const bool wide = nt > 8 * Z;  // rows enough for groups of eight
-  const int group = wide ? 8 : 4;
+  float* part = reinterpret_cast<float*>(smem);
   // h of this CTA's rows of x, in shared memory, a warp per row
-  __half* hs = reinterpret_cast<__half*>(smem + size_t(FUSED ? 2 : 1) * cols * 512);  // [row of x][rank]
+  __half* hs = reinterpret_cast<__half*>(part + (FUSED ? 2 : 1) * cols * PS);  // [row of x][rank + 8]
   if (!FUSED) wait_primary();
   if (p.n_adapters > 0) {
     for (int k = warp; k < FT; k += FTHREADS / 32) {
-      const int i = (k / (2 * group) * Z + z) * 2 * group + k % (2 * group);  // k-th row of this CTA's groups
+      const int i = (k / 8 * Z + z) * 8 + k % 8;  // k-th row of this CTA's groups
       if (i >= nt) break;
       const int ad = ids[i];
       if (ad < 0) continue;
       if (FUSED) {  // the parts of the row's own adapter, scaled
         const float sc = p.scales ? __ldg(p.scales + ad) : 1.f;
         for (int r = lane; r < p.rank; r += 32) {
-          const float* src = part + (cols + i) * 128 + ad * p.rank + r;
+          const float* src = part + (cols + i) * PS + ad * p.rank + r;
           float d = 0.f;
           if (Z == 1) {
             d = *src;
@@ -416,18 +439,48 @@ __global__ void __launch_bounds__(FTHREADS, 1)
 #pragma unroll
             for (int q = 0; q < 8; ++q) d += u[q];
           }
-          hs[i * p.rank + r] = __float2half_rn(d * sc);
+          hs[i * (p.rank + 8) + r] = __float2half_rn(d * sc);
         }
       } else if (lane < p.rank / 8) {
-        reinterpret_cast<uint4*>(hs + i * p.rank)[lane] = reinterpret_cast<const uint4*>(p.h + int64_t(t0 + i) * p.rank)[lane];
+        reinterpret_cast<uint4*>(hs + i * (p.rank + 8))[lane] = reinterpret_cast<const uint4*>(p.h + int64_t(t0 + i) * p.rank)[lane];
       }
     }
     __syncthreads();
+    if (warp >= 2 && warp < 10)
+      while (used.g * 8 < nt) {
+        const Products after = loaded;
+        uint2 lo[8], hi[8];
+        load_batch(p, loaded, ids, nt, Z, b_at, low, high, lo, hi);
+        use_batch(p, used, hs, part + 16 * (warp - 2) + (lane >> 2), b_lo, b_hi);
+        used = after;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) b_lo[i] = lo[i], b_hi[i] = hi[i];
+      }
+    __syncthreads();
   }
-  if (warp >= 2 && warp < 10 && !abort_flag) {
-    const int c = (warp & 3) * 32 + lane, half = (warp - 2) >> 2;
-    if (wide) few_outputs<8>(p, part, ids, hs, n0, t0, nt, z, Z, c, half);
-    else few_outputs<4>(p, part, ids, hs, n0, t0, nt, z, Z, c, half);
+  // this CTA's rows, a warp a row: the parts of the sum, in rank order, and the bias, rounded once
+  const int n = n0 + 4 * lane;
+  if (n < p.n && !abort_flag) {
+    float4 bias = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (p.bias) {
+      const uint2 u = __ldg(reinterpret_cast<const uint2*>(p.bias + n));
+      const float2 lo = __half22float2(*reinterpret_cast<const __half2*>(&u.x)), hi = __half22float2(*reinterpret_cast<const __half2*>(&u.y));
+      bias = make_float4(lo.x, lo.y, hi.x, hi.y);
+    }
+#pragma unroll 2
+    for (int k = warp; k < FT; k += FTHREADS / 32) {
+      const int i = (k / 8 * Z + z) * 8 + k % 8;
+      if (i >= nt) break;
+      const float* src = part + i * PS + 4 * lane;
+      float4 v = bias;
+      float4 u[8];
+#pragma unroll
+      for (int q = 0; q < 8; ++q)
+        u[q] = q >= Z ? make_float4(0.f, 0.f, 0.f, 0.f) : Z == 1 ? *reinterpret_cast<const float4*>(src) : ld_cluster_f32x4(cluster_addr(src, uint32_t(q)));
+#pragma unroll
+      for (int q = 0; q < 8; ++q) v.x += u[q].x, v.y += u[q].y, v.z += u[q].z, v.w += u[q].w;
+      *reinterpret_cast<uint2*>(p.out + (t0 + i) * p.out_stride + n) = make_uint2(pack_half2(v.x, v.y), pack_half2(v.z, v.w));
+    }
   }
   if (Z > 1) cluster_sync();  // no CTA leaves while another reads its part
   if (warp == 1) {
@@ -1249,6 +1302,12 @@ void lora_matmul(const kh_lora_matmul_args* args, cudaStream_t st) {
   const bool adapters = a.n_adapters > 0;
   if (adapters && !fuses(a)) {
     if (shrinks_rows(a)) {
+      // (with the next kernel's split of an SM's memory, so that its CTAs may start beside these)
+      static std::atomic<uint64_t> configured{0};
+      once_per_device(configured, [] {
+        KH_CUDA(cudaFuncSetAttribute(lora_shrink_rows_kernel, cudaFuncAttributePreferredSharedMemoryCarveout,
+                                     cudaSharedmemCarveoutMaxShared));
+      });
       lora_shrink_rows_kernel<<<unsigned(a.rows), 512, 0, st>>>(p);
       KH_CUDA(cudaGetLastError());
     } else {
