@@ -194,12 +194,14 @@ struct Products {
 __device__ __forceinline__ void load_batch(const LoraParams& p, Products& s, const int* ids, int nt, int step, const __half* b,
                                            bool low, bool high, uint2 (&lo)[8], uint2 (&hi)[8]) {
   const int q4 = (threadIdx.x & 3) * 4;
-  const bool some = s.g * 8 < nt;
+  const uint32_t stride = uint32_t(p.n) * uint32_t(p.rank);  // below 2^23
+#pragma unroll
+  for (int i = 0; i < 8; ++i) lo[i] = hi[i] = make_uint2(0, 0);
+  if (s.g * 8 >= nt) return;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    lo[i] = hi[i] = make_uint2(0, 0);
-    if (some && s.leaders) {
-      const __half* src = b + s.adapter() * (int64_t(p.n) * p.rank) + s.k;
+    if (s.leaders) {
+      const __half* src = b + uint64_t(uint32_t(s.adapter())) * stride + s.k;
       if (s.k + q4 < p.rank) {
         if (low) lo[i] = __ldg(reinterpret_cast<const uint2*>(src));
         if (high) hi[i] = __ldg(reinterpret_cast<const uint2*>(src + 8 * p.rank));
@@ -207,7 +209,7 @@ __device__ __forceinline__ void load_batch(const LoraParams& p, Products& s, con
       s.next(p.rank);
     }
   }
-  if (some && !s.leaders) {
+  if (!s.leaders) {
     s.g += step;
     s.find(ids, nt, step);
   }
@@ -247,6 +249,7 @@ __global__ void __maxnreg__(FUSED ? 168 : 112)
   __shared__ uint32_t tmem_holder;
   __shared__ volatile int abort_flag;
   __shared__ int ids[FT];
+  __shared__ float row_scale[FT];  // (FUSED)
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int z = blockIdx.x % Z, n0 = int(blockIdx.x / Z) * 128;
@@ -369,7 +372,11 @@ __global__ void __maxnreg__(FUSED ? 168 : 112)
         for (int j = 0; j < 4; ++j)
           if (lo[j] < hi[j]) {
             const int ad = known_adapter(p, id[j]);
-            for (int t = lo[j]; t < hi[j]; ++t) ids[t - t0] = ad;
+            const float sc = FUSED && ad >= 0 && p.scales ? __ldg(p.scales + ad) : 1.f;
+            for (int t = lo[j]; t < hi[j]; ++t) {
+              ids[t - t0] = ad;
+              if (FUSED) row_scale[t - t0] = sc;
+            }
           }
         more = __all_sync(0xffffffffu, lo[3] < t0 + nt);
       }
@@ -414,6 +421,10 @@ __global__ void __maxnreg__(FUSED ? 168 : 112)
   }
   fence_before_sync();
   __syncthreads();
+  // outputs that this lane stores, and their bias
+  const int n = n0 + 4 * lane;
+  uint2 bias_bits = make_uint2(0, 0);
+  if (p.bias && n < p.n) bias_bits = __ldg(reinterpret_cast<const uint2*>(p.bias + n));
   if (Z > 1) cluster_sync();
   float* part = reinterpret_cast<float*>(smem);
   // h of this CTA's rows of x, in shared memory, a warp per row
@@ -426,7 +437,7 @@ __global__ void __maxnreg__(FUSED ? 168 : 112)
       const int ad = ids[i];
       if (ad < 0) continue;
       if (FUSED) {  // the parts of the row's own adapter, scaled
-        const float sc = p.scales ? __ldg(p.scales + ad) : 1.f;
+        const float sc = row_scale[i];
         for (int r = lane; r < p.rank; r += 32) {
           const float* src = part + (cols + i) * PS + ad * p.rank + r;
           float d = 0.f;
@@ -459,14 +470,10 @@ __global__ void __maxnreg__(FUSED ? 168 : 112)
     __syncthreads();
   }
   // this CTA's rows, a warp a row: the parts of the sum, in rank order, and the bias, rounded once
-  const int n = n0 + 4 * lane;
   if (n < p.n && !abort_flag) {
-    float4 bias = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (p.bias) {
-      const uint2 u = __ldg(reinterpret_cast<const uint2*>(p.bias + n));
-      const float2 lo = __half22float2(*reinterpret_cast<const __half2*>(&u.x)), hi = __half22float2(*reinterpret_cast<const __half2*>(&u.y));
-      bias = make_float4(lo.x, lo.y, hi.x, hi.y);
-    }
+    const float2 bias_lo = __half22float2(*reinterpret_cast<const __half2*>(&bias_bits.x));
+    const float2 bias_hi = __half22float2(*reinterpret_cast<const __half2*>(&bias_bits.y));
+    const float4 bias = make_float4(bias_lo.x, bias_lo.y, bias_hi.x, bias_hi.y);
 #pragma unroll 2
     for (int k = warp; k < FT; k += FTHREADS / 32) {
       const int i = (k / 8 * Z + z) * 8 + k % 8;
