@@ -489,8 +489,20 @@ __global__ void __launch_bounds__(TCfg<D>::THREADS, TCfg<D>::ONE ? 1 : 2)
   const int all = (nk + KEYS - 1) / KEYS, per = (all + p.nsplit - 1) / p.nsplit;
   const int t0 = min(split * per, all), nkt = min(t0 + per, all) - t0;
   const int n0_of = pair ? nkt : (nkt + 1) / 2, n1_of = pair ? nkt : nkt / 2;  // tiles of the streams
+  auto load_tile = [&](int j, bool is_v) {  // of K or V into its ring, by one thread
+    const int st = is_v ? j % C::VS : j % C::KS;
+    uint64_t* full = is_v ? &v_full[st] : &k_full[st];
+    mbar_arrive_expect_tx(full, C::KTILE);
+    uint8_t* dst = (is_v ? sV : sK) + st * C::KTILE;
+    for (int c = 0; c < C::PANELS; ++c)
+      tma_load_2d(dst + c * C::KPANEL, is_v ? &tmv : &tmk, full, hk * D + c * C::PCOLS, int(k0) + (t0 + j) * KEYS);
+  };
+  constexpr int AHEAD = C::VS / 2;
 
   if (threadIdx.x == 0) {
+    prefetch_tmap(&tmq);
+    prefetch_tmap(&tmk);
+    prefetch_tmap(&tmv);
     mbar_init(q_full, 1);
     for (int g = 0; g < 2; ++g) {
       mbar_init(&s_full[g], 1);
@@ -511,9 +523,18 @@ __global__ void __launch_bounds__(TCfg<D>::THREADS, TCfg<D>::ONE ? 1 : 2)
     mbar_init(v_tail, 1);
     *abort_flag = 0;
     fence_barrier_init();
-    prefetch_tmap(&tmq);
-    prefetch_tmap(&tmk);
-    prefetch_tmap(&tmv);
+    // the first loads, while the other warps come up
+    if (nkt > 0) {
+      const int tiles = pair ? 2 : 1;
+      mbar_arrive_expect_tx(q_full, tiles * C::PANELS * qpt * G * C::ROWB);
+      for (int g = 0; g < tiles; ++g)
+        for (int c = 0; c < C::PANELS; ++c)
+          tma_load_3d(sQ + g * C::QTILE + c * C::QPANEL, &tmq, q_full, c * C::PCOLS, hk * G, int(q0) + qb + g * qpt);
+      for (int j = 0; j <= AHEAD; ++j) {
+        if (j < nkt) load_tile(j, false);
+        if (j < AHEAD && j < nkt) load_tile(j, true);
+      }
+    }
   }
   if (warp == 1) tmem_alloc(tmem_holder, C::COLS);
   fence_before_sync();
@@ -527,26 +548,17 @@ __global__ void __launch_bounds__(TCfg<D>::THREADS, TCfg<D>::ONE ? 1 : 2)
   if (warp < C::FIRST) {
     if (C::ONE) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::REGS_ISSUE));
     if (warp == 0 && nkt > 0) {
-      const int tiles = pair ? 2 : 1;
-      if (lane == 0) {
-        mbar_arrive_expect_tx(q_full, tiles * C::PANELS * qpt * G * C::ROWB);
-        for (int g = 0; g < tiles; ++g)
-          for (int c = 0; c < C::PANELS; ++c)
-            tma_load_3d(sQ + g * C::QTILE + c * C::QPANEL, &tmq, q_full, c * C::PCOLS, hk * G, int(q0) + qb + g * qpt);
-      }
       uint32_t pend_k = 0, pend_v = 0;  // last issued parity per ring slot (bit 1: issued)
+      for (int j = 0; j <= AHEAD && j < nkt; ++j) {
+        pend_k |= 2u << (2 * j);
+        if (j < AHEAD) pend_v |= 2u << (2 * j);
+      }
       auto load = [&](int j, bool is_v) -> bool {
         if (j >= nkt) return true;
         const int st = is_v ? j % C::VS : j % C::KS;
         const uint32_t u = uint32_t(is_v ? j / C::VS : j / C::KS) & 1;
-        uint64_t* full = is_v ? &v_full[st] : &k_full[st];
         if (!wwait(is_v ? &v_empty[st] : &k_empty[st], u ^ 1, is_v ? 102 : 101)) return false;
-        if (lane == 0) {
-          mbar_arrive_expect_tx(full, C::KTILE);
-          uint8_t* dst = (is_v ? sV : sK) + st * C::KTILE;
-          for (int c = 0; c < C::PANELS; ++c)
-            tma_load_2d(dst + c * C::KPANEL, is_v ? &tmv : &tmk, full, hk * D + c * C::PCOLS, int(k0) + (t0 + j) * KEYS);
-        }
+        if (lane == 0) load_tile(j, is_v);
         __syncwarp();
         uint32_t& pend = is_v ? pend_v : pend_k;
         pend = (pend & ~(3u << (2 * st))) | ((2u | u) << (2 * st));
@@ -563,9 +575,7 @@ __global__ void __launch_bounds__(TCfg<D>::THREADS, TCfg<D>::ONE ? 1 : 2)
       };
       // Tile j's rows are looked at before V of tile j + AHEAD is loaded, whose slot is free once the product
       // of tile j - AHEAD is done: the clearing runs ahead of the products.
-      constexpr int AHEAD = C::VS / 2;
-      bool ok = load(0, false);
-      for (int j = 0; j < AHEAD && ok; ++j) ok = load(j + 1, false) && load(j, true);
+      bool ok = true;
       if (p.mask) load_mask(0);
       for (int j = 0; j < nkt && ok; ok = ok && load(j + AHEAD + 1, false) && load(j + AHEAD, true), ++j) {
         if (!p.mask && (t0 + j + 1) * KEYS <= nk) continue;
