@@ -368,7 +368,7 @@ __global__ void __launch_bounds__(128) cross_join_kernel(const CrossParams p) {
 //              from TMEM, V as an MN-major operand) into its O columns;
 //   8 warps    softmax, four to a stream, one thread per row: its KEYS scores in registers, P (f16)
 //              written over S in TMEM.
-// The two streams are two row tiles over the same K and V tiles (heads of 128); where the CTA's rows fit
+// The two streams are two row tiles over the same K and V tiles (see row_tiles); where the CTA's rows fit
 // one tile, they take its even and odd key tiles instead and add up their (m, l, O) at the end. S of the next
 // tile is issued behind P V of the last one, in order, so P may lie over S, and a full S means that the
 // products before it are done; one stream's softmax runs under the other's products.
@@ -389,7 +389,6 @@ constexpr int TROWS = 128;
 template <int D>
 struct TCfg {
   static constexpr bool ONE = D == 128;              // one CTA per SM
-  static constexpr int ROW_TILES = ONE ? 2 : 1;      // of a CTA, at most
   static constexpr int KEYS = ONE ? 128 : 64;
   static constexpr int HALVES = ONE ? 2 : 1;         // parts in which P goes into its products
   static constexpr int FIRST = ONE ? 4 : 2;          // first softmax warp (setmaxnreg acts on whole warpgroups)
@@ -402,8 +401,8 @@ struct TCfg {
   static constexpr int QPANEL = TROWS * ROWB, QTILE = PANELS * QPANEL;
   static constexpr int KPANEL = KEYS * ROWB, KTILE = PANELS * KPANEL;
   static constexpr int KS = ONE ? 3 : 4, VS = ONE ? 2 : 4;  // ring stages
-  // (with one row tile, 2 KB beside it to exchange the streams' m and l; with two, the unused second tile)
-  static constexpr int K_OFF = ROW_TILES == 2 ? 2 * QTILE : QTILE + 2048;
+  // (a CTA of one row tile exchanges its streams' m and l in the second one's space)
+  static constexpr int K_OFF = 2 * QTILE;
   static constexpr int V_OFF = K_OFF + KS * KTILE;
   static constexpr int BAR_OFF = V_OFF + VS * KTILE;
   static constexpr int USED = BAR_OFF + 320 + 1024;
@@ -449,7 +448,8 @@ __device__ __forceinline__ bool quarter_any(int quarter, bool pred) {
   }
 }
 
-template <int D>
+// ROW_TILES: of a CTA, at most.
+template <int D, int ROW_TILES>
 __global__ void __launch_bounds__(TCfg<D>::THREADS, TCfg<D>::ONE ? 1 : 2)
     cross_tile_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant__ CUtensorMap tmk,
                       const __grid_constant__ CUtensorMap tmv, const CrossParams p) {
@@ -482,9 +482,9 @@ __global__ void __launch_bounds__(TCfg<D>::THREADS, TCfg<D>::ONE ? 1 : 2)
   int nq, nk;
   seq_range(p.q_starts, s, p.q_rows, p.max_q, q0, nq);
   seq_range(p.k_starts, s, p.kv_rows, p.max_k, k0, nk);
-  const int qb = blockIdx.x * C::ROW_TILES * qpt;  // first query of the CTA
+  const int qb = blockIdx.x * ROW_TILES * qpt;  // first query of the CTA
   if (qb >= nq) return;
-  const bool pair = C::ROW_TILES == 2 && nq - qb > qpt;  // two row tiles (else the streams share one tile's states)
+  const bool pair = ROW_TILES == 2 && nq - qb > qpt;  // two row tiles (else the streams share one tile's states)
   // key tiles of this split
   const int all = (nk + KEYS - 1) / KEYS, per = (all + p.nsplit - 1) / p.nsplit;
   const int t0 = min(split * per, all), nkt = min(t0 + per, all) - t0;
@@ -898,12 +898,17 @@ bool takes_rows_kernel(const kh_cross_attention_args& a) {
 
 constexpr int SMS = 148;  // of a B200: the split must not depend on the device the size is asked on
 
+// Row tiles of a CTA of the tile kernel: two where a CTA's time is mostly its start and end (60 sequences of
+// 400-600 queries, 12 heads of 64: on 64 states 46 us against 58 with one, on 256 71 against 82; on 512
+// equal, on 1,024 57 against 51). With heads of 128, one CTA to an SM, always.
+int row_tiles(const kh_cross_attention_args& a) { return a.head_dim == 128 || a.max_k <= 256 ? 2 : 1; }
+
 // CTAs that a sequence's states are split over: as many as fill the SMs (four CTAs each of the rows
 // kernel, one or two of the tile kernel), each with enough states to pay for the join.
 int splits(const kh_cross_attention_args& a) {
   const int64_t G = a.q_heads / a.kv_heads;
   const bool few = takes_rows_kernel(a);
-  const int64_t cta_rows = (a.head_dim == 128 ? 2 : 1) * (TROWS / G);
+  const int64_t cta_rows = row_tiles(a) * (TROWS / G);
   const int64_t blocks = few ? 1 : (a.max_q + cta_rows - 1) / cta_rows;
   const int64_t ctas = std::max<int64_t>(1, blocks * a.kv_heads * a.n_seqs);
   const int64_t want = (few ? 4 * SMS : a.head_dim == 128 ? SMS : 2 * SMS) / ctas;
@@ -920,6 +925,18 @@ void launch_rows(const CUtensorMap& tk, const CUtensorMap& tv, const CrossParams
     KH_CUDA(cudaFuncSetAttribute(cross_rows_kernel<D, RW>, cudaFuncAttributeMaxDynamicSharedMemorySize, RCfg<D, RW>::SMEM));
   });
   cross_rows_kernel<D, RW><<<dim3(p.nsplit, p.kv_heads, p.n_seqs), RW * 32, RCfg<D, RW>::SMEM, st>>>(tk, tv, p);
+}
+
+template <int D, int ROW_TILES>
+void launch_tiles(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const CrossParams& p, cudaStream_t st) {
+  using C = TCfg<D>;
+  static std::atomic<uint64_t> configured{0};
+  once_per_device(configured, [] {
+    KH_CUDA(cudaFuncSetAttribute(cross_tile_kernel<D, ROW_TILES>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
+  });
+  const int rows = ROW_TILES * (TROWS / p.G);
+  const dim3 grid(unsigned((p.max_q + rows - 1) / rows), unsigned(p.kv_heads * p.nsplit), unsigned(p.n_seqs));
+  cross_tile_kernel<D, ROW_TILES><<<grid, C::THREADS, C::SMEM, st>>>(tq, tk, tv, p);
 }
 
 template <int D>
@@ -946,19 +963,15 @@ void launch(const CrossParams& p, const kh_cross_attention_args& a, bool states,
     else launch_rows<D, 4>(tk, tv, p, st);
   } else {
     using C = TCfg<D>;
-    static std::atomic<uint64_t> configured{0};
-    once_per_device(configured, [] {
-      KH_CUDA(cudaFuncSetAttribute(cross_tile_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
-    });
     const int qpt = TROWS / p.G;
     CUtensorMap tq;
     encode_tensor_map_f16_3d(&tq, a.q, {uint64_t(D), uint64_t(a.q_heads), uint64_t(a.q_rows)}, D, uint64_t(a.q_stride),
                              {uint32_t(C::PCOLS), uint32_t(p.G), uint32_t(qpt)}, C::ROWB);
     if (states) state_maps(C::PCOLS, C::KEYS, C::ROWB);
     else tk = tv = tq;
-    const int rows = C::ROW_TILES * qpt;
-    const dim3 grid(unsigned((a.max_q + rows - 1) / rows), unsigned(a.kv_heads * p.nsplit), unsigned(a.n_seqs));
-    cross_tile_kernel<D><<<grid, C::THREADS, C::SMEM, st>>>(tq, tk, tv, p);
+    if constexpr (D == 128) launch_tiles<D, 2>(tq, tk, tv, p, st);
+    else if (row_tiles(a) == 2) launch_tiles<D, 2>(tq, tk, tv, p, st);
+    else launch_tiles<D, 1>(tq, tk, tv, p, st);
   }
   KH_CUDA(cudaGetLastError());
   if (p.nsplit > 1) {
