@@ -110,6 +110,7 @@ __global__ void __launch_bounds__(RW * 32)
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int split = blockIdx.x, hk = blockIdx.y, s = blockIdx.z;
+  launch_dependents();
   if (lane == 0) {
     for (int i = 0; i < C::STAGES; ++i) mbar_init(&bars[warp][i], 1);
     fence_barrier_init();
@@ -316,47 +317,64 @@ __global__ void __launch_bounds__(RW * 32)
   }
 }
 
-// ---- joining the splits: one CTA of 4 warps per (query, head), a warp every fourth split ----
+// ---- joining the splits: WARPS warps per (query, head), each every WARPS-th split ----
+//
+// CTAs of 4 warps, launched while the parts are made. Few rows: 4 warps to one, for the loads in flight. Many:
+// one (11 sequences of up to 660 queries, heads of 128, 3 splits: 22.8 us with the parts, 28.9 with 4).
 
-template <int D>
-__global__ void __launch_bounds__(128) cross_join_kernel(const CrossParams p) {
+template <int D, int WARPS>
+__global__ void __launch_bounds__(128) cross_join_kernel(const CrossParams p, int64_t rows) {
   constexpr int V = D / 32;
   __shared__ float so[4][D], sl[4];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int64_t t = blockIdx.x;
+  const int64_t t = int64_t(blockIdx.x) * (4 / WARPS) + warp / WARPS;
   const int64_t per_seq = int64_t(p.max_q) * p.q_heads;
   const int s = int(t / per_seq);
   const int i = int((t - s * per_seq) / p.q_heads), h = int(t % p.q_heads);
-  int64_t q0;
-  int nq;
-  seq_range(p.q_starts, s, p.q_rows, p.max_q, q0, nq);
-  if (i >= nq) return;
-  // the largest reference point first (a lane per split), then the sums, with independent loads
-  float m = -INFINITY;
-  for (int z = lane; z < p.nsplit; z += 32) m = fmaxf(m, p.part_ml[part_index(p, z, s, i, h)].x);
-  for (int w = 16; w; w >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, w));
-  float l = 0.f, o[V] = {};
+  int64_t q0 = 0;
+  int nq = 0;
+  if (t < rows) seq_range(p.q_starts, s, p.q_rows, p.max_q, q0, nq);
+  wait_primary();
+  const bool in = i < nq;  // (WARPS 4: the same for the CTA)
+  float o[V] = {}, l = 0.f;
+  if (in) {
+    // the largest reference point first (a lane per split), then the sums, with independent loads
+    float m = -INFINITY;
+    for (int z = lane; z < p.nsplit; z += 32) m = fmaxf(m, p.part_ml[part_index(p, z, s, i, h)].x);
+    for (int w = 16; w; w >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, w));
 #pragma unroll 4
-  for (int z = warp; z < p.nsplit; z += 4) {
-    const int64_t at = part_index(p, z, s, i, h);
-    const float2 ml = p.part_ml[at];
-    float v[V];
+    for (int z = warp % WARPS; z < p.nsplit; z += WARPS) {
+      const int64_t at = part_index(p, z, s, i, h);
+      const float2 ml = p.part_ml[at];
+      float v[V];
 #pragma unroll
-    for (int e = 0; e < V; ++e) v[e] = p.part_o[at * D + lane * V + e];
-    const float f = ml.x == -INFINITY ? 0.f : ex2_approx(ml.x - m);
-    l += f * ml.y;
+      for (int e = 0; e < V; ++e) v[e] = p.part_o[at * D + lane * V + e];
+      const float f = ml.x == -INFINITY ? 0.f : ex2_approx(ml.x - m);
+      l += f * ml.y;
 #pragma unroll
-    for (int e = 0; e < V; ++e) o[e] += f == 0.f ? 0.f : f * v[e];  // (without a kept state O holds anything)
+      for (int e = 0; e < V; ++e) o[e] += f == 0.f ? 0.f : f * v[e];  // (without a kept state O holds anything)
+    }
   }
+  if (WARPS > 1) {
 #pragma unroll
-  for (int e = 0; e < V; ++e) so[warp][lane * V + e] = o[e];
-  if (lane == 0) sl[warp] = l;
-  __syncthreads();
-  l = (sl[0] + sl[1]) + (sl[2] + sl[3]);
+    for (int e = 0; e < V; ++e) so[warp][lane * V + e] = o[e];
+    if (lane == 0) sl[warp] = l;
+    __syncthreads();
+    if (warp > 0) return;
+    l = (sl[0] + sl[1]) + (sl[2] + sl[3]);
+#pragma unroll
+    for (int e = 0; e < V; ++e)
+      o[e] = (so[0][lane * V + e] + so[1][lane * V + e]) + (so[2][lane * V + e] + so[3][lane * V + e]);
+  }
+  if (!in) return;
   const float inv = l == 0.f ? 0.f : 1.f / l;
-  if (threadIdx.x < D)
-    p.out[(q0 + i) * p.out_stride + h * D + threadIdx.x] =
-        __float2half_rn(((so[0][threadIdx.x] + so[1][threadIdx.x]) + (so[2][threadIdx.x] + so[3][threadIdx.x])) * inv);
+  __half* dst = p.out + (q0 + i) * p.out_stride + h * D + lane * V;
+  if constexpr (V == 1) {
+    dst[0] = __float2half_rn(o[0] * inv);
+  } else {
+#pragma unroll
+    for (int e = 0; e < V; e += 2) reinterpret_cast<uint32_t*>(dst)[e / 2] = pack_half2(o[e] * inv, o[e + 1] * inv);
+  }
 }
 
 // ---- tiles of 128 rows on the tensor cores ----
@@ -475,6 +493,7 @@ __global__ void __launch_bounds__(TCfg<D>::THREADS, TCfg<D>::ONE ? 1 : 2)
   uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(v_clear + C::VS);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_holder + 1);
 
+  launch_dependents();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int hk = blockIdx.y % p.kv_heads, split = blockIdx.y / p.kv_heads, s = blockIdx.z;
   const int G = p.G, qpt = TROWS / G;  // queries of a row tile
@@ -927,6 +946,8 @@ void launch_rows(const CUtensorMap& tk, const CUtensorMap& tv, const CrossParams
   cross_rows_kernel<D, RW><<<dim3(p.nsplit, p.kv_heads, p.n_seqs), RW * 32, RCfg<D, RW>::SMEM, st>>>(tk, tv, p);
 }
 
+constexpr int64_t JOIN_ROWS = 1024;  // from here on a warp to a row (8 rows, 64 splits: 52 us, 62 with a warp)
+
 template <int D, int ROW_TILES>
 void launch_tiles(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const CrossParams& p, cudaStream_t st) {
   using C = TCfg<D>;
@@ -976,8 +997,17 @@ void launch(const CrossParams& p, const kh_cross_attention_args& a, bool states,
   KH_CUDA(cudaGetLastError());
   if (p.nsplit > 1) {
     const int64_t rows = int64_t(p.n_seqs) * p.max_q * p.q_heads;
-    cross_join_kernel<D><<<unsigned(rows), 128, 0, st>>>(p);
-    KH_CUDA(cudaGetLastError());
+    const bool many = rows > JOIN_ROWS;
+    cudaLaunchAttribute attr = {};
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(unsigned(many ? (rows + 3) / 4 : rows), 1, 1);
+    cfg.blockDim = dim3(128, 1, 1);
+    cfg.stream = st;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    KH_CUDA(cudaLaunchKernelEx(&cfg, many ? cross_join_kernel<D, 1> : cross_join_kernel<D, 4>, p, rows));
   }
 }
 
