@@ -39,6 +39,7 @@ struct NormParams {
   uint32_t groups;  // rows * blocks of this launch
   int q_heads, k_heads, D, R;
   uint32_t q_blocks, blocks;  // blocks of U heads of a row: those of q, all
+  uint32_t lane_inv;          // 1024 / chunks of a head, rounded up
   float eps, inv_d;
   bool interleaved;
 };
@@ -122,15 +123,27 @@ __device__ __forceinline__ void coefficients(float (&wc)[VEC], float (&ws)[VEC],
 // stores are whole heads side by side; the chunk that the rotation mixes with comes from its lane. MODE:
 // 0 no rotation, 1 pairs R / 2 apart, 2 neighbouring pairs. Next to the loads it is the instructions that
 // count (packed f32x2 arithmetic, one mode to a kernel): 65,536 rows of 24 heads of 64 take 77 us (5.3 TB/s;
-// 91 us with every mode in one kernel, 160 instructions to a chunk, and 83 us with the kernel below).
-template <typename T, int VEC, int U, int MODE>
-__global__ void __launch_bounds__(256) qk_norm_rope_lanes_kernel(const NormParams p, int lanes_log2) {
-  const uint32_t lanes = 1u << lanes_log2;
-  const uint32_t thread = blockIdx.x * 256u + threadIdx.x;
-  const int c = int(thread & (lanes - 1));  // chunk
-  const uint32_t group = thread >> lanes_log2;
+// 91 us with every mode in one kernel, 160 instructions to a chunk, and 83 us with the kernel below). Heads
+// whose chunks are no power of two (!POW2) share a warp whole: 35,149 rows of 20 heads of 80, 57 us against
+// 65 with 16 lanes to their 10 chunks.
+template <typename T, int VEC, int U, int MODE, bool POW2>
+__global__ void __launch_bounds__(256) qk_norm_rope_lanes_kernel(const NormParams p, int lanes) {
+  const int lane = threadIdx.x & 31;
+  int c;           // chunk
+  uint32_t group;  // blocks of heads, in order
+  bool in;         // (all stay for the shuffles)
+  if (POW2) {
+    const uint32_t log2 = 31 - __clz(lanes);
+    group = (blockIdx.x * 256u + threadIdx.x) >> log2;
+    c = lane & (lanes - 1);
+    in = group < p.groups;
+  } else {  // whole heads to a warp, lanes behind the last one idle; lane / lanes is exact below 33
+    const uint32_t nth = uint32_t(lane) * p.lane_inv >> 10, of = 32u * p.lane_inv >> 10;
+    c = lane - int(nth) * lanes;
+    group = (blockIdx.x * 8u + (threadIdx.x >> 5)) * of + nth;
+    in = nth < of && group < p.groups;
+  }
   const uint32_t row = group / p.blocks, block = group - row * p.blocks;
-  const bool in = group < p.groups && c < p.D / VEC;  // (all stay for the shuffles)
   const bool is_k = block >= p.q_blocks;
   const int head0 = int(is_k ? block - p.q_blocks : block) * U;
   const int nheads = in ? min(U, (is_k ? p.k_heads : p.q_heads) - head0) : 0;
@@ -200,11 +213,23 @@ __global__ void __launch_bounds__(256) qk_norm_rope_lanes_kernel(const NormParam
     for (int e = 0; e < VEC; e += 2) ss = sm100::ffma2(a[u].pair(e), a[u].pair(e), ss);
     scale[u] = ss.x + ss.y;
   }
-  for (uint32_t o = lanes >> 1; o; o >>= 1)
+  if (POW2) {
+    for (int o = lanes >> 1; o; o >>= 1)
 #pragma unroll
-    for (int u = 0; u < U; ++u) scale[u] += __shfl_xor_sync(0xffffffffu, scale[u], o);
+      for (int u = 0; u < U; ++u) scale[u] += __shfl_xor_sync(0xffffffffu, scale[u], o);
+  } else {  // towards the head's first lane, and back
+    for (int o = 16; o; o >>= 1)
+      if (o < lanes)
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          const float t = __shfl_down_sync(0xffffffffu, scale[u], o);
+          if (c + o < lanes) scale[u] += t;
+        }
+#pragma unroll
+    for (int u = 0; u < U; ++u) scale[u] = __shfl_sync(0xffffffffu, scale[u], lane - c);
+  }
 
-  const int src = (threadIdx.x & 31) - c + other;
+  const int src = lane - c + other;
   T* yr = static_cast<T*>(p.out) + row * p.out_stride + col;
 #pragma unroll
   for (int u = 0; u < U; ++u) {
@@ -372,13 +397,14 @@ __global__ void __launch_bounds__(256) qk_norm_rope_kernel(const NormParams p, i
 // PAIRS 0: the kernel with one chunk to a thread.
 template <typename T, int VEC, int PAIRS, int U>
 void launch(NormParams p, int64_t rows, cudaStream_t st) {
-  const int units = PAIRS ? (p.D / VEC + 1) / 2 : p.D / VEC;
   int log2 = 0;
-  while ((std::max(PAIRS, 1) << log2) < units) ++log2;
+  while ((std::max(PAIRS, 1) << log2) < (p.D / VEC + 1) / 2) ++log2;
+  const int lanes = p.D / VEC, heads = PAIRS ? 32 >> log2 : 32 / lanes;  // heads (of U blocks) of a warp
   p.q_blocks = uint32_t((p.q_heads + U - 1) / U);
   p.blocks = p.q_blocks + uint32_t((p.k_heads + U - 1) / U);
+  p.lane_inv = uint32_t((1024 + lanes - 1) / lanes);
   // 32-bit thread indexes: launches of as many whole rows as stay below 2^31 threads
-  const int64_t most = ((int64_t(1) << 31) - 256) / (int64_t(p.blocks) << log2);
+  const int64_t most = ((int64_t(1) << 31) - 8192) / 32 * heads / p.blocks;
   for (int64_t r = 0; r < rows; r += most) {
     const int64_t n = std::min(most, rows - r);
     NormParams q = p;
@@ -386,12 +412,16 @@ void launch(NormParams p, int64_t rows, cudaStream_t st) {
     q.x = static_cast<const T*>(p.x) + r * p.x_stride;
     q.out = static_cast<T*>(p.out) + r * p.out_stride;
     if (p.R) q.positions = p.positions + r;
-    const int64_t threads = (int64_t(q.groups) << log2);
-    const unsigned grid = unsigned((threads + 255) / 256);
+    const unsigned grid = unsigned((q.groups + 8 * heads - 1) / (8 * heads));
     if constexpr (PAIRS == 0) {
-      if (!p.R) qk_norm_rope_lanes_kernel<T, VEC, U, 0><<<grid, 256, 0, st>>>(q, log2);
-      else if (!p.interleaved) qk_norm_rope_lanes_kernel<T, VEC, U, 1><<<grid, 256, 0, st>>>(q, log2);
-      else qk_norm_rope_lanes_kernel<T, VEC, U, 2><<<grid, 256, 0, st>>>(q, log2);
+      const int mode = !p.R ? 0 : !p.interleaved ? 1 : 2;
+      auto go = [&](auto* kernel) { kernel<<<grid, 256, 0, st>>>(q, lanes); };
+      if ((lanes & (lanes - 1)) == 0)
+        go(mode == 0 ? qk_norm_rope_lanes_kernel<T, VEC, U, 0, true> : mode == 1 ? qk_norm_rope_lanes_kernel<T, VEC, U, 1, true>
+                                                                                 : qk_norm_rope_lanes_kernel<T, VEC, U, 2, true>);
+      else
+        go(mode == 0 ? qk_norm_rope_lanes_kernel<T, VEC, U, 0, false> : mode == 1 ? qk_norm_rope_lanes_kernel<T, VEC, U, 1, false>
+                                                                                  : qk_norm_rope_lanes_kernel<T, VEC, U, 2, false>);
     } else {
       qk_norm_rope_kernel<T, VEC, PAIRS, U><<<grid, 256, 0, st>>>(q, log2);
     }

@@ -728,3 +728,47 @@ def test_two_captured_layers_replayed_at_once():
     kb().operator_status(stream())
     for t, w in zip(ts, want):
         assert torch.equal(t["y"], w)
+
+
+@pytest.mark.parametrize("dtype", ["f16", "f32"])
+@pytest.mark.parametrize("D", list(range(8, 129, 8)) + [136, 176, 224, 256])
+def test_norm_every_chunk_count(dtype, D):
+    """Heads of 1 to 32 chunks of a load each, with the rotation over all, a part, and none of the head."""
+    torch = torch_()
+    g = gen(D)
+    rows, qh, kh = 37, 5, 2
+    x = randn(g, rows, (qh + kh) * D + 8, dtype=getattr(torch, "float16" if dtype == "f16" else "float32"))
+    qw, kw = 1 + 0.1 * randn(g, D, dtype=torch.float32), 1 + 0.1 * randn(g, D, dtype=torch.float32)
+    pos = torch.randint(0, 50, (rows,), generator=g, device="cuda").int()
+    for R, inter in ((D, False), (D, True), (D // 16 * 8, False), (D // 16 * 8, True), (0, False)):
+        table = angle_table(50, R) if R else None
+        out = torch.full_like(x, 7.0)
+        kb().qk_norm_rope(norm_args(x, out, qh, kh, D, R, inter, table, pos if R else None, qw, kw), stream())
+        kb().operator_status(stream())
+        want, top = norm_ref(x, qh, kh, D, R, inter, table, pos, qw, kw)
+        close(out[:, :(qh + kh) * D], want, norm_tol(x, want, top), (R, inter))
+        assert (out[:, (qh + kh) * D:] == 7).all()
+
+
+@pytest.mark.parametrize("D,H,KV", [(32, 4, 4), (64, 2, 2), (64, 6, 2)])
+@pytest.mark.parametrize("masked", [False, True])
+def test_cross_many_queries_on_short_states(D, H, KV, masked):
+    """Two row tiles to a CTA: lengths on both sides of a tile, one key tile and several, none."""
+    torch = torch_()
+    ql, kl = [300, 140, 1, 128, 129, 17], [256, 65, 64, 0, 1, 200]
+    q, k, v, qs, ks, scale = cross_case(D + H, ql, kl, H, KV, D, pad=8, first=2)
+    mask = None
+    if masked:
+        mask = (torch.rand(k.shape[0], generator=gen(3), device="cuda") > 0.5).float()
+        mask[ks[1]:ks[2]] = 0
+    out = cross_check(q, k, v, qs, ks, H, KV, D, scale, mask)
+    assert (out[qs[3]:qs[4], :H * D] == 0).all()
+    if masked:
+        assert (out[qs[1]:qs[2], :H * D] == 0).all()
+
+
+@pytest.mark.parametrize("D", [32, 64, 128])
+def test_cross_join_of_many_rows(D):
+    """Split states of so many rows that a warp joins each, with sequences shorter than the bounds."""
+    q, k, v, qs, ks, scale = cross_case(D + 1, [400, 3, 250], [3000, 40, 1500], 3, 1, D)
+    cross_check(q, k, v, qs, ks, 3, 1, D, scale)
