@@ -1178,17 +1178,25 @@ void launch_ex(F* kernel, dim3 grid, int threads, size_t smem, int cluster, bool
   KH_CUDA(cudaLaunchKernelEx(&cfg, kernel, args...));
 }
 
-// Whether a tile of 128 rows holds so many adapters (no more than it has segments) that a product for
-// each costs more than the tile is worth.
-bool scattered(const kh_lora_matmul_args& a) { return a.rows < 8 * int64_t(a.n_segs) && a.n_adapters > 16; }
-// h by a CTA per row: few rows (each reads its adapter's A through L2), or scattered ones (400 rows of 40
-// adapters, 1,024 -> 4,096: the whole call 63 us, with h by tiles 80; 1,000 rows of 100: 38 against 47).
-bool shrinks_rows(const kh_lora_matmul_args& a) {
-  return scattered(a) || (a.rows <= FT && a.rows * a.rank * int64_t(a.k) <= (int64_t(1) << 24));
+// Adapters that a tile of 128 rows holds, about: no more than there are, nor than its segments.
+int64_t tile_adapters(const kh_lora_matmul_args& a) {
+  return std::min<int64_t>({int64_t(a.n_adapters), 128, std::max<int64_t>(1, 128 * int64_t(a.n_segs) / a.rows)});
 }
-// Rows of x as the columns of the product: W is read once per 128 rows. Scattered rows take it up to four
-// times (250 rows of 100 adapters, 768 -> 2,304: 36 us against 94; 400 of 40, 1,024 -> 4,096: 63 against 179).
-bool takes_few(const kh_lora_matmul_args& a) { return a.rows <= FT || (a.rows <= 4 * FT && scattered(a)); }
+// h by a CTA per row, which reads its adapter's A through L2, instead of by tiles, which take a product
+// for each adapter. Few rows (128 of rank 64, 4,096 values to a sum, are too many already); a few hundred
+// of some adapters (216 rows of 5, 1,024 -> 2,304, rank 8: the whole call 21 us against 26; 689 of 5,
+// 4,096 -> 384, rank 16: 32 against 26); any number of many (1,095 of 16, 384 -> 1,024: 24 against 30).
+bool shrinks_rows(const kh_lora_matmul_args& a) {
+  const int64_t work = a.rows * a.rank * int64_t(a.k), adapters = tile_adapters(a);
+  return (a.rows <= FT && work <= (1 << 24)) || (adapters > 4 && work <= (1 << 23)) || adapters >= 16;
+}
+// Rows of x as the columns of the product: W is read once per 128 rows, where a pair's tile takes a product
+// for each of its adapters. Up to 128 rows; of many adapters up to four times that (187 rows of 16 adapters,
+// 768 -> 384: 18 us against 50; 477 of 23 to a tile 19 against 27, of 16 41 against 27).
+bool takes_few(const kh_lora_matmul_args& a) {
+  const int64_t blocks = (a.rows + FT - 1) / FT;
+  return blocks <= 1 || (blocks <= 4 && tile_adapters(a) >= 5 * blocks);
+}
 // h from the same launch: every cluster makes it for itself, so A is read once per 128 outputs.
 bool fuses(const kh_lora_matmul_args& a) { return takes_few(a) && a.n_adapters > 0 && a.n_adapters * a.rank <= 128; }
 
