@@ -325,17 +325,15 @@ __global__ void __maxnreg__(FUSED ? 168 : 112)
       if (!wwait(&full[st], ph, 233)) { ok = false; break; }
       fence_after_sync();
       const uint64_t dw = desc_sw128(smem + st * stage_bytes), dx = desc_sw128(smem + st * stage_bytes + X_OFF);
-      if (lead) {
 #pragma unroll
-        for (int k = 0; k < 4; ++k) mma_f16(tmem, dw + uint64_t(2 * k), dx + uint64_t(2 * k), idesc, (kb | k) ? 1u : 0u);
-        if (FUSED) {  // (rows of the A tile past the adapters hold anything; so do their lanes)
-          const uint64_t da = desc_sw128(smem + st * stage_bytes + 16384);
+      for (int k = 0; k < 4; ++k) mma_f16_if(lead, tmem, dw + uint64_t(2 * k), dx + uint64_t(2 * k), idesc, (kb | k) ? 1u : 0u);
+      if (FUSED) {  // (rows of the A tile past the adapters hold anything; so do their lanes)
+        const uint64_t da = desc_sw128(smem + st * stage_bytes + 16384);
 #pragma unroll
-          for (int k = 0; k < 4; ++k)
-            mma_f16(tmem + tcols / 2, da + uint64_t(2 * k), dx + uint64_t(2 * k), idesc, (kb | k) ? 1u : 0u);
-        }
-        mma_commit(&empty[st]);
+        for (int k = 0; k < 4; ++k)
+          mma_f16_if(lead, tmem + tcols / 2, da + uint64_t(2 * k), dx + uint64_t(2 * k), idesc, (kb | k) ? 1u : 0u);
       }
+      mma_commit_if(lead, &empty[st]);
       __syncwarp();
       if (++st == stages) {
         st = 0;
@@ -566,7 +564,8 @@ __global__ void __launch_bounds__(224) lora_shrink_tile_kernel(const __grid_cons
     return __all_sync(0xffffffffu, mbar_wait(bar, parity, code));
   };
 
-  if (warp == 0) {
+  if (warp == 0) {  // all lanes in step, one issues (and so below)
+    const bool lead = elect_one();
     bool ok = true;
     int xs = 0, issued = 0;
     uint32_t u = 0;
@@ -574,10 +573,8 @@ __global__ void __launch_bounds__(224) lora_shrink_tile_kernel(const __grid_cons
       // past the first round it is known whether any row has an adapter (if none, x was loaded in vain)
       if (kb == xstages && (!wwait(listed, 0, 200) || pieces.count == 0)) break;
       if (!wwait(&x_empty[xs], u ^ 1, 201)) { ok = false; break; }
-      if (lane == 0) {
-        mbar_arrive_expect_tx(&x_full[xs], 16384);
-        tma_load_2d(sX + xs * 16384, &tmx, &x_full[xs], (kb0 + kb) * 64, r0);
-      }
+      mbar_arrive_expect_tx_if(lead, &x_full[xs], 16384);
+      tma_load_2d_if(lead, sX + xs * 16384, &tmx, &x_full[xs], (kb0 + kb) * 64, r0);
       __syncwarp();
       ++issued;
       if (++xs == xstages) {
@@ -643,16 +640,15 @@ __global__ void __launch_bounds__(224) lora_shrink_tile_kernel(const __grid_cons
     if (lane == 0) pieces.count = np;
     __syncwarp();
     mbar_arrive(listed);
+    const bool lead = elect_one();
     bool ok = true;
     int as = 0;
     uint32_t v = 0, pend = 0;  // pend: two bits a stage: issued, parity
     for (int kb = 0; kb < nk && ok; ++kb)
       for (int i = 0; i < np; ++i) {
         if (!wwait(&a_empty[as], v ^ 1, 202)) { ok = false; break; }
-        if (lane == 0) {
-          mbar_arrive_expect_tx(&a_full[as], a_bytes);
-          tma_load_2d(sA + as * a_bytes, &tma, &a_full[as], (kb0 + kb) * 64, pieces.id[i] * p.rank);
-        }
+        mbar_arrive_expect_tx_if(lead, &a_full[as], a_bytes);
+        tma_load_2d_if(lead, sA + as * a_bytes, &tma, &a_full[as], (kb0 + kb) * 64, pieces.id[i] * p.rank);
         __syncwarp();
         pend = (pend & ~(3u << (2 * as))) | ((2u | v) << (2 * as));
         if (++as == astages) {
@@ -681,20 +677,18 @@ __global__ void __launch_bounds__(224) lora_shrink_tile_kernel(const __grid_cons
         if (!wwait(&a_full[as], av, 206)) { ok = false; break; }
         fence_after_sync();
         const uint64_t da = desc_sw128(sA + as * a_bytes);
-        if (lead) {
-          const uint32_t off[4] = {o.x, o.y, o.z, o.w};
+        const uint32_t off[4] = {o.x, o.y, o.z, o.w};
 #pragma unroll
-          for (int k = 0; k < 4; ++k)
-            mma_f16_lanes(tmem, dx + uint64_t(2 * k), da + uint64_t(2 * k), idesc, (kb | k) ? 1u : 0u, off);
-          mma_commit(&a_empty[as]);
-        }
+        for (int k = 0; k < 4; ++k)
+          mma_f16_lanes_if(lead, tmem, dx + uint64_t(2 * k), da + uint64_t(2 * k), idesc, (kb | k) ? 1u : 0u, off);
+        mma_commit_if(lead, &a_empty[as]);
         __syncwarp();
         if (++as == astages) {
           as = 0;
           av ^= 1;
         }
       }
-      if (ok && lead) mma_commit(&x_empty[xs]);
+      mma_commit_if(ok && lead, &x_empty[xs]);
       __syncwarp();
       if (++xs == xstages) {
         xs = 0;
@@ -998,13 +992,11 @@ __global__ void __launch_bounds__(PCfg<BN>::THREADS, 1)
           } else {
             const uint4 o0 = notes[stage].off[0], o1 = notes[stage].off[1];
             const int steps = notes[stage].steps;
-            if (lead) {
-              const uint32_t off[8] = {o0.x, o0.y, o0.z, o0.w, o1.x, o1.y, o1.z, o1.w};
+            const uint32_t off[8] = {o0.x, o0.y, o0.z, o0.w, o1.x, o1.y, o1.z, o1.w};
 #pragma unroll
-              for (int k = 0; k < BK / 16; ++k)
-                if (k < steps) mma_f16_pair_lanes(d, da + uint64_t(k * 2), db + uint64_t(k * 2), idesc, 1u, off);
-              mma_commit_pair_both(&empty[stage]);
-            }
+            for (int k = 0; k < BK / 16; ++k)
+              mma_f16_pair_lanes_if(lead && k < steps, d, da + uint64_t(k * 2), db + uint64_t(k * 2), idesc, 1u, off);
+            mma_commit_pair_both_if(lead, &empty[stage]);
           }
           __syncwarp();
           if (++stage == STAGES) {
@@ -1337,7 +1329,8 @@ void lora_matmul(const kh_lora_matmul_args* args, cudaStream_t st) {
       encode_tensor_map_f16(&ta, a.lora_a, uint64_t(a.n_adapters) * a.rank, uint64_t(a.k), uint64_t(a.k), 64, R16, 128);
       const int64_t tiles = (a.rows + 127) / 128;
       int Z = 1;  // CTAs that split a tile's sum: while SMs are idle, at least two K blocks each
-      while (Z < 8 && 2 * Z * tiles <= CLUSTER_CTAS && 4 * Z <= (a.k + 63) / 64) Z *= 2;
+      const int at_once = R16 <= 32 ? 2 * CLUSTER_CTAS : CLUSTER_CTAS;  // (two CTAs an SM up to rank 32)
+      while (Z < 8 && 2 * Z * tiles <= at_once && 4 * Z <= (a.k + 63) / 64) Z *= 2;
       // many tiles: rings so short that four CTAs share an SM (up to rank 32) and cover each other's waits
       const int xstages = tiles > 2 * SMS ? 2 : SXS, astages = R16 > 32 || tiles > 2 * SMS ? 4 : SAS;
       const size_t smem = size_t(xstages) * 16384 + size_t(astages) * R16 * 128 + 1024;

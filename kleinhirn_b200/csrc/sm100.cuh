@@ -250,13 +250,14 @@ __device__ __forceinline__ void mma_f16_ts(uint32_t tmem_d, uint32_t tmem_a, uin
 }
 
 // mma_f16 that leaves the TMEM lanes (rows of D) whose bit is set in off[lane / 32] as they are.
-__device__ __forceinline__ void mma_f16_lanes(uint32_t tmem_d, uint64_t da, uint64_t db, uint32_t idesc, uint32_t acc,
-                                              const uint32_t (&off)[4]) {
+__device__ __forceinline__ void mma_f16_lanes_if(bool lead, uint32_t tmem_d, uint64_t da, uint64_t db, uint32_t idesc,
+                                                 uint32_t acc, const uint32_t (&off)[4]) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\t"
+      "{\n\t.reg .pred p, q;\n\t"
       "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%5, %6, %7, %8}, p;\n\t}" ::"r"(tmem_d),
-      "l"(da), "l"(db), "r"(idesc), "r"(acc), "r"(off[0]), "r"(off[1]), "r"(off[2]), "r"(off[3])
+      "setp.ne.b32 q, %9, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%5, %6, %7, %8}, p;\n\t}" ::"r"(tmem_d),
+      "l"(da), "l"(db), "r"(idesc), "r"(acc), "r"(off[0]), "r"(off[1]), "r"(off[2]), "r"(off[3]), "r"(uint32_t(lead))
       : "memory");
 }
 
@@ -407,6 +408,15 @@ __device__ __forceinline__ void tma_load_2d_pair(void* dst, const CUtensorMap* m
       : "memory");
 }
 // The same, and the arrival that announces its bytes, under a predicate (see mma_f16_if).
+__device__ __forceinline__ void tma_load_2d_if(bool lead, void* dst, const CUtensorMap* map, uint64_t* bar, int x, int y) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\t"
+      "setp.ne.b32 q, %5, 0;\n\t"
+      "@q cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];\n\t}" ::"r"(
+          smem_u32(dst)),
+      "l"(map), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(uint32_t(lead))
+      : "memory");
+}
 __device__ __forceinline__ void tma_load_2d_pair_if(bool lead, void* dst, const CUtensorMap* map, uint32_t bar, int x, int y) {
   asm volatile(
       "{\n\t.reg .pred q;\n\t"
@@ -455,14 +465,15 @@ __device__ __forceinline__ void mma_f16_pair(uint32_t tmem_d, uint64_t da, uint6
       : "memory");
 }
 // The same, leaving rows of D as they are: bit of row r in off[r / 32] (rows 128 and on: the peer's).
-__device__ __forceinline__ void mma_f16_pair_lanes(uint32_t tmem_d, uint64_t da, uint64_t db, uint32_t idesc,
-                                                   uint32_t acc, const uint32_t (&off)[8]) {
+__device__ __forceinline__ void mma_f16_pair_lanes_if(bool lead, uint32_t tmem_d, uint64_t da, uint64_t db, uint32_t idesc,
+                                                      uint32_t acc, const uint32_t (&off)[8]) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\t"
+      "{\n\t.reg .pred p, q;\n\t"
       "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, {%5, %6, %7, %8, %9, %10, %11, %12}, p;\n\t}" ::"r"(tmem_d),
+      "setp.ne.b32 q, %13, 0;\n\t"
+      "@q tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, {%5, %6, %7, %8, %9, %10, %11, %12}, p;\n\t}" ::"r"(tmem_d),
       "l"(da), "l"(db), "r"(idesc), "r"(acc), "r"(off[0]), "r"(off[1]), "r"(off[2]), "r"(off[3]), "r"(off[4]),
-      "r"(off[5]), "r"(off[6]), "r"(off[7])
+      "r"(off[5]), "r"(off[6]), "r"(off[7]), "r"(uint32_t(lead))
       : "memory");
 }
 // Arrives on the mbarrier at the same shared-memory offset in both CTAs of the pair once the
