@@ -55,9 +55,11 @@ __device__ __forceinline__ int known_adapter(const LoraParams& p, int id) {
   return -1;
 }
 __device__ __forceinline__ int adapter_of(const LoraParams& p, int seg) { return known_adapter(p, __ldg(p.ids + seg)); }
-// First segment that ends behind row r (n_segs if none), found by a whole warp, 32 probes a round; with
-// one row to a segment (a step of single tokens) it is segment r, which the first round looks at too.
-__device__ __forceinline__ int first_seg(const LoraParams& p, int r) {
+// First segment that ends behind row r (n_segs if none), found by a whole warp, 32 probes a round; with one
+// row to a segment (a step of single tokens) it is segment r, which the first round looks at too. Where the
+// caller's first round reads all segments anyway (`reads` of them), the first of all.
+__device__ __forceinline__ int first_seg(const LoraParams& p, int r, int reads) {
+  if (p.n_segs <= reads) return 0;
   const int lane = threadIdx.x & 31;
   const int guess = min(r, p.n_segs - 1), g0 = seg_start(p, guess), g1 = seg_start(p, guess + 1);
   int lo = 0, hi = p.n_segs;
@@ -93,7 +95,7 @@ __device__ __forceinline__ float dot8(uint4 a, uint4 b, float acc) {
 __global__ void __launch_bounds__(512) lora_shrink_rows_kernel(const LoraParams p) {
   launch_dependents();
   const int t = blockIdx.x, lane = threadIdx.x & 31;
-  const int seg = first_seg(p, t);
+  const int seg = first_seg(p, t, 0);
   if (seg >= p.n_segs || t < seg_start(p, seg) || t >= seg_start(p, p.n_segs)) return;
   const int ad = adapter_of(p, seg);
   if (ad < 0) return;
@@ -352,7 +354,7 @@ __global__ void __maxnreg__(FUSED ? 168 : 112)
     for (int t = lane; t < FT; t += 32) ids[t] = -1;
     __syncwarp();
     if (p.n_adapters > 0) {
-      for (int s = first_seg(p, t0), more = 1; more && s < p.n_segs; s += 128) {
+      for (int s = first_seg(p, t0, 128), more = 1; more && s < p.n_segs; s += 128) {
         // four segments a lane, their loads together
         int lo[4], hi[4], id[4];
 #pragma unroll
@@ -536,6 +538,8 @@ __global__ void __launch_bounds__(224) lora_shrink_tile_kernel(const __grid_cons
            *done = a_empty + SAS, *drain = done + 1, *listed = drain + 1;
   launch_dependents();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) prefetch_tmap(&tmx);
+  if (threadIdx.x == 192) prefetch_tmap(&tma);
   const int z = blockIdx.x % Z, r0 = int(blockIdx.x / Z) * 128;
   const uint32_t cols = R16 <= 32 ? 32u : R16 <= 64 ? 64u : 128u;
   if (threadIdx.x == 0) {
@@ -592,7 +596,7 @@ __global__ void __launch_bounds__(224) lora_shrink_tile_kernel(const __grid_cons
     int n = 0;
     for (int r = lane; r < 128; r += 32) pieces.row_id[r] = -1;
     __syncwarp();
-    for (int s = first_seg(p, r0), more = 1; more && s < p.n_segs; s += 128) {
+    for (int s = first_seg(p, r0, 128), more = 1; more && s < p.n_segs; s += 128) {
       // four segments a lane, their loads together
       int lo[4], hi[4], id[4];
 #pragma unroll
@@ -625,11 +629,7 @@ __global__ void __launch_bounds__(224) lora_shrink_tile_kernel(const __grid_cons
           uint32_t* off = reinterpret_cast<uint32_t*>(&pieces.off[at]);
 #pragma unroll
           for (int w = 0; w < 4; ++w) atomicAnd(off + w, ~lanes_on(lo[j], hi[j], w));
-          const float sc = p.scales ? __ldg(p.scales + ad) : 1.f;
-          for (int r = lo[j]; r < hi[j]; ++r) {
-            pieces.row_id[r] = ad;
-            pieces.row_scale[r] = sc;
-          }
+          for (int r = lo[j]; r < hi[j]; ++r) pieces.row_id[r] = ad;
         }
         n += __popc(added);  // (at most 128: every one has a row of its own)
         __syncwarp();
@@ -705,10 +705,13 @@ __global__ void __launch_bounds__(224) lora_shrink_tile_kernel(const __grid_cons
     __syncwarp();
   } else {
     const int quarter = warp & 3, r = quarter * 32 + lane, t = r0 + r;
-    const bool ok = wwait(listed, 0, 210) && wwait(done, 0, 208) && !abort_flag;
+    bool ok = wwait(listed, 0, 210);
+    int ad = ok ? pieces.row_id[r] : -1;
+    const float s = ad >= 0 && p.scales ? __ldg(p.scales + ad) : 1.f;
+    pieces.row_scale[r] = s;
+    ok = ok && wwait(done, 0, 208) && !abort_flag;
     fence_after_sync();
-    const int ad = ok ? pieces.row_id[r] : -1;
-    const float s = pieces.row_scale[r];  // (used where ad >= 0)
+    if (!ok) ad = -1;
     const bool any = nk > 0 && pieces.count > 0;  // else the accumulator was never written
     const uint32_t taddr = tmem + (uint32_t(quarter * 32) << 16);
     float* part = reinterpret_cast<float*>(smem) + r * (R16 + 4);  // split sums, over the stages (all read)
@@ -1023,7 +1026,7 @@ __global__ void __launch_bounds__(PCfg<BN>::THREADS, 1)
       bool ok = true;
       for (int t = pair; t < tiles && ok; t += npairs) {
         const int r0 = (m_first + t / n_tiles) * 2 * BM, r1 = min(r0 + 2 * BM, end);
-        int s = first_seg(p, r0);
+        int s = first_seg(p, r0, 32);
         for (bool more = true; more && ok; s += 32) {
           const int i = s + lane;
           int lo = 0, hi = 0, id = -1;
