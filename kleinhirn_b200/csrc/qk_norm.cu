@@ -124,10 +124,11 @@ __device__ __forceinline__ void coefficients(float (&wc)[VEC], float (&ws)[VEC],
 // 0 no rotation, 1 pairs R / 2 apart, 2 neighbouring pairs. Next to the loads it is the instructions that
 // count (packed f32x2 arithmetic, one mode to a kernel): 65,536 rows of 24 heads of 64 take 77 us (5.3 TB/s;
 // 91 us with every mode in one kernel, 160 instructions to a chunk, and 83 us with the kernel below). Heads
-// whose chunks are no power of two (!POW2) share a warp whole: 35,149 rows of 20 heads of 80, 57 us against
-// 65 with 16 lanes to their 10 chunks.
+// whose chunks are no power of two (!POW2) share a warp whole: 35,149 rows of 20 heads of 80, 55 us against
+// 65 with 16 lanes to their 10 chunks. Four CTAs to an SM where 64 registers hold it (neighbouring pairs: 20,011 rows
+// of 20 heads of 128, 39 us against 43; pairs R / 2 apart would spill: 99 against 77).
 template <typename T, int VEC, int U, int MODE, bool POW2>
-__global__ void __launch_bounds__(256) qk_norm_rope_lanes_kernel(const NormParams p, int lanes) {
+__global__ void __launch_bounds__(256, MODE != 2 ? 3 : POW2 ? 4 : 0) qk_norm_rope_lanes_kernel(const NormParams p, int lanes) {
   const int lane = threadIdx.x & 31;
   int c;           // chunk
   uint32_t group;  // blocks of heads, in order
