@@ -772,3 +772,61 @@ def test_cross_join_of_many_rows(D):
     """Split states of so many rows that a warp joins each, with sequences shorter than the bounds."""
     q, k, v, qs, ks, scale = cross_case(D + 1, [400, 3, 250], [3000, 40, 1500], 3, 1, D)
     cross_check(q, k, v, qs, ks, 3, 1, D, scale)
+
+
+@pytest.mark.parametrize("ql,kl", [([1, 2], [4000, 2500]), ([300, 20], [2500, 1100])])
+def test_cross_split_states_captured(ql, kl):
+    """Parts and their join in a graph, behind and ahead of other work on the same buffers."""
+    torch = torch_()
+    H, KV, D = 4, 2, 64
+    q, k, v, qs, ks, scale = cross_case(81, ql, kl, H, KV, D)
+    out = torch.zeros(q.shape[0], H * D, dtype=torch.float16, device="cuda")
+    dq, dk = i32(qs), i32(ks)  # (the graph reads them)
+    a = cross_args(q, k, v, out, dq, dk, H, KV, D, scale, max(ql), max(kl))
+    assert a.workspace_bytes > 0
+    kb().cross_attention_f16(a, stream())
+    torch.cuda.synchronize()
+    eager, twice = out.clone(), torch.zeros_like(out)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        for _ in range(3):
+            a._ws.fill_(0xff)
+            kb().cross_attention_f16(a, torch.cuda.current_stream().cuda_stream)
+            twice.copy_(out)
+            out.zero_()
+    for _ in range(5):
+        twice.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(twice[:qs[-1]], eager[:qs[-1]])
+    kb().operator_status(stream())
+    want, tol = cross_ref(q, k, v, qs, ks, H, KV, D, scale)
+    close(eager[:qs[-1]], want[:qs[-1]], tol[:qs[-1]])
+
+
+@pytest.mark.parametrize("lens,na", [([1] * 40, 40), ([1] * 200, 60), ([50] * 6, 3), ([1] * 5, 2)])
+def test_lora_captured_back_to_back(lens, na):
+    """The two launches of a projection in a graph, several projections on one workspace."""
+    torch = torch_()
+    x, w, bias, a, b, scales, st = lora_case(82, lens, 512, 520, 16, na)
+    ids = [(i * 3) % na for i in range(len(lens))]
+    want, tol = lora_ref(x, w, bias, a, b, scales, st, ids)
+    outs = [torch.zeros(x.shape[0], 520, dtype=torch.float16, device="cuda") for _ in range(4)]
+    calls = [lora_args(x, w, bias, a, b, scales, i32(st), i32(ids), o) for o in outs]
+    for c in calls:
+        c._starts = i32(st), i32(ids)
+        c.seg_starts, c.seg_adapters = (t.data_ptr() for t in c._starts)
+        c.workspace = calls[0].workspace
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        for c in calls:
+            kb().lora_matmul_f16(c, torch.cuda.current_stream().cuda_stream)
+    for _ in range(3):
+        for o in outs:
+            o.fill_(7)
+        graph.replay()
+        torch.cuda.synchronize()
+        kb().operator_status(stream())
+        for o in outs:
+            close(o[:st[-1]], want[:st[-1]], tol[:st[-1]])
+            assert (o[st[-1]:] == 7).all()
