@@ -511,7 +511,7 @@ struct ShrinkPieces {  // the adapters of a tile
   int count;
   int id[128];
   uint4 off[128];         // lanes of other rows
-  int row_id[128];        // adapter of each row, -1 for none
+  int row_id[128];        // adapter of each row, -1 for none (from the warps that write h)
   float row_scale[128];
 };
 
@@ -594,8 +594,6 @@ __global__ void __launch_bounds__(224) lora_shrink_tile_kernel(const __grid_cons
     // the adapters of these rows, each with all its rows
     const int last = seg_start(p, p.n_segs);  // rows from here on are not written
     int n = 0;
-    for (int r = lane; r < 128; r += 32) pieces.row_id[r] = -1;
-    __syncwarp();
     for (int s = first_seg(p, r0, 128), more = 1; more && s < p.n_segs; s += 128) {
       // four segments a lane, their loads together
       int lo[4], hi[4], id[4];
@@ -612,6 +610,7 @@ __global__ void __launch_bounds__(224) lora_shrink_tile_kernel(const __grid_cons
       }
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
+        if (!__any_sync(0xffffffffu, lo[j] < hi[j])) continue;
         const int ad = lo[j] < hi[j] ? known_adapter(p, id[j]) : -1;
         // an adapter that is in the list already takes these rows too; a new one's first lane adds it
         int at = -1;
@@ -629,7 +628,6 @@ __global__ void __launch_bounds__(224) lora_shrink_tile_kernel(const __grid_cons
           uint32_t* off = reinterpret_cast<uint32_t*>(&pieces.off[at]);
 #pragma unroll
           for (int w = 0; w < 4; ++w) atomicAnd(off + w, ~lanes_on(lo[j], hi[j], w));
-          for (int r = lo[j]; r < hi[j]; ++r) pieces.row_id[r] = ad;
         }
         n += __popc(added);  // (at most 128: every one has a row of its own)
         __syncwarp();
@@ -706,7 +704,10 @@ __global__ void __launch_bounds__(224) lora_shrink_tile_kernel(const __grid_cons
   } else {
     const int quarter = warp & 3, r = quarter * 32 + lane, t = r0 + r;
     bool ok = wwait(listed, 0, 210);
-    int ad = ok ? pieces.row_id[r] : -1;
+    int ad = -1;
+    for (int i = 0, np = ok ? pieces.count : 0; i < np; ++i)
+      if (!((reinterpret_cast<const uint32_t*>(&pieces.off[i])[quarter] >> lane) & 1u)) ad = pieces.id[i];
+    pieces.row_id[r] = ad;
     const float s = ad >= 0 && p.scales ? __ldg(p.scales + ad) : 1.f;
     pieces.row_scale[r] = s;
     ok = ok && wwait(done, 0, 208) && !abort_flag;
