@@ -1333,7 +1333,9 @@ void lora_matmul(const kh_lora_matmul_args* args, cudaStream_t st) {
       encode_tensor_map_f16(&ta, a.lora_a, uint64_t(a.n_adapters) * a.rank, uint64_t(a.k), uint64_t(a.k), 64, R16, 128);
       const int64_t tiles = (a.rows + 127) / 128;
       int Z = 1;  // CTAs that split a tile's sum: while SMs are idle, at least two K blocks each
-      const int at_once = R16 <= 32 ? 2 * CLUSTER_CTAS : CLUSTER_CTAS;  // (two CTAs an SM up to rank 32)
+      // (two CTAs an SM up to rank 32: 43 tiles of 1,536 -> 384, rank 16, the whole call 22 us against 24 with
+      // a bound of 128 CTAs and 26 with 400)
+      const int at_once = R16 <= 32 ? 2 * CLUSTER_CTAS : CLUSTER_CTAS;
       while (Z < 8 && 2 * Z * tiles <= at_once && 4 * Z <= (a.k + 63) / 64) Z *= 2;
       // many tiles: rings so short that four CTAs share an SM (up to rank 32) and cover each other's waits
       const int xstages = tiles > 2 * SMS ? 2 : SXS, astages = R16 > 32 || tiles > 2 * SMS ? 4 : SAS;
