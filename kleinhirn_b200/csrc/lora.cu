@@ -1205,8 +1205,10 @@ void launch_few(const LoraParams& p, const kh_lora_matmul_args& a, cudaStream_t 
   const int cols = int(std::min<int64_t>(FT, (a.rows + 15) / 16 * 16));
   const int stages = std::min(12, FSMEM / ((FUSED ? 32768 : 16384) + cols * 128));
   const int n_tiles = (a.n + 127) / 128, nk = (a.k + 63) / 64;
-  int Z = 1;  // CTAs that split the sum of 128 outputs: while SMs are idle, at least a K block each
-  while (Z < 8 && 2 * Z * n_tiles <= CLUSTER_CTAS && 2 * Z <= nk) Z *= 2;
+  // CTAs that split the sum of 128 outputs: while SMs are idle, at least two K blocks each (one: 32 rows
+  // 768 -> 768, 9.3 us against 8.8)
+  int Z = 1;
+  while (Z < 8 && 2 * Z * n_tiles <= CLUSTER_CTAS && 4 * Z <= nk) Z *= 2;
   CUtensorMap tx, tw, ta;
   encode_tensor_map_f16(&tx, a.x, uint64_t(a.rows), uint64_t(a.k), uint64_t(a.x_stride), 64, uint32_t(cols), 128);
   encode_tensor_map_f16(&tw, a.w, uint64_t(a.n), uint64_t(a.k), uint64_t(a.k), 64, 128, 128);
