@@ -830,3 +830,11 @@ def test_lora_captured_back_to_back(lens, na):
         for o in outs:
             close(o[:st[-1]], want[:st[-1]], tol[:st[-1]])
             assert (o[st[-1]:] == 7).all()
+
+
+@pytest.mark.parametrize("lens,na", [([16] * 8, 8), ([30, 1, 60, 20], 3), ([25] * 20, 16), ([40] * 24, 5)])
+@pytest.mark.parametrize("K,N,R", [(1536, 136, 128), (2048, 1024, 24)])
+def test_lora_adapters_of_a_tile_shared_by_clusters(lens, na, K, N, R):
+    """Few row tiles of several adapters: their h is made by clusters that share the adapters."""
+    x, w, bias, a, b, scales, st = lora_case(K + na, lens, K, N, R, na, first=2)
+    lora_check(x, w, bias, a, b, scales, st, [(i * 3) % (na + 1) - 1 for i in range(len(lens))])
