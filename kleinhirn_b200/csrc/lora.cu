@@ -1182,9 +1182,10 @@ int64_t tile_adapters(const kh_lora_matmul_args& a) {
   return std::min<int64_t>({int64_t(a.n_adapters), 128, std::max<int64_t>(1, 128 * int64_t(a.n_segs) / a.rows)});
 }
 // h by a CTA per row, which reads its adapter's A through L2, instead of by tiles, which take a product
-// for each adapter. Few rows (128 of rank 64, 4,096 values to a sum, are too many already); a few hundred
-// of some adapters (216 rows of 5, 1,024 -> 2,304, rank 8: the whole call 21 us against 26; 689 of 5,
-// 4,096 -> 384, rank 16: 32 against 26); any number of many (1,095 of 16, 384 -> 1,024: 24 against 30).
+// for each adapter. Few rows (120 of rank 64, 4,096 values to a sum, are too many already: 32 us against
+// 28); a few hundred of some adapters (268 rows of 5, 384 -> 768, rank 24: the whole call 16 us against 19;
+// 689 of 5, 4,096 -> 384, rank 16, are too many: 32 against 26); any number of many (198 of 32 to a tile,
+// 4,096 -> 2,304, rank 16: 27 against 34; about equal from 1,000 on).
 bool shrinks_rows(const kh_lora_matmul_args& a) {
   const int64_t work = a.rows * a.rank * int64_t(a.k), adapters = tile_adapters(a);
   return (a.rows <= FT && work <= (1 << 24)) || (adapters > 4 && work <= (1 << 23)) || adapters >= 16;
