@@ -18,6 +18,7 @@
 
 #include <algorithm>
 #include <atomic>
+#include <cmath>
 
 #include "runtime.h"
 #include "sm100.cuh"
@@ -1361,10 +1362,15 @@ void lora_matmul(const kh_lora_matmul_args* args, cudaStream_t st) {
     if (fuses(a)) launch_few<true>(p, a, st);
     else launch_few<false>(p, a, st);
   } else {
-    // The tile width whose rounds over the SM pairs are over soonest; a narrower tile costs a little more
-    // than its share (the same x for fewer columns).
-    const int64_t m_tiles = (a.rows + 255) / 256, pairs = device_sms() / 2;
-    auto cost = [&](int bn) { return double((m_tiles * ((a.n + bn - 1) / bn) + pairs - 1) / pairs) * (bn + 24); };
+    // The tile width that is over soonest: a tile costs its columns and, as a constant, what it reads of x and
+    // its adapters' products; a last round that is not full counts in part, as pairs start one after another
+    // and the first ones have the tile more (24 texts of 4,254 rows, 768 -> 2,304, 2.07 rounds of 256 columns
+    // or 2.76 of 192: 25.5 us against 28.5; 9,974 rows 1,024 -> 1,152: 128 columns 40.6, 192 35.6, 256 36.5).
+    const double m_tiles = double((a.rows + 255) / 256), pairs = device_sms() / 2;
+    auto cost = [&](int bn) {
+      const double rounds = std::max(1.0, m_tiles * ((a.n + bn - 1) / bn) / pairs);
+      return (rounds + (rounds < 2 ? 0.35 : 0.15) * (std::ceil(rounds) - rounds)) * (bn + (adapters ? 80 : 24));
+    };
     if (cost(256) <= cost(192) && cost(256) <= cost(128)) launch_pair<256>(p, a, adapters, st);
     else if (cost(192) <= cost(128)) launch_pair<192>(p, a, adapters, st);
     else launch_pair<128>(p, a, adapters, st);
