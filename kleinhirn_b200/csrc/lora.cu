@@ -1,7 +1,7 @@
 // A projection with the low-rank adapters of many requests.
 //
 // out[t] = x[t] W^T + bias + s_a (x[t] A_a^T) B_a^T, a the adapter of the segment of rows that t lies
-// in. Two launches: h[t] = s_a x[t] A_a^T (rank values a row, rounded to f16: 2^-11 of the adapter's
+// in. Two launches (one where few rows' adapters are few, see lora_few_kernel): h[t] = s_a x[t] A_a^T (rank values a row, rounded to f16: 2^-11 of the adapter's
 // own part), then the projection with h B_a^T added to the same f32 accumulators, rounded once. The
 // second launch starts while the first runs (programmatic dependent launch) and waits for it where it
 // needs h, behind the projection's own products.
@@ -136,6 +136,8 @@ __global__ void __launch_bounds__(512) lora_shrink_rows_kernel(const LoraParams 
 // adapters meanwhile.
 // FUSED: where all adapters' A together have at most 128 rows, they are a second operand tile of every
 // stage, h comes out of the same pass over x, and there is no launch before this one.
+// 64 rows of 48 adapters of rank 16, 4,096 -> 4,096: 18.8 us, of it 2.6 to the first tile, 4 to 6 for W (46 MB
+// with the adapters), 5 for the sum, the adapters and the outputs.
 
 constexpr int FT = 128;      // rows of x, at most
 constexpr int FTHREADS = 352;
@@ -779,6 +781,8 @@ __global__ void __launch_bounds__(224) lora_shrink_tile_kernel(const __grid_cons
 //   TMA (tiles with rows that are not to be written: straight from registers); the last warp finds the
 //   adapters of the tiles ahead, in lists of up to 16 from 32 segments (found by the TMA warp itself, the
 //   dependent loads of the search held up the K blocks: 7 % on 65,536 rows of 768 -> 2,304).
+// 256 texts of 68,000 rows, 768 -> 2,304, 16 adapters of rank 32: 197 us, 1,280 TFLOP/s, the tensor pipe 72 %
+// busy under the power cap; h before it 25 us (its x 4 TB/s).
 
 constexpr int BM = 128;
 constexpr int BK = 64;
