@@ -1,10 +1,11 @@
 // A projection with the low-rank adapters of many requests.
 //
 // out[t] = x[t] W^T + bias + s_a (x[t] A_a^T) B_a^T, a the adapter of the segment of rows that t lies
-// in. Two launches (one where few rows' adapters are few, see lora_few_kernel): h[t] = s_a x[t] A_a^T (rank values a row, rounded to f16: 2^-11 of the adapter's
+// in. Two launches: h[t] = s_a x[t] A_a^T (rank values a row, rounded to f16: 2^-11 of the adapter's
 // own part), then the projection with h B_a^T added to the same f32 accumulators, rounded once. The
 // second launch starts while the first runs (programmatic dependent launch) and waits for it where it
-// needs h, behind the projection's own products.
+// needs h, behind the projection's own products. (One launch where few rows have few adapters: see
+// lora_few_kernel.)
 //
 // Few rows (takes_few): bound by reading W, A and B once; lora_shrink_rows_kernel and
 // lora_few_kernel. Many rows: bound by the tensor cores;
