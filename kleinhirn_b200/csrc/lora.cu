@@ -220,21 +220,27 @@ __device__ __forceinline__ void load_batch(const LoraParams& p, Products& s, con
     s.find(ids, nt, step);
   }
 }
-// part: the sum at row 0 of x and this lane's output; hs: h [row of x][rank + 8]
+// part: the sum at row 0 of x and this lane's output; hs: h [row of x][rank + 8]. A product is taken over in the
+// columns of its own adapter's rows alone: the zeros that stand for the other rows' h would turn an infinity
+// in this adapter's B into a NaN in their outputs.
 __device__ __forceinline__ void use_batch(const LoraParams& p, Products s, const __half* hs, float* part, const uint2 (&lo)[8],
                                           const uint2 (&hi)[8]) {
   const int lane = threadIdx.x & 31, q4 = (lane & 3) * 4;
   float* dst = part + (s.g * 8 + 2 * (lane & 3)) * PS;
   float acc[4] = {dst[0], dst[PS], dst[8], dst[PS + 8]};
+  const int column0 = __shfl_sync(0xffffffffu, s.mine, 8 * (lane & 3)), column1 = __shfl_sync(0xffffffffu, s.mine, 8 * (lane & 3) + 4);
   const __half* h = hs + (s.g * 8 + (lane >> 2)) * (p.rank + 8) + q4;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
+    if (!s.leaders) break;
+    const int id = s.adapter();
     uint2 v = make_uint2(0, 0);
-    if (s.leaders) {
-      if (s.adapter() == s.mine && s.k + q4 < p.rank) v = *reinterpret_cast<const uint2*>(h + s.k);
-      s.next(p.rank);
-    }
-    mma_16816(acc, lo[i].x, hi[i].x, lo[i].y, hi[i].y, v.x, v.y);
+    if (id == s.mine && s.k + q4 < p.rank) v = *reinterpret_cast<const uint2*>(h + s.k);
+    s.next(p.rank);
+    float sum[4] = {acc[0], acc[1], acc[2], acc[3]};
+    mma_16816(sum, lo[i].x, hi[i].x, lo[i].y, hi[i].y, v.x, v.y);
+    if (id == column0) acc[0] = sum[0], acc[2] = sum[2];
+    if (id == column1) acc[1] = sum[1], acc[3] = sum[3];
   }
   dst[0] = acc[0];
   dst[PS] = acc[1];

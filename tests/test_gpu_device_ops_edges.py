@@ -1,0 +1,41 @@
+"""Operators on caller-owned device buffers where one request's values, a value's range or several
+reports at once could reach what they must not: against the definitions in 64 bits, with the
+tolerances of test_gpu_device_ops.py."""
+import pytest
+from test_gpu_device_ops import H16, close, cross_args, gen, i32, kb, lora_args, lora_case, lora_ref, randn, starts_of, stream, torch_
+
+pytestmark = pytest.mark.gpu
+
+
+# every kernel choice of the projection: (lens, ids, adapters, K, N, R)
+LORA_CHOICES = [
+    ([1] * 24, [0, 1, -1, 2, 1, 0] * 4, 3, 256, 200, 16),                          # one launch, h beside the product
+    ([1, 3, 0, 2, 5, 1] * 4, [0, 1, 2, -1, 2, 1] * 4, 3, 1024, 264, 40),            # up to 128 rows
+    ([2, 1] * 90, [(i * 7) % 41 - 1 for i in range(180)], 40, 256, 264, 16),        # a few hundred of many adapters
+    ([37, 90, 1, 0, 130, 64], [0, 1, -1, 2, 1, 2], 3, 256, 328, 24),                # tiles of the tensor cores
+    ([1, 2] * 450, [(i * 7) % 6 - 1 for i in range(900)], 5, 128, 264, 8),          # the same, scattered rows
+]
+
+
+@pytest.mark.parametrize("value", [float("inf"), float("nan")])
+@pytest.mark.parametrize("lens,ids,na,K,N,R", LORA_CHOICES)
+def test_lora_infinities_of_an_adapter_stay_in_its_rows(lens, ids, na, K, N, R, value):
+    """An adapter that rows of the call use holds infinities or NaN in some outputs' rows of B, another one
+    in A: the rows of other adapters, and rows without one, are as by the definition."""
+    torch = torch_()
+    x, w, bias, a, b, scales, st = lora_case(K + N, lens, K, N, R, na, pad=8)
+    want, tol = lora_ref(x[:, :K], w, bias, a, b, scales, st, ids)
+    b[1, ::7] = value
+    a[2, R - 1, 3] = value
+    out = torch.full((x.shape[0], N), 7.0, dtype=torch.float16, device="cuda")
+    kb().lora_matmul_f16(lora_args(x, w, bias, a, b, scales, i32(st), i32(ids), out), stream())
+    kb().operator_status(stream())
+    row_id = torch.tensor([ad for n, ad in zip(lens, ids) for _ in range(n)], device="cuda")
+    hit = torch.zeros(st[-1], N, dtype=torch.bool, device="cuda")
+    hit[(row_id == 1), ::7] = True
+    hit[row_id == 2] = True
+    assert hit.any() and not hit.all()
+    got = out[:st[-1]]
+    assert not got[hit].isfinite().any()
+    keep = ~hit
+    close(got[keep], want[:st[-1]][keep], tol[:st[-1]][keep])
