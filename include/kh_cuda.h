@@ -332,7 +332,8 @@ int kh_cross_attention_f16(const kh_cross_attention_args* args, void* stream);
  * of x belong to request i, whose adapter is a = seg_adapters[i]:
  *   out = x w^T + bias + scales[a] (x lora_a[a]^T) lora_b[a]^T
  * f16 operands, f32 sums, the rank-sized product (with its scale) rounded to f16 once and added to the
- * same f32 accumulator as the projection; the output is rounded once. A negative id is a request
+ * same f32 accumulator as the projection; the output is rounded once. A row with a rank-sized product
+ * beyond f16's 65,504 is made in f32 throughout (many times slower). A negative id is a request
  * without an adapter; an id of n_adapters or more counts as none and gives a status. out shares no
  * value with what the call reads (not in place).
  * Limits: k, n and rank multiples of 8, k and n in [8, 65,536], rank in [8, 128] (pad a smaller one

@@ -2,7 +2,7 @@
 //
 // out[t] = x[t] W^T + bias + s_a (x[t] A_a^T) B_a^T, a the adapter of the segment of rows that t lies
 // in. Two launches: h[t] = s_a x[t] A_a^T (rank values a row, rounded to f16: 2^-11 of the adapter's
-// own part), then the projection with h B_a^T added to the same f32 accumulators, rounded once. The
+// own part; rows with a value beyond f16: see row_beyond_f16), then the projection with h B_a^T added to the same f32 accumulators, rounded once. The
 // second launch starts while the first runs (programmatic dependent launch) and waits for it where it
 // needs h, behind the projection's own products. (One launch where few rows have few adapters: see
 // lora_few_kernel.)
@@ -90,6 +90,48 @@ __device__ __forceinline__ float dot8(uint4 a, uint4 b, float acc) {
     acc = fmaf(u.x, v.x, fmaf(u.y, v.y, acc));
   }
   return acc;
+}
+
+// Dot product of k values by a whole warp, the same in every lane.
+__device__ __forceinline__ float warp_dot(const __half* x, const __half* y, int k) {
+  const uint4 *u = reinterpret_cast<const uint4*>(x), *v = reinterpret_cast<const uint4*>(y);
+  float d = 0.f;
+#pragma unroll 1
+  for (int i = threadIdx.x & 31; i < k / 8; i += 32) d = dot8(__ldg(u + i), __ldg(v + i), d);
+  for (int o = 16; o; o >>= 1) d += __shfl_xor_sync(0xffffffffu, d, o);
+  return d;
+}
+// h is an f16 operand, so a value of it beyond 65,504 is an infinity, and all that it is multiplied with is
+// infinite or NaN. A row with such outputs comes here, to one warp: its h in f32, and where a value may have
+// been too large (2^15: this sum's order is another one) `count` outputs from n0 on again, put(j, value) by every
+// lane. Otherwise the row is infinite by the definition, and stays as it is.
+template <class Put>
+__device__ __forceinline__ void row_beyond_f16(const LoraParams& p, int64_t row, int ad, int n0, int count, Put put) {
+  const int lane = threadIdx.x & 31;
+  const __half* x = p.x + row * p.x_stride;
+  const float s = p.scales ? __ldg(p.scales + ad) : 1.f;
+  float h[4] = {};  // rank value lane + 32 i
+  bool beyond = false;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll 1
+    for (int r = 32 * i; r < min(32 * i + 32, p.rank); ++r) {
+      const float d = warp_dot(x, p.a + (int64_t(ad) * p.rank + r) * p.k, p.k) * s;
+      if (lane == (r & 31)) h[i] = d;
+      beyond |= fabsf(d) >= 32768.f && fabsf(d) < INFINITY;
+    }
+  if (!beyond) return;
+#pragma unroll 1
+  for (int j = 0; j < count; ++j) {
+    const int n = n0 + j;
+    const __half* b = p.b + (int64_t(ad) * p.n + n) * p.rank;
+    float d = 0.f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (lane + 32 * i < p.rank) d = fmaf(h[i], __half2float(b[lane + 32 * i]), d);
+    for (int o = 16; o; o >>= 1) d += __shfl_xor_sync(0xffffffffu, d, o);
+    put(j, warp_dot(x, p.w + int64_t(n) * p.k, p.k) + d + (p.bias ? __half2float(p.bias[n]) : 0.f));
+  }
 }
 
 // ---- few rows: h, one CTA of 16 warps per row, a warp one of the rank's dot products at a time ----
@@ -480,13 +522,14 @@ __global__ void __maxnreg__(FUSED ? 168 : 112)
     __syncthreads();
   }
   // this CTA's rows, a warp a row: the parts of the sum, in rank order, and the bias, rounded once
+  uint32_t not_finite = 0;  // rows of this warp with an output of this lane that is infinite or NaN
   if (n < p.n && !abort_flag) {
     const float2 bias_lo = __half22float2(*reinterpret_cast<const __half2*>(&bias_bits.x));
     const float2 bias_hi = __half22float2(*reinterpret_cast<const __half2*>(&bias_bits.y));
     const float4 bias = make_float4(bias_lo.x, bias_lo.y, bias_hi.x, bias_hi.y);
 #pragma unroll 2
-    for (int k = warp; k < FT; k += FTHREADS / 32) {
-      const int i = (k / 8 * Z + z) * 8 + k % 8;
+    for (int j = 0; warp + j * (FTHREADS / 32) < FT; ++j) {
+      const int k = warp + j * (FTHREADS / 32), i = (k / 8 * Z + z) * 8 + k % 8;
       if (i >= nt) break;
       const float* src = part + i * PS + 4 * lane;
       float4 v = bias;
@@ -497,7 +540,17 @@ __global__ void __maxnreg__(FUSED ? 168 : 112)
 #pragma unroll
       for (int q = 0; q < 8; ++q) v.x += u[q].x, v.y += u[q].y, v.z += u[q].z, v.w += u[q].w;
       *reinterpret_cast<uint2*>(p.out + (t0 + i) * p.out_stride + n) = make_uint2(pack_half2(v.x, v.y), pack_half2(v.z, v.w));
+      const float zero = fmaf(v.x, 0.f, fmaf(v.y, 0.f, fmaf(v.z, 0.f, v.w * 0.f)));
+      if (zero != 0.f) not_finite |= 1u << j;
     }
+  }
+  for (not_finite = __reduce_or_sync(0xffffffffu, not_finite); not_finite; not_finite &= not_finite - 1) {
+    const int k = warp + (__ffs(not_finite) - 1) * (FTHREADS / 32), i = (k / 8 * Z + z) * 8 + k % 8;
+    if (ids[i] < 0) continue;
+    __half* dst = p.out + (t0 + i) * p.out_stride + n0;
+    row_beyond_f16(p, t0 + i, ids[i], n0, min(128, p.n - n0), [&](int j, float v) {
+      if (lane == 0) dst[j] = __float2half_rn(v);
+    });
   }
   if (Z > 1) cluster_sync();  // no CTA leaves while another reads its part
   if (warp == 1) {
@@ -1107,6 +1160,7 @@ __global__ void __launch_bounds__(PCfg<BN>::THREADS, 1)
       fence_after_sync();
       const uint32_t taddr = tmem + (uint32_t(q * 32) << 16) + uint32_t(buf * BN + g * 64);
       const int row = row0 + r;
+      float2 zero = make_float2(0.f, 0.f);  // NaN once an output is infinite or NaN
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
         uint32_t a[32];
@@ -1131,12 +1185,27 @@ __global__ void __launch_bounds__(PCfg<BN>::THREADS, 1)
             const float2 v = fadd2(make_float2(__uint_as_float(a[8 * c8 + 2 * e]), __uint_as_float(a[8 * c8 + 2 * e + 1])),
                                    __half22float2(bh[e]));
             u[e] = pack_half2(v.x, v.y);
+            zero = ffma2(v, make_float2(0.f, 0.f), zero);
           }
           const uint4 o = make_uint4(u[0], u[1], u[2], u[3]);
           if (inside) *reinterpret_cast<uint4*>(stile + r * 128 + (((4 * half + c8) ^ (r & 7)) * 16)) = o;
           else if (row >= begin && row < end && n < p.n)
             *reinterpret_cast<uint4*>(p.out + row * p.out_stride + n) = o;
         }
+      }
+      if (p.n_adapters > 0) {
+        uint32_t rows = __ballot_sync(0xffffffffu, zero.x + zero.y != 0.f && row >= begin && row < end);
+        for (; rows; rows &= rows - 1) {
+          const int rr = q * 32 + __ffs(rows) - 1, again = row0 + rr, seg = first_seg(p, again, 0);
+          const int ad = seg < p.n_segs && again >= seg_start(p, seg) ? adapter_of(p, seg) : -1;
+          if (ad < 0) continue;
+          row_beyond_f16(p, again, ad, nc, min(64, p.n - nc), [&](int j, float v) {
+            if (lane) return;
+            if (inside) *reinterpret_cast<__half*>(stile + rr * 128 + (((j >> 3) ^ (rr & 7)) * 16) + (j & 7) * 2) = __float2half_rn(v);
+            else p.out[again * p.out_stride + nc + j] = __float2half_rn(v);
+          });
+        }
+        __syncwarp();
       }
       fence_proxy_async_smem();
       named_bar(1 + g, 128);

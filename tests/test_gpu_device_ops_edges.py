@@ -39,3 +39,47 @@ def test_lora_infinities_of_an_adapter_stay_in_its_rows(lens, ids, na, K, N, R, 
     assert not got[hit].isfinite().any()
     keep = ~hit
     close(got[keep], want[:st[-1]][keep], tol[:st[-1]][keep])
+
+
+@pytest.mark.parametrize("lens,ids,na,K,N,R", LORA_CHOICES)
+def test_lora_rank_product_beyond_f16(lens, ids, na, K, N, R):
+    """A large scale with a small B: s x A^T passes 65,504 in some rows of an adapter, the output does not."""
+    torch = torch_()
+    x, w, bias, a, b, scales, st = lora_case(K + R, lens, K, N, R, na, pad=8)
+    scales[1] = 2.0 ** 16
+    b[1] = (b[1].float() * 2.0 ** -12).half()
+    if na > 3:
+        scales[3], b[3] = -2.0 ** 20, (b[3].float() * 2.0 ** -16).half()
+    h = x[:st[-1], :K].double() @ a[1].double().T * scales[1]
+    assert (h.abs() > 65504).any() and (h.abs() < 65504).any()
+    want, tol = lora_ref(x[:, :K], w, bias, a, b, scales, st, ids)
+    assert want[:st[-1]].abs().max() < 60000
+    out = torch.full((x.shape[0], N + 8), 7.0, dtype=torch.float16, device="cuda")
+    kb().lora_matmul_f16(lora_args(x, w, bias, a, b, scales, i32(st), i32(ids), out), stream())
+    kb().operator_status(stream())
+    close(out[:st[-1], :N], want[:st[-1]], tol[:st[-1]])
+    assert (out[st[-1]:] == 7).all() and (out[:, N:] == 7).all()
+
+
+@pytest.mark.parametrize("lens,ids,na,K,N,R", LORA_CHOICES)
+def test_lora_infinite_rows_stay_infinite(lens, ids, na, K, N, R):
+    """A row of x with a NaN, one with an infinity, and outputs beyond f16: as by the definition."""
+    torch = torch_()
+    x, w, bias, a, b, scales, st = lora_case(K + R, lens, K, N, R, na)
+    x[0, 5], x[st[-1] - 1, K - 1] = float("nan"), float("inf")
+    bias[8:16] = 65504.0
+    w[9], w[12] = 0.0, 0.0
+    w[9, :], w[12, 0] = w[9, :], 65504.0
+    ref_x = x[:, :K].clone()
+    ref_x[[0, st[-1] - 1]] = 0
+    want, tol = lora_ref(ref_x, w, bias, a, b, scales, st, ids)
+    out = torch.full((x.shape[0], N), 7.0, dtype=torch.float16, device="cuda")
+    kb().lora_matmul_f16(lora_args(x, w, bias, a, b, scales, i32(st), i32(ids), out), stream())
+    kb().operator_status(stream())
+    assert out[0].isnan().all() and not out[st[-1] - 1].isfinite().any()
+    mid, low = want[1:st[-1] - 1], tol[1:st[-1] - 1]
+    got = out[1:st[-1] - 1]
+    sure = (mid.abs() + low < 65504)  # (values next to the border may round either way)
+    close(got[sure], mid[sure], low[sure])
+    over = mid.abs() - low > 65520
+    assert over.any() and got[over].isinf().all() and (got[over].sign() == mid[over].sign()).all()
