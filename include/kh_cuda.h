@@ -364,7 +364,8 @@ int kh_lora_matmul_f16(const kh_lora_matmul_args* args, void* stream);
 /* Waits for `stream` (as cudaStreamSynchronize) and reports what the three operators above met on the
  * current device since the last report: KH_OK; KH_ERR_ARG for a position outside its table or an
  * adapter id that does not exist; KH_ERR_CUDA for a pipeline wait that gave up (the output is then
- * partly written). Reading clears it. Not while a capture is under way. */
+ * partly written), also where both were met: kh_last_error names everything. Reading clears it. Not
+ * while a capture is under way (KH_ERR_ARG; the capture goes on). */
 int kh_operator_status(void* stream);
 
 /* ---- failure-path self-tests (no counterpart in the reference) ----
@@ -377,11 +378,16 @@ int kh_operator_status(void* stream);
  *   limit_us microseconds (1 to 1e6); the wait gives up and records its code as a pipeline wait
  *   that timed out does; the call synchronizes, returns KH_ERR_CUDA ("pipeline wait timed out")
  *   and latches it in ctx.
+ * kh_selftest_operator_status: records codes on the current device, in the order of `stream`, as the
+ *   kernels of kh_qk_norm_rope (norm_index: not 0 for a position outside its table),
+ *   kh_cross_attention_f16 (cross_wait: of a wait that gave up) and kh_lora_matmul_f16 (lora_wait;
+ *   lora_index: an adapter id that does not exist) would; kh_operator_status reports and clears them.
  * kh_selftest_tensor_maps: `threads` host threads (1-64) fetch `iters` TMA descriptors each from
  *   the library's descriptor cache over more keys than it keeps; returns how many differ from a
  *   fresh encoding (0 expected), or -1 on an error. */
 int kh_inject_cuda_error(kh_ctx* ctx, const char* what);
 int kh_selftest_wait_limit(kh_ctx* ctx, int limit_us);
+int kh_selftest_operator_status(int norm_index, int cross_wait, int lora_wait, int lora_index, void* stream);
 int64_t kh_selftest_tensor_maps(int threads, int iters);
 
 #ifdef __cplusplus

@@ -79,6 +79,7 @@ _SIGS = {
     "kh_operator_status": ([_P], ctypes.c_int),
     "kh_inject_cuda_error": ([_P, ctypes.c_char_p], ctypes.c_int),
     "kh_selftest_wait_limit": ([_P, ctypes.c_int], ctypes.c_int),
+    "kh_selftest_operator_status": ([ctypes.c_int] * 4 + [_P], ctypes.c_int),
     "kh_selftest_tensor_maps": ([ctypes.c_int, ctypes.c_int], ctypes.c_int64),
 }
 
@@ -203,6 +204,13 @@ def operator_status(stream: int = 0) -> None:
     position or adapter id outside its table, or gave up a pipeline wait (the report clears it)."""
     lib = load_library()
     _check(lib, lib.kh_operator_status(stream or None))
+
+
+def selftest_operator_status(norm_index: int = 0, cross_wait: int = 0, lora_wait: int = 0, lora_index: int = 0,
+                             stream: int = 0) -> None:
+    """kh_selftest_operator_status: records codes for operator_status as the operators' kernels would."""
+    lib = load_library()
+    _check(lib, lib.kh_selftest_operator_status(norm_index, cross_wait, lora_wait, lora_index, stream or None))
 
 
 def selftest_tensor_maps(threads: int, iters: int) -> int:

@@ -1098,6 +1098,12 @@ int kh_selftest_wait_limit(kh_ctx* ctx, int limit_us) {
   });
 }
 
+int kh_selftest_operator_status(int norm_index, int cross_wait, int lora_wait, int lora_index, void* stream) {
+  return guard(nullptr, Latch::No, [&] {
+    kh::selftest_operator_status({norm_index, cross_wait, lora_wait, lora_index}, static_cast<cudaStream_t>(stream));
+  });
+}
+
 int64_t kh_selftest_tensor_maps(int threads, int iters) {
   int64_t bad = -1;
   const int st = guard(nullptr, Latch::No, [&] { bad = kh::selftest_tensor_maps(threads, iters); });

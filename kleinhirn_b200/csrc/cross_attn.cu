@@ -1086,14 +1086,10 @@ void cross_attention(const kh_cross_attention_args* args, cudaStream_t st) {
   else launch<128>(p, a, states, st);
 }
 
-int cross_attention_error_code() {
-  int v = 0;
-  KH_CUDA(cudaMemcpyFromSymbol(&v, sm100::kh_tc_error, sizeof(int)));
-  if (v) {
-    const int zero = 0;
-    KH_CUDA(cudaMemcpyToSymbol(sm100::kh_tc_error, &zero, sizeof(int)));
-  }
-  return v;
+int* cross_attention_wait_word() {
+  void* p = nullptr;
+  KH_CUDA(cudaGetSymbolAddress(&p, sm100::kh_tc_error));
+  return static_cast<int*>(p);
 }
 
 }  // namespace kh

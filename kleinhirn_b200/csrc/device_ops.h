@@ -16,15 +16,20 @@ void cross_attention(const kh_cross_attention_args* a, cudaStream_t st);
 int64_t lora_matmul_workspace(const kh_lora_matmul_args* a);
 void lora_matmul(const kh_lora_matmul_args* a, cudaStream_t st);
 
-// Synchronizes `st`; throws what the operators met on the current device since the last report
-// (ArgError: a position or an adapter id outside its table; CudaError: a wait that gave up).
+// Synchronizes `st`; throws all that the operators met on the current device since the last report
+// (CudaError where a wait gave up, else ArgError: a position or an adapter id outside its table).
 void operator_status(cudaStream_t st);
+// Records codes as the operators' kernels would (0: none), in the order of OperatorWord.
+void selftest_operator_status(const int (&codes)[4], cudaStream_t st);
 
-// Code each operator's kernels left on the current device (0: none), read and cleared.
-constexpr int OP_BAD_INDEX = 1;  // a position or an adapter id outside its table; others: waits
-int qk_norm_error_code();
-int cross_attention_error_code();
-int lora_error_code();
+// Words in which the operators' kernels leave what they meet, on the current device. A bad index and a wait that
+// gave up have a word each, so that neither hides the other.
+enum OperatorWord { NORM_INDEX, CROSS_WAIT, LORA_WAIT, LORA_INDEX, OPERATOR_WORDS };
+constexpr int OP_BAD_INDEX = 1;  // of an index word; a wait's is the code of the first that gave up
+int* qk_norm_index_word();
+int* cross_attention_wait_word();
+int* lora_wait_word();
+int* lora_index_word();
 
 // Shared argument checks (ArgError with the entry point's name).
 void check_that(bool ok, const char* fn, const char* what);

@@ -31,6 +31,8 @@ namespace {
 
 using namespace sm100;
 
+__device__ int kh_lora_index_error = 0;  // (a wait that gave up: kh_tc_error)
+
 struct LoraParams {
   const __half* x;
   const __half* w;
@@ -53,7 +55,7 @@ __device__ __forceinline__ int seg_start(const LoraParams& p, int i) {
 // An id as an adapter, -1 for none; one that does not exist counts as none and is reported.
 __device__ __forceinline__ int known_adapter(const LoraParams& p, int id) {
   if (id < p.n_adapters) return id < 0 ? -1 : id;
-  atomicCAS(&kh_tc_error, 0, OP_BAD_INDEX);
+  atomicOr(&kh_lora_index_error, OP_BAD_INDEX);
   return -1;
 }
 __device__ __forceinline__ int adapter_of(const LoraParams& p, int seg) { return known_adapter(p, __ldg(p.ids + seg)); }
@@ -1457,14 +1459,16 @@ void lora_matmul(const kh_lora_matmul_args* args, cudaStream_t st) {
   }
 }
 
-int lora_error_code() {
-  int v = 0;
-  KH_CUDA(cudaMemcpyFromSymbol(&v, sm100::kh_tc_error, sizeof(int)));
-  if (v) {
-    const int zero = 0;
-    KH_CUDA(cudaMemcpyToSymbol(sm100::kh_tc_error, &zero, sizeof(int)));
-  }
-  return v;
+int* lora_wait_word() {
+  void* p = nullptr;
+  KH_CUDA(cudaGetSymbolAddress(&p, sm100::kh_tc_error));
+  return static_cast<int*>(p);
+}
+
+int* lora_index_word() {
+  void* p = nullptr;
+  KH_CUDA(cudaGetSymbolAddress(&p, kh_lora_index_error));
+  return static_cast<int*>(p);
 }
 
 }  // namespace kh

@@ -518,14 +518,10 @@ void qk_norm_rope(const kh_qk_norm_rope_args* args, cudaStream_t st) {
   }
 }
 
-int qk_norm_error_code() {
-  int v = 0;
-  KH_CUDA(cudaMemcpyFromSymbol(&v, kh_norm_error, sizeof(int)));
-  if (v) {
-    const int zero = 0;
-    KH_CUDA(cudaMemcpyToSymbol(kh_norm_error, &zero, sizeof(int)));
-  }
-  return v;
+int* qk_norm_index_word() {
+  void* p = nullptr;
+  KH_CUDA(cudaGetSymbolAddress(&p, kh_norm_error));
+  return static_cast<int*>(p);
 }
 
 }  // namespace kh

@@ -83,3 +83,108 @@ def test_lora_infinite_rows_stay_infinite(lens, ids, na, K, N, R):
     close(got[sure], mid[sure], low[sure])
     over = mid.abs() - low > 65520
     assert over.any() and got[over].isinf().all() and (got[over].sign() == mid[over].sign()).all()
+
+
+# ---- reports ----
+
+def bad_norm_call():
+    """A norm with a position outside its table."""
+    torch, k = torch_(), kb()
+    x, table = randn(gen(1), 3, 64), torch.zeros(4, 128, device="cuda")
+    pos = i32([0, 4, 1])
+    a = k.QkNormRopeArgs(dtype=k.KH_F16, q_heads=1, head_dim=64, rotary_dim=64, eps=1e-6, rows=3, x_stride=64, out_stride=64,
+                         table_rows=4, x=x.data_ptr(), out=x.data_ptr(), cossin=table.data_ptr(), positions=pos.data_ptr())
+    a._keep = x, table, pos
+    return a
+
+
+def bad_lora_call():
+    """A projection with an adapter id that does not exist."""
+    torch = torch_()
+    x, w, bias, a, b, scales, st = lora_case(2, [2, 2], 64, 64, 8, 2)
+    starts, ids, out = i32(st), i32([0, 2]), torch.zeros(x.shape[0], 64, dtype=torch.float16, device="cuda")
+    args = lora_args(x, w, bias, a, b, scales, starts, ids, out)
+    args._keep = x, w, bias, a, b, scales, starts, ids, out
+    return args
+
+
+def test_status_reports_every_operator():
+    """What two operators met before one report is in that report, and cleared by it."""
+    k = kb()
+    k.qk_norm_rope(bad_norm_call(), stream())
+    k.lora_matmul_f16(bad_lora_call(), stream())
+    with pytest.raises(k.KhError) as e:
+        k.operator_status(stream())
+    assert e.value.status == 1 and "position" in str(e.value) and "adapter id" in str(e.value)
+    k.operator_status(stream())
+
+
+def test_status_of_one_stream_keeps_to_it():
+    """The report of a stream waits for that stream and finds what it met, beside work on another one."""
+    torch, k = torch_(), kb()
+    side = torch.cuda.Stream()
+    a = bad_lora_call()
+    torch.cuda.synchronize()
+    busy = torch.empty(1 << 28, dtype=torch.uint8, device="cuda")
+    for _ in range(20):
+        busy.fill_(1)
+    k.lora_matmul_f16(a, side.cuda_stream)
+    with pytest.raises(k.KhError, match="adapter id"):
+        k.operator_status(side.cuda_stream)
+    k.operator_status(side.cuda_stream)
+    torch.cuda.synchronize()
+
+
+def test_status_of_a_capturing_stream_is_refused():
+    """The report is refused before anything is done to the capture, which goes on."""
+    torch, k = torch_(), kb()
+    x, w, bias, a, b, scales, st = lora_case(3, [5, 6], 64, 64, 8, 2)
+    starts, ids, out = i32(st), i32([0, 1]), torch.zeros(x.shape[0], 64, dtype=torch.float16, device="cuda")
+    args = lora_args(x, w, bias, a, b, scales, starts, ids, out)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        st_ = torch.cuda.current_stream().cuda_stream
+        k.lora_matmul_f16(args, st_)
+        with pytest.raises(k.KhError, match="captur") as e:
+            k.operator_status(st_)
+        assert e.value.status == 1
+    graph.replay()
+    torch.cuda.synchronize()
+    k.operator_status(stream())
+    want, tol = lora_ref(x, w, bias, a, b, scales, st, [0, 1])
+    close(out[:st[-1]], want[:st[-1]], tol[:st[-1]])
+
+
+def test_status_puts_waits_before_indexes_and_loses_neither():
+    """A wait that gave up is reported as such, whatever was met before it, and everything is named."""
+    k = kb()
+    names = {"norm_index": "position", "cross_wait": "kh_cross_attention_f16: pipeline", "lora_wait": "kh_lora_matmul_f16: pipeline",
+             "lora_index": "adapter id"}
+    for bits in range(1, 16):
+        met = [n for i, n in enumerate(names) if bits >> i & 1]
+        for n in reversed(met):  # (an adapter id first, a wait of the same operator behind it)
+            k.selftest_operator_status(**{n: 100 + len(n) if "wait" in n else 1}, stream=stream())
+        with pytest.raises(k.KhError) as e:
+            k.operator_status(stream())
+        assert e.value.status == (3 if any("wait" in n for n in met) else 1), met
+        for n, text in names.items():
+            assert (text in str(e.value)) == (n in met)
+        for n in met:
+            assert "wait" not in n or f"code {100 + len(n)}" in str(e.value)
+        k.operator_status(stream())
+
+
+def test_status_of_a_bad_id_with_a_wait_that_gave_up():
+    """The kernel's own report of an adapter id leaves room for a wait's, before and after it."""
+    k = kb()
+    for first in (True, False):
+        if first:
+            k.selftest_operator_status(lora_wait=233, stream=stream())
+        k.lora_matmul_f16(bad_lora_call(), stream())
+        if not first:
+            k.selftest_operator_status(lora_wait=233, stream=stream())
+        with pytest.raises(k.KhError, match="code 233.*adapter id") as e:
+            k.operator_status(stream())
+        assert e.value.status == 3
+        k.operator_status(stream())
