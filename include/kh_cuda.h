@@ -260,7 +260,8 @@ int kh_attention_f16_noalloc_status(void* stream);
  *   same time need a workspace each.
  * - A workspace needs no initial contents, must be 256-byte aligned and holds nothing afterwards.
  * - Segment starts ([n + 1] int32, not decreasing) live on the device, so a captured call serves
- *   other lengths. Starts outside the buffer are cut to its rows. Rows before the first start and
+ *   other lengths. Starts outside the buffer are cut to its rows; with decreasing ones the values of
+ *   the rows are unspecified, and nothing outside the buffers is read or written. Rows before the first start and
  *   behind the last are not written.
  * - Sizes the kernels do not take are KH_ERR_ARG, said before anything is queued. What only the
  *   device can see (a position outside its table, an adapter id that does not exist, a pipeline wait
@@ -362,8 +363,9 @@ int64_t kh_lora_matmul_f16_workspace(const kh_lora_matmul_args* args);
 int kh_lora_matmul_f16(const kh_lora_matmul_args* args, void* stream);
 
 /* Waits for `stream` (as cudaStreamSynchronize) and reports what the three operators above met on the
- * current device since the last report: KH_OK; KH_ERR_ARG for a position outside its table or an
- * adapter id that does not exist; KH_ERR_CUDA for a pipeline wait that gave up (the output is then
+ * current device since the last report: KH_OK; KH_ERR_ARG for a position outside its table, an
+ * adapter id that does not exist or, where a projection meets them, segment starts that decrease
+ * (its rows there are unspecified); KH_ERR_CUDA for a pipeline wait that gave up (the output is then
  * partly written), also where both were met: kh_last_error names everything. Reading clears it. Not
  * while a capture is under way (KH_ERR_ARG; the capture goes on). */
 int kh_operator_status(void* stream);
@@ -381,7 +383,7 @@ int kh_operator_status(void* stream);
  * kh_selftest_operator_status: records codes on the current device, in the order of `stream`, as the
  *   kernels of kh_qk_norm_rope (norm_index: not 0 for a position outside its table),
  *   kh_cross_attention_f16 (cross_wait: of a wait that gave up) and kh_lora_matmul_f16 (lora_wait;
- *   lora_index: an adapter id that does not exist) would; kh_operator_status reports and clears them.
+ *   lora_index: 1 for an adapter id that does not exist, 2 for starts that decrease) would; kh_operator_status reports and clears them.
  * kh_selftest_tensor_maps: `threads` host threads (1-64) fetch `iters` TMA descriptors each from
  *   the library's descriptor cache over more keys than it keeps; returns how many differ from a
  *   fresh encoding (0 expected), or -1 on an error. */

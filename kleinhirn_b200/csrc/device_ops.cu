@@ -91,7 +91,8 @@ void operator_status(cudaStream_t st) {
   wait("kh_cross_attention_f16", c.v[CROSS_WAIT]);
   wait("kh_lora_matmul_f16", c.v[LORA_WAIT]);
   if (c.v[NORM_INDEX]) add("kh_qk_norm_rope: a position outside [0, table_rows)");
-  if (c.v[LORA_INDEX]) add("kh_lora_matmul_f16: an adapter id of n_adapters or more");
+  if (c.v[LORA_INDEX] & OP_BAD_INDEX) add("kh_lora_matmul_f16: an adapter id of n_adapters or more");
+  if (c.v[LORA_INDEX] & OP_BAD_STARTS) add("kh_lora_matmul_f16: segment starts that decrease (some rows are without their adapter)");
   if (c.v[CROSS_WAIT] || c.v[LORA_WAIT]) throw CudaError(met);
   if (!met.empty()) throw ArgError(met);
 }

@@ -25,7 +25,9 @@ void selftest_operator_status(const int (&codes)[4], cudaStream_t st);
 // Words in which the operators' kernels leave what they meet, on the current device. A bad index and a wait that
 // gave up have a word each, so that neither hides the other.
 enum OperatorWord { NORM_INDEX, CROSS_WAIT, LORA_WAIT, LORA_INDEX, OPERATOR_WORDS };
-constexpr int OP_BAD_INDEX = 1;  // of an index word; a wait's is the code of the first that gave up
+// Bits of an index word (a wait's is the code of the first that gave up).
+constexpr int OP_BAD_INDEX = 1;   // a position or an adapter id outside its table
+constexpr int OP_BAD_STARTS = 2;  // segment starts that decrease
 int* qk_norm_index_word();
 int* cross_attention_wait_word();
 int* lora_wait_word();

@@ -573,10 +573,11 @@ __global__ void __maxnreg__(FUSED ? 168 : 112)
 
 constexpr int SXS = 4;  // x stages
 constexpr int SAS = 8;  // A stages, at most
+constexpr int LISTED = 128;  // adapters of a tile, at most: its rows
 struct ShrinkPieces {  // the adapters of a tile
   int count;
-  int id[128];
-  uint4 off[128];         // lanes of other rows
+  int id[LISTED];
+  uint4 off[LISTED];      // lanes of other rows
   int row_id[128];        // adapter of each row, -1 for none (from the warps that write h)
   float row_scale[128];
 };
@@ -684,10 +685,14 @@ __global__ void __launch_bounds__(224) lora_shrink_tile_kernel(const __grid_cons
         int at = -1;
         for (int k = 0; k < n; ++k) at = pieces.id[k] == ad ? k : at;
         const uint32_t peers = __match_any_sync(0xffffffffu, ad);
-        const bool adds = ad >= 0 && at < 0 && lane == __ffs(peers) - 1;
-        const uint32_t added = __ballot_sync(0xffffffffu, adds);
-        if (ad >= 0 && at < 0) at = n + __popc(added & ((1u << (__ffs(peers) - 1)) - 1u));
-        if (adds) {
+        const bool fresh = ad >= 0 && at < 0;
+        const uint32_t added = __ballot_sync(0xffffffffu, fresh && lane == __ffs(peers) - 1);
+        if (fresh) at = n + __popc(added & ((1u << (__ffs(peers) - 1)) - 1u));
+        if (at >= LISTED) {  // only where starts decrease: else every adapter has a row of its own
+          atomicOr(&kh_lora_index_error, OP_BAD_STARTS);
+          ad = -1;
+        }
+        if (ad >= 0 && fresh && lane == __ffs(peers) - 1) {
           pieces.id[at] = ad;
           pieces.off[at] = make_uint4(~0u, ~0u, ~0u, ~0u);
         }
@@ -697,7 +702,7 @@ __global__ void __launch_bounds__(224) lora_shrink_tile_kernel(const __grid_cons
 #pragma unroll
           for (int w = 0; w < 4; ++w) atomicAnd(off + w, ~lanes_on(lo[j], hi[j], w));
         }
-        n += __popc(added);  // (at most 128: every one has a row of its own)
+        n = min(n + __popc(added), LISTED);
         __syncwarp();
       }
       more = __all_sync(0xffffffffu, lo[3] < 128);

@@ -85,6 +85,26 @@ def test_lora_infinite_rows_stay_infinite(lens, ids, na, K, N, R):
     assert over.any() and got[over].isinf().all() and (got[over].sign() == mid[over].sign()).all()
 
 
+def test_lora_starts_that_go_back_and_forth():
+    """Starts that decrease again and again name 300 adapters for the two first rows: the list of a tile's
+    adapters holds no more than it has room for, the report says so, and the next call is as ever."""
+    torch, k = torch_(), kb()
+    na, rows = 300, 2500
+    x, w, bias, a, b, scales, st = lora_case(5, [rows], 1024, 64, 8, na)
+    starts, ids = i32([0, 2] * (na // 2) + [rows]), i32(list(range(na)))
+    out = torch.full((x.shape[0], 80), 7.0, dtype=torch.float16, device="cuda")
+    k.lora_matmul_f16(lora_args(x, w, bias, a, b, scales, starts, ids, out), stream())
+    with pytest.raises(k.KhError, match="starts that decrease") as e:
+        k.operator_status(stream())
+    assert e.value.status == 1
+    assert (out[rows:] == 7).all() and (out[:, 64:] == 7).all()
+    starts, ids = i32(st), i32([na - 1])
+    k.lora_matmul_f16(lora_args(x, w, bias, a, b, scales, starts, ids, out), stream())
+    k.operator_status(stream())
+    want, tol = lora_ref(x, w, bias, a, b, scales, st, [na - 1])
+    close(out[:rows, :64], want[:rows], tol[:rows])
+
+
 # ---- reports ----
 
 def bad_norm_call():
