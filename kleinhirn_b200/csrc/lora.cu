@@ -407,33 +407,31 @@ __global__ void __maxnreg__(FUSED ? 168 : 112)
   } else if (warp == 10) {
     for (int t = lane; t < FT; t += 32) ids[t] = -1;
     __syncwarp();
-    if (p.n_adapters > 0) {
-      for (int s = first_seg(p, t0, 128), more = 1; more && s < p.n_segs; s += 128) {
-        // four segments a lane, their loads together
-        int lo[4], hi[4], id[4];
+    for (int s = first_seg(p, t0, 128), more = 1; more && s < p.n_segs; s += 128) {
+      // four segments a lane, their loads together
+      int lo[4], hi[4], id[4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int i = s + 32 * j + lane;
-          lo[j] = hi[j] = t0 + nt;
-          id[j] = -1;
-          if (i < p.n_segs) {
-            lo[j] = max(seg_start(p, i), t0);
-            hi[j] = min(seg_start(p, i + 1), t0 + nt);
-            id[j] = __ldg(p.ids + i);
+      for (int j = 0; j < 4; ++j) {
+        const int i = s + 32 * j + lane;
+        lo[j] = hi[j] = t0 + nt;
+        id[j] = -1;
+        if (i < p.n_segs) {
+          lo[j] = max(seg_start(p, i), t0);
+          hi[j] = min(seg_start(p, i + 1), t0 + nt);
+          id[j] = __ldg(p.ids + i);
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (lo[j] < hi[j]) {
+          const int ad = known_adapter(p, id[j]);
+          const float sc = FUSED && ad >= 0 && p.scales ? __ldg(p.scales + ad) : 1.f;
+          for (int t = lo[j]; t < hi[j]; ++t) {
+            ids[t - t0] = ad;
+            if (FUSED) row_scale[t - t0] = sc;
           }
         }
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          if (lo[j] < hi[j]) {
-            const int ad = known_adapter(p, id[j]);
-            const float sc = FUSED && ad >= 0 && p.scales ? __ldg(p.scales + ad) : 1.f;
-            for (int t = lo[j]; t < hi[j]; ++t) {
-              ids[t - t0] = ad;
-              if (FUSED) row_scale[t - t0] = sc;
-            }
-          }
-        more = __all_sync(0xffffffffu, lo[3] < t0 + nt);
-      }
+      more = __all_sync(0xffffffffu, lo[3] < t0 + nt);
     }
     __syncwarp();
     named_bar(1, 32 * 9);
@@ -1143,6 +1141,9 @@ __global__ void __launch_bounds__(PCfg<BN>::THREADS, 1)
         }
       }
       if (!ok) *abort_flag = 1;
+    } else {  // every id is one that does not exist; no product needs a list
+      for (int i = int(blockIdx.x) * 32 + lane; i < p.n_segs; i += int(gridDim.x) * 32)
+        if (seg_start(p, i) < seg_start(p, i + 1)) adapter_of(p, i);
     }
   } else {
     const int q = warp & 3;

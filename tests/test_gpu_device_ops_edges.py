@@ -208,3 +208,25 @@ def test_status_of_a_bad_id_with_a_wait_that_gave_up():
             k.operator_status(stream())
         assert e.value.status == 3
         k.operator_status(stream())
+
+
+@pytest.mark.parametrize("lens", [[30, 20], [300, 0, 200], [1] * 700])
+def test_lora_ids_without_adapters_are_reported(lens):
+    """With no adapters at all every id is one that does not exist: none is used, and the report says so;
+    the id of a segment without rows is not looked at."""
+    torch, k = torch_(), kb()
+    for bad in (False, True):
+        x, w, bias, a, b, scales, st = lora_case(8, lens, 128, 264, 8, 1)
+        starts, ids = i32(st), i32([0 if n == 0 else -1 for n in lens])
+        if bad:
+            ids[len(lens) - 1] = 0
+        out = torch.zeros(x.shape[0], 264, dtype=torch.float16, device="cuda")
+        args = lora_args(x, w, bias, a, b, scales, starts, ids, out)
+        args.n_adapters, args.lora_a, args.lora_b, args.scales = 0, None, None, None
+        k.lora_matmul_f16(args, stream())
+        if bad:
+            with pytest.raises(k.KhError, match="adapter id"):
+                k.operator_status(stream())
+        k.operator_status(stream())
+        want, tol = lora_ref(x, w, bias, a, b, scales, st, [-1] * len(lens))
+        close(out[:st[-1]], want[:st[-1]], tol[:st[-1]])
