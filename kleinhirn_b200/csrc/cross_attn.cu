@@ -403,6 +403,7 @@ __global__ void __launch_bounds__(128) cross_join_kernel(const CrossParams p, in
 // polynomial on the FMA pipe instead: no faster, as the clock falls with the power they take.)
 
 constexpr int TROWS = 128;
+constexpr float EXACT_REF = 4194304.f;  // half a unit of 2^22 in the last place: 2^-2
 
 template <int D>
 struct TCfg {
@@ -793,6 +794,16 @@ __global__ void __launch_bounds__(TCfg<D>::THREADS, TCfg<D>::ONE ? 1 : 2)
         }
       }
       const float ref = m == -INFINITY ? 0.f : m;
+      // 2^(s scale - m) in one step keeps the bits of the product that m, the rounded one, lacks: up to half a
+      // unit of m in the last place, far outside f16 for the largest. There the products are rounded first.
+      float mul = p.scale_log2;
+      if (__any_sync(0xffffffffu, fabsf(ref) > EXACT_REF)) {
+        mul = 1.f;
+#pragma unroll
+        for (int c = 0; c < W; ++c)
+#pragma unroll
+          for (int i = 0; i < 32; ++i) sr[c][i] = __float_as_uint(__fmul_rn(__uint_as_float(sr[c][i]), p.scale_log2));
+      }
       float2 ls[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
       constexpr int CHUNK = C::ONE ? 32 : 8;  // packed pairs stored at a time, as the registers allow
 #pragma unroll
@@ -802,7 +813,7 @@ __global__ void __launch_bounds__(TCfg<D>::THREADS, TCfg<D>::ONE ? 1 : 2)
         for (int i = 0; i < CHUNK; ++i) {
           const int k = 2 * (c + i);
           const float2 x = ffma2(make_float2(__uint_as_float(sr[k / 32][k & 31]), __uint_as_float(sr[k / 32][(k + 1) & 31])),
-                                 twice(p.scale_log2), twice(-ref));
+                                 twice(mul), twice(-ref));
           const float2 e = make_float2(ex2_approx(x.x), ex2_approx(x.y));
           ls[i & 1] = fadd2(ls[i & 1], e);
           pk[i] = pack_half2(e.x, e.y);

@@ -230,3 +230,35 @@ def test_lora_ids_without_adapters_are_reported(lens):
         k.operator_status(stream())
         want, tol = lora_ref(x, w, bias, a, b, scales, st, [-1] * len(lens))
         close(out[:st[-1]], want[:st[-1]], tol[:st[-1]])
+
+
+# ---- attention ----
+
+def ones_case(top, lens_q, lens_k, D):
+    """Queries of a row's constant and states of a state's constant: every score is one product."""
+    torch = torch_()
+    qs, ks = starts_of(lens_q), starts_of(lens_k)
+    q = (top - 3.0 * torch.arange(qs[-1], device="cuda"))[:, None].expand(-1, D).half().contiguous()
+    order = torch.cat([torch.randperm(n, generator=torch.Generator().manual_seed(n)) for n in lens_k]).cuda()
+    k = (top - 8.0 * order)[:, None].expand(-1, D).half().contiguous()
+    return q, k, randn(gen(D), ks[-1], D), qs, ks, order
+
+
+@pytest.mark.parametrize("ql,kl", [([2, 16], [300, 500]), ([150, 300], [300, 500]), ([128], [700])])
+@pytest.mark.parametrize("D", [32, 64, 128])
+def test_cross_scores_far_beyond_the_exponent(ql, kl, D):
+    """Scores of 2^28 and more in powers of two, neighbours 2^13 and more apart (a rounding of the largest is
+    2^6 at most): the output is the value of the best state, whatever the steps of f32 are up there."""
+    torch = torch_()
+    q, k, v, qs, ks, order = ones_case(8000.0, ql, kl, D)
+    s = (q[:, :1].double() @ k[:, :1].double().T).abs() * D * 0.125 * 1.4427
+    assert (s[:, order == 0] > 2.0 ** 27).all()
+    out = torch.full_like(q, 7.0)
+    a = cross_args(q, k, v, out, i32(qs), i32(ks), 1, 1, D, 0.125, max(ql), max(kl))
+    kb().cross_attention_f16(a, stream())
+    kb().operator_status(stream())
+    for i in range(len(ql)):
+        best = v[ks[i] + int(order[ks[i]:ks[i + 1]].argmin())].double()
+        want = best.expand(ql[i], D)
+        # one state of weight 1: the exponential (2^-22), its f16 rounding and the sum's division, the output's rounding
+        close(out[qs[i]:qs[i + 1]], want, (2 * H16 + 2.0 ** -20) * want.abs() + 2.0 ** -24)
