@@ -3,9 +3,10 @@
 // For query row i of sequence s and query head h, with G = q_heads / kv_heads and K the kept states of
 // s: out = sum_j p_j v_j, p the softmax over j in K of scale q_i,h . k_j,h/G; zero where K is empty.
 // Both kernels make one pass over the states with a running reference point m (log2 units) and the sum
-// l of 2^(s - m): m moves only when a score exceeds it by more than 8, so the accumulated output is
-// rescaled seldom and p stays within 2^8, where f16 (the operand of the product with v) rounds it by
-// 2^-11 as anywhere; m, l, scores and the output accumulate in f32.
+// l of p = 2^(s - m + LIFT): m moves only when a score exceeds it by more than RISE, so the accumulated output
+// is rescaled seldom. p is f16 as the operand of the product with v: at most 2^(LIFT + RISE + 1), rounded by
+// 2^-11, and below 2^-14 by up to 2^-25, which is 2^-32 of the largest (m is a score, so the largest p is
+// 2^LIFT or more); l adds the f32 values. m, l, scores and the output accumulate in f32.
 // The G query heads of a key head are rows of the same tile (row = query * G + head), so k and v are
 // read once for them.
 //
@@ -82,6 +83,7 @@ __device__ __forceinline__ uint32_t pack_half2(float a, float b) {
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 
+constexpr float LIFT = 7.f, RISE = 7.f;  // (m - LIFT may round to m - 8: 2^15 at most)
 constexpr int RSTEP = 16;  // states of a step
 
 template <int D, int RW>
@@ -227,7 +229,7 @@ __global__ void __launch_bounds__(RW * 32)
 #pragma unroll
     for (int r = 0; r < 2; ++r)
       top[r] = fmaxf(fmaxf(sc[0][2 * r], sc[0][2 * r + 1]), fmaxf(sc[1][2 * r], sc[1][2 * r + 1]));
-    if (__any_sync(0xffffffffu, top[0] > m[0] + 8.f || top[1] > m[1] + 8.f)) {
+    if (__any_sync(0xffffffffu, top[0] - m[0] > RISE || top[1] - m[1] > RISE)) {
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
         top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 1));
@@ -243,7 +245,7 @@ __global__ void __launch_bounds__(RW * 32)
         }
       }
     }
-    const float ref[2] = {m[0] == -INFINITY ? 0.f : m[0], m[1] == -INFINITY ? 0.f : m[1]};
+    const float ref[2] = {m[0] == -INFINITY ? 0.f : m[0] - LIFT, m[1] == -INFINITY ? 0.f : m[1] - LIFT};
     uint32_t pa[2][2];
 #pragma unroll
     for (int b = 0; b < 2; ++b)
@@ -773,7 +775,7 @@ __global__ void __launch_bounds__(TCfg<D>::THREADS, TCfg<D>::ONE ? 1 : 2)
         for (int i = 0; i < 32; i += 2)
           mr[(i >> 1) & 3] = fmax3(mr[(i >> 1) & 3], __uint_as_float(sr[c][i]), __uint_as_float(sr[c][i + 1]));
       const float cand = fmaxf(fmaxf(mr[0], mr[1]), fmaxf(mr[2], mr[3])) * p.scale_log2;
-      const bool moves = cand > m + 8.f;  // (also the first kept state: m = -inf)
+      const bool moves = cand - m > RISE;  // (also the first kept state: m = -inf)
       if (__any_sync(0xffffffffu, moves)) {
         const float corr = moves ? ex2_approx(m - cand) : 1.f;
         if (moves) m = cand;
@@ -793,7 +795,7 @@ __global__ void __launch_bounds__(TCfg<D>::THREADS, TCfg<D>::ONE ? 1 : 2)
           tmem_st_wait();
         }
       }
-      const float ref = m == -INFINITY ? 0.f : m;
+      const float ref = m == -INFINITY ? 0.f : m - LIFT;
       // 2^(s scale - m) in one step keeps the bits of the product that m, the rounded one, lacks: up to half a
       // unit of m in the last place, far outside f16 for the largest. There the products are rounded first.
       float mul = p.scale_log2;

@@ -262,3 +262,32 @@ def test_cross_scores_far_beyond_the_exponent(ql, kl, D):
         want = best.expand(ql[i], D)
         # one state of weight 1: the exponential (2^-22), its f16 rounding and the sum's division, the output's rounding
         close(out[qs[i]:qs[i + 1]], want, (2 * H16 + 2.0 ** -20) * want.abs() + 2.0 ** -24)
+
+
+@pytest.mark.parametrize("n_q", [1, 150])
+@pytest.mark.parametrize("far", [16.0, 18.0, 20.0])
+@pytest.mark.parametrize("D", [32, 64, 128])
+def test_cross_many_small_probabilities(n_q, far, D):
+    """One state with a score 16 to 20 above 20,000 equal ones, which together still weigh 2^-9 to 2^-15: each
+    of their probabilities is off by half a step of f16, relative (2^-11) or of its smallest values at the size
+    in which they are kept (2^-25 where the largest is 2^7 or more: 2^-32 of it). 300 heads, so that no part of
+    the states has a reference of its own."""
+    torch = torch_()
+    n, heads = 20_000, 300
+    q = torch.ones(n_q, heads * D, dtype=torch.float16, device="cuda")
+    k = torch.zeros(n, heads * D, dtype=torch.float16, device="cuda")
+    k[777] = far / 8  # (exact in f16; scale 8 / D)
+    head = 1 + 0.25 * randn(gen(4), n, D)
+    head[777] = 0
+    v = head.repeat(1, heads)
+    out = torch.zeros_like(q)
+    a = cross_args(q, k, v, out, i32([0, n_q]), i32([0, n]), heads, heads, D, 8.0 / D, n_q, n)
+    assert a.workspace_bytes == 0
+    kb().cross_attention_f16(a, stream())
+    kb().operator_status(stream())
+    p = torch.softmax(k[:, :D].double().sum(1) * (8.0 / D), 0)
+    size = p @ head.double().abs()
+    # relative: the probabilities' and the output's rounding, and sums in f32 of n / 64 terms a part (2^-24 each,
+    # twice where the tensor core cuts): 2^-14.7
+    tol = (2 * H16 + 2.0 ** -14) * size + n * 2.0 ** -32 * head.double().abs().max() + 2.0 ** -25
+    close(out.view(n_q, heads, D), (p @ head.double()).expand(n_q, heads, D), tol.expand(n_q, heads, D))
