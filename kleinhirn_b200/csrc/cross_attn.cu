@@ -969,7 +969,9 @@ void launch_tiles(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMa
     KH_CUDA(cudaFuncSetAttribute(cross_tile_kernel<D, ROW_TILES>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
   });
   const int rows = ROW_TILES * (TROWS / p.G);
-  const dim3 grid(unsigned((p.max_q + rows - 1) / rows), unsigned(p.kv_heads * p.nsplit), unsigned(p.n_seqs));
+  // (no sequence has more queries than the buffer has rows, however generous max_q is)
+  const int64_t most = std::min<int64_t>(p.max_q, p.q_rows);
+  const dim3 grid(unsigned((most + rows - 1) / rows), unsigned(p.kv_heads * p.nsplit), unsigned(p.n_seqs));
   cross_tile_kernel<D, ROW_TILES><<<grid, C::THREADS, C::SMEM, st>>>(tq, tk, tv, p);
 }
 

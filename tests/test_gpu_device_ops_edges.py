@@ -2,7 +2,7 @@
 reports at once could reach what they must not: against the definitions in 64 bits, with the
 tolerances of test_gpu_device_ops.py."""
 import pytest
-from test_gpu_device_ops import H16, close, cross_args, gen, i32, kb, lora_args, lora_case, lora_ref, randn, starts_of, stream, torch_
+from test_gpu_device_ops import H16, close, cross_args, cross_ref, gen, i32, kb, lora_args, lora_case, lora_ref, randn, starts_of, stream, torch_
 
 pytestmark = pytest.mark.gpu
 
@@ -291,3 +291,22 @@ def test_cross_many_small_probabilities(n_q, far, D):
     # twice where the tensor core cuts): 2^-14.7
     tol = (2 * H16 + 2.0 ** -14) * size + n * 2.0 ** -32 * head.double().abs().max() + 2.0 ** -25
     close(out.view(n_q, heads, D), (p @ head.double()).expand(n_q, heads, D), tol.expand(n_q, heads, D))
+
+
+def test_cross_generous_bounds():
+    """max_q and max_k at their limits, for buffers of a few hundred rows, with many sequences without rows:
+    the CTAs are those that the buffers can need."""
+    torch = torch_()
+    H = KV = 12
+    D, n = 64, 500
+    ql, kl = [3, 140, 0, 20] + [0] * (n - 4), [70, 200, 9, 0] + [1] * (n - 4)
+    qs, ks = starts_of(ql), starts_of(kl)
+    q, kv = randn(gen(6), qs[-1], H * D, scale=1.5), randn(gen(7), ks[-1], 2 * KV * D)
+    k, v = kv[:, :KV * D], kv[:, KV * D:]
+    out = torch.full_like(q, 7.0)
+    a = cross_args(q, k, v, out, i32(qs), i32(ks), H, KV, D, 0.125, 1 << 24, 1 << 24)
+    assert a.workspace_bytes == 0
+    kb().cross_attention_f16(a, stream())
+    kb().operator_status(stream())
+    want, tol = cross_ref(q, k, v, qs, ks, H, KV, D, 0.125)
+    close(out, want, tol)
