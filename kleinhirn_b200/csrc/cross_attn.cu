@@ -32,6 +32,8 @@ namespace {
 
 using namespace sm100;
 
+constexpr float LIFT = 7.f, RISE = 7.f;  // (m - LIFT may round to m - 8: 2^15 at most)
+
 struct CrossParams {
   const __half* q;
   const __half* k;
@@ -71,19 +73,6 @@ __device__ __forceinline__ int64_t part_index(const CrossParams& p, int z, int s
 // Bound: HBM (2 D 2 bytes per state and key head, each read once), by the bytes in flight: 64 requests of
 // one query on 200-512 states, 12 heads of 64, took 25 us with loads one step ahead in registers.
 
-__device__ __forceinline__ void mma_16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
-                                          uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
-__device__ __forceinline__ uint32_t pack_half2(float a, float b) {
-  const __half2 h = __floats2half2_rn(a, b);
-  return *reinterpret_cast<const uint32_t*>(&h);
-}
-
-constexpr float LIFT = 7.f, RISE = 7.f;  // (m - LIFT may round to m - 8: 2^15 at most)
 constexpr int RSTEP = 16;  // states of a step
 
 template <int D, int RW>

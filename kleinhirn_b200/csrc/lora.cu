@@ -79,10 +79,6 @@ __device__ __forceinline__ int first_seg(const LoraParams& p, int r, int reads) 
   return lo;
 }
 
-__device__ __forceinline__ uint32_t pack_half2(float a, float b) {
-  const __half2 h = __floats2half2_rn(a, b);
-  return *reinterpret_cast<const uint32_t*>(&h);
-}
 __device__ __forceinline__ float dot8(uint4 a, uint4 b, float acc) {
   const __half2* x = reinterpret_cast<const __half2*>(&a);
   const __half2* y = reinterpret_cast<const __half2*>(&b);
@@ -200,13 +196,6 @@ __device__ __forceinline__ float ld_cluster_f32(uint32_t addr) {
   float v;
   asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
   return v;
-}
-__device__ __forceinline__ void mma_16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
-                                          uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
 constexpr int PS = 132;  // row stride of the parts of the sum: [row of x][output], f32

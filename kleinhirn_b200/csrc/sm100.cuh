@@ -82,9 +82,6 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, int co
   return mbar_wait_for(bar, parity, code, WAIT_LIMIT_NS);
 }
 
-// Prefetch of a line into L2.
-__device__ __forceinline__ void prefetch_l2(const void* p) { asm volatile("prefetch.global.L2 [%0];" ::"l"(p)); }
-
 // Prefetch of a 2-D tensor-map box into L2 (no shared memory, no completion).
 __device__ __forceinline__ void tma_prefetch_2d(const CUtensorMap* map, int x, int y) {
   asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global [%0, {%1, %2}];" ::"l"(map), "r"(x), "r"(y) : "memory");
@@ -213,6 +210,20 @@ __device__ __forceinline__ uint64_t desc_sw128(const void* smem) {
   return ((addr >> 4) & 0x3FFFull) | (1ull << 16) | (64ull << 32) | (1ull << 46) | (2ull << 61);
 }
 
+// Two f32 values as an operand word.
+__device__ __forceinline__ uint32_t pack_half2(float a, float b) {
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+// Product of one warp on registers, m16n8k16: few rows, whose operands are not worth a tile.
+__device__ __forceinline__ void mma_16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                          uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
 // True in one lane of a converged warp. An MMA warp runs its loop with all lanes (so that descriptors and
 // addresses stay warp-uniform values) and issues from this one.
 __device__ __forceinline__ bool elect_one() {
@@ -239,16 +250,6 @@ __device__ __forceinline__ void mma_f16(uint32_t tmem_d, uint64_t da, uint64_t d
       : "memory");
 }
 
-// The same with the A operand in TMEM: lane = row, 8 columns per K step of 16 f16 values.
-__device__ __forceinline__ void mma_f16_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t db, uint32_t idesc, uint32_t acc) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(tmem_d),
-      "r"(tmem_a), "l"(db), "r"(idesc), "r"(acc)
-      : "memory");
-}
-
 // mma_f16 that leaves the TMEM lanes (rows of D) whose bit is set in off[lane / 32] as they are.
 __device__ __forceinline__ void mma_f16_lanes_if(bool lead, uint32_t tmem_d, uint64_t da, uint64_t db, uint32_t idesc,
                                                  uint32_t acc, const uint32_t (&off)[4]) {
@@ -272,6 +273,7 @@ __device__ __forceinline__ void mma_f16_if(bool lead, uint32_t tmem_d, uint64_t 
       "l"(da), "l"(db), "r"(idesc), "r"(acc), "r"(uint32_t(lead))
       : "memory");
 }
+// (A in TMEM: lane = row, 8 columns per K step of 16 f16 values)
 __device__ __forceinline__ void mma_f16_ts_if(bool lead, uint32_t tmem_d, uint32_t tmem_a, uint64_t db, uint32_t idesc,
                                               uint32_t acc) {
   asm volatile(
