@@ -1262,11 +1262,14 @@ int64_t tile_adapters(const kh_lora_matmul_args& a) {
 // h by a CTA per row, which reads its adapter's A through L2, instead of by tiles, which take a product
 // for each adapter. Few rows (120 of rank 64, 4,096 values to a sum, are too many already: 32 us against
 // 28); a few hundred of some adapters (268 rows of 5, 384 -> 768, rank 24: the whole call 16 us against 19;
-// 689 of 5, 4,096 -> 384, rank 16, are too many: 32 against 26); any number of many (198 of 32 to a tile,
-// 4,096 -> 2,304, rank 16: 27 against 34; about equal from 1,000 on).
+// 689 of 5, 4,096 -> 384, rank 16, are too many: 32 against 26); some thousand of many (2,000 of 25 to a tile,
+// 768 -> 768, rank 16: 39 against 42; 6,000: 69 against 49); any number where a tile would take more products
+// than the rank is worth (20,000 single rows, 4,096 -> 4,096, rank 64: 3,154 against 3,537; 64 to a tile, rank 16:
+// 1,432 against 1,847, rank 64: 2,561 against 2,045).
 bool shrinks_rows(const kh_lora_matmul_args& a) {
   const int64_t work = a.rows * a.rank * int64_t(a.k), adapters = tile_adapters(a);
-  return (a.rows <= FT && work <= (1 << 24)) || (adapters > 4 && work <= (1 << 23)) || adapters >= 16;
+  return (a.rows <= FT && work <= (1 << 24)) || (adapters > 4 && work <= (1 << 23)) || (adapters >= 16 && work <= (1 << 25)) ||
+         (adapters >= 56 && 2 * adapters >= 3 * a.rank);
 }
 // Rows of x as the columns of the product: W is read once per 128 rows, where a pair's tile takes a product
 // for each of its adapters. Up to 128 rows; of many adapters up to four times that (187 rows of 16 adapters,
