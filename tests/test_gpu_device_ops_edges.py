@@ -310,3 +310,87 @@ def test_cross_generous_bounds():
     kb().operator_status(stream())
     want, tol = cross_ref(q, k, v, qs, ks, H, KV, D, 0.125)
     close(out, want, tol)
+
+
+@pytest.mark.parametrize("G", [5, 9, 16, 17, 33, 48, 64])
+@pytest.mark.parametrize("ql,kl", [([1, 1, 1], [300, 0, 70]), ([1, 4, 90], [70, 300, 129])])
+def test_cross_many_query_heads_to_a_key_head(G, ql, kl):
+    """Tiles whose rows no whole number of queries fills, and single tokens on both kernels."""
+    for D in (32, 64, 128):
+        torch = torch_()
+        KV = 2
+        g = gen(G + D)
+        qs, ks = starts_of(ql), starts_of(kl)
+        q, kv = randn(g, qs[-1], KV * G * D, scale=1.5), randn(g, ks[-1], 2 * KV * D)
+        k, v = kv[:, :KV * D], kv[:, KV * D:]
+        out = torch.full((qs[-1], KV * G * D + 8), 7.0, dtype=torch.float16, device="cuda")
+        a = cross_args(q, k, v, out, i32(qs), i32(ks), KV * G, KV, D, D ** -0.5, max(ql), max(kl))
+        kb().cross_attention_f16(a, stream())
+        kb().operator_status(stream())
+        want, tol = cross_ref(q, k, v, qs, ks, KV * G, KV, D, D ** -0.5)
+        close(out[:, :KV * G * D], want, tol)
+        assert (out[:, KV * G * D:] == 7).all()
+
+
+@pytest.mark.parametrize("max_q", [1, 30])
+def test_cross_most_sequences(max_q):
+    """65,535 sequences of no or one query, on no or one state: the output is the state's value."""
+    torch = torch_()
+    n, D = 65535, 64
+    has_q = torch.rand(n, generator=gen(1), device="cuda") > 0.3
+    has_k = torch.rand(n, generator=gen(2), device="cuda") > 0.3
+    qs = torch.cat([torch.zeros(1, device="cuda"), has_q.cumsum(0)]).int()
+    ks = torch.cat([torch.zeros(1, device="cuda"), has_k.cumsum(0)]).int()
+    q, k = randn(gen(3), int(qs[-1]), D), randn(gen(4), int(ks[-1]), D)
+    v = randn(gen(5), int(ks[-1]), D)
+    out = torch.full_like(q, 7.0)
+    b = kb()
+    a = b.CrossAttentionArgs(n_seqs=n, q_heads=1, kv_heads=1, head_dim=D, max_q=max_q, max_k=1, scale=0.125, q_rows=q.shape[0],
+                             kv_rows=k.shape[0], q_stride=D, k_stride=D, v_stride=D, out_stride=D, q=q.data_ptr(), k=k.data_ptr(),
+                             v=v.data_ptr(), out=out.data_ptr(), q_starts=qs.data_ptr(), k_starts=ks.data_ptr())
+    assert b.cross_attention_f16_workspace(a) == 0
+    b.cross_attention_f16(a, stream())
+    b.operator_status(stream())
+    want = torch.zeros_like(q)
+    both = has_q & has_k
+    want[qs[:-1][both].long()] = v[ks[:-1][both].long()]
+    # (a weight of one: the exponential of 2^7 and its sum, each within 2^-22)
+    close(out, want.double(), H16 * want.double().abs() + 2.0 ** -25)
+
+
+def test_lora_most_segments():
+    """65,535 segments of no to three rows, of 60 adapters, on both sides of a tile's 128 rows."""
+    torch = torch_()
+    n = 65535
+    lens = [(i * 7 + i // 11) % 4 for i in range(n)]
+    x, w, bias, a, b, scales, st = lora_case(9, lens, 64, 72, 8, 60)
+    ids = torch.tensor([(i * 13) % 61 - 1 for i in range(n)], device="cuda", dtype=torch.int32)
+    out = torch.full((x.shape[0], 72), 7.0, dtype=torch.float16, device="cuda")
+    starts = i32(st)
+    kb().lora_matmul_f16(lora_args(x, w, bias, a, b, scales, starts, ids, out), stream())
+    kb().operator_status(stream())
+    row = torch.repeat_interleave(ids, torch.tensor(lens, device="cuda")).long()
+    xx = x[:st[-1]].double()
+    y, size = xx @ w.double().T + bias.double(), xx.abs() @ w.double().abs().T + bias.double().abs()
+    tol = 64 * 2.0 ** -23 * size
+    for ad in range(60):
+        r = row == ad
+        h, hs = xx[r] @ a[ad].double().T * scales[ad].double(), xx[r].abs() @ a[ad].double().abs().T * scales[ad].double()
+        y[r] += h @ b[ad].double().T
+        tol[r] += (H16 * h.abs() + 64 * 2.0 ** -23 * hs + 2.0 ** -25) @ b[ad].double().abs().T + 8 * 2.0 ** -23 * (h.abs() @ b[ad].double().abs().T)
+    close(out[:st[-1]], y, tol + H16 * (y.abs() + tol) + 2.0 ** -25)
+    assert (out[st[-1]:] == 7).all()
+
+
+def test_streams_by_handle():
+    """The legacy stream and the thread's own by their handles, and a stream of the caller's."""
+    torch, k = torch_(), kb()
+    for handle in (0, 1, 2, torch.cuda.Stream().cuda_stream):
+        x, w, bias, a, b, scales, st = lora_case(4, [5, 6], 64, 64, 8, 2)
+        starts, ids, out = i32(st), i32([0, 1]), torch.zeros(x.shape[0], 64, dtype=torch.float16, device="cuda")
+        args = lora_args(x, w, bias, a, b, scales, starts, ids, out)
+        torch.cuda.synchronize()
+        k.lora_matmul_f16(args, handle)
+        k.operator_status(handle)
+        want, tol = lora_ref(x, w, bias, a, b, scales, st, [0, 1])
+        close(out[:st[-1]], want[:st[-1]], tol[:st[-1]])
