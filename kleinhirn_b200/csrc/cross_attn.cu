@@ -1036,6 +1036,8 @@ void cross_attention(const kh_cross_attention_args* args, cudaStream_t st) {
   check_that(a.q && a.out && a.q_starts && a.k_starts && (!states || (a.k && a.v)), fn, "null pointer argument");
   check_that(aligned(a.q) && aligned(a.out) && aligned(a.k) && aligned(a.v), fn,
              "q, k, v and out must be 16-byte aligned");
+  check_that(aligned4(a.key_mask) && aligned4(a.q_starts) && aligned4(a.k_starts), fn,
+             "key_mask, q_starts and k_starts must be 4-byte aligned");
   const int64_t qw = int64_t(a.q_heads) * a.head_dim, kw = int64_t(a.kv_heads) * a.head_dim;
   const int64_t lim = int64_t(1) << 31;
   check_that(a.q_stride >= qw && a.out_stride >= qw && a.q_stride < lim && a.out_stride < lim &&
@@ -1043,6 +1045,8 @@ void cross_attention(const kh_cross_attention_args* args, cudaStream_t st) {
              fn, "a stride is shorter than its rows (or 2^31 and more)");
   check_that(a.q_stride % 8 == 0 && a.out_stride % 8 == 0 && a.k_stride % 8 == 0 && a.v_stride % 8 == 0, fn,
              "strides must be multiples of 8");
+  check_that(a.out != a.q || a.out_stride == a.q_stride, fn, "out may be q with the same stride alone");
+  check_that(!states || (a.out != a.k && a.out != a.v), fn, "out may not be k or v: every query reads them");
   const int64_t need = cross_attention_workspace(args);
   check_that(need == 0 || (a.workspace && int64_t(a.workspace_bytes) >= need), fn, "workspace too small");
   check_that((reinterpret_cast<uintptr_t>(a.workspace) & 255) == 0, fn, "workspace must be 256-byte aligned");

@@ -35,6 +35,7 @@ int* lora_index_word();
 
 // Shared argument checks (ArgError with the entry point's name).
 void check_that(bool ok, const char* fn, const char* what);
+inline bool aligned4(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 3) == 0; }
 // The stream belongs to the current device.
 void check_stream(const char* fn, cudaStream_t st);
 // Memory a kernel on the current device can use: device memory of that device, managed or page-locked

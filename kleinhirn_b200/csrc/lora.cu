@@ -1357,6 +1357,8 @@ void lora_matmul(const kh_lora_matmul_args* args, cudaStream_t st) {
   check_that(aligned(a.x) && aligned(a.w) && aligned(a.bias) && aligned(a.lora_a) && aligned(a.lora_b) &&
                  aligned(a.out),
              fn, "x, w, bias, lora_a, lora_b and out must be 16-byte aligned");
+  check_that(aligned4(a.scales) && aligned4(a.seg_starts) && aligned4(a.seg_adapters), fn,
+             "scales, seg_starts and seg_adapters must be 4-byte aligned");
   const int64_t lim = int64_t(1) << 31;
   check_that(a.x_stride >= a.k && a.out_stride >= a.n && a.x_stride < lim && a.out_stride < lim &&
                  a.x_stride % 8 == 0 && a.out_stride % 8 == 0,

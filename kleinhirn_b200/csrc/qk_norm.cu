@@ -476,11 +476,9 @@ void qk_norm_rope(const kh_qk_norm_rope_args* args, cudaStream_t st) {
   if (a.rotary_dim) {
     check_that(a.cossin && a.positions, fn, "null cossin or positions");
     check_that(a.table_rows >= 1, fn, "table_rows must be at least 1");
-    check_that(reinterpret_cast<uintptr_t>(a.cossin) % 4 == 0 && reinterpret_cast<uintptr_t>(a.positions) % 4 == 0,
-               fn, "cossin and positions must be 4-byte aligned");
+    check_that(aligned4(a.cossin) && aligned4(a.positions), fn, "cossin and positions must be 4-byte aligned");
   }
-  check_that(reinterpret_cast<uintptr_t>(a.q_weight) % 4 == 0 && reinterpret_cast<uintptr_t>(a.k_weight) % 4 == 0, fn,
-             "weights must be 4-byte aligned");
+  check_that(aligned4(a.q_weight) && aligned4(a.k_weight), fn, "weights must be 4-byte aligned");
   check_stream(fn, st);
   check_device_memory(fn, "x", a.x);
   check_device_memory(fn, "out", a.out);
