@@ -251,7 +251,8 @@ int kh_attention_f16_noalloc_status(void* stream);
  * of every query and key head with the position rotation, attention over states of another length,
  * and a projection with the low-rank adapters of many requests. Common to the three:
  * - Every pointer of an argument struct is device memory of the current device (or null where the
- *   field says so), owned by the caller; strides are in elements. Nothing is allocated. The struct
+ *   field says so), owned by the caller; strides are in elements. int32 and f32 arrays are aligned to
+ *   their 4 bytes. Nothing is allocated. The struct
  *   itself is host memory and has been read when the call returns.
  * - The work is queued on `stream` (a cudaStream_t of the current device, NULL for the legacy default
  *   stream); the call returns once it is queued. Calls may be captured into a CUDA graph; the graph
@@ -271,7 +272,8 @@ int kh_attention_f16_noalloc_status(void* stream);
  * (the q heads first, as in a plan's qkv buffer; what follows them in a row is not read). For every
  * row and head y = x / sqrt(mean(x^2) + eps) * w, then the first rotary_dim values of y are rotated by
  * the row's position: (a, b) -> (a cos - b sin, b cos + a sin) for the pairs (d, d + rotary_dim / 2),
- * or (2 d, 2 d + 1) when interleaved, d < rotary_dim / 2. All of it in f32, rounded to dtype once.
+ * or (2 d, 2 d + 1) when interleaved, d < rotary_dim / 2. All of it in f32 (the squares too, so f32
+ * values are below 1e18), rounded to dtype once.
  * cossin: f32 [table_rows][2 * rotary_dim], cos of pair d at column d, sin at rotary_dim + d (the
  * layout of a plan's cossin buffer). out may be x itself (with the same stride), else they must not
  * overlap. A position outside [0, table_rows) gives a zero row and a status.
@@ -300,8 +302,9 @@ int kh_qk_norm_rope(const kh_qk_norm_rope_args* args, void* stream);
  * rows [q_starts[s], q_starts[s + 1]) and the state rows [k_starts[s], k_starts[s + 1]); query head h
  * reads key / value head h / (q_heads / kv_heads); out = softmax(scale q k^T) v over the states whose
  * key_mask is above 0.5. A row without a kept state is exactly zero, whatever k and v hold there.
- * f16 operands; scores, sums and the accumulated output in f32, the probabilities rounded to f16 for
- * the product with v, the output once. max_q and max_k bound the lengths (they size the grid and the
+ * f16 operands; scores (finite in f32, scaled), sums and the accumulated output in f32; the
+ * probabilities rounded to f16 for the product with v (by 2^-11 of each, or 2^-32 of the largest), the
+ * output once. max_q and max_k bound the lengths (they size the grid and the
  * split): of a longer sequence, query rows past max_q are not written and states past max_k not read.
  * out may be q itself (with the same stride); else it shares no value with what the call reads.
  * Limits: head_dim 32, 64 or 128; kv_heads divides q_heads (at most 1,024), at most 64 query heads to
@@ -311,7 +314,7 @@ typedef struct kh_cross_attention_args {
   int32_t n_seqs; /* 0: nothing to do */
   int32_t q_heads, kv_heads, head_dim;
   int32_t max_q, max_k; /* >= 0 */
-  float scale; /* > 0, finite */
+  float scale; /* > 0, at most 1e30 */
   int64_t q_rows, kv_rows; /* rows of the buffers */
   int64_t q_stride, k_stride, v_stride, out_stride;
   const void* q; /* f16 [q_rows][q_heads * head_dim] */
@@ -325,7 +328,7 @@ typedef struct kh_cross_attention_args {
   uint64_t workspace_bytes;
 } kh_cross_attention_args;
 /* Bytes of workspace of such a call (pointers and strides are not read), or -1 and kh_last_error. They
- * depend on the head counts, n_seqs, max_q and max_k, and need not grow with each of them. */
+ * depend on the head counts, head_dim, n_seqs, max_q and max_k, and need not grow with each. */
 int64_t kh_cross_attention_f16_workspace(const kh_cross_attention_args* args);
 int kh_cross_attention_f16(const kh_cross_attention_args* args, void* stream);
 

@@ -912,7 +912,7 @@ void check_sizes(const char* fn, const kh_cross_attention_args* args) {
              "q_rows and kv_rows must be in [0, 2^31)");
 }
 
-// One m16 block of rows to a key head: the kernel that streams k and v through registers.
+// One m16 block of rows to a key head: the kernel whose warps stream k and v through rings of their own.
 bool takes_rows_kernel(const kh_cross_attention_args& a) {
   return int64_t(a.max_q) * (a.q_heads / a.kv_heads) <= 16;
 }
@@ -1029,7 +1029,7 @@ void cross_attention(const kh_cross_attention_args* args, cudaStream_t st) {
   const char* fn = "kh_cross_attention_f16";
   check_sizes(fn, args);
   const kh_cross_attention_args& a = *args;
-  check_that(a.scale > 0.f && a.scale <= 1e30f, fn, "scale must be above 0 and finite");
+  check_that(a.scale > 0.f && a.scale <= 1e30f, fn, "scale must be above 0, at most 1e30");
   if (a.n_seqs == 0 || a.max_q == 0 || a.q_rows == 0) return;
   const bool states = a.kv_rows > 0 && a.max_k > 0;
   auto aligned = [](const void* x) { return (reinterpret_cast<uintptr_t>(x) & 15) == 0; };

@@ -12,6 +12,11 @@
 // lora_shrink_tile_kernel (HBM: reads x once) and lora_pair_kernel. A row tile that holds rows of
 // several adapters takes one more product per adapter, whose output lanes of other rows are switched
 // off in the instruction, so no operand is masked or copied, and rows of one adapter need not be neighbours.
+// (h is made with one product an adapter and tile; the projection lists a tile's adapters from 32 segments at a
+// time, so one that comes back in later segments takes a product again: 1,000 single rows of 60 adapters take
+// 233 to a tile of 256 rows.)
+// Times beside the kernels and rules are of calls in a graph, unless a single launch is named; calls queued one by
+// one from a program take 1 to 2 us more.
 
 #include "device_ops.h"
 
@@ -177,7 +182,7 @@ __global__ void __launch_bounds__(512) lora_shrink_rows_kernel(const LoraParams 
 // adapters meanwhile.
 // FUSED: where all adapters' A together have at most 128 rows, they are a second operand tile of every
 // stage, h comes out of the same pass over x, and there is no launch before this one.
-// 64 rows of 48 adapters of rank 16, 4,096 -> 4,096: 18.8 us, of it 2.6 to the first tile, 4 to 6 for W (46 MB
+// 64 rows of 48 adapters of rank 16, 4,096 -> 4,096: 19.2 us, of it 2.6 to the first tile, 4 to 6 for W (46 MB
 // with the adapters), 5 for the sum, the adapters and the outputs.
 
 constexpr int FT = 128;      // rows of x, at most
@@ -835,8 +840,8 @@ __global__ void __launch_bounds__(224) lora_shrink_tile_kernel(const __grid_cons
 //   TMA (tiles with rows that are not to be written: straight from registers); the last warp finds the
 //   adapters of the tiles ahead, in lists of up to 16 from 32 segments (found by the TMA warp itself, the
 //   dependent loads of the search held up the K blocks: 7 % on 65,536 rows of 768 -> 2,304).
-// 256 texts of 68,000 rows, 768 -> 2,304, 16 adapters of rank 32: 197 us, 1,280 TFLOP/s, the tensor pipe 72 %
-// busy under the power cap; h before it 25 us (its x 4 TB/s).
+// 256 texts of 68,000 rows, 768 -> 2,304, 16 adapters of rank 32: 199 us by itself, 1,270 TFLOP/s, the tensor
+// pipe 71 % busy under the power cap; h before it 24 us by itself (its x 4 TB/s). The call: 232 to 270 in a graph.
 
 constexpr int BM = 128;
 constexpr int BK = 64;

@@ -5,12 +5,11 @@
 // position. Everything between the load and the store is f32; one rounding at the store.
 //
 // Bound: HBM, each value read and written once (7 operations per value).
-// Layout: a head is cut into chunks of VEC values (one load each), and a thread owns two chunks of the
-// same head, the pair that the rotation mixes (chunk i and the one R / 2 values on; neighbours when
-// the pairs are neighbours or behind R), so the rotation needs no exchange. LANES threads, a power of
-// two, hold a head and add their squares by shuffles. A thread takes U heads of the same row: it loads
-// the angles and weights once, folds them into coefficients w cos and w sin (the scale of a head
-// comes last), and has 2 U loads in flight.
+// Layout: a head is cut into chunks of VEC values (one load each). In the usual kernel a thread owns one chunk and
+// takes the chunk that the rotation mixes with it from that chunk's lane; in the one for other heads it owns both,
+// and the rotation needs no exchange. The threads of a head add their squares by shuffles. A thread takes U heads
+// of the same row: it loads the angles and weights once, folds them into coefficients w cos and w sin (the scale
+// of a head comes last), and has the loads of all its heads in flight.
 
 #include "device_ops.h"
 
@@ -125,8 +124,8 @@ __device__ __forceinline__ void coefficients(float (&wc)[VEC], float (&ws)[VEC],
 // count (packed f32x2 arithmetic, one mode to a kernel): 65,536 rows of 24 heads of 64 take 77 us (5.3 TB/s;
 // 91 us with every mode in one kernel, 160 instructions to a chunk, and 83 us with the kernel below). Heads
 // whose chunks are no power of two (!POW2) share a warp whole: 35,149 rows of 20 heads of 80, 55 us against
-// 65 with 16 lanes to their 10 chunks. Four CTAs to an SM where 64 registers hold it (neighbouring pairs: 20,011 rows
-// of 20 heads of 128, 39 us against 43; pairs R / 2 apart would spill: 99 against 77).
+// 65 with 16 lanes to their 10 chunks. Four CTAs to an SM for neighbouring pairs, though 64 registers spill 36 bytes
+// (20,011 rows of 20 heads of 128, 39 us against 43); pairs R / 2 apart would spill more (99 against 77).
 template <typename T, int VEC, int U, int MODE, bool POW2>
 __global__ void __launch_bounds__(256, MODE != 2 ? 3 : POW2 ? 4 : 0) qk_norm_rope_lanes_kernel(const NormParams p, int lanes) {
   const int lane = threadIdx.x & 31;
@@ -255,7 +254,8 @@ __global__ void __launch_bounds__(256, MODE != 2 ? 3 : POW2 ? 4 : 0) qk_norm_rop
   }
 }
 
-// Heads of more chunks, and unaligned ones. PAIRS: chunk pairs of a thread (1, or 4 for the one-value
+// Heads of more chunks, and unaligned ones: a thread owns chunk i of a head and the one R / 2 values on (neighbours
+// where the pairs are neighbours or behind R). LANES threads, a power of two, hold a head. PAIRS: chunk pairs of a thread (1, or 4 for the one-value
 // chunks of unaligned heads). LANES * PAIRS pairs cover D <= 256.
 template <typename T, int VEC, int PAIRS, int U>
 __global__ void __launch_bounds__(256) qk_norm_rope_kernel(const NormParams p, int lanes_log2) {
