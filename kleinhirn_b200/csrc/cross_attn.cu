@@ -784,16 +784,22 @@ __global__ void __launch_bounds__(TCfg<D>::THREADS, TCfg<D>::ONE ? 1 : 2)
           tmem_st_wait();
         }
       }
-      const float ref = m == -INFINITY ? 0.f : m - LIFT;
+      float ref = m == -INFINITY ? 0.f : m - LIFT;
       // 2^(s scale - m) in one step keeps the bits of the product that m, the rounded one, lacks: up to half a
-      // unit of m in the last place, far outside f16 for the largest. There the products are rounded first.
-      float mul = p.scale_log2;
-      if (__any_sync(0xffffffffu, fabsf(ref) > EXACT_REF)) {
-        mul = 1.f;
+      // unit of m in the last place, far outside f16 for the largest. There the products of the row are rounded
+      // first, and the exponents taken back to the scale of scores (a factor of the row's own instead takes a
+      // register that the others lack: 5 % slower).
+      const bool far = fabsf(ref) > EXACT_REF;
+      if (__any_sync(0xffffffffu, far)) {
+        const float back = 1.f / p.scale_log2;
 #pragma unroll
         for (int c = 0; c < W; ++c)
 #pragma unroll
-          for (int i = 0; i < 32; ++i) sr[c][i] = __float_as_uint(__fmul_rn(__uint_as_float(sr[c][i]), p.scale_log2));
+          for (int i = 0; i < 32; ++i) {
+            const float s = __uint_as_float(sr[c][i]);
+            sr[c][i] = __float_as_uint(far ? (__fmul_rn(s, p.scale_log2) - ref) * back : s);
+          }
+        if (far) ref = 0.f;
       }
       float2 ls[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
       constexpr int CHUNK = C::ONE ? 32 : 8;  // packed pairs stored at a time, as the registers allow
@@ -804,7 +810,7 @@ __global__ void __launch_bounds__(TCfg<D>::THREADS, TCfg<D>::ONE ? 1 : 2)
         for (int i = 0; i < CHUNK; ++i) {
           const int k = 2 * (c + i);
           const float2 x = ffma2(make_float2(__uint_as_float(sr[k / 32][k & 31]), __uint_as_float(sr[k / 32][(k + 1) & 31])),
-                                 twice(mul), twice(-ref));
+                                 twice(p.scale_log2), twice(-ref));
           const float2 e = make_float2(ex2_approx(x.x), ex2_approx(x.y));
           ls[i & 1] = fadd2(ls[i & 1], e);
           pk[i] = pack_half2(e.x, e.y);

@@ -394,3 +394,24 @@ def test_streams_by_handle():
         k.operator_status(handle)
         want, tol = lora_ref(x, w, bias, a, b, scales, st, [0, 1])
         close(out[:st[-1]], want[:st[-1]], tol[:st[-1]])
+
+
+@pytest.mark.parametrize("D", [32, 64, 128])
+def test_cross_scores_of_a_row_leave_the_others_alone(D):
+    """One query with scores beyond 2^22 among others of its tile: theirs are the same bits as without it."""
+    torch = torch_()
+    n_q, n_k, row = 150, 700, 5
+    g = gen(D)
+    q, k, v = randn(g, n_q, D, scale=1.5 / 64), randn(g, n_k, D), randn(g, n_k, D)
+    outs = []
+    for top in (0.02, 60000.0):
+        q[row] = top
+        out = torch.zeros_like(q)
+        a = cross_args(q, k, v, out, i32([0, n_q]), i32([0, n_k]), 1, 1, D, 8.0, n_q, n_k)
+        kb().cross_attention_f16(a, stream())
+        kb().operator_status(stream())
+        outs.append(out)
+    s = (q[row].double() @ k.double().T).abs().max() * 8 * 1.4427
+    assert s > 2.0 ** 22
+    others = torch.arange(n_q, device="cuda") != row
+    assert torch.equal(outs[0][others], outs[1][others]) and not torch.equal(outs[0][row], outs[1][row])
