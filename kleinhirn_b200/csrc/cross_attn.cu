@@ -223,9 +223,9 @@ __global__ void __launch_bounds__(RW * 32)
       for (int r = 0; r < 2; ++r) {
         top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 1));
         top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 2));
-        const float mn = fmaxf(m[r], top[r]);
-        const float corr = mn > m[r] ? ex2_approx(m[r] - mn) : 1.f;  // (0 from m = -inf)
-        m[r] = mn;
+        const bool moves = top[r] - m[r] > RISE;  // the row's own: another one's scores leave its bits alone
+        const float corr = moves ? ex2_approx(m[r] - top[r]) : 1.f;  // (0 from m = -inf)
+        if (moves) m[r] = top[r];
         l[r] *= corr;
 #pragma unroll
         for (int e = 0; e < E; ++e) {

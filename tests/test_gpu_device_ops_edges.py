@@ -415,3 +415,23 @@ def test_cross_scores_of_a_row_leave_the_others_alone(D):
     assert s > 2.0 ** 22
     others = torch.arange(n_q, device="cuda") != row
     assert torch.equal(outs[0][others], outs[1][others]) and not torch.equal(outs[0][row], outs[1][row])
+
+
+@pytest.mark.parametrize("D", [32, 64, 128])
+def test_cross_few_rows_leave_one_another_alone(D):
+    """Up to 16 rows share a block of products: a row's bits are those that it has beside other rows."""
+    torch = torch_()
+    n_q, n_k = 12, 900
+    g = gen(D)
+    q, k, v = randn(g, n_q, D, scale=1.5), randn(g, n_k, D), randn(g, n_k, D)
+    k *= torch.linspace(0.2, 3, n_k, device="cuda")[:, None].half()  # the largest scores grow along the states
+    outs = []
+    for size in (1.0, 0.1, 4.0):
+        q2 = q * size
+        q2[5] = q[5]
+        out = torch.zeros_like(q)
+        a = cross_args(q2, k, v, out, i32([0, n_q]), i32([0, n_k]), 1, 1, D, 0.125, n_q, n_k)
+        kb().cross_attention_f16(a, stream())
+        kb().operator_status(stream())
+        outs.append(out[5])
+    assert torch.equal(outs[0], outs[1]) and torch.equal(outs[0], outs[2])
