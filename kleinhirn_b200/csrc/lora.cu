@@ -2,10 +2,10 @@
 //
 // out[t] = x[t] W^T + bias + s_a (x[t] A_a^T) B_a^T, a the adapter of the segment of rows that t lies
 // in. Two launches: h[t] = s_a x[t] A_a^T (rank values a row, rounded to f16: 2^-11 of the adapter's
-// own part; rows with a value beyond f16: see row_beyond_f16), then the projection with h B_a^T added to the same f32 accumulators, rounded once. The
-// second launch starts while the first runs (programmatic dependent launch) and waits for it where it
-// needs h, behind the projection's own products. (One launch where few rows have few adapters: see
-// lora_few_kernel.)
+// own part; rows with a value beyond f16: see row_beyond_f16), then the projection with h B_a^T added to
+// the same f32 accumulators, rounded once. The second launch starts while the first runs (programmatic
+// dependent launch) and waits for it where it needs h, behind the projection's own products. (One launch
+// where few rows have few adapters: see lora_few_kernel.)
 //
 // Few rows (takes_few): bound by reading W, A and B once; lora_shrink_rows_kernel and
 // lora_few_kernel. Many rows: bound by the tensor cores;
@@ -538,6 +538,7 @@ __global__ void __maxnreg__(FUSED ? 168 : 112)
       if (zero != 0.f) not_finite |= 1u << j;
     }
   }
+  __syncwarp();  // (such a row is written again, over what other lanes wrote)
   for (not_finite = __reduce_or_sync(0xffffffffu, not_finite); not_finite; not_finite &= not_finite - 1) {
     const int k = warp + (__ffs(not_finite) - 1) * (FTHREADS / 32), i = (k / 8 * Z + z) * 8 + k % 8;
     if (ids[i] < 0) continue;
@@ -1197,6 +1198,7 @@ __global__ void __launch_bounds__(PCfg<BN>::THREADS, 1)
       }
       if (p.n_adapters > 0) {
         uint32_t rows = __ballot_sync(0xffffffffu, zero.x + zero.y != 0.f && row >= begin && row < end);
+        __syncwarp();  // (such a row is written again, over what its own lane wrote)
         for (; rows; rows &= rows - 1) {
           const int rr = q * 32 + __ffs(rows) - 1, again = row0 + rr, seg = first_seg(p, again, 0);
           const int ad = seg < p.n_segs && again >= seg_start(p, seg) ? adapter_of(p, seg) : -1;
